@@ -45,6 +45,9 @@ HIP_SOURCES = [
     ("block_ops.hip", []),
     ("softmax.hip", []),
     ("distributions.hip", []),
+    ("kv_cache.hip", []),
+    ("kv_attention.hip", []),
+    ("token_logprobs.hip", []),
 ]
 
 HIP_FLAGS = [

@@ -28,6 +28,15 @@ class EmberError(RuntimeError):
     pass
 
 
+class KVCacheView(C.Structure):
+    """ember_kv_cache: where a 4-bit key/value cache lies and how it is cut
+    (addresses of device memory, and sizes)."""
+
+    _fields_ = [("k_codes", _vp), ("k_scales", _vp), ("v_codes", _vp), ("v_scales", _vp), ("page_table", _vp),
+                ("pages", _i64), ("heads", _i64), ("page_size", _i64), ("head_dim", _i64),
+                ("sequences", _i64), ("max_pages", _i64)]
+
+
 def exported_symbols() -> list[str]:
     """Every function name include/ember_amd.h declares (operators.def expanded)."""
     names: list[str] = []
@@ -99,6 +108,17 @@ def lib() -> C.CDLL:
     L.adamw_step.argtypes = [C.POINTER(_vp)] * 4 + [C.POINTER(_i64), C.c_int] + [C.c_double] * 5 + [_i64]
     L.sgd_step.restype = C.c_int
     L.sgd_step.argtypes = [C.POINTER(_vp)] * 3 + [C.POINTER(_i64), C.c_int] + [C.c_double] * 2
+    cache = C.POINTER(KVCacheView)
+    L.kv_cache_write.restype = C.c_int
+    L.kv_cache_write.argtypes = [cache, _vp, _vp] + [_i64] * 4 + [_vp] * 3
+    L.kv_cache_read.restype = C.c_int
+    L.kv_cache_read.argtypes = [cache, _vp, _vp] + [_i64] * 4 + [_vp] * 2
+    L.kv_cache_attention.restype = C.c_int
+    L.kv_cache_attention.argtypes = [cache, _vp, _vp, _vp, _i64, _i64, C.c_float, C.c_int] + [_i64] * 6 + [_vp] * 2
+    L.token_logprobs.restype = C.c_int
+    L.token_logprobs.argtypes = [_vp, _i64, _vp, _i64, _i64] + [_vp] * 5 + [C.c_int]
+    L.token_logprobs_bwd.restype = C.c_int
+    L.token_logprobs_bwd.argtypes = [_vp, _i64] + [_vp] * 6 + [_i64] * 3
     _lib = L
     return L
 

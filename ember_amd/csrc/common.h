@@ -39,7 +39,9 @@ enum ScratchSlot {
     kScratchColSum = 3,
     kScratchGemmSplit = 4,
     kScratchAttnOrder = 5,
-    kScratchSlots = 6
+    kScratchKvAttention = 6,
+    kScratchLogprobs = 7,
+    kScratchSlots = 8
 };
 
 // The library-wide switch set by ember_set_deterministic.

@@ -335,6 +335,106 @@ int layernorm_bwd(const float *x, const float *gamma, const float *mean, const f
                   const float *dy, const float *dres, float *dx, float *dgamma, float *dbeta,
                   int64_t rows, int64_t d);
 
+/* ---- key/value cache in 4 bits (new; no reference counterpart) ----
+ *
+ * Keys and values of tokens already seen, for decoding.  A token's head row of
+ * D elements is cut into groups of 32 neighbours; a group is held as 32 E2M1
+ * codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign bit, 8) that share one scale
+ * 2^e, stored as the byte e + 127 (the OCP MXFP4 format).  e is the smallest
+ * number with amax <= 6 * 2^e, but at least -119; each element is rounded to
+ * the nearest code times 2^e, ties to the even code.  A group of zeros has the
+ * scale byte 127; one that holds a NaN or a size from 2^127 on has the byte 255
+ * and reads back as NaN.
+ *
+ * Codes are (pages, heads, page_size, D/2) bytes, element 2i of a row in the
+ * low nibble of byte i and 2i+1 in the high one; scales are (pages, heads,
+ * page_size, D/32) bytes; k_ and v_ arrays alike.  Sequence b's tokens
+ * i*page_size .. (i+1)*page_size - 1 lie on page page_table[b*max_pages + i];
+ * pages may be shared by sequences that only read them.  A token whose page is
+ * outside [0, pages) or past the table is not there: it is not written, reads
+ * back as zero and is not attended to.
+ *
+ * heads >= 1, D in {32, 64, 128}, page_size a power of two from 16 to 65536,
+ * at most 2^31 - 1 pages and max_pages * page_size at most 2^31 - 2^16.  The
+ * arrays are device memory, 16-byte aligned, of the caller's; the struct
+ * itself is host memory, read during the call only.
+ *
+ * A call works on T rows per sequence: row t is token start[b] + t of sequence
+ * b, and is valid where t < count[b].  start and count are int32 device arrays
+ * of `sequences` elements; NULL start is 0 for all, NULL count is T for all.
+ * Counts outside [0, T] are taken as the nearer end; tokens below 0 are not
+ * there.  Element (b, t, h, d) of an fp32 operand lives at b*sb + h*sh + t*ss +
+ * d (strides as in attention_fwd: multiples of 4, 16-byte aligned pointers, row
+ * strides below 2^24; none negative).  T * heads is below 2^31 - 2^16, and
+ * sequences at most 65535. */
+typedef struct ember_kv_cache {
+    void *k_codes, *k_scales, *v_codes, *v_scales;
+    const int32_t *page_table; /* (sequences, max_pages) */
+    int64_t pages, heads, page_size, head_dim;
+    int64_t sequences, max_pages;
+} ember_kv_cache;
+
+/* Rounds the valid rows of k and v into the cache.  Two valid rows must not
+ * land on the same slot (a page written through two table entries).  next,
+ * when not NULL, is an int32 device array that gets start[b] + the number of
+ * valid rows, where the sequence's next call starts; it must not be start. */
+int kv_cache_write(const ember_kv_cache *cache, const float *k, const float *v, int64_t T,
+                   int64_t in_sb, int64_t in_sh, int64_t in_ss, const int32_t *start,
+                   const int32_t *count, int32_t *next);
+/* The values that the cache holds for the valid rows; rows that are not valid
+ * are written as zeros. */
+int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, int64_t T, int64_t out_sb,
+                  int64_t out_sh, int64_t out_ss, const int32_t *start, const int32_t *count);
+/* Attention of T query rows per sequence over the cache, whose tokens 0 ..
+ * start[b] + count[b] - 1 (the rows' own among them) have been written.  Query
+ * head h of q_heads reads cache head h / (q_heads / heads); q_heads is a
+ * multiple of heads.  With s[t][j] = scale * <q_t, k_j>, key j is visible to
+ * the valid row t iff j < start + count and, when causal, j <= start + t;
+ * o_t = softmax_j(s[t][.]) v, lse_t = ln sum_j exp(s[t][j]) (may be NULL),
+ * dense (sequences, q_heads, T).  A row that is not valid, or sees no key,
+ * gets o = 0 and lse = -infinity.  Keys and values enter exactly and q in full
+ * fp32: products are those of an fp32 attention over kv_cache_read's values.
+ * A row of q that holds an infinity or a NaN gets NaN; keys and values that
+ * read back as NaN reach the rows that see them, and no others.  scale is
+ * finite and >= 0; T * q_heads / heads is at most 2^30, and sequences * heads *
+ * T * q_heads / heads at most 2^24.  Uses library scratch; o must not overlap
+ * q. */
+int kv_cache_attention(const ember_kv_cache *cache, const float *q, float *o, float *lse, int64_t T,
+                       int64_t q_heads, float scale, int causal, int64_t in_sb, int64_t in_sh,
+                       int64_t in_ss, int64_t out_sb, int64_t out_sh, int64_t out_ss,
+                       const int32_t *start, const int32_t *count);
+
+/* ---- log probabilities by token id (new; no reference counterpart) ----
+ *
+ * logits is (rows, classes) with row r at logits + r*row_stride (row_stride >=
+ * classes).  Per row, with lse = ln sum_j exp(x_j) and p_j = exp(x_j - lse):
+ *   logp    = x[tokens[r]] - lse, or 0 where tokens[r] is outside [0, classes)
+ *             (a padded place)
+ *   entropy = -sum_j p_j ln p_j  (in nats; a logit of -infinity adds nothing)
+ *   top_tokens, top_logp (rows, top): the `top` largest logits' ids, largest
+ *             first and of equal ones the lowest id first, and their log
+ *             probabilities; top from 0 (both may be NULL) to min(64, classes)
+ * lse and entropy may be NULL.  A row that holds a NaN or +infinity, or only
+ * -infinity, gives NaN in logp (of a token in range), entropy and top_logp,
+ * and in lse NaN, or -infinity if it holds nothing else; where NaN stands in
+ * the order of top_tokens is not specified.  tokens are int32 device memory.
+ * Uses library scratch.
+ * classes from 1 to 2^31 - 2^16. */
+int token_logprobs(const float *logits, int64_t row_stride, const int32_t *tokens, int64_t rows,
+                   int64_t classes, float *logp, float *lse, float *entropy, int32_t *top_tokens,
+                   float *top_logp, int top);
+/* Its gradient: from the upstream gradients d_logp and d_entropy (rows; either
+ * may be NULL, 0) and the forward's lse and entropy (entropy may be NULL where
+ * d_entropy is),
+ *   d_logits[r][j] = d_logp * ([j == tokens[r]] - p_j)
+ *                    - d_entropy * p_j * (ln p_j + entropy),
+ * d_logp taken as 0 where tokens[r] is out of range; row r at d_logits +
+ * r*out_stride.  d_logits may be logits itself (with the same stride); it
+ * must not overlap it otherwise. */
+int token_logprobs_bwd(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
+                       const float *entropy, const float *d_logp, const float *d_entropy, float *d_logits,
+                       int64_t out_stride, int64_t rows, int64_t classes);
+
 #undef EMBER_BINARY_OP
 #undef EMBER_SCALAR_OP
 #undef EMBER_BROADCAST_OP

@@ -1,0 +1,305 @@
+"""The 4-bit cache through the C ABI against a NumPy oracle: what is written is
+right to the bit, at the right slots and nowhere else; what is read back is the
+same; attention over it agrees with float64 for one row and many, page ends,
+padded batches, rows that see nothing, and slots that hold no numbers."""
+
+import numpy as np
+import pytest
+
+import gpu_helpers as G
+from ember_amd import capi
+from oracle import serving
+from serving_helpers import Bytes, Pair, ints, table
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(rng, *shape):
+    return rng.standard_normal(shape).astype(np.float32)
+
+
+def same_slots(p):
+    for name, dev, host in (("codes", p.codes, p.host.codes), ("scales", p.scales, p.host.scales)):
+        for d, h in zip(dev, host):
+            np.testing.assert_array_equal(d.numpy(), h, err_msg=name)
+
+
+# ---- writing and reading ----
+
+
+def hard_rows(D):
+    """Rows whose groups are zeros, ties, borders of the scale, and no numbers."""
+    rng = np.random.default_rng(5)
+    rows = [np.zeros(32), -np.zeros(32), np.linspace(-6, 6, 32), np.linspace(-1, 1, 32) * 1e-30, np.full(32, 1e-45),
+            np.array([6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5] * 4), -np.array([6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5] * 4),
+            np.nextafter(np.float32(6), np.float32(7)) * np.linspace(-1, 1, 32), np.full(32, 1.5), np.full(32, -3 * 2.0 ** 90),
+            np.linspace(0, 1.99 * 2.0 ** 126, 32), np.linspace(-1, 1, 32) * 2.0 ** -119, np.linspace(-1, 1, 32) * 2.0 ** -122]
+    for bad in (np.inf, -np.inf, np.nan, 2.0 ** 127, np.finfo(np.float32).max):
+        x = rng.standard_normal(32)
+        x[7] = bad
+        rows.append(x)
+    rows += [rng.standard_normal(32) * 10.0 ** rng.integers(-30, 30) for _ in range(110)]
+    x = np.array(rows, np.float32)  # a multiple of 4 groups
+    return x[:len(x) // (D // 32) * (D // 32)].reshape(-1, D)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_write_rounds_as_the_format_says(D):
+    x = hard_rows(D)
+    T = len(x)
+    p = Pair((T + 15) // 16, 1, 16, D, [np.arange((T + 15) // 16)])
+    p.write(x[None, :, None], -x[None, ::-1, None])
+    same_slots(p)
+    k, v = p.read(T)
+    for got, ref in zip((k, v), p.host.read(T)):
+        np.testing.assert_array_equal(got, ref.astype(np.float32))
+
+
+@pytest.mark.parametrize("B, T, H, D, page, start, count", [
+    (1, 1, 1, 32, 16, None, None),
+    (3, 5, 2, 64, 16, [0, 14, 31], None),            # across page ends
+    (4, 7, 5, 128, 32, [3, 0, 57, 20], [7, 0, 4, 9]),  # none valid, some valid, a count past T
+    (2, 33, 3, 32, 64, [0, 40], [33, 20]),
+    (3, 4, 1, 64, 16, [-2, 62, 1000], None),         # before the sequence, past its table
+    (2, 600, 16, 128, 256, [1, 100], [600, 411]),
+])
+def test_write_and_read_slots(B, T, H, D, page, start, count):
+    rng = np.random.default_rng(B * T + D)
+    places = -(-(max(start or [0]) + T) // page) if max(start or [0]) < 900 else 64 // page
+    tab, pages = table(rng, B, places)
+    p = Pair(pages, H, page, D, tab, fill=0x5A)
+    got, ref = p.write(normal(rng, B, T, H, D), normal(rng, B, T, H, D), start, count, stride_pad=4)
+    np.testing.assert_array_equal(got, ref)
+    same_slots(p)
+    for got, ref in zip(p.read(T, start, count), p.host.read(T, start, count)):
+        np.testing.assert_array_equal(got, ref.astype(np.float32))
+
+
+@pytest.mark.parametrize("fault", [-1, 7, 2 ** 31 - 1, -2 ** 31])
+def test_pages_that_are_not_there(fault):
+    """Tokens of a page outside the cache are dropped, read as zero and not seen."""
+    rng = np.random.default_rng(11)
+    tab = np.array([[0, fault, 2], [3, 4, fault]], np.int32)
+    p = Pair(7, 2, 16, 64, tab)
+    k, v = normal(rng, 2, 48, 2, 64), normal(rng, 2, 48, 2, 64)
+    p.write(k, v)
+    same_slots(p)
+    for got, ref in zip(p.read(48), p.host.read(48)):
+        np.testing.assert_array_equal(got, ref.astype(np.float32))
+    p.check_attention(normal(rng, 2, 3, 4, 64), True, start=[45, 20])
+    p.check_attention(normal(rng, 2, 1, 4, 64), True, start=[17, 47])
+
+
+def test_next_without_rows_and_no_next():
+    p = Pair(2, 1, 16, 32, [[0], [1]])
+    start, nxt = ints([3, 9]), ints([-1, -1])
+    p.write(np.ones((2, 1, 1, 32), np.float32), np.ones((2, 1, 1, 32), np.float32), [3, 9])
+    G.say("kv_cache_write of no rows")
+    capi.check(capi.lib().kv_cache_write(p.view, None, None, 0, 0, 0, 0, start.ptr, None, nxt.ptr), "kv_cache_write")
+    np.testing.assert_array_equal(nxt.numpy(), [3, 9])
+    same_slots(p)
+
+
+# ---- attention ----
+
+
+def filled(rng, B, H, page, D, L, fill=255):
+    """A cache of B sequences with L tokens each (slots past them hold `fill`)."""
+    tab, pages = table(rng, B, -(-L // page))
+    p = Pair(pages, H, page, D, tab, fill)
+    p.write(normal(rng, B, L, H, D), normal(rng, B, L, H, D))
+    return p
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("L", [1, 2, 15, 16, 17, 31, 33, 64, 127, 200])
+def test_one_token(D, L):
+    rng = np.random.default_rng(L + D)
+    p = filled(rng, 2, 2, 16, D, L)
+    p.check_attention(normal(rng, 2, 1, 4, D), True, start=[L - 1, (L - 1) // 2])
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8, 9, 16, 17])
+@pytest.mark.parametrize("T", [1, 3, 8])
+def test_groups_of_heads(group, T):
+    rng = np.random.default_rng(group * T)
+    p = filled(rng, 2, 3, 32, 64, 90)
+    p.check_attention(normal(rng, 2, T, 3 * group, 64), True, start=[90 - T, 7])
+
+
+@pytest.mark.parametrize("D, T, G_, L, causal", [
+    (128, 40, 4, 150, True), (64, 33, 1, 97, True), (32, 70, 2, 130, True), (128, 64, 1, 64, True), (64, 129, 3, 200, False),
+    (32, 5, 1, 300, False), (128, 17, 8, 80, False),
+])
+def test_many_rows(D, T, G_, L, causal):
+    rng = np.random.default_rng(D + T)
+    p = filled(rng, 2, 2, 16, D, L)
+    p.check_attention(normal(rng, 2, T, 2 * G_, D), causal, start=[L - T, (L - T) // 3])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("T", [4, 50])
+def test_padded_batch_and_empty_rows(causal, T):
+    """Counts below T, sequences with nothing in them, rows before the start."""
+    rng = np.random.default_rng(T)
+    p = filled(rng, 5, 2, 16, 64, 80)
+    o, lse = p.check_attention(normal(rng, 5, T, 6, 64), causal, start=[80 - T, 3, 0, 0, -2], count=[T, 2, 0, 1, T - 1])
+    assert (o[2] == 0).all() and np.isneginf(lse[2]).all()
+    assert (o[1, 2:] == 0).all() and np.isneginf(lse[1, :, 2:]).all()
+    if causal:
+        assert (o[4, :2] == 0).all() and np.isneginf(lse[4, :, :2]).all()
+
+
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_what_is_no_number_reaches_only_who_sees_it(T, D):
+    """NaN keys and values late in a sequence: rows before them stay finite."""
+    rng = np.random.default_rng(T + D)
+    L = 70
+    tab, pages = table(rng, 2, 5)
+    p = Pair(pages, 2, 16, D, tab)
+    k, v = normal(rng, 2, L, 2, D), normal(rng, 2, L, 2, D)
+    v[0, L - 1, 0, D - 1] = np.nan
+    v[1, L - T // 2 - 1, 1, 0] = np.inf
+    k[1, L - 1, 0, 3] = np.nan
+    p.write(k, v)
+    q = normal(rng, 2, T, 4, D)
+    o, _ = p.check_attention(q, True, start=[L - T, L - T])
+    assert np.isnan(o[0, -1, 0, D - 32:]).all() and np.isfinite(o[0, -1, 0, :D - 32]).all()
+    if T > 1:
+        assert np.isfinite(o[0, :-1]).all()
+    p.check_attention(q, True, start=[L - T - 10, 5])
+
+
+def test_long_sequence_and_splits():
+    """Keys split over workgroups, and joined: 5000 tokens of one sequence."""
+    rng = np.random.default_rng(3)
+    p = filled(rng, 1, 1, 256, 32, 5000)
+    p.check_attention(normal(rng, 1, 1, 2, 32), True, start=[4999])
+    p.check_attention(normal(rng, 1, 2, 1, 32), True, start=[130])
+
+
+def test_scores_of_all_sizes():
+    """Scores from -300 to 300, growing along the keys (the maximum is raised often), and scale 0."""
+    rng = np.random.default_rng(8)
+    tab, pages = table(rng, 1, 10)
+    p = Pair(pages, 1, 16, 64, tab)
+    k = normal(rng, 1, 160, 1, 64) * np.linspace(0.01, 40, 160, dtype=np.float32)[None, :, None, None]
+    p.write(k, normal(rng, 1, 160, 1, 64))
+    q = normal(rng, 1, 5, 4, 64)
+    o, lse = p.attention(q, True, start=[155])
+    ro, rl, weight, reach = p.host.attention(q, True, G.scale_for(64), [155], None)
+    off = 2 * 2.0 ** -24 * (64 + 8) * reach.transpose(0, 2, 1)[..., None]
+    assert (np.abs(o - ro) <= (2 * off + 2.0 ** -23 * 176) * weight).all()
+    p.check_attention(q, True, scale=0.0, start=[155])
+
+
+def test_a_row_of_q_that_is_no_number():
+    rng = np.random.default_rng(9)
+    p = filled(rng, 1, 1, 16, 64, 40)
+    q = normal(rng, 1, 3, 2, 64)
+    q[0, 1, 0, 5] = np.inf
+    q[0, 2, 1, 7] = np.nan
+    o, lse = p.attention(q, True, start=[37])
+    assert np.isnan(o[0, 1, 0]).all() and np.isnan(o[0, 2, 1]).all() and np.isnan(lse[0, 0, 1]) and np.isnan(lse[0, 1, 2])
+    fine = np.isfinite(q).all(-1)
+    ro = p.host.attention(np.where(fine[..., None], q, 0), True, G.scale_for(64), [37], None)[0]
+    np.testing.assert_allclose(o[fine], ro[fine], rtol=0, atol=2e-5)
+
+
+def test_small_and_large_sizes_of_numbers():
+    """Queries near the ends of fp32's range meet keys near the others."""
+    rng = np.random.default_rng(10)
+    tab, pages = table(rng, 1, 2)
+    p = Pair(pages, 1, 16, 32, tab)
+    k = normal(rng, 1, 20, 1, 32) * np.float32(2.0 ** -60)
+    p.write(k, normal(rng, 1, 20, 1, 32) * np.float32(2.0 ** 100))
+    p.check_attention(normal(rng, 1, 2, 1, 32) * np.float32(2.0 ** 60), True, start=[18])
+
+
+def test_layouts_and_no_lse():
+    rng = np.random.default_rng(12)
+    p = filled(rng, 2, 2, 32, 128, 50)
+    q = normal(rng, 2, 9, 4, 128)
+    o1, _ = p.check_attention(q, True, start=[41, 20])
+    o2, _ = p.check_attention(q, True, start=[41, 20], head_major=True)
+    o3, none = p.check_attention(q, True, start=[41, 20], want_lse=False)
+    assert none is None
+    np.testing.assert_array_equal(o1, o2)
+    np.testing.assert_array_equal(o1, o3)
+
+
+def test_shared_pages():
+    """Two sequences whose first pages are the same ones."""
+    rng = np.random.default_rng(13)
+    p = Pair(4, 1, 16, 64, [[0, 1, 2], [0, 1, 3]])
+    k, v = normal(rng, 1, 32, 1, 64), normal(rng, 1, 32, 1, 64)
+    both = lambda x: np.concatenate([x, np.zeros_like(x)])  # noqa: E731
+    p.write(both(k), both(v), count=[32, 0])
+    p.write(normal(rng, 2, 5, 1, 64), normal(rng, 2, 5, 1, 64), start=[32, 32])
+    p.check_attention(normal(rng, 2, 5, 2, 64), True, start=[32, 32])
+
+
+def test_calls_repeat_to_the_bit():
+    rng = np.random.default_rng(14)
+    p = filled(rng, 3, 4, 64, 128, 700)
+    q = normal(rng, 3, 1, 16, 128)
+    first = p.attention(q, True, start=[699, 300, 64])
+    for _ in range(3):
+        again = p.attention(q, True, start=[699, 300, 64])
+        for a, b in zip(first, again):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_far_slots():
+    """Pages whose codes lie past 2^32 bytes from the first."""
+    pages, heads, page, D = 70000, 2, 512, 128   # 64 bytes a row: 4.6 GB of codes each
+    G.say("kv cache of 70000 pages")
+    per = heads * page * D // 2
+    codes = [capi.DeviceArray((pages * per // 4,)) for _ in range(2)]
+    scales = [capi.DeviceArray((pages * per // 64,)) for _ in range(2)]
+    rng = np.random.default_rng(15)
+    tab = Bytes(np.array([[pages - 1, 3]], np.int32))
+    near = Pair(2, heads, page, D, [[0, 1]])
+    far = capi.KVCacheView(codes[0].ptr, scales[0].ptr, codes[1].ptr, scales[1].ptr, tab.ptr, pages, heads, page, D, 1, 2)
+    k, v, q = normal(rng, 1, 600, heads, D), normal(rng, 1, 600, heads, D), normal(rng, 1, 1, 4, D)
+    near.write(k, v)
+    want = near.attention(q, True, start=[599])
+    near.view = far
+    near.write(k, v)
+    for a, b in zip(want, near.attention(q, True, start=[599])):
+        np.testing.assert_array_equal(a, b)
+    for a, b in zip(near.read(600), near.host.read(600)):
+        np.testing.assert_array_equal(a, b.astype(np.float32))
+
+
+def test_written_step_by_step_as_at_once():
+    """A prompt, then tokens one by one: the same cache and, row for row, the same attention as in one call."""
+    rng = np.random.default_rng(16)
+    B, L, H, D = 2, 45, 2, 64
+    k, v, q = (normal(rng, B, L, H, D) for _ in range(3))
+    tab, pages = table(rng, B, 3)
+    whole = Pair(pages, H, 16, D, tab)
+    whole.write(k, v)
+    o, lse = whole.check_attention(q, True)
+    steps = Pair(pages, H, 16, D, tab)
+    at = np.zeros(B, np.int32)
+    for t0, t1 in [(0, 30), *[(t, t + 1) for t in range(30, L)]]:
+        nxt, _ = steps.write(k[:, t0:t1], v[:, t0:t1], start=at)
+        so, sl = steps.attention(q[:, t0:t1], True, start=at)
+        np.testing.assert_allclose(so, o[:, t0:t1], rtol=0, atol=4e-6)
+        np.testing.assert_allclose(sl, lse[:, :, t0:t1], rtol=0, atol=4e-6)
+        at = nxt
+    np.testing.assert_array_equal(at, [L, L])
+    for a, b in zip((*whole.codes, *whole.scales), (*steps.codes, *steps.scales)):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+
+
+def test_oracle_values_agree_with_what_is_read():
+    rng = np.random.default_rng(17)
+    x = normal(rng, 4, 128)
+    codes, scales = serving.quantise(x)
+    back = serving.values(codes, scales)
+    # Half a step of the grid: at most 1 of 6 in the top half of a group, 1/6 of amax.
+    amax = np.abs(x).reshape(4, 4, 32).max(-1)
+    assert (np.abs(back - x).reshape(4, 4, 32) <= amax[..., None] / 3).all()
