@@ -23,11 +23,12 @@
 //     or p for the odd one.  So a wave has 8 rows in 16 columns, and no value of V
 //     is moved between lanes or within a register.
 // A workgroup is 4 waves that take turns at tiles of 32 keys and join at the
-// end; a sequence's keys are cut into `splits` parts, each with a workgroup of
-// its own, and kv_attention_join adds the parts.
+// end; a unit's keys are cut into pieces, each with a workgroup of its own, and
+// kv_attention_join adds them.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.h"
 #include "split_bf16.h"
@@ -40,8 +41,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNone = -3.402823466e38f;  // the running maximum before any key
 constexpr float kRaise = 8.0f;
 constexpr int kWaves = 4;
-constexpr int kTile = 32;  // keys
-constexpr int kRows = 8;   // rows per workgroup
+constexpr int kTile = 32;        // keys
+constexpr int kRows = 8;         // rows per workgroup
+constexpr int kPerCu = 3;        // workgroups that a CU holds at once
+constexpr int kMostPlan = 1024;  // sequences that are planned for; with more, a unit is not cut
 
 struct KvAttnArgs {
     KvCache c;
@@ -49,10 +52,55 @@ struct KvAttnArgs {
     float *o, *lse;
     RowStrides qs, os;
     const int32_t *start, *count;
-    float *part;  // O (rows, D) of each (unit, split), then m and l of each row
-    int T, q_heads, group, tiles, splits, causal;
+    float *part;  // O (rows, D) of each workgroup, then m and l of each row; null: units are not cut
+    int T, q_heads, group, tiles, blocks, causal;
     float scale2;  // scale * log2(e)
 };
+
+// Tokens that a sequence has after the call, as far as its table has room.
+__device__ __forceinline__ int length_of(const KvAttnArgs &a, Span sp)
+{
+    const int64_t room = (int64_t)a.c.max_pages << a.c.page_shift;
+    return (int)max(min((int64_t)sp.start + sp.count, room), (int64_t)0);
+}
+
+template <class V>
+__device__ __forceinline__ V wave_sum(V v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// How the keys are cut: into pieces of `per` tiles, the same for every unit (a
+// sequence's cache head and its 8 rows), so that no workgroup has more than
+// another however the sequences' lengths differ.  per is the smallest, in steps
+// of an eighth, that needs no more workgroups than there are.  Each wave finds
+// it for itself; sequences are taken 64 at a time.
+struct Plan {
+    int per;
+    __device__ __forceinline__ int pieces(int tiles) const { return max((tiles + per - 1) / per, 1); }
+};
+
+__device__ __forceinline__ int tiles_of(const KvAttnArgs &a, int b)
+{
+    return b < a.c.sequences ? (length_of(a, span_of(a.start, a.count, b, a.T)) + kTile - 1) / kTile : 0;
+}
+
+__device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
+{
+    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles, most = a.blocks / units;
+    const int mine = tiles_of(a, lane);
+    auto sum = [&](auto f) {
+        auto n = wave_sum(lane < a.c.sequences ? f(mine) : decltype(f(0))(0));
+        for (int b = 64; b < a.c.sequences; b += 64) n += wave_sum(b + lane < a.c.sequences ? f(tiles_of(a, b + lane)) : decltype(f(0))(0));
+        return n;
+    };
+    // The sum of all tiles may pass 32 bits; as a float it is near enough.
+    Plan p = {(int)fmaxf(sum([](int n) { return (float)n; }) / most, 1.0f)};
+    while (sum([&](int n) { return p.pieces(n); }) > most) p.per += p.per / 8 + 1;
+    return p;
+}
 
 __device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c)
 {
@@ -68,7 +116,8 @@ __device__ __forceinline__ unsigned fp4_bf16(unsigned w, float scale)
 // N bytes (a power of two up to 16) as words; the pointer is aligned to N.
 template <int N>
 struct Words {
-    unsigned w[N < 4 ? 1 : N / 4];
+    static constexpr int kWords = N < 4 ? 1 : N / 4;
+    unsigned w[kWords];
     __device__ __forceinline__ void load(const uint8_t *p)
     {
         if constexpr (N == 16) {
@@ -88,42 +137,50 @@ struct Words {
     __device__ __forceinline__ void zero()
     {
 #pragma unroll
-        for (unsigned &x : w) x = 0;
-    }
-    __device__ __forceinline__ unsigned byte(int i) const  // i known when compiled, or N <= 4
-    {
-        return (w[i >> 2] >> (8 * (i & 3))) & 0xff;
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
 };
 
-// What a lane holds of 16 keys and values.
-template <int D>
-struct Piece {
-    Words<D / 8> k;
-    unsigned ks;
-    Words<D / 32> v[4];
-    Words<D / 8> vs;  // the scales of its 4 tokens
-    bool there;
+// The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
+// head h, or -1.  b, h and pos are the same in all lanes, so the table is read
+// through the scalar cache.
+__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
+{
+    typedef const __attribute__((address_space(4))) int32_t *scalar;
+    const int place = pos >> c.page_shift;
+    if (place >= c.max_pages) return -1;
+    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + place];
+    if ((unsigned)page >= (unsigned)c.pages) return -1;
+    return (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+}
 
-    // Key `pos` (a multiple of 16) is the first; pages hold whole pieces.
-    __device__ __forceinline__ void load(const KvCache &c, int b, int h, int pos, int lane)
+// What a lane holds of 16 keys, and of 16 values.  Where there are none (at < 0)
+// it takes the cache's first ones, which then count for nothing.
+template <int D>
+struct Keys {
+    Words<D / 8> code;
+    unsigned scale;
+    __device__ __forceinline__ void load(const KvCache &c, int64_t at, int lane)
     {
-        const int64_t slot = slot_of(c, b, pos);
-        there = slot >= 0;
-        if (!there) {
-            k.zero(), vs.zero(), ks = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i].zero();
-            return;
-        }
-        const int64_t at = slot + ((int64_t)h << c.page_shift);
         const int col = lane & 15, r = lane >> 4;
-        k.load(c.k_codes + (at + col) * (D / 2) + r * (D / 8));
-        ks = c.k_scales[(at + col) * (D / 32) + r * D / 128];
-        const uint8_t *vp = c.v_codes + (at + 4 * r) * (D / 2) + col * (D / 32);
+        at = max(at, (int64_t)0);
+        code.load(c.k_codes + at * (D / 2) + (col * (D / 2) + r * (D / 8)));
+        scale = (c.k_scales + at * (D / 32))[col * (D / 32) + r * D / 128];
+    }
+};
+
+template <int D>
+struct Values {
+    Words<D / 32> code[4];
+    Words<D / 8> scale;  // of its 4 tokens
+    __device__ __forceinline__ void load(const KvCache &c, int64_t at, int lane)
+    {
+        const int col = lane & 15, r = lane >> 4;
+        at = max(at, (int64_t)0);
+        const uint8_t *p = c.v_codes + at * (D / 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i].load(vp + i * (D / 2));
-        vs.load(c.v_scales + (at + 4 * r) * (D / 32));
+        for (int i = 0; i < 4; ++i) code[i].load(p + ((4 * r + i) * (D / 2) + col * (D / 32)));
+        scale.load(c.v_scales + at * (D / 32) + 4 * r * (D / 32));
     }
 };
 
@@ -137,8 +194,40 @@ __device__ __forceinline__ void cut3(float x, unsigned &hi, unsigned &mid, unsig
     lo = float_bits(x) & 0xffff0000u;
 }
 
+// Where a workgroup stands: its unit, its piece of the unit's keys, and, for
+// the join, the unit's first workgroup (its further ones follow `units` apart).
+struct Place {
+    int b, unit, piece, pieces, first;
+};
+
+// The place of workgroup `block`; b = -1 where the plan needs fewer.
+__device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block)
+{
+    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles;
+    int before = 0;
+    for (int b0 = 0; b0 < a.c.sequences; b0 += 64) {
+        const int n = b0 + lane < a.c.sequences ? p.pieces(tiles_of(a, b0 + lane)) : 0;
+        int upto = n;  // of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o, 64);
+            upto += lane >= o ? x : 0;
+        }
+        const int64_t past = __ballot(block >= before + upto * units);
+        const int at = __popcll(past);
+        if (at < 64) {
+            const int first = before + (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at)) * units;
+            const int i = block - first, piece = i / units;
+            if (b0 + at >= a.c.sequences) break;
+            return {b0 + at, i - piece * units, piece, __builtin_amdgcn_readlane(n, at), first};
+        }
+        before += __builtin_amdgcn_readlane(upto, 63) * units;
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
 template <int D>
-__global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
+__global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAttnArgs a)
 {
     constexpr int KS = D / 32;  // contraction steps of S, and pairs of elements of a lane of O
     constexpr int STR = D + 4;
@@ -147,19 +236,28 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, r = lane >> 4, row8 = col >> 1;
     const bool odd = col & 1;
-    const int split = blockIdx.x % a.splits;
-    const int unit = blockIdx.x / a.splits, tile = unit % a.tiles, bh = unit / a.tiles;
-    const int b = bh / a.c.heads, h = bh - b * a.c.heads;
+    const int units = a.c.heads * a.tiles;
+    Plan plan = {0x40000000};
+    Place pl;
+    if (a.part) {
+        plan = make_plan(a);
+        pl = place_of(a, plan, blockIdx.x);
+        if (pl.b < 0) return;
+    } else {
+        const int b = blockIdx.x / units;
+        pl = {b, (int)blockIdx.x - b * units, 0, 1, 0};
+    }
+    const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
+    const int h = unit / a.tiles, tile = unit - h * a.tiles;
     const Span sp = span_of(a.start, a.count, b, a.T);
-    const int64_t room = (int64_t)a.c.max_pages << a.c.page_shift;
-    const int len = (int)max(min((int64_t)sp.start + sp.count, room), (int64_t)0);
+    const int len = length_of(a, sp);
 
     // This lane's row, and the first key that it does not see.
     const int row = tile * kRows + row8, t = row / a.group, g = row - t * a.group;
     const bool valid = t < sp.count;
     const int last_t = min((tile * kRows + kRows - 1) / a.group, sp.count - 1);
     auto limit_of = [&](int t) { return a.causal ? (int)max(min((int64_t)sp.start + t + 1, (int64_t)len), (int64_t)0) : len; };
-    const int keys = tile * kRows / a.group < sp.count ? limit_of(last_t) : 0;  // all that the workgroup's rows see
+    const int keys = tile * kRows / a.group < sp.count && a.c.pages ? limit_of(last_t) : 0;  // all that the workgroup's rows see
     const int limit = valid ? limit_of(t) : keys;
     const int sure = keys ? limit_of(tile * kRows / a.group) : 0;  // every row sees the keys before
 
@@ -185,36 +283,41 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
     float m = kNone, l = 0.0f;
     const int shift = odd ? 0 : 16;
 
-    const int n = (keys + kTile - 1) / kTile, per = (n + a.splits - 1) / a.splits;
-    const int end = min(n, (split + 1) * per);
-    for (int tl = split * per + wave; tl < end; tl += kWaves) {
-        Piece<D> pc[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) pc[j].load(a.c, b, h, tl * kTile + 16 * j, lane);
+    const int n = (keys + kTile - 1) / kTile;
+    const int end = pl.piece + 1 < pl.pieces ? min(n, (pl.piece + 1) * plan.per) : n;
+    int tl = __builtin_amdgcn_readfirstlane(pl.piece * plan.per) + wave;
+    int64_t at[2], ahead[2];
+    Keys<D> kk[2];
+    Values<D> vv[2];
+    // One tile; the next one's keys are loaded as soon as this one's are used,
+    // and its values after this one's.
+    auto step = [&](auto more) {
         float s[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f32x4 sum = {0, 0, 0, 0};
-            const float scale = scale_of(pc[j].ks);
-            // The small parts first.
+            f32x4 sum[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            const float scale = scale_of(kk[j].scale);
 #pragma unroll
-            for (int part = 2; part >= 0; --part)
+            for (int x = 0; x < KS; ++x) {
+                const unsigned w = kk[j].code.w[x];
+                const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
 #pragma unroll
-                for (int x = 0; x < KS; ++x) {
-                    const unsigned w = pc[j].k.w[x];
-                    const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
-                    sum = mfma_16x16x32(k, q[x][part], sum);
-                }
+                for (int part = 0; part < 3; ++part) sum[part] = mfma_16x16x32(k, q[x][part], sum[part]);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = sum[i] * a.scale2;
+            for (int i = 0; i < 4; ++i) s[j][i] = ((sum[2][i] + sum[1][i]) + sum[0][i]) * a.scale2;
         }
-        const bool partly = tl * kTile + kTile > sure || !pc[0].there || !pc[1].there;
+        if constexpr (more.value) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) kk[j].load(a.c, ahead[j], lane);
+        }
+        const bool partly = tl * kTile + kTile > sure || at[0] < 0 || at[1] < 0;
         if (partly) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (tl * kTile + 16 * j + 4 * r + i >= limit || !pc[j].there) s[j][i] = -INFINITY;
+                    if (tl * kTile + 16 * j + 4 * r + i >= limit || at[j] < 0) s[j][i] = -INFINITY;
         }
         float top = kNone;
 #pragma unroll
@@ -232,8 +335,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[x][i] *= f;
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        auto values = [&](auto J) {
+            constexpr int j = decltype(J)::value;
             u32x4 p[3];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -248,8 +351,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
             bool spoilt = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const unsigned word = pc[j].vs.w[i * D / 128];
-                const unsigned byte = (word >> (8 * ((i * (D / 32) & 3) + gv))) & 0xff;
+                const unsigned byte = (vv[j].scale.w[i * D / 128] >> (8 * ((i * (D / 32) & 3) + gv))) & 0xff;
                 vscale[i] = scale_of(byte);
                 spoilt |= byte > kMostScale;
             }
@@ -257,12 +359,10 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
                 // A value that is no number, in a place that some rows do not
                 // see (or that was never written): zero in the product, and
                 // NaN given to the rows that do see it.
-                const int64_t slot = slot_of(a.c, b, tl * kTile + 16 * j);
                 bool mine = false;
-                for (int x = 0; x < 16; ++x) {
-                    const int64_t at = slot + ((int64_t)h << a.c.page_shift) + x;
-                    mine |= pc[j].there && tl * kTile + 16 * j + x < limit && a.c.v_scales[at * (D / 32) + r * D / 128] > kMostScale;
-                }
+                for (int x = 0; x < 16; ++x)
+                    mine |= at[j] >= 0 && tl * kTile + 16 * j + x < limit &&
+                            a.c.v_scales[(at[j] + x) * (D / 32) + r * D / 128] > kMostScale;
 #pragma unroll
                 for (int x = 0; x < KS; ++x)
 #pragma unroll
@@ -271,25 +371,48 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
                 for (int i = 0; i < 4; ++i)
                     if (vscale[i] >= scale_of(kMostScale + 1)) {
                         vscale[i] = 1.0f;
-                        pc[j].v[i].zero();
+                        vv[j].code[i].zero();
                     }
             }
+            u32x4 v[KS];
+            auto convert = [&](auto X) {
+                constexpr int x = decltype(X)::value;
 #pragma unroll
-            for (int part = 2; part >= 0; --part) {
-                auto step = [&](auto S) {
-                    constexpr int x = decltype(S)::value;
-                    const u32x4 v = {fp4_bf16<x>(pc[j].v[0].w[0], vscale[0]), fp4_bf16<x>(pc[j].v[1].w[0], vscale[1]),
-                                     fp4_bf16<x>(pc[j].v[2].w[0], vscale[2]), fp4_bf16<x>(pc[j].v[3].w[0], vscale[3])};
-                    acc[x] = mfma_16x16x32(v, p[part], acc[x]);
-                };
-                step(std::integral_constant<int, 0>{});
-                if constexpr (KS > 1) step(std::integral_constant<int, 1>{});
-                if constexpr (KS > 2) {
-                    step(std::integral_constant<int, 2>{});
-                    step(std::integral_constant<int, 3>{});
-                }
+                for (int i = 0; i < 4; ++i) v[x][i] = fp4_bf16<x>(vv[j].code[i].w[0], vscale[i]);
+            };
+            convert(std::integral_constant<int, 0>{});
+            if constexpr (KS > 1) convert(std::integral_constant<int, 1>{});
+            if constexpr (KS > 2) {
+                convert(std::integral_constant<int, 2>{});
+                convert(std::integral_constant<int, 3>{});
+            }
+#pragma unroll
+            for (int part = 2; part >= 0; --part)  // the small parts first
+#pragma unroll
+                for (int x = 0; x < KS; ++x) acc[x] = mfma_16x16x32(v[x], p[part], acc[x]);
+        };
+        values(std::integral_constant<int, 0>{});
+        values(std::integral_constant<int, 1>{});
+        if constexpr (more.value) {
+            tl += kWaves;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                vv[j].load(a.c, ahead[j], lane);
+                at[j] = ahead[j];
+                ahead[j] = tl + kWaves < end ? row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j) : -1;
             }
         }
+    };
+    if (tl < end) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            at[j] = row_of(a.c, b, h, tl * kTile + 16 * j);
+            kk[j].load(a.c, at[j], lane);
+            vv[j].load(a.c, at[j], lane);
+            ahead[j] = tl + kWaves < end ? row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j) : -1;
+        }
+        while (tl + kWaves < end) step(std::true_type{});
+        step(std::false_type{});
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -315,7 +438,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
         }
         const int row = tile * kRows + rw, t = row / a.group, g = row - t * a.group;
         if (t >= a.T) continue;
-        if (a.splits > 1) {
+        if (pl.pieces > 1) {
             const int64_t block = blockIdx.x;
             *(f32x4 *)(a.part + (block * kRows + rw) * D + d) = o;
             if (d == 0) {
@@ -332,27 +455,32 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(KvAttnArgs a)
     }
 }
 
-// Adds the parts of each row: D/4 lanes a row.
+// Adds the parts of each row of the units that were cut: a workgroup per unit
+// and sequence, 8 rows of D/4 lanes.
 template <int D>
-__global__ __launch_bounds__(256) void kv_attention_join(KvAttnArgs a, int units)
+__global__ __launch_bounds__(kRows * D / 4) void kv_attention_join(KvAttnArgs a)
 {
-    constexpr int LPR = D / 4;
-    const int64_t at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;  // (unit, row of the tile)
-    const int d = threadIdx.x % LPR * 4;
-    const int64_t unit = at / kRows;
-    if (unit >= units) return;
-    const int rw = (int)(at % kRows), tile = (int)(unit % a.tiles), bh = (int)(unit / a.tiles);
-    const int b = bh / a.c.heads, h = bh - b * a.c.heads;
+    const int units = a.c.heads * a.tiles, b = blockIdx.x / units, unit = blockIdx.x - b * units;
+    const Plan plan = make_plan(a);
+    // The sequence's first workgroup.
+    const int lane = threadIdx.x & 63;
+    int first = 0;
+    for (int b0 = 0; b0 < b; b0 += 64) first += wave_sum(b0 + lane < b ? plan.pieces(tiles_of(a, b0 + lane)) : 0);
+    first = first * units + unit;
+    const int pieces = plan.pieces(tiles_of(a, b));
+    if (pieces == 1) return;
+    const int rw = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const int h = unit / a.tiles, tile = unit - h * a.tiles;
     const int row = tile * kRows + rw, t = row / a.group, g = row - t * a.group;
     if (t >= a.T) return;
     const Span sp = span_of(a.start, a.count, b, a.T);
-    const float *st = a.part + (int64_t)units * a.splits * kRows * D;
+    const float *st = a.part + (int64_t)a.blocks * kRows * D;
     float top = kNone;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, st[((unit * a.splits + s) * kRows + rw) * 2]);
+    for (int s = 0; s < pieces; ++s) top = fmaxf(top, st[((int64_t)(first + s * units) * kRows + rw) * 2]);
     float sum = 0.0f;
     f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) {
-        const int64_t i = (unit * a.splits + s) * kRows + rw;
+    for (int s = 0; s < pieces; ++s) {
+        const int64_t i = (int64_t)(first + s * units) * kRows + rw;
         const float f = __builtin_amdgcn_exp2f(st[2 * i] - top);
         sum += f * st[2 * i + 1];
         o += f * *(const f32x4 *)(a.part + i * D + d);
@@ -367,23 +495,21 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttnArgs a, int units
 template <int D>
 int launch(KvAttnArgs &a)
 {
-    const int64_t units = (int64_t)a.c.sequences * a.c.heads * a.tiles;
-    // Enough workgroups for the chip, 4 of them to a CU, and at least 64 keys
-    // each of the longest sequence that the table has room for.
-    const int64_t room = (int64_t)a.c.max_pages << a.c.page_shift;
-    const int cus = std::max(device_cu_count(), 1);
-    const int64_t want = std::min((4 * cus + units - 1) / units, room / 64);
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, 256));
-    if (units * a.splits * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
-    if (a.splits > 1) {
-        a.part = (float *)scratch(kScratchKvAttention, (size_t)units * a.splits * kRows * (D + 2) * sizeof(float));
+    const int64_t all = (int64_t)a.c.sequences * a.c.heads * a.tiles;  // units
+    if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
+    // One round of workgroups over the chip; where the units alone are about as
+    // many, two pieces each, so that the longest sequence does not decide.
+    const int64_t slots = (int64_t)kPerCu * std::max(device_cu_count(), 1);
+    const bool cut = a.c.sequences <= kMostPlan && all <= 16 * slots;
+    a.blocks = (int)(cut ? std::max(slots, 2 * all) : all);
+    if (cut) {
+        a.part = (float *)scratch(kScratchKvAttention, (size_t)a.blocks * kRows * (D + 2) * sizeof(float));
         if (!a.part) return EMBER_ERR_OUT_OF_MEMORY;
     }
-    hipLaunchKernelGGL(kv_attention_kernel<D>, dim3((unsigned)(units * a.splits)), dim3(64 * kWaves), 0, 0, a);
+    hipLaunchKernelGGL(kv_attention_kernel<D>, dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     if (!launch_ok("kv_attention")) return EMBER_ERR_DEVICE;
-    if (a.splits > 1) {
-        constexpr int rpb = 256 / (D / 4);
-        hipLaunchKernelGGL(kv_attention_join<D>, dim3((unsigned)((units * kRows + rpb - 1) / rpb)), dim3(256), 0, 0, a, (int)units);
+    if (cut) {
+        hipLaunchKernelGGL(kv_attention_join<D>, dim3((unsigned)all), dim3(kRows * D / 4), 0, 0, a);
         if (!launch_ok("kv_attention_join")) return EMBER_ERR_DEVICE;
     }
     return EMBER_OK;
