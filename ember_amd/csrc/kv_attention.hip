@@ -23,14 +23,16 @@
 //     or p for the odd one.  So a wave has 8 rows in 16 columns, and no value of V
 //     is moved between lanes or within a register.
 // A workgroup is 4 waves that take turns at tiles of 32 keys and join at the
-// end; a unit's keys are cut into pieces, each with a workgroup of its own, and
-// kv_attention_join adds them.
+// end.  A unit's keys are cut into pieces, each with a workgroup of its own; the
+// last of them to be done (by a count that they all add to) joins the pieces, in
+// their order.
 #include <math.h>
 
 #include <algorithm>
 #include <type_traits>
 
 #include "kv_cache.h"
+#include "lds_dma.h"
 #include "split_bf16.h"
 
 namespace ember {
@@ -45,6 +47,7 @@ constexpr int kTile = 32;        // keys
 constexpr int kRows = 8;         // rows per workgroup
 constexpr int kPerCu = 3;        // workgroups that a CU holds at once
 constexpr int kMostPlan = 1024;  // sequences that are planned for; with more, a unit is not cut
+constexpr int kMostUnits = 1 << 14;  // that are cut
 
 struct KvAttnArgs {
     KvCache c;
@@ -52,9 +55,9 @@ struct KvAttnArgs {
     float *o, *lse;
     RowStrides qs, os;
     const int32_t *start, *count;
-    float *part;  // O (rows, D) of each workgroup, then m and l of each row; null: units are not cut
+    float *part;  // of each workgroup: O (rows, D), then m and l of each row; null: units are not cut
     int T, q_heads, group, tiles, blocks, causal;
-    float scale2;  // scale * log2(e)
+    float scale2;  // scale * log2(e), above 0
 };
 
 // Tokens that a sequence has after the call, as far as its table has room.
@@ -64,13 +67,33 @@ __device__ __forceinline__ int length_of(const KvAttnArgs &a, Span sp)
     return (int)max(min((int64_t)sp.start + sp.count, room), (int64_t)0);
 }
 
+// Sums over the lanes up to this one (a wave's lanes, in register moves).
+template <int CTRL, int ROWS, class V>
+__device__ __forceinline__ V moved_in(V v)
+{
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V v)
+{
+    v += moved_in<0x111, 0xf>(v);  // from 1, 2, 4 and 8 lanes below, within 16
+    v += moved_in<0x112, 0xf>(v);
+    v += moved_in<0x114, 0xf>(v);
+    v += moved_in<0x118, 0xf>(v);
+    v += moved_in<0x142, 0xa>(v);  // the last lane of the 16 below, and of the 32 below
+    v += moved_in<0x143, 0xc>(v);
+    return v;
+}
 template <class V>
 __device__ __forceinline__ V wave_sum(V v)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63));
 }
+
+// Units that are cut: how many of their workgroups are done.  Zero between
+// calls: the last one, which all the others have added to, clears its unit's.
+// All calls run on the null stream, so no two use it at once.
+__device__ unsigned g_done[kMostUnits];
 
 // How the keys are cut: into pieces of `per` tiles, the same for every unit (a
 // sequence's cache head and its 8 rows), so that no workgroup has more than
@@ -194,8 +217,8 @@ __device__ __forceinline__ void cut3(float x, unsigned &hi, unsigned &mid, unsig
     lo = float_bits(x) & 0xffff0000u;
 }
 
-// Where a workgroup stands: its unit, its piece of the unit's keys, and, for
-// the join, the unit's first workgroup (its further ones follow `units` apart).
+// Where a workgroup stands: its unit, its piece of the unit's keys, and the
+// unit's first workgroup (its further ones follow `units` apart).
 struct Place {
     int b, unit, piece, pieces, first;
 };
@@ -207,23 +230,31 @@ __device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block
     int before = 0;
     for (int b0 = 0; b0 < a.c.sequences; b0 += 64) {
         const int n = b0 + lane < a.c.sequences ? p.pieces(tiles_of(a, b0 + lane)) : 0;
-        int upto = n;  // of the lanes up to this one
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(upto, o, 64);
-            upto += lane >= o ? x : 0;
-        }
-        const int64_t past = __ballot(block >= before + upto * units);
-        const int at = __popcll(past);
+        const int upto = wave_scan(n);
+        const int at = __popcll(__ballot(block >= before + upto * units));  // sequences that end before
         if (at < 64) {
-            const int first = before + (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at)) * units;
-            const int i = block - first, piece = i / units;
-            if (b0 + at >= a.c.sequences) break;
-            return {b0 + at, i - piece * units, piece, __builtin_amdgcn_readlane(n, at), first};
+            const int pieces = __builtin_amdgcn_readlane(n, at);
+            const int from = before + (__builtin_amdgcn_readlane(upto, at) - pieces) * units;
+            const int piece = (block - from) / units, unit = block - from - piece * units;
+            return {b0 + at, unit, piece, pieces, from + unit};
         }
         before += __builtin_amdgcn_readlane(upto, 63) * units;
     }
     return {-1, 0, 0, 0, 0};
+}
+
+// Parts of a unit's result go from one workgroup to another of the same launch,
+// which may be on another XCD with an L2 of its own: stores and loads at device
+// scope pass the L2s by.  (A release fence would write a whole L2 back.)
+__device__ __forceinline__ void put2(float *p, float x, float y)
+{
+    const uint64_t v = (uint64_t)__builtin_bit_cast(unsigned, y) << 32 | __builtin_bit_cast(unsigned, x);
+    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 get2(const float *p)
+{
+    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return f32x2{__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32))};
 }
 
 template <int D>
@@ -233,6 +264,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
     constexpr int STR = D + 4;
     __shared__ float slab[kWaves][kRows * STR];
     __shared__ float stat[kWaves][kRows][2];
+    __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, r = lane >> 4, row8 = col >> 1;
     const bool odd = col & 1;
@@ -281,7 +313,8 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
 #pragma unroll
     for (int s = 0; s < KS; ++s) acc[s] = f32x4{0, 0, 0, 0};
     float m = kNone, l = 0.0f;
-    const int shift = odd ? 0 : 16;
+    const unsigned half = odd ? 0x03020c0cu : 0x0c0c0302u;  // a float's upper half as the upper or the lower of two
+    const unsigned turn = 8 * (col * D / 512) + 9;          // the byte of the lane's group of 32 to bits 23 .. 30
 
     const int n = (keys + kTile - 1) / kTile;
     const int end = pl.piece + 1 < pl.pieces ? min(n, (pl.piece + 1) * plan.per) : n;
@@ -295,17 +328,17 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
         float s[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f32x4 sum[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            f32x4 sum = {0, 0, 0, 0};
             const float scale = scale_of(kk[j].scale);
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
                 const unsigned w = kk[j].code.w[x];
                 const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
 #pragma unroll
-                for (int part = 0; part < 3; ++part) sum[part] = mfma_16x16x32(k, q[x][part], sum[part]);
+                for (int part = 2; part >= 0; --part) sum = mfma_16x16x32(k, q[x][part], sum);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = ((sum[2][i] + sum[1][i]) + sum[0][i]) * a.scale2;
+            for (int i = 0; i < 4; ++i) s[j][i] = sum[i];
         }
         if constexpr (more.value) {
 #pragma unroll
@@ -319,11 +352,12 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
                 for (int i = 0; i < 4; ++i)
                     if (tl * kTile + 16 * j + 4 * r + i >= limit || at[j] < 0) s[j][i] = -INFINITY;
         }
-        float top = kNone;
+        float top = s[0][0];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
+        top *= a.scale2;
         if (__any(top > m + kRaise)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -340,39 +374,43 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
             u32x4 p[3];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(s[j][i] - m);
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[j][i], a.scale2, -m));
                 l += e;
                 unsigned hi, mid, lo;
                 cut3(e, hi, mid, lo);
-                p[0][i] = hi >> shift, p[1][i] = mid >> shift, p[2][i] = lo >> shift;
+                p[0][i] = __builtin_amdgcn_perm(0, hi, half), p[1][i] = __builtin_amdgcn_perm(0, mid, half);
+                p[2][i] = __builtin_amdgcn_perm(0, lo, half);
             }
+            // The scale's byte turned to where a float has its exponent: no
+            // other bit of it counts.
             float vscale[4];
-            const int gv = col * D / 512;  // the lane's group of 32
-            bool spoilt = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const unsigned byte = (vv[j].scale.w[i * D / 128] >> (8 * ((i * (D / 32) & 3) + gv))) & 0xff;
-                vscale[i] = scale_of(byte);
-                spoilt |= byte > kMostScale;
+                const unsigned w = vv[j].scale.w[i * D / 128];
+                vscale[i] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(w, w, turn + 8 * (i * (D / 32) & 3)));
             }
-            if (partly && __any(spoilt)) {
-                // A value that is no number, in a place that some rows do not
-                // see (or that was never written): zero in the product, and
+            if (partly) {
+                // Is a value no number, in a place that some rows do not see
+                // (or that was never written)?  Then zero in the product, and
                 // NaN given to the rows that do see it.
-                bool mine = false;
-                for (int x = 0; x < 16; ++x)
-                    mine |= at[j] >= 0 && tl * kTile + 16 * j + x < limit &&
-                            a.c.v_scales[(at[j] + x) * (D / 32) + r * D / 128] > kMostScale;
+                bool spoilt[4];
 #pragma unroll
-                for (int x = 0; x < KS; ++x)
+                for (int i = 0; i < 4; ++i) spoilt[i] = ((float_bits(vscale[i]) >> 23) & 0xff) > kMostScale;
+                if (__any(spoilt[0] || spoilt[1] || spoilt[2] || spoilt[3])) {
+                    bool mine = false;
+                    for (int x = 0; x < 16; ++x)
+                        mine |= at[j] >= 0 && tl * kTile + 16 * j + x < limit &&
+                                a.c.v_scales[(at[j] + x) * (D / 32) + r * D / 128] > kMostScale;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[x][i] = mine ? NAN : acc[x][i];
+                    for (int x = 0; x < KS; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (vscale[i] >= scale_of(kMostScale + 1)) {
-                        vscale[i] = 1.0f;
-                        vv[j].code[i].zero();
+                        for (int i = 0; i < 4; ++i) acc[x][i] = mine ? NAN : acc[x][i];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        vscale[i] = spoilt[i] ? 1.0f : vscale[i];
+                        vv[j].code[i].w[0] = spoilt[i] ? 0 : vv[j].code[i].w[0];
                     }
+                }
             }
             u32x4 v[KS];
             auto convert = [&](auto X) {
@@ -424,72 +462,56 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
 #pragma unroll
         for (int i = 0; i < 4; ++i) slab[wave][row8 * STR + (4 * r + i) * (D / 16) + 2 * x + odd] = acc[x][i];
     __syncthreads();
-    for (int at = threadIdx.x; at < kRows * D / 4; at += 64 * kWaves) {
-        const int rw = at / (D / 4), d = at % (D / 4) * 4;
-        float top = kNone, sum = 0.0f;
+    const int rw = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    const bool works = rw < kRows;
+    float top = kNone, sum = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    if (works) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stat[w][rw][0]);
-        f32x4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float f = __builtin_amdgcn_exp2f(stat[w][rw][0] - top);
             sum += f * stat[w][rw][1];
             o += f * *(const f32x4 *)&slab[w][rw * STR + d];
         }
-        const int row = tile * kRows + rw, t = row / a.group, g = row - t * a.group;
-        if (t >= a.T) continue;
-        if (pl.pieces > 1) {
-            const int64_t block = blockIdx.x;
-            *(f32x4 *)(a.part + (block * kRows + rw) * D + d) = o;
-            if (d == 0) {
-                float *st = a.part + (int64_t)gridDim.x * kRows * D + (block * kRows + rw) * 2;
-                st[0] = top, st[1] = sum;
+    }
+    if (pl.pieces > 1) {
+        constexpr int PART = kRows * (D + 2);
+        if (works) {
+            float *mine = a.part + (int64_t)blockIdx.x * PART;
+            put2(mine + rw * D + d, o[0], o[1]);
+            put2(mine + rw * D + d + 2, o[2], o[3]);
+            if (d == 0) put2(mine + kRows * D + 2 * rw, top, sum);
+        }
+        wait_vmem();  // the stores have reached memory
+        __syncthreads();
+        unsigned *done = &g_done[b * units + unit];
+        if (threadIdx.x == 0) last = __hip_atomic_fetch_add(done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)pl.pieces - 1;
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) __hip_atomic_store(done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (works) {
+            const float *from = a.part + (int64_t)pl.first * PART;
+            const int64_t step = (int64_t)units * PART;
+            top = kNone, sum = 0.0f, o = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < pl.pieces; ++i, from += step) {
+                const f32x2 st = get2(from + kRows * D + 2 * rw), o0 = get2(from + rw * D + d), o1 = get2(from + rw * D + d + 2);
+                const float to = fmaxf(top, st[0]), f = __builtin_amdgcn_exp2f(top - to), g = __builtin_amdgcn_exp2f(st[0] - to);
+                top = to;
+                sum = sum * f + st[1] * g;
+                o = o * f + f32x4{o0[0], o0[1], o1[0], o1[1]} * g;
             }
-        } else {
-            const int head = h * a.group + g;
-            const bool empty = t >= sp.count || sum == 0.0f;
-            *(f32x4 *)(a.o + b * a.os.sb + head * a.os.sh + t * a.os.ss + d) = empty ? f32x4{0, 0, 0, 0} : o / sum;
-            if (a.lse && d == 0)
-                a.lse[((int64_t)b * a.q_heads + head) * a.T + t] = empty ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
         }
     }
-}
-
-// Adds the parts of each row of the units that were cut: a workgroup per unit
-// and sequence, 8 rows of D/4 lanes.
-template <int D>
-__global__ __launch_bounds__(kRows * D / 4) void kv_attention_join(KvAttnArgs a)
-{
-    const int units = a.c.heads * a.tiles, b = blockIdx.x / units, unit = blockIdx.x - b * units;
-    const Plan plan = make_plan(a);
-    // The sequence's first workgroup.
-    const int lane = threadIdx.x & 63;
-    int first = 0;
-    for (int b0 = 0; b0 < b; b0 += 64) first += wave_sum(b0 + lane < b ? plan.pieces(tiles_of(a, b0 + lane)) : 0);
-    first = first * units + unit;
-    const int pieces = plan.pieces(tiles_of(a, b));
-    if (pieces == 1) return;
-    const int rw = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-    const int h = unit / a.tiles, tile = unit - h * a.tiles;
-    const int row = tile * kRows + rw, t = row / a.group, g = row - t * a.group;
-    if (t >= a.T) return;
-    const Span sp = span_of(a.start, a.count, b, a.T);
-    const float *st = a.part + (int64_t)a.blocks * kRows * D;
-    float top = kNone;
-    for (int s = 0; s < pieces; ++s) top = fmaxf(top, st[((int64_t)(first + s * units) * kRows + rw) * 2]);
-    float sum = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
-    for (int s = 0; s < pieces; ++s) {
-        const int64_t i = (int64_t)(first + s * units) * kRows + rw;
-        const float f = __builtin_amdgcn_exp2f(st[2 * i] - top);
-        sum += f * st[2 * i + 1];
-        o += f * *(const f32x4 *)(a.part + i * D + d);
+    if (works) {
+        const int row = tile * kRows + rw, t = row / a.group, head = h * a.group + row - t * a.group;
+        if (t >= a.T) return;
+        const bool empty = t >= sp.count || sum == 0.0f;
+        *(f32x4 *)(a.o + b * a.os.sb + head * a.os.sh + t * a.os.ss + d) = empty ? f32x4{0, 0, 0, 0} : o / sum;
+        if (a.lse && d == 0)
+            a.lse[((int64_t)b * a.q_heads + head) * a.T + t] = empty ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
     }
-    const int head = h * a.group + g;
-    const bool empty = t >= sp.count || sum == 0.0f;
-    *(f32x4 *)(a.o + b * a.os.sb + head * a.os.sh + t * a.os.ss + d) = empty ? f32x4{0, 0, 0, 0} : o / sum;
-    if (a.lse && d == 0)
-        a.lse[((int64_t)b * a.q_heads + head) * a.T + t] = empty ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 template <int D>
@@ -500,7 +522,7 @@ int launch(KvAttnArgs &a)
     // One round of workgroups over the chip; where the units alone are about as
     // many, two pieces each, so that the longest sequence does not decide.
     const int64_t slots = (int64_t)kPerCu * std::max(device_cu_count(), 1);
-    const bool cut = a.c.sequences <= kMostPlan && all <= 16 * slots;
+    const bool cut = a.c.sequences <= kMostPlan && all <= kMostUnits;
     a.blocks = (int)(cut ? std::max(slots, 2 * all) : all);
     if (cut) {
         a.part = (float *)scratch(kScratchKvAttention, (size_t)a.blocks * kRows * (D + 2) * sizeof(float));
@@ -508,10 +530,6 @@ int launch(KvAttnArgs &a)
     }
     hipLaunchKernelGGL(kv_attention_kernel<D>, dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     if (!launch_ok("kv_attention")) return EMBER_ERR_DEVICE;
-    if (cut) {
-        hipLaunchKernelGGL(kv_attention_join<D>, dim3((unsigned)all), dim3(kRows * D / 4), 0, 0, a);
-        if (!launch_ok("kv_attention_join")) return EMBER_ERR_DEVICE;
-    }
     return EMBER_OK;
 }
 
@@ -538,6 +556,9 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     a.start = start, a.count = count;
     a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / a.c.heads);
     a.tiles = (int)((T * a.group + kRows - 1) / kRows);
-    a.causal = causal != 0, a.scale2 = scale * kLog2e;
+    a.causal = causal != 0;
+    // Above 0, so that a masked score stays -infinity under it; a scale of 0 then
+    // gives scores that differ by nothing.
+    a.scale2 = std::max(scale * kLog2e, 1e-37f);
     return a.c.D == 128 ? launch<128>(a) : a.c.D == 64 ? launch<64>(a) : launch<32>(a);
 }
