@@ -9,29 +9,35 @@
 // Sums over parts of a row join by
 //   s = sum s_i f_i,  w = sum (w_i + (m_i - m) s_i) f_i,  f_i = e^(m_i - m).
 //
-// A workgroup takes a segment of a row into registers (32 floats a thread), so
-// that the maximum is known before the sums without a second read; segments of
-// a row are joined by token_logprobs_join.  HBM-bound: 4 bytes per logit.
+// A thread takes 16 logits at a time into registers, so that their maximum is
+// known before the sums, and the next 16 are on their way meanwhile; where rows
+// are few, a row is cut over workgroups, and the last of them to be done (by a
+// count that they add to) joins their sums.  HBM-bound: 4 bytes per logit.
 //
 // The `top` largest: floats are ordered as unsigned integers (all bits turned
 // over where the sign is set, else the sign alone), with the complement of the
 // index below them, so that one comparison of 64 bits has the order asked for.
-// Each wave keeps its best in order, one per lane.  A first bound is the k-th
-// largest of its lanes' largest, to 16 bits, found by halving on ballots; the
-// few elements from it on are put in one by one.
+// Each wave keeps its best in order, one per lane, and tests each logit against
+// the last of them; before it has any, against the k-th largest of its lanes'
+// largest (found to 16 bits, by halving on ballots), so that few are put in that
+// do not stay.
 #include <math.h>
 
 #include <algorithm>
 
 #include "common.h"
+#include "lds_dma.h"
 
 namespace ember {
 namespace {
 
 constexpr int kMostTop = 64;
 constexpr int kThreads = 256;
-constexpr int kPerThread = 32;
-constexpr int kSegment = kThreads * kPerThread;
+constexpr int kPerThread = 16;
+constexpr int kChunk = kThreads * kPerThread;
+constexpr int kMostRows = 1 << 13;  // that are cut
+constexpr int kKeys = 2048;         // of lists that are joined at a time
+constexpr float kLog2e = 1.4426950408889634f;
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows start anywhere
 
@@ -41,22 +47,28 @@ struct ScoreArgs {
     float *logp, *lse, *entropy;
     int32_t *top_tokens;
     float *top_logp;
-    float *part;      // m, s, w of each (row, segment)
-    uint64_t *lists;  // its best, `top` keys
+    char *part;  // of each workgroup: m, s, w, and its waves' best (`top` keys each); null: rows are not cut
     int64_t stride;
-    int rows, classes, segments, top;
+    int rows, classes, chunks, pieces, per, top;  // chunks of a row, pieces that it is cut into, chunks of a piece
+    int row0;
 };
+
+// Rows that are cut: how many of their workgroups are done.  Zero between
+// launches: the last one, which all the others have added to, clears its row's.
+// All calls run on the null stream, so no two use it at once.
+__device__ unsigned g_rows_done[kMostRows];
 
 struct Sums {
     float m, s, w;
 };
 
-// One side's part of a sum whose maximum is m.  Nothing is added where it holds
-// nothing but -infinity (no inf - inf) or is too far below (no 0 * inf).
+// One side's part of a sum whose maximum is m.  A side that holds nothing but
+// -infinity stays 0 (no inf - inf); one that is too far below adds no w (no 0 *
+// inf), but a NaN in its s stays.
 __device__ __forceinline__ Sums moved(Sums a, float m)
 {
     const float d = a.s == 0.0f ? 0.0f : a.m - m, f = expf(d);
-    return f == 0.0f ? Sums{m, 0.0f, 0.0f} : Sums{m, a.s * f, (a.w + d * a.s) * f};
+    return {m, a.s * f, f == 0.0f ? 0.0f : (a.w + d * a.s) * f};
 }
 
 __device__ __forceinline__ Sums join(Sums a, Sums b)
@@ -69,7 +81,7 @@ __device__ __forceinline__ Sums join(Sums a, Sums b)
 __device__ __forceinline__ uint64_t key_of(float x, int i)
 {
     const unsigned u = __builtin_bit_cast(unsigned, x + 0.0f);  // -0 as 0
-    const unsigned v = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+    const unsigned v = x == x ? u ^ ((unsigned)((int)u >> 31) | 0x80000000u) : 0xffffffffu;
     return ((uint64_t)v << 32) | (0xffffffffu - (unsigned)i);
 }
 __device__ __forceinline__ float value_of(uint64_t key)
@@ -89,16 +101,19 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane)
 }
 
 // A wave's `top` largest keys, the largest in lane 0.  Empty places hold 0,
-// below every key of a float.
+// below every key of a float.  Only keys above `last` are taken: the lowest that
+// is kept, or a bound that at least `top` others are known to pass.
 struct Best {
-    uint64_t mine = 0, last = 0;  // last: the lowest that is kept
+    uint64_t mine = 0, last = 0;
     __device__ __forceinline__ void put(uint64_t key, int top)  // the same in every lane
     {
-        const int at = __popcll(__ballot(mine > key));
-        const uint64_t up = ((uint64_t)(unsigned)__shfl_up((int)(mine >> 32), 1, 64) << 32) | (unsigned)__shfl_up((int)(unsigned)mine, 1, 64);
-        const int lane = threadIdx.x & 63;
-        mine = lane < at ? mine : lane == at ? key : up;
-        last = lane_key(mine, top - 1);
+        const int at = __popcll(__ballot(mine > key)), lane = threadIdx.x & 63;
+        // From the lane below (a wave's shift by one, in registers).
+        const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(mine >> 32), 0x138, 0xf, 0xf, false);
+        const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)mine, 0x138, 0xf, 0xf, false);
+        mine = lane < at ? mine : lane == at ? key : ((uint64_t)hi << 32) | lo;
+        const uint64_t l = lane_key(mine, top - 1);
+        last = l > last ? l : last;
     }
     // Takes in one key of each lane (0: none).
     __device__ __forceinline__ void take(uint64_t key, int top)
@@ -107,6 +122,34 @@ struct Best {
             const uint64_t k = lane_key(key, __builtin_ctzll(left));
             if (k > last) put(k, top);
         }
+    }
+    // Of one key of each lane, at least `top` of which count: the k-th largest,
+    // cut to 16 bits, is a bound (none if fewer lanes have one).
+    __device__ __forceinline__ void raise(unsigned upper, int top)
+    {
+        unsigned bound = 0;
+        for (unsigned bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+            if (__popcll(__ballot(upper >= (bound | bit))) >= top) bound |= bit;
+        const uint64_t l = bound ? ((uint64_t)bound << 32) - 1 : 0;
+        last = l > last ? l : last;
+    }
+    // Takes in n sorted lists of `top` keys, one after the other in `lists`.
+    __device__ __forceinline__ void join(const uint64_t *lists, int n, int top)
+    {
+        const int lane = threadIdx.x & 63;
+        uint64_t head = 0;
+        if (n >= 64) {
+            for (int i = lane; i < n; i += 64) head = lists[i * top] > head ? lists[i * top] : head;
+        } else if (lane / n < top) {
+            head = lists[lane % n * top + lane / n];
+        }
+        raise((unsigned)(head >> 32), top);
+        for (int i = lane; i - lane < n; i += 64)
+            for (int at = 0; at < top; ++at) {
+                const uint64_t k = i < n ? lists[i * top + at] : 0;
+                if (!__any(k > last)) break;  // nor the lists' further ones
+                take(k, top);
+            }
     }
 };
 
@@ -134,108 +177,154 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, int row, Sums t, uint
     }
 }
 
-template <bool TOP>
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
+// Sums over 16 more logits; missing ones are -infinity.
+__device__ __forceinline__ void add(Sums &t, const f4 *x, float most)
 {
-    __shared__ Sums sums[4];
-    __shared__ uint64_t lists[4][kMostTop];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
-    const int64_t first = (int64_t)seg * kSegment;
-    const float *p = a.x + row * a.stride + first;
-    const int n = (int)min((int64_t)kSegment, a.classes - first);
-
-    f4 x[kPerThread / 4];
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kPerThread / 4; ++j) {
-        const int c = 4 * (kThreads * j + (int)threadIdx.x);
-        if (c + 4 <= n) {
-            x[j] = *(const f4 *)(p + c);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[j][i] = c + i < n ? p[c + i] : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, x[j][i]);
+    const float m = fmaxf(t.m, most), ref = m == -INFINITY ? 0.0f : m;
+    if (__any(t.m < m)) {
+        t = moved(t, ref);
+        t.m = m;
     }
-    Sums t = {m, 0.0f, 0.0f};
-    const float ref = m == -INFINITY ? 0.0f : m;
+    float s = t.s, w = t.w;
 #pragma unroll
     for (int j = 0; j < kPerThread / 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float d = x[j][i] - ref, e = expf(d);
-            t.s += e;
-            t.w += e == 0.0f ? 0.0f : d * e;
+            const float d = x[j][i] - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
+            s += e;
+            w = fmaf(d, e, w);
         }
-    t = wave_join(t);
-    if (lane == 0) sums[wave] = t;
-
-    if (TOP) {
-        // The lanes' largest, and the k-th of them from below.
-        unsigned most = 0;
-        auto key = [&](int j, int i) {
-            const int c = 4 * (kThreads * j + (int)threadIdx.x) + i;
-            return c < n ? key_of(x[j][i], (int)first + c) : 0;
-        };
-#pragma unroll
-        for (int j = 0; j < kPerThread / 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) most = max(most, (unsigned)(key(j, i) >> 32));
-        unsigned bound = 0;
-        for (unsigned bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-            if (__popcll(__ballot(most >= (bound | bit))) >= a.top) bound |= bit;
-        Best best;
-        best.last = bound ? ((uint64_t)bound << 32) - 1 : 0;
+    if (__any(w != w)) {  // -infinity among them: 0 there, and not 0 * inf
+        w = t.w;
 #pragma unroll
         for (int j = 0; j < kPerThread / 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint64_t k = key(j, i);
-                for (uint64_t left = __ballot(k > best.last); left; left &= left - 1) {
-                    const uint64_t one = lane_key(k, __builtin_ctzll(left));
-                    if (one <= best.last) continue;
-                    best.put(one, a.top);
-                    if (bound) best.last = max(best.last, ((uint64_t)bound << 32) - 1);
+                const float d = x[j][i] - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
+                w += e == 0.0f ? 0.0f : d * e;
+            }
+    }
+    t.s = s, t.w = w;
+}
+
+// Between workgroups of a launch, past the L2s of their XCDs.
+__device__ __forceinline__ void put8(void *p, uint64_t v)
+{
+    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get8(const void *p)
+{
+    return __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
+{
+    __shared__ Sums sums[4];
+    __shared__ uint64_t lists[TOP ? kKeys : 1];
+    __shared__ bool last;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int index = blockIdx.x / a.pieces, piece = blockIdx.x - index * a.pieces, row = a.row0 + index;
+    const float *p = a.x + row * a.stride;
+    const int end = min((piece + 1) * a.per, a.chunks);
+
+    f4 x[kPerThread / 4], next[kPerThread / 4];
+    auto load = [&](f4 *to, int chunk) {
+        const int64_t first = (int64_t)chunk * kChunk + 4 * (int)threadIdx.x;
+        if ((int64_t)(chunk + 1) * kChunk <= a.classes) {
+#pragma unroll
+            for (int j = 0; j < kPerThread / 4; ++j) to[j] = *(const f4 *)(p + first + 4 * kThreads * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPerThread / 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t c = first + 4 * kThreads * j + i;
+                    to[j][i] = c < a.classes ? p[c] : -INFINITY;
+                }
+        }
+    };
+    Sums t = {-INFINITY, 0.0f, 0.0f};
+    Best best;
+    load(next, piece * a.per);
+    for (int chunk = piece * a.per; chunk < end; ++chunk) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kPerThread / 4; ++j) {
+            x[j] = next[j];
+            most = fmaxf(most, fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+        }
+        if (chunk + 1 < end) load(next, chunk + 1);
+        add(t, x, most);
+        if (TOP) {
+            if (chunk == piece * a.per) best.raise((unsigned)(key_of(most, 0) >> 32), a.top);
+            const int64_t first = (int64_t)chunk * kChunk + 4 * (int)threadIdx.x;
+#pragma unroll
+            for (int j = 0; j < kPerThread / 4; ++j) {
+                // Below the last that is kept?  (A NaN is never below.)
+                const float least = value_of(best.last + 1);
+                const bool any = !(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) < least);
+                if (!__any(any)) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t c = first + 4 * kThreads * j + i;
+                    best.take(c < a.classes ? key_of(x[j][i], (int)c) : 0, a.top);
                 }
             }
-        if (lane < a.top) lists[wave][lane] = best.mine;
+        }
+    }
+    t = wave_join(t);
+    if (lane == 0) sums[wave] = t;
+    if (a.pieces > 1) {
+        const int64_t size = 16 + 32 * (int64_t)a.top;
+        char *mine = a.part + blockIdx.x * size;
+        if (TOP && lane < a.top) put8(mine + 16 + 8 * (wave * a.top + lane), best.mine);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            t = join(join(sums[0], sums[1]), join(sums[2], sums[3]));
+            put8(mine, (uint64_t)__builtin_bit_cast(unsigned, t.s) << 32 | __builtin_bit_cast(unsigned, t.m));
+            put8(mine + 8, __builtin_bit_cast(unsigned, t.w));
+        }
+        wait_vmem();  // the stores have reached memory
+        __syncthreads();
+        if (threadIdx.x == 0)
+            last = __hip_atomic_fetch_add(&g_rows_done[index], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.pieces - 1;
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) __hip_atomic_store(&g_rows_done[index], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const char *from = a.part + (int64_t)index * a.pieces * size;
+        t = {-INFINITY, 0.0f, 0.0f};
+        for (int i = threadIdx.x; i < a.pieces; i += kThreads) {
+            const uint64_t ms = get8(from + i * size), w = get8(from + i * size + 8);
+            t = join(t, Sums{__builtin_bit_cast(float, (unsigned)ms), __builtin_bit_cast(float, (unsigned)(ms >> 32)),
+                             __builtin_bit_cast(float, (unsigned)w)});
+        }
+        t = wave_join(t);
+        if (lane == 0) sums[wave] = t;
+        if (TOP) {
+            best = Best();
+            const int at_once = kKeys / (4 * a.top);  // pieces
+            for (int i0 = 0; i0 < a.pieces; i0 += at_once) {
+                const int n = min(at_once, a.pieces - i0), keys = 4 * a.top;
+                __syncthreads();
+                for (int i = threadIdx.x; i < n * keys; i += kThreads) {
+                    const int pc = i / keys;
+                    lists[i] = get8(from + (i0 + pc) * size + 16 + 8 * (i - pc * keys));
+                }
+                __syncthreads();
+                if (wave == 0) best.join(lists, 4 * n, a.top);
+            }
+        }
+    } else if (TOP) {
+        if (lane < a.top) lists[wave * a.top + lane] = best.mine;
     }
     __syncthreads();
     if (wave) return;
     t = join(join(sums[0], sums[1]), join(sums[2], sums[3]));
-    Best best;
-    if (TOP) {
-        if (lane < a.top) best.mine = lists[0][lane];
-        best.last = lane_key(best.mine, a.top - 1);
-#pragma unroll
-        for (int w = 1; w < 4; ++w) best.take(lane < a.top ? lists[w][lane] : 0, a.top);
+    if (TOP && a.pieces == 1) {
+        best = Best();
+        best.join(lists, 4, a.top);
     }
-    if (a.segments == 1) {
-        finish(a, row, t, best.mine);
-        return;
-    }
-    if (lane == 0) *(Sums *)(a.part + 3 * (int64_t)blockIdx.x) = t;
-    if (TOP && lane < a.top) a.lists[(int64_t)blockIdx.x * a.top + lane] = best.mine;
-}
-
-// One wave per row.
-__global__ __launch_bounds__(64) void token_logprobs_join(ScoreArgs a)
-{
-    const int row = blockIdx.x, lane = threadIdx.x;
-    const int64_t first = (int64_t)row * a.segments;
-    Sums t = {-INFINITY, 0.0f, 0.0f};
-    for (int s = lane; s < a.segments; s += 64) t = join(t, *(const Sums *)(a.part + 3 * (first + s)));
-    t = wave_join(t);
-    Best best;
-    if (a.top)
-        for (int s = 0; s < a.segments; s += 64)
-            for (int i = 0; i < a.top; ++i) {
-                const uint64_t k = s + lane < a.segments ? a.lists[(first + s + lane) * a.top + i] : 0;
-                if (!__any(k > best.last)) break;  // nor the lists' further ones
-                best.take(k, a.top);
-            }
     finish(a, row, t, best.mine);
 }
 
@@ -295,28 +384,32 @@ extern "C" int token_logprobs(const float *logits, int64_t row_stride, const int
 {
     using namespace ember;
     const char *what = "token_logprobs";
-    const int64_t segments = (classes + kSegment - 1) / kSegment;
-    if (rows < 0 || classes < 1 || classes > kMostClasses || row_stride < classes || top < 0 || top > kMostTop || top > classes ||
-        rows > kMostBlocks / segments)
+    if (rows < 0 || rows > 0x7fffffff || classes < 1 || classes > kMostClasses || row_stride < classes || top < 0 || top > kMostTop ||
+        top > classes)
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
     if (rows == 0) return EMBER_OK;
     if (!logits || !tokens || !logp || (top && (!top_tokens || !top_logp)) ||
         (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)logp | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)top_tokens | (uintptr_t)top_logp) & 3))
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
-    ScoreArgs a = {logits, tokens, logp, lse, entropy, top_tokens, top_logp, nullptr, nullptr, row_stride, (int)rows, (int)classes, (int)segments, top};
-    const int64_t blocks = rows * segments;
-    if (segments > 1) {
-        const size_t lists = ((size_t)blocks * 12 + 15) / 16 * 16;
-        char *ws = (char *)scratch(kScratchLogprobs, lists + (size_t)blocks * top * 8);
-        if (!ws) return EMBER_ERR_OUT_OF_MEMORY;
-        a.part = (float *)ws, a.lists = (uint64_t *)(ws + lists);
+    ScoreArgs a = {logits, tokens, logp, lse, entropy, top_tokens, top_logp, nullptr, row_stride, (int)rows, (int)classes};
+    a.chunks = (int)((classes + kChunk - 1) / kChunk), a.top = top;
+    // A row to a workgroup, unless there are too few for the chip (8 of them fit
+    // on a CU): then pieces, but of a chunk at least.
+    const int64_t slots = std::min<int64_t>(8 * (int64_t)std::max(device_cu_count(), 1), kMostRows);
+    a.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, slots / rows));
+    a.per = (a.chunks + a.pieces - 1) / a.pieces;
+    a.pieces = (a.chunks + a.per - 1) / a.per;
+    if (a.pieces > 1) {  // then there are no more rows than slots
+        a.part = (char *)scratch(kScratchLogprobs, (size_t)rows * a.pieces * (16 + 32 * top));
+        if (!a.part) return EMBER_ERR_OUT_OF_MEMORY;
     }
-    if (top) hipLaunchKernelGGL(token_logprobs_kernel<true>, dim3((unsigned)blocks), dim3(kThreads), 0, 0, a);
-    else hipLaunchKernelGGL(token_logprobs_kernel<false>, dim3((unsigned)blocks), dim3(kThreads), 0, 0, a);
-    if (!launch_ok("token_logprobs")) return EMBER_ERR_DEVICE;
-    if (segments > 1) {
-        hipLaunchKernelGGL(token_logprobs_join, dim3((unsigned)rows), dim3(64), 0, 0, a);
-        if (!launch_ok("token_logprobs_join")) return EMBER_ERR_DEVICE;
+    const int64_t most = kMostBlocks / a.pieces;
+    for (int64_t row = 0; row < rows; row += most) {
+        a.row0 = (int)row;
+        const unsigned blocks = (unsigned)(std::min(most, rows - row) * a.pieces);
+        if (top) hipLaunchKernelGGL(token_logprobs_kernel<true>, dim3(blocks), dim3(kThreads), 0, 0, a);
+        else hipLaunchKernelGGL(token_logprobs_kernel<false>, dim3(blocks), dim3(kThreads), 0, 0, a);
+        if (!launch_ok("token_logprobs")) return EMBER_ERR_DEVICE;
     }
     return EMBER_OK;
 }

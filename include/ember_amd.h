@@ -418,8 +418,7 @@ int kv_cache_attention(const ember_kv_cache *cache, const float *q, float *o, fl
  * -infinity, gives NaN in logp (of a token in range), entropy and top_logp,
  * and in lse NaN, or -infinity if it holds nothing else; where NaN stands in
  * the order of top_tokens is not specified.  tokens are int32 device memory.
- * Uses library scratch.
- * classes from 1 to 2^31 - 2^16. */
+ * Uses library scratch.  At most 2^31 - 1 rows, classes from 1 to 2^31 - 2^16. */
 int token_logprobs(const float *logits, int64_t row_stride, const int32_t *tokens, int64_t rows,
                    int64_t classes, float *logp, float *lse, float *entropy, int32_t *top_tokens,
                    float *top_logp, int top);
