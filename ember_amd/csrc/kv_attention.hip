@@ -34,6 +34,7 @@
 #include "kv_cache.h"
 #include "lds_dma.h"
 #include "split_bf16.h"
+#include "wave.h"
 
 namespace ember {
 namespace {
@@ -65,29 +66,6 @@ __device__ __forceinline__ int length_of(const KvAttnArgs &a, Span sp)
 {
     const int64_t room = (int64_t)a.c.max_pages << a.c.page_shift;
     return (int)max(min((int64_t)sp.start + sp.count, room), (int64_t)0);
-}
-
-// Sums over the lanes up to this one (a wave's lanes, in register moves).
-template <int CTRL, int ROWS, class V>
-__device__ __forceinline__ V moved_in(V v)
-{
-    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-}
-template <class V>
-__device__ __forceinline__ V wave_scan(V v)
-{
-    v += moved_in<0x111, 0xf>(v);  // from 1, 2, 4 and 8 lanes below, within 16
-    v += moved_in<0x112, 0xf>(v);
-    v += moved_in<0x114, 0xf>(v);
-    v += moved_in<0x118, 0xf>(v);
-    v += moved_in<0x142, 0xa>(v);  // the last lane of the 16 below, and of the 32 below
-    v += moved_in<0x143, 0xc>(v);
-    return v;
-}
-template <class V>
-__device__ __forceinline__ V wave_sum(V v)
-{
-    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_scan(v)), 63));
 }
 
 // Units that are cut: how many of their workgroups are done.  Zero between
@@ -230,7 +208,7 @@ __device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block
     int before = 0;
     for (int b0 = 0; b0 < a.c.sequences; b0 += 64) {
         const int n = b0 + lane < a.c.sequences ? p.pieces(tiles_of(a, b0 + lane)) : 0;
-        const int upto = wave_scan(n);
+        const int upto = wave_scan_sum(n);
         const int at = __popcll(__ballot(block >= before + upto * units));  // sequences that end before
         if (at < 64) {
             const int pieces = __builtin_amdgcn_readlane(n, at);
@@ -243,17 +221,13 @@ __device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block
     return {-1, 0, 0, 0, 0};
 }
 
-// Parts of a unit's result go from one workgroup to another of the same launch,
-// which may be on another XCD with an L2 of its own: stores and loads at device
-// scope pass the L2s by.  (A release fence would write a whole L2 back.)
 __device__ __forceinline__ void put2(float *p, float x, float y)
 {
-    const uint64_t v = (uint64_t)__builtin_bit_cast(unsigned, y) << 32 | __builtin_bit_cast(unsigned, x);
-    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    put8(p, (uint64_t)float_bits(y) << 32 | float_bits(x));
 }
 __device__ __forceinline__ f32x2 get2(const float *p)
 {
-    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t v = get8(p);
     return f32x2{__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32))};
 }
 
@@ -486,21 +460,29 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
         }
         wait_vmem();  // the stores have reached memory
         __syncthreads();
-        unsigned *done = &g_done[b * units + unit];
-        if (threadIdx.x == 0) last = __hip_atomic_fetch_add(done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)pl.pieces - 1;
+        if (threadIdx.x == 0) last = last_of(&g_done[b * units + unit], pl.pieces);
         __syncthreads();
         if (!last) return;
-        if (threadIdx.x == 0) __hip_atomic_store(done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (works) {
             const float *from = a.part + (int64_t)pl.first * PART;
             const int64_t step = (int64_t)units * PART;
             top = kNone, sum = 0.0f, o = f32x4{0, 0, 0, 0};
-            for (int i = 0; i < pl.pieces; ++i, from += step) {
-                const f32x2 st = get2(from + kRows * D + 2 * rw), o0 = get2(from + rw * D + d), o1 = get2(from + rw * D + d + 2);
-                const float to = fmaxf(top, st[0]), f = __builtin_amdgcn_exp2f(top - to), g = __builtin_amdgcn_exp2f(st[0] - to);
-                top = to;
-                sum = sum * f + st[1] * g;
-                o = o * f + f32x4{o0[0], o0[1], o1[0], o1[1]} * g;
+            constexpr int N = 6;  // pieces whose loads are in flight at once
+            for (int i = 0; i < pl.pieces; i += N) {
+                f32x2 st[N], o0[N], o1[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float *one = from + min(i + j, pl.pieces - 1) * step;
+                    st[j] = get2(one + kRows * D + 2 * rw), o0[j] = get2(one + rw * D + d), o1[j] = get2(one + rw * D + d + 2);
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    if (i + j >= pl.pieces) break;
+                    const float to = fmaxf(top, st[j][0]), f = __builtin_amdgcn_exp2f(top - to), g = __builtin_amdgcn_exp2f(st[j][0] - to);
+                    top = to;
+                    sum = sum * f + st[j][1] * g;
+                    o = o * f + f32x4{o0[j][0], o0[j][1], o1[j][0], o1[j][1]} * g;
+                }
             }
         }
     }

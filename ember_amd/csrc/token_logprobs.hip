@@ -27,6 +27,7 @@
 
 #include "common.h"
 #include "lds_dma.h"
+#include "wave.h"
 
 namespace ember {
 namespace {
@@ -100,6 +101,24 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane)
            (unsigned)__builtin_amdgcn_readlane((int)(unsigned)k, lane);
 }
 
+// What the lanes of a wave have written to LDS is there for all of them.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Appends the lanes' keys above `last` to `found`, which has c; returns how many
+// there are then (those past kFound are not kept).
+constexpr int kFound = 128;
+__device__ __forceinline__ int gather(uint64_t *found, int c, uint64_t key, uint64_t last)
+{
+    const uint64_t some = __ballot(key > last);
+    const int at = c + __builtin_amdgcn_mbcnt_hi((unsigned)(some >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
+    if (key > last && at < kFound) found[at] = key;
+    return c + __popcll(some);
+}
+
 // A wave's `top` largest keys, the largest in lane 0.  Empty places hold 0,
 // below every key of a float.  Only keys above `last` are taken: the lowest that
 // is kept, or a bound that at least `top` others are known to pass.
@@ -133,8 +152,29 @@ struct Best {
         const uint64_t l = bound ? ((uint64_t)bound << 32) - 1 : 0;
         last = l > last ? l : last;
     }
+    // The `top` largest of c keys in `found` (c <= kFound), each put where the
+    // number of larger ones says; `found` is used up.
+    __device__ __forceinline__ void sort(uint64_t *found, int c, int top)
+    {
+        const int lane = threadIdx.x & 63;
+        wave_sync();
+        const uint64_t k0 = lane < c ? found[lane] : 0, k1 = lane + 64 < c ? found[lane + 64] : 0;
+        int r0 = 0, r1 = 0;
+#pragma unroll 8
+        for (int i = 0; i < c; ++i) {
+            const uint64_t k = found[i];
+            r0 += k > k0, r1 += k > k1;
+        }
+        wave_sync();
+        if (lane < c && r0 < top) found[r0] = k0;
+        if (lane + 64 < c && r1 < top) found[r1] = k1;
+        wave_sync();
+        mine = lane < min(c, top) ? found[lane] : 0;
+        const uint64_t l = lane_key(mine, top - 1);
+        last = l > last ? l : last;
+    }
     // Takes in n sorted lists of `top` keys, one after the other in `lists`.
-    __device__ __forceinline__ void join(const uint64_t *lists, int n, int top)
+    __device__ __forceinline__ void join(const uint64_t *lists, int n, int top, uint64_t *found)
     {
         const int lane = threadIdx.x & 63;
         uint64_t head = 0;
@@ -144,20 +184,25 @@ struct Best {
             head = lists[lane % n * top + lane / n];
         }
         raise((unsigned)(head >> 32), top);
-        for (int i = lane; i - lane < n; i += 64)
-            for (int at = 0; at < top; ++at) {
-                const uint64_t k = i < n ? lists[i * top + at] : 0;
-                if (!__any(k > last)) break;  // nor the lists' further ones
-                take(k, top);
-            }
+        auto all = [&](auto f) {
+            for (int i = lane; i - lane < n; i += 64)
+                for (int at = 0; at < top; ++at) {
+                    const uint64_t k = i < n ? lists[i * top + at] : 0;
+                    if (!__any(k > last)) break;  // nor the lists' further ones
+                    f(k);
+                }
+        };
+        int c = gather(found, 0, mine, 0);
+        all([&](uint64_t k) { c = gather(found, c, k, last); });
+        if (c <= kFound) sort(found, c, top);
+        else all([&](uint64_t k) { take(k, top); });
     }
 };
 
 __device__ __forceinline__ Sums wave_join(Sums a)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join(a, Sums{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.w, o, 64)});
-    return a;
+    a = moved(a, wave_max(a.m));
+    return {a.m, wave_sum(a.s), wave_sum(a.w)};
 }
 
 // The row's results, from its sums; `best` is lane i's i-th key.  One wave.
@@ -207,21 +252,11 @@ __device__ __forceinline__ void add(Sums &t, const f4 *x, float most)
     t.s = s, t.w = w;
 }
 
-// Between workgroups of a launch, past the L2s of their XCDs.
-__device__ __forceinline__ void put8(void *p, uint64_t v)
-{
-    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ uint64_t get8(const void *p)
-{
-    return __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 template <bool TOP>
 __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
 {
     __shared__ Sums sums[4];
-    __shared__ uint64_t lists[TOP ? kKeys : 1];
+    __shared__ uint64_t lists[TOP ? kKeys : 1], found[TOP ? 4 : 1][kFound];
     __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int index = blockIdx.x / a.pieces, piece = blockIdx.x - index * a.pieces, row = a.row0 + index;
@@ -257,19 +292,29 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         if (chunk + 1 < end) load(next, chunk + 1);
         add(t, x, most);
         if (TOP) {
-            if (chunk == piece * a.per) best.raise((unsigned)(key_of(most, 0) >> 32), a.top);
             const int64_t first = (int64_t)chunk * kChunk + 4 * (int)threadIdx.x;
+            auto all = [&](auto f) {
 #pragma unroll
-            for (int j = 0; j < kPerThread / 4; ++j) {
-                // Below the last that is kept?  (A NaN is never below.)
-                const float least = value_of(best.last + 1);
-                const bool any = !(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) < least);
-                if (!__any(any)) continue;
+                for (int j = 0; j < kPerThread / 4; ++j) {
+                    // Below the last that is kept?  (A NaN is never below.)
+                    const float least = value_of(best.last + 1);
+                    if (!__any(!(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) < least))) continue;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t c = first + 4 * kThreads * j + i;
-                    best.take(c < a.classes ? key_of(x[j][i], (int)c) : 0, a.top);
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t c = first + 4 * kThreads * j + i;
+                        f(c < a.classes ? key_of(x[j][i], (int)c) : 0);
+                    }
                 }
+            };
+            auto take = [&](uint64_t k) { best.take(k, a.top); };
+            if (chunk == piece * a.per) {
+                best.raise((unsigned)(key_of(most, 0) >> 32), a.top);
+                int c = 0;
+                all([&](uint64_t k) { c = gather(found[wave], c, k, best.last); });
+                if (c <= kFound) best.sort(found[wave], c, a.top);
+                else all(take);
+            } else {
+                all(take);
             }
         }
     }
@@ -287,11 +332,9 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         }
         wait_vmem();  // the stores have reached memory
         __syncthreads();
-        if (threadIdx.x == 0)
-            last = __hip_atomic_fetch_add(&g_rows_done[index], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.pieces - 1;
+        if (threadIdx.x == 0) last = last_of(&g_rows_done[index], a.pieces);
         __syncthreads();
         if (!last) return;
-        if (threadIdx.x == 0) __hip_atomic_store(&g_rows_done[index], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const char *from = a.part + (int64_t)index * a.pieces * size;
         t = {-INFINITY, 0.0f, 0.0f};
         for (int i = threadIdx.x; i < a.pieces; i += kThreads) {
@@ -307,12 +350,18 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
             for (int i0 = 0; i0 < a.pieces; i0 += at_once) {
                 const int n = min(at_once, a.pieces - i0), keys = 4 * a.top;
                 __syncthreads();
-                for (int i = threadIdx.x; i < n * keys; i += kThreads) {
-                    const int pc = i / keys;
-                    lists[i] = get8(from + (i0 + pc) * size + 16 + 8 * (i - pc * keys));
+                // All of a thread's loads in flight at once.
+                uint64_t k[kKeys / kThreads];
+#pragma unroll
+                for (int j = 0; j < kKeys / kThreads; ++j) {
+                    const int i = min(j * kThreads + (int)threadIdx.x, n * keys - 1), pc = i / keys;
+                    k[j] = get8(from + (i0 + pc) * size + 16 + 8 * (i - pc * keys));
                 }
+#pragma unroll
+                for (int j = 0; j < kKeys / kThreads; ++j)
+                    if (j * kThreads + (int)threadIdx.x < n * keys) lists[j * kThreads + threadIdx.x] = k[j];
                 __syncthreads();
-                if (wave == 0) best.join(lists, 4 * n, a.top);
+                if (wave == 0) best.join(lists, 4 * n, a.top, found[0]);
             }
         }
     } else if (TOP) {
@@ -323,7 +372,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
     t = join(join(sums[0], sums[1]), join(sums[2], sums[3]));
     if (TOP && a.pieces == 1) {
         best = Best();
-        best.join(lists, 4, a.top);
+        best.join(lists, 4, a.top, found[0]);
     }
     finish(a, row, t, best.mine);
 }
