@@ -47,6 +47,7 @@ HIP_SOURCES = [
     ("distributions.hip", []),
     ("kv_cache.hip", []),
     ("kv_attention.hip", []),
+    ("kv_attention_rows.hip", []),
     ("token_logprobs.hip", []),
 ]
 

@@ -1,0 +1,167 @@
+// kv_attention.h -- what the kernels of attention over the 4-bit cache share (not
+// part of the public ABI): arguments, how keys are cut into pieces, and the parts
+// of an fp32 operand.
+#pragma once
+
+#include <math.h>
+
+#include "kv_cache.h"
+#include "split_bf16.h"
+#include "wave.h"
+
+namespace ember {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNone = -3.402823466e38f;  // the running maximum before any key
+constexpr float kRaise = 8.0f;
+constexpr int kWaves = 4;        // of a workgroup
+constexpr int kMostPlan = 1024;  // sequences that are planned for; with more, a unit is not cut
+constexpr int kMostUnits = 1 << 14;  // that are cut
+
+struct KvAttnArgs {
+    KvCache c;
+    const float *q;
+    float *o, *lse;
+    RowStrides qs, os;
+    const int32_t *start, *count;
+    float *part;  // of each workgroup: O (rows, D), then m and l of each row; null: units are not cut
+    int T, q_heads, group, tiles, blocks, causal;  // tiles: of rows, of a head
+    int keys, least;  // keys of a tile, tiles of a piece at least
+    float scale2;  // scale * log2(e), above 0
+};
+
+// Tokens that a sequence has after the call, as far as its table has room.
+__device__ __forceinline__ int length_of(const KvAttnArgs &a, Span sp)
+{
+    const int64_t room = (int64_t)a.c.max_pages << a.c.page_shift;
+    return (int)max(min((int64_t)sp.start + sp.count, room), (int64_t)0);
+}
+
+// How the keys are cut: into pieces of `per` tiles, the same for every unit (a
+// sequence's cache head and a tile of its rows), so that no workgroup has more than
+// another however the sequences' lengths differ.  per is the smallest, in steps
+// of an eighth, that needs no more workgroups than there are.  Each wave finds
+// it for itself; sequences are taken 64 at a time.  Pieces are not made smaller than
+// a join is worth.
+struct Plan {
+    int per;
+    __device__ __forceinline__ int pieces(int tiles) const { return max((tiles + per - 1) / per, 1); }
+};
+
+__device__ __forceinline__ int tiles_of(const KvAttnArgs &a, int b)
+{
+    return b < a.c.sequences ? (length_of(a, span_of(a.start, a.count, b, a.T)) + a.keys - 1) / a.keys : 0;
+}
+
+__device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
+{
+    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles, most = a.blocks / units;
+    const int mine = tiles_of(a, lane);
+    auto sum = [&](auto f) {
+        auto n = wave_sum(lane < a.c.sequences ? f(mine) : decltype(f(0))(0));
+        for (int b = 64; b < a.c.sequences; b += 64) n += wave_sum(b + lane < a.c.sequences ? f(tiles_of(a, b + lane)) : decltype(f(0))(0));
+        return n;
+    };
+    // The sum of all tiles may pass 32 bits; as a float it is near enough.
+    Plan p = {max((int)(sum([](int n) { return (float)n; }) / most), a.least)};
+    while (sum([&](int n) { return p.pieces(n); }) > most) p.per += p.per / 8 + 1;
+    return p;
+}
+
+__device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <int S>
+__device__ __forceinline__ unsigned fp4_bf16(unsigned w, float scale)
+{
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, S));
+}
+
+// The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
+// head h, or -1.  b, h and pos are the same in all lanes, so the table is read
+// through the scalar cache.
+__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
+{
+    typedef const __attribute__((address_space(4))) int32_t *scalar;
+    const int place = pos >> c.page_shift;
+    if (place >= c.max_pages) return -1;
+    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + place];
+    if ((unsigned)page >= (unsigned)c.pages) return -1;
+    return (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+}
+
+// The upper halves of three floats' parts: hi, mid and lo of x.
+__device__ __forceinline__ void cut3(float x, unsigned &hi, unsigned &mid, unsigned &lo)
+{
+    hi = float_bits(x) & 0xffff0000u;
+    x -= __builtin_bit_cast(float, hi);
+    mid = float_bits(x) & 0xffff0000u;
+    x -= __builtin_bit_cast(float, mid);
+    lo = float_bits(x) & 0xffff0000u;
+}
+
+// Where a workgroup stands: its unit, its piece of the unit's keys, and the
+// unit's first workgroup (its further ones follow `units` apart).
+struct Place {
+    int b, unit, piece, pieces, first;
+};
+
+// The place of workgroup `block`; b = -1 where the plan needs fewer.
+__device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block)
+{
+    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles;
+    int before = 0;
+    for (int b0 = 0; b0 < a.c.sequences; b0 += 64) {
+        const int n = b0 + lane < a.c.sequences ? p.pieces(tiles_of(a, b0 + lane)) : 0;
+        const int upto = wave_scan_sum(n);
+        const int at = __popcll(__ballot(block >= before + upto * units));  // sequences that end before
+        if (at < 64) {
+            const int pieces = __builtin_amdgcn_readlane(n, at);
+            const int from = before + (__builtin_amdgcn_readlane(upto, at) - pieces) * units;
+            const int piece = (block - from) / units, unit = block - from - piece * units;
+            return {b0 + at, unit, piece, pieces, from + unit};
+        }
+        before += __builtin_amdgcn_readlane(upto, 63) * units;
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
+__device__ __forceinline__ void put2(float *p, float x, float y)
+{
+    put8(p, (uint64_t)float_bits(y) << 32 | float_bits(x));
+}
+__device__ __forceinline__ f32x2 get2(const float *p)
+{
+    const uint64_t v = get8(p);
+    return f32x2{__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32))};
+}
+
+// The first key that row t of a sequence with `len` tokens does not see.
+__device__ __forceinline__ int limit_of(const KvAttnArgs &a, Span sp, int len, int t)
+{
+    return a.causal ? (int)max(min((int64_t)sp.start + t + 1, (int64_t)len), (int64_t)0) : len;
+}
+
+// A unit's workgroup: its place, or b = -1.
+__device__ __forceinline__ Place start_block(const KvAttnArgs &a, Plan &plan)
+{
+    const int units = a.c.heads * a.tiles;
+    plan = {0x40000000};
+    if (a.part) {
+        plan = make_plan(a);
+        return place_of(a, plan, blockIdx.x);
+    }
+    const int b = blockIdx.x / units;
+    return {b, (int)blockIdx.x - b * units, 0, 1, 0};
+}
+
+// Attention for many rows (kv_attention_rows.hip).
+int launch_kv_attention_rows(KvAttnArgs &a);
+// Fills in how the keys are cut, for workgroups of `rows` rows of which a CU
+// holds per_cu, and tiles of `keys` keys; records and returns a status.
+int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu);
+
+}  // namespace ember

@@ -26,93 +26,25 @@
 // end.  A unit's keys are cut into pieces, each with a workgroup of its own; the
 // last of them to be done (by a count that they all add to) joins the pieces, in
 // their order.
-#include <math.h>
-
 #include <algorithm>
 #include <type_traits>
 
-#include "kv_cache.h"
+#include "kv_attention.h"
 #include "lds_dma.h"
-#include "split_bf16.h"
-#include "wave.h"
 
 namespace ember {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNone = -3.402823466e38f;  // the running maximum before any key
-constexpr float kRaise = 8.0f;
-constexpr int kWaves = 4;
-constexpr int kTile = 32;        // keys
-constexpr int kRows = 8;         // rows per workgroup
-constexpr int kPerCu = 3;        // workgroups that a CU holds at once
-constexpr int kMostPlan = 1024;  // sequences that are planned for; with more, a unit is not cut
-constexpr int kMostUnits = 1 << 14;  // that are cut
-
-struct KvAttnArgs {
-    KvCache c;
-    const float *q;
-    float *o, *lse;
-    RowStrides qs, os;
-    const int32_t *start, *count;
-    float *part;  // of each workgroup: O (rows, D), then m and l of each row; null: units are not cut
-    int T, q_heads, group, tiles, blocks, causal;
-    float scale2;  // scale * log2(e), above 0
-};
-
-// Tokens that a sequence has after the call, as far as its table has room.
-__device__ __forceinline__ int length_of(const KvAttnArgs &a, Span sp)
-{
-    const int64_t room = (int64_t)a.c.max_pages << a.c.page_shift;
-    return (int)max(min((int64_t)sp.start + sp.count, room), (int64_t)0);
-}
+constexpr int kTile = 32;  // keys
+constexpr int kRows = 8;   // rows per workgroup
+constexpr int kPerCu = 3;  // workgroups that a CU holds at once
+constexpr int kLeast = 8;  // tiles of a piece: two for each wave
+constexpr int kFewRows = 32;
 
 // Units that are cut: how many of their workgroups are done.  Zero between
 // calls: the last one, which all the others have added to, clears its unit's.
 // All calls run on the null stream, so no two use it at once.
 __device__ unsigned g_done[kMostUnits];
-
-// How the keys are cut: into pieces of `per` tiles, the same for every unit (a
-// sequence's cache head and its 8 rows), so that no workgroup has more than
-// another however the sequences' lengths differ.  per is the smallest, in steps
-// of an eighth, that needs no more workgroups than there are.  Each wave finds
-// it for itself; sequences are taken 64 at a time.
-struct Plan {
-    int per;
-    __device__ __forceinline__ int pieces(int tiles) const { return max((tiles + per - 1) / per, 1); }
-};
-
-__device__ __forceinline__ int tiles_of(const KvAttnArgs &a, int b)
-{
-    return b < a.c.sequences ? (length_of(a, span_of(a.start, a.count, b, a.T)) + kTile - 1) / kTile : 0;
-}
-
-__device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
-{
-    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles, most = a.blocks / units;
-    const int mine = tiles_of(a, lane);
-    auto sum = [&](auto f) {
-        auto n = wave_sum(lane < a.c.sequences ? f(mine) : decltype(f(0))(0));
-        for (int b = 64; b < a.c.sequences; b += 64) n += wave_sum(b + lane < a.c.sequences ? f(tiles_of(a, b + lane)) : decltype(f(0))(0));
-        return n;
-    };
-    // The sum of all tiles may pass 32 bits; as a float it is near enough.
-    Plan p = {(int)fmaxf(sum([](int n) { return (float)n; }) / most, 1.0f)};
-    while (sum([&](int n) { return p.pieces(n); }) > most) p.per += p.per / 8 + 1;
-    return p;
-}
-
-__device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <int S>
-__device__ __forceinline__ unsigned fp4_bf16(unsigned w, float scale)
-{
-    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, S));
-}
 
 // N bytes (a power of two up to 16) as words; the pointer is aligned to N.
 template <int N>
@@ -141,19 +73,6 @@ struct Words {
         for (int i = 0; i < kWords; ++i) w[i] = 0;
     }
 };
-
-// The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
-// head h, or -1.  b, h and pos are the same in all lanes, so the table is read
-// through the scalar cache.
-__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
-{
-    typedef const __attribute__((address_space(4))) int32_t *scalar;
-    const int place = pos >> c.page_shift;
-    if (place >= c.max_pages) return -1;
-    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + place];
-    if ((unsigned)page >= (unsigned)c.pages) return -1;
-    return (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
-}
 
 // What a lane holds of 16 keys, and of 16 values.  Where there are none (at < 0)
 // it takes the cache's first ones, which then count for nothing.
@@ -185,52 +104,6 @@ struct Values {
     }
 };
 
-// The upper halves of three floats' parts: hi, mid and lo of x.
-__device__ __forceinline__ void cut3(float x, unsigned &hi, unsigned &mid, unsigned &lo)
-{
-    hi = float_bits(x) & 0xffff0000u;
-    x -= __builtin_bit_cast(float, hi);
-    mid = float_bits(x) & 0xffff0000u;
-    x -= __builtin_bit_cast(float, mid);
-    lo = float_bits(x) & 0xffff0000u;
-}
-
-// Where a workgroup stands: its unit, its piece of the unit's keys, and the
-// unit's first workgroup (its further ones follow `units` apart).
-struct Place {
-    int b, unit, piece, pieces, first;
-};
-
-// The place of workgroup `block`; b = -1 where the plan needs fewer.
-__device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block)
-{
-    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles;
-    int before = 0;
-    for (int b0 = 0; b0 < a.c.sequences; b0 += 64) {
-        const int n = b0 + lane < a.c.sequences ? p.pieces(tiles_of(a, b0 + lane)) : 0;
-        const int upto = wave_scan_sum(n);
-        const int at = __popcll(__ballot(block >= before + upto * units));  // sequences that end before
-        if (at < 64) {
-            const int pieces = __builtin_amdgcn_readlane(n, at);
-            const int from = before + (__builtin_amdgcn_readlane(upto, at) - pieces) * units;
-            const int piece = (block - from) / units, unit = block - from - piece * units;
-            return {b0 + at, unit, piece, pieces, from + unit};
-        }
-        before += __builtin_amdgcn_readlane(upto, 63) * units;
-    }
-    return {-1, 0, 0, 0, 0};
-}
-
-__device__ __forceinline__ void put2(float *p, float x, float y)
-{
-    put8(p, (uint64_t)float_bits(y) << 32 | float_bits(x));
-}
-__device__ __forceinline__ f32x2 get2(const float *p)
-{
-    const uint64_t v = get8(p);
-    return f32x2{__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32))};
-}
-
 template <int D>
 __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAttnArgs a)
 {
@@ -243,16 +116,9 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
     const int col = lane & 15, r = lane >> 4, row8 = col >> 1;
     const bool odd = col & 1;
     const int units = a.c.heads * a.tiles;
-    Plan plan = {0x40000000};
-    Place pl;
-    if (a.part) {
-        plan = make_plan(a);
-        pl = place_of(a, plan, blockIdx.x);
-        if (pl.b < 0) return;
-    } else {
-        const int b = blockIdx.x / units;
-        pl = {b, (int)blockIdx.x - b * units, 0, 1, 0};
-    }
+    Plan plan;
+    const Place pl = start_block(a, plan);
+    if (pl.b < 0) return;
     const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
     const int h = unit / a.tiles, tile = unit - h * a.tiles;
     const Span sp = span_of(a.start, a.count, b, a.T);
@@ -262,10 +128,9 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
     const int row = tile * kRows + row8, t = row / a.group, g = row - t * a.group;
     const bool valid = t < sp.count;
     const int last_t = min((tile * kRows + kRows - 1) / a.group, sp.count - 1);
-    auto limit_of = [&](int t) { return a.causal ? (int)max(min((int64_t)sp.start + t + 1, (int64_t)len), (int64_t)0) : len; };
-    const int keys = tile * kRows / a.group < sp.count && a.c.pages ? limit_of(last_t) : 0;  // all that the workgroup's rows see
-    const int limit = valid ? limit_of(t) : keys;
-    const int sure = keys ? limit_of(tile * kRows / a.group) : 0;  // every row sees the keys before
+    const int keys = tile * kRows / a.group < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the workgroup's rows see
+    const int limit = valid ? limit_of(a, sp, len, t) : keys;
+    const int sure = keys ? limit_of(a, sp, len, tile * kRows / a.group) : 0;  // every row sees the keys before
 
     u32x4 q[KS][3];
     {
@@ -499,23 +364,33 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
 template <int D>
 int launch(KvAttnArgs &a)
 {
-    const int64_t all = (int64_t)a.c.sequences * a.c.heads * a.tiles;  // units
-    if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
-    // One round of workgroups over the chip; where the units alone are about as
-    // many, two pieces each, so that the longest sequence does not decide.
-    const int64_t slots = (int64_t)kPerCu * std::max(device_cu_count(), 1);
-    const bool cut = a.c.sequences <= kMostPlan && all <= kMostUnits;
-    a.blocks = (int)(cut ? std::max(slots, 2 * all) : all);
-    if (cut) {
-        a.part = (float *)scratch(kScratchKvAttention, (size_t)a.blocks * kRows * (D + 2) * sizeof(float));
-        if (!a.part) return EMBER_ERR_OUT_OF_MEMORY;
-    }
+    const int st = cut_keys(a, kRows, kTile, kLeast, kPerCu);
+    if (st) return st;
     hipLaunchKernelGGL(kv_attention_kernel<D>, dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
-    if (!launch_ok("kv_attention")) return EMBER_ERR_DEVICE;
-    return EMBER_OK;
+    return launch_ok("kv_attention") ? EMBER_OK : EMBER_ERR_DEVICE;
 }
 
 }  // namespace
+
+int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
+{
+    a.tiles = (int)(((int64_t)a.T * a.group + rows - 1) / rows);
+    a.keys = keys, a.least = least;
+    const int64_t all = (int64_t)a.c.sequences * a.c.heads * a.tiles;  // units
+    if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
+    // One round of workgroups over the chip; where the units alone are about as
+    // many, two pieces each, so that the longest sequence does not decide.  With
+    // many units none is cut.
+    const int64_t slots = (int64_t)per_cu * std::max(device_cu_count(), 1);
+    const bool cut = a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * slots);
+    a.blocks = (int)(cut ? std::max(slots, 2 * all) : all);
+    if (cut) {
+        a.part = (float *)scratch(kScratchKvAttention, (size_t)a.blocks * rows * (a.c.D + 2) * sizeof(float));
+        if (!a.part) return EMBER_ERR_OUT_OF_MEMORY;
+    }
+    return EMBER_OK;
+}
+
 }  // namespace ember
 
 extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, float *o, float *lse, int64_t T, int64_t q_heads,
@@ -537,10 +412,10 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     a.qs = {in_sb, in_sh, in_ss}, a.os = {out_sb, out_sh, out_ss};
     a.start = start, a.count = count;
     a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / a.c.heads);
-    a.tiles = (int)((T * a.group + kRows - 1) / kRows);
     a.causal = causal != 0;
     // Above 0, so that a masked score stays -infinity under it; a scale of 0 then
     // gives scores that differ by nothing.
     a.scale2 = std::max(scale * kLog2e, 1e-37f);
+    if (T * a.group > kFewRows) return launch_kv_attention_rows(a);
     return a.c.D == 128 ? launch<128>(a) : a.c.D == 64 ? launch<64>(a) : launch<32>(a);
 }

@@ -1,0 +1,373 @@
+// kv_attention_rows.hip -- attention of many query rows over the 4-bit cache: a
+// prompt read in pieces, on what is cached.
+//
+// The same sums as in kv_attention.hip, on v_mfma_f32_32x32x16_bf16: a workgroup
+// has 128 rows, 32 to a wave, and its waves share tiles of 64 keys and values
+// that are converted to bf16 once and laid out in LDS as the matrix core takes
+// them, so that the conversion is a small part of the work:
+//   S^T (32 keys x 32 rows) = K . Q^T, Q's three parts in registers;
+//   O^T (D x 32 rows) += V^T . P^T, P's three parts from S^T's registers: lane l
+//     holds column l % 32 and, of each 16 keys, those of its half h = l / 32: 4h ..
+//     4h+3 and 8+4h .. 8+4h+3.  V^T lies in LDS with its keys in that order.
+// Two tiles of LDS: while one is worked on, the next is converted into the other
+// and the one after is loaded; one barrier a tile.
+//
+// LDS: K rows are D bf16 long, V^T rows 64, cut into pieces of 16 bytes whose
+// place in the row is turned by the row's number (k_place, v_place), so that
+// neither the 32 rows that a wave reads at once nor the ones that it writes lie
+// in the same banks.
+//
+// Work: 12 * T * keys * D matrix operations a head where 4 are the definition's.
+#include <type_traits>
+
+#include "kv_attention.h"
+#include "lds_dma.h"
+
+namespace ember {
+namespace {
+
+constexpr int kTile = 64;    // keys
+constexpr int kRows = 128;   // rows per workgroup
+constexpr int kPerCu = 2;    // workgroups that a CU holds at once
+constexpr int kLeast = 8;    // tiles of a piece
+
+// As in kv_attention.hip.
+__device__ unsigned g_done[kMostUnits];
+
+template <int D>
+struct Lds {
+    uint4 k[kTile * D / 8], v[kTile * D / 8];  // bf16
+    // Of the tile's 64 tokens and each group of 32, whether the values are no
+    // numbers (bytes: token within the group of D); then, of each 16 tokens,
+    // whether they are not there.
+    unsigned flags[16 * (D / 32) + 4];
+};
+
+// The piece of 16 bytes where elements 8c .. 8c+7 of key `key` are, and where V^T
+// has piece c (of 8) of its row d.
+template <int D>
+__device__ __forceinline__ int k_place(int key, int c)
+{
+    constexpr int N = D / 8;
+    return key * N + (c ^ (D == 128 ? key & 15 : D == 64 ? key & 7 : (key >> 1) & 3));
+}
+template <int D>
+__device__ __forceinline__ int v_place(int d, int c)
+{
+    return d * 8 + (c ^ ((d ^ (d / (D / 16))) & 7));
+}
+
+// What a thread loads of a tile: a quarter of a key's row, and of 4 tokens' values
+// D/16 elements each.  A wave's keys and values are the tile's tokens 16w ..
+// 16w+15, which are on one page.
+template <int D>
+struct Raw {
+    static constexpr int KW = D / 32 == 1 ? 1 : D / 32;  // words of a quarter row
+    unsigned k[KW], ks, v[4], vs[KW];
+    bool there;
+
+    __device__ __forceinline__ void load(const KvCache &c, int64_t at, int thread)
+    {
+        there = at >= 0;
+        at = at < 0 ? 0 : at;
+        const int key = (thread >> 2) & 15, r = thread & 3;
+        const uint8_t *kp = c.k_codes + at * (D / 2) + (key * (D / 2) + r * (D / 8));
+        words(kp, k);
+        ks = (c.k_scales + at * (D / 32))[key * (D / 32) + r * D / 128];
+        const int quad = (thread >> 4) & 3, col = thread & 15;
+        const uint8_t *vp = c.v_codes + at * (D / 2) + (4 * quad * (D / 2) + col * (D / 32));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (D == 128) v[i] = *(const unsigned *)(vp + i * (D / 2));
+            else if constexpr (D == 64) v[i] = *(const uint16_t *)(vp + i * (D / 2));
+            else v[i] = vp[i * (D / 2)];
+        }
+        words(c.v_scales + at * (D / 32) + 4 * quad * (D / 32), vs);
+    }
+    __device__ __forceinline__ static void words(const uint8_t *p, unsigned *w)
+    {
+        if constexpr (D == 128) {
+            const u32x4 x = *(const u32x4 *)p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = x[i];
+        } else if constexpr (D == 64) {
+            const uint2 x = *(const uint2 *)p;
+            w[0] = x.x, w[1] = x.y;
+        } else {
+            w[0] = *(const unsigned *)p;
+        }
+    }
+
+    // Converts and writes them.
+    __device__ __forceinline__ void put(Lds<D> &lds, int thread) const
+    {
+        const int key = thread >> 2, r = thread & 3;
+        const float kscale = scale_of(ks);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+            lds.k[k_place<D>(key, r * (D / 32) + i)] = uint4{fp4_bf16<0>(k[i], kscale), fp4_bf16<1>(k[i], kscale),
+                                                            fp4_bf16<2>(k[i], kscale), fp4_bf16<3>(k[i], kscale)};
+        const int quad = thread >> 4, col = thread & 15;
+        float scale[4];
+        unsigned w[4], bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned byte = (vs[i * D / 128] >> (8 * ((i * (D / 32) & 3) + col * D / 512))) & 0xff;
+            const bool spoilt = byte > kMostScale;
+            bad |= spoilt ? 1u << (8 * i) : 0;
+            w[i] = spoilt ? 0 : v[i];  // zero in the products
+            scale[i] = spoilt ? 1.0f : scale_of(byte);
+        }
+        if (col % (16 / (D / 32)) == 0) lds.flags[16 * (col * D / 512) + quad] = bad;
+        if ((thread & 63) == 0) lds.flags[16 * (D / 32) + (thread >> 6)] = there ? 0 : 1;
+        // Keys 16s .. +15 of a row of V^T: the 8 of half 0, then those of half 1;
+        // a quad is 8 bytes.
+        const int s = quad >> 2, piece = 2 * s + (quad & 1), half = (quad >> 1) & 1;
+        uint2 *to = (uint2 *)lds.v;
+        auto pair = [&](auto X) {
+            constexpr int x = decltype(X)::value;
+            const unsigned a = fp4_bf16<x>(w[0], scale[0]), b = fp4_bf16<x>(w[1], scale[1]);
+            const unsigned e = fp4_bf16<x>(w[2], scale[2]), f = fp4_bf16<x>(w[3], scale[3]);
+            const int d = col * (D / 16) + 2 * x;
+            to[2 * v_place<D>(d, piece) + half] = uint2{__builtin_amdgcn_perm(b, a, 0x05040100), __builtin_amdgcn_perm(f, e, 0x05040100)};
+            to[2 * v_place<D>(d + 1, piece) + half] = uint2{__builtin_amdgcn_perm(b, a, 0x07060302), __builtin_amdgcn_perm(f, e, 0x07060302)};
+        };
+        pair(std::integral_constant<int, 0>{});
+        if constexpr (D > 32) pair(std::integral_constant<int, 1>{});
+        if constexpr (D > 64) {
+            pair(std::integral_constant<int, 2>{});
+            pair(std::integral_constant<int, 3>{});
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma32(uint4 a, u32x4 b, f32x16 c)
+{
+    return mfma_32x32x16(u32x4{a.x, a.y, a.z, a.w}, b, c);
+}
+
+// Two floats' upper halves as a packed pair.
+__device__ __forceinline__ unsigned upper_halves(float x0, float x1)
+{
+    return __builtin_amdgcn_perm(float_bits(x1), float_bits(x0), 0x07060302);
+}
+__device__ __forceinline__ float lower_part(float x)
+{
+    return x - __builtin_bit_cast(float, float_bits(x) & 0xffff0000u);
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(KvAttnArgs a)
+{
+    constexpr int KS = D / 16, DB = D / 32;
+    __shared__ Lds<D> lds[2];
+    __shared__ bool last;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    const int units = a.c.heads * a.tiles;
+    Plan plan;
+    const Place pl = start_block(a, plan);
+    if (pl.b < 0) return;
+    const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
+    // The last rows see most keys: they start first.
+    const int h = unit / a.tiles, tile = a.tiles - 1 - (unit - h * a.tiles);
+    const Span sp = span_of(a.start, a.count, b, a.T);
+    const int len = length_of(a, sp);
+
+    // This lane's row, and the first key that it does not see.
+    const int row = tile * kRows + wave * 32 + l32, t = row / a.group, g = row - t * a.group;
+    const bool valid = t < sp.count;
+    const int first_t = tile * kRows / a.group, last_t = min((tile * kRows + kRows - 1) / a.group, sp.count - 1);
+    const int keys = first_t < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the workgroup's rows see
+    const int limit = valid ? limit_of(a, sp, len, t) : keys;
+    // All of the wave's rows see the keys before `sure`, none those from `seen` on.
+    const int wave_row = tile * kRows + wave * 32;
+    const int sure = min(keys, limit_of(a, sp, len, wave_row / a.group));
+    const int seen = wave_row / a.group < sp.count ? min(keys, limit_of(a, sp, len, (wave_row + 31) / a.group)) : 0;
+
+    u32x4 q[KS][3];
+    {
+        const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + 8 * half;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f32x4 x = valid ? *(const f32x4 *)(src + 16 * s + 4 * i) : f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x0 = x[2 * j], x1 = x[2 * j + 1];
+                    q[s][0][2 * i + j] = upper_halves(x0, x1);
+                    x0 = lower_part(x0), x1 = lower_part(x1);
+                    q[s][1][2 * i + j] = upper_halves(x0, x1);
+                    x0 = lower_part(x0), x1 = lower_part(x1);
+                    q[s][2][2 * i + j] = upper_halves(x0, x1);
+                }
+            }
+    }
+
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = zero16();
+    float m = kNone, l = 0.0f;
+
+    const int n = (keys + kTile - 1) / kTile;
+    const int first = __builtin_amdgcn_readfirstlane(pl.piece * plan.per);
+    const int end = pl.piece + 1 < pl.pieces ? min(n, first + plan.per) : n;
+
+    auto block = [&](const Lds<D> &at, int key0, auto KB) {
+        constexpr int kb = decltype(KB)::value;
+        f32x16 s = zero16();
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+            const uint4 k = at.k[k_place<D>(32 * kb + l32, 2 * x + half)];
+#pragma unroll
+            for (int part = 2; part >= 0; --part) s = mfma32(k, q[x][part], s);
+        }
+        const bool partly = key0 + 32 > sure || (at.flags[16 * DB + 2 * kb] | at.flags[16 * DB + 2 * kb + 1]);
+        if (__builtin_amdgcn_readfirstlane(partly)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (key0 + acc_row(i, half) >= limit || at.flags[16 * DB + 2 * kb + i / 8]) s[i] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top *= a.scale2;
+        if (__any(top > m + kRaise)) {
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            u32x4 p[3];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i], a.scale2, -m));
+                float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i + 1], a.scale2, -m));
+                l += e0;
+                l += e1;
+                p[0][i] = upper_halves(e0, e1);
+                e0 = lower_part(e0), e1 = lower_part(e1);
+                p[1][i] = upper_halves(e0, e1);
+                e0 = lower_part(e0), e1 = lower_part(e1);
+                p[2][i] = upper_halves(e0, e1);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const uint4 v = at.v[v_place<D>(32 * d + l32, 2 * (2 * kb + st) + half)];
+#pragma unroll
+                for (int part = 2; part >= 0; --part) acc[d] = mfma32(v, p[part], acc[d]);
+            }
+        }
+    };
+
+    auto piece_at = [&](int tl) { return tl < end ? row_of(a.c, b, h, tl * kTile + 16 * wave) : -1; };
+    Raw<D> raw;
+    if (first < end) {
+        raw.load(a.c, piece_at(first), threadIdx.x);
+        raw.put(lds[0], threadIdx.x);
+        if (first + 1 < end) raw.load(a.c, piece_at(first + 1), threadIdx.x);
+        __syncthreads();
+    }
+    for (int tl = first; tl < end; ++tl) {
+        const Lds<D> &at = lds[(tl - first) & 1];
+        if (tl + 1 < end) {
+            raw.put(lds[(tl - first + 1) & 1], threadIdx.x);
+            if (tl + 2 < end) raw.load(a.c, piece_at(tl + 2), threadIdx.x);
+        }
+        const int key0 = tl * kTile;
+        if (key0 < seen) {
+            // Values that are no numbers: NaN for the rows that see them.
+            unsigned bad = lane < 16 * DB ? at.flags[lane] : 0;
+            if (__any(bad)) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    for (int x = 0; x < kTile; ++x)
+                        if ((at.flags[16 * d + x / 4] >> (8 * (x & 3)) & 1) && key0 + x < limit && !at.flags[16 * DB + x / 16])
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[d][i] = NAN;
+            }
+            block(at, key0, std::integral_constant<int, 0>{});
+            if (key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
+        }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    if (pl.pieces > 1) {
+        constexpr int PART = kRows * (D + 2), SUMS = kRows * D;
+        float *mine = a.part + (int64_t)blockIdx.x * PART;
+        const int at = wave * 32 * D + 2 * lane;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float *to = mine + at + (8 * d + i) * 128;
+                put8(to, (uint64_t)float_bits(acc[d][2 * i + 1]) << 32 | float_bits(acc[d][2 * i]));
+            }
+        if (half == 0) put2(mine + SUMS + 2 * (wave * 32 + l32), m, l);
+        wait_vmem();  // the stores have reached memory
+        __syncthreads();
+        if (threadIdx.x == 0) last = last_of(&g_done[b * units + unit], pl.pieces);
+        __syncthreads();
+        if (!last) return;
+        const float *from = a.part + (int64_t)pl.first * PART;
+        m = kNone, l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] = zero16();
+        for (int i = 0; i < pl.pieces; ++i, from += (int64_t)units * PART) {
+            const f32x2 st = get2(from + SUMS + 2 * (wave * 32 + l32));
+            const float to = fmaxf(m, st[0]), f = __builtin_amdgcn_exp2f(m - to), e = __builtin_amdgcn_exp2f(st[0] - to);
+            m = to;
+            l = l * f + st[1] * e;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const f32x2 x = get2(from + at + (8 * d + j) * 128);
+                    acc[d][2 * j] = acc[d][2 * j] * f + x[0] * e;
+                    acc[d][2 * j + 1] = acc[d][2 * j + 1] * f + x[1] * e;
+                }
+        }
+    }
+    if (t >= a.T) return;
+    const int head = h * a.group + g;
+    const bool empty = !valid || l == 0.0f;
+    const float inv = 1.0f / l;
+    float *o = a.o + b * a.os.sb + head * a.os.sh + t * a.os.ss + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f32x4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = empty ? 0.0f : acc[d][4 * i + j] * inv;
+            *(f32x4 *)(o + 32 * d + 8 * i) = x;
+        }
+    if (a.lse && half == 0)
+        a.lse[((int64_t)b * a.q_heads + head) * a.T + t] = empty ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+template <int D>
+int launch(KvAttnArgs &a)
+{
+    const int st = cut_keys(a, kRows, kTile, kLeast, kPerCu);
+    if (st) return st;
+    hipLaunchKernelGGL(kv_attention_rows_kernel<D>, dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
+    return launch_ok("kv_attention_rows") ? EMBER_OK : EMBER_ERR_DEVICE;
+}
+
+}  // namespace
+
+int launch_kv_attention_rows(KvAttnArgs &a)
+{
+    return a.c.D == 128 ? launch<128>(a) : a.c.D == 64 ? launch<64>(a) : launch<32>(a);
+}
+
+}  // namespace ember

@@ -179,6 +179,16 @@ def test_long_sequence_and_splits():
     p.check_attention(normal(rng, 1, 2, 1, 32), True, start=[130])
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("T", [20, 70])
+def test_many_rows_and_splits(D, T):
+    """Many rows with their keys split over workgroups, sequences of very different lengths."""
+    rng = np.random.default_rng(D * T)
+    p = filled(rng, 3, 1, 64, D, 1700)
+    p.check_attention(normal(rng, 3, T, 2, D), True, start=[1700 - T, 600, 0], count=[T, T, 3])
+    p.check_attention(normal(rng, 3, T, 2, D), False, start=[1700 - T, 600, 0], count=[T, 5, T])
+
+
 def test_scores_of_all_sizes():
     """Scores from -300 to 300, growing along the keys (the maximum is raised often), and scale 0."""
     rng = np.random.default_rng(8)
