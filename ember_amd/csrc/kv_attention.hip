@@ -39,7 +39,7 @@ constexpr int kTile = 32;  // keys
 constexpr int kRows = 8;   // rows per workgroup
 constexpr int kPerCu = 3;  // workgroups that a CU holds at once
 constexpr int kLeast = 8;  // tiles of a piece: two for each wave
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 40;
 
 // Units that are cut: how many of their workgroups are done.  Zero between
 // calls: the last one, which all the others have added to, clears its unit's.

@@ -27,7 +27,6 @@ namespace ember {
 namespace {
 
 constexpr int kTile = 64;    // keys
-constexpr int kRows = 128;   // rows per workgroup
 constexpr int kPerCu = 2;    // workgroups that a CU holds at once
 constexpr int kLeast = 8;    // tiles of a piece
 
@@ -156,14 +155,17 @@ __device__ __forceinline__ float lower_part(float x)
     return x - __builtin_bit_cast(float, float_bits(x) & 0xffff0000u);
 }
 
-template <int D>
+// KW = 1: 128 rows, every wave takes all keys of a tile.  KW = 2: 64 rows, a wave
+// takes 32 keys of a tile, and pairs of waves join at the end.
+template <int D, int KW>
 __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(KvAttnArgs a)
 {
     constexpr int KS = D / 16, DB = D / 32;
+    constexpr int kRows = 32 * kWaves / KW;  // rows per workgroup
     __shared__ Lds<D> lds[2];
     __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l32 = lane & 31, half = lane >> 5;
+    const int l32 = lane & 31, half = lane >> 5, rows32 = wave / KW;
     const int units = a.c.heads * a.tiles;
     Plan plan;
     const Place pl = start_block(a, plan);
@@ -175,13 +177,13 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(
     const int len = length_of(a, sp);
 
     // This lane's row, and the first key that it does not see.
-    const int row = tile * kRows + wave * 32 + l32, t = row / a.group, g = row - t * a.group;
+    const int row = tile * kRows + rows32 * 32 + l32, t = row / a.group, g = row - t * a.group;
     const bool valid = t < sp.count;
     const int first_t = tile * kRows / a.group, last_t = min((tile * kRows + kRows - 1) / a.group, sp.count - 1);
     const int keys = first_t < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the workgroup's rows see
     const int limit = valid ? limit_of(a, sp, len, t) : keys;
     // All of the wave's rows see the keys before `sure`, none those from `seen` on.
-    const int wave_row = tile * kRows + wave * 32;
+    const int wave_row = tile * kRows + rows32 * 32;
     const int sure = min(keys, limit_of(a, sp, len, wave_row / a.group));
     const int seen = wave_row / a.group < sp.count ? min(keys, limit_of(a, sp, len, (wave_row + 31) / a.group)) : 0;
 
@@ -293,49 +295,69 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(
 #pragma unroll
                             for (int i = 0; i < 16; ++i) acc[d][i] = NAN;
             }
-            block(at, key0, std::integral_constant<int, 0>{});
-            if (key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
+            if (KW == 1 || wave % 2 == 0) block(at, key0, std::integral_constant<int, 0>{});
+            if ((KW == 1 || wave % 2 == 1) && key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
         }
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
 
-    if (pl.pieces > 1) {
-        constexpr int PART = kRows * (D + 2), SUMS = kRows * D;
-        float *mine = a.part + (int64_t)blockIdx.x * PART;
-        const int at = wave * 32 * D + 2 * lane;
+    auto take_in = [&](float m1, float l1, auto value) {  // another part of this wave's rows
+        const float to = fmaxf(m, m1), f = __builtin_amdgcn_exp2f(m - to), e = __builtin_amdgcn_exp2f(m1 - to);
+        m = to;
+        l = l * f + l1 * e;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float *to = mine + at + (8 * d + i) * 128;
-                put8(to, (uint64_t)float_bits(acc[d][2 * i + 1]) << 32 | float_bits(acc[d][2 * i]));
+                const f32x2 x = value(8 * d + i);
+                acc[d][2 * i] = acc[d][2 * i] * f + x[0] * e;
+                acc[d][2 * i + 1] = acc[d][2 * i + 1] * f + x[1] * e;
             }
-        if (half == 0) put2(mine + SUMS + 2 * (wave * 32 + l32), m, l);
+    };
+    if (KW == 2) {
+        // The tiles' LDS is free (a barrier ends the loop).
+        f32x2 *part = (f32x2 *)lds + rows32 * (16 * D + 64) + lane;
+        if (wave % 2 == 1) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[64 * (8 * d + i)] = f32x2{acc[d][2 * i], acc[d][2 * i + 1]};
+            part[16 * D] = f32x2{m, l};
+        }
+        __syncthreads();
+        if (wave % 2 == 0) {
+            const f32x2 st = part[16 * D];
+            take_in(st[0], st[1], [&](int i) { return part[64 * i]; });
+        }
+    }
+    const bool keeps = wave % KW == 0 && wave_row / a.group < a.T;  // has rows to write
+    if (pl.pieces > 1) {
+        constexpr int PART = kRows * (D + 2), SUMS = kRows * D;
+        float *mine = a.part + (int64_t)blockIdx.x * PART;
+        const int at = rows32 * 32 * D + 2 * lane;
+        if (keeps) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) put2(mine + at + (8 * d + i) * 128, acc[d][2 * i], acc[d][2 * i + 1]);
+            if (half == 0) put2(mine + SUMS + 2 * (rows32 * 32 + l32), m, l);
+        }
         wait_vmem();  // the stores have reached memory
         __syncthreads();
         if (threadIdx.x == 0) last = last_of(&g_done[b * units + unit], pl.pieces);
         __syncthreads();
-        if (!last) return;
+        if (!last || !keeps) return;
         const float *from = a.part + (int64_t)pl.first * PART;
         m = kNone, l = 0.0f;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
         for (int i = 0; i < pl.pieces; ++i, from += (int64_t)units * PART) {
-            const f32x2 st = get2(from + SUMS + 2 * (wave * 32 + l32));
-            const float to = fmaxf(m, st[0]), f = __builtin_amdgcn_exp2f(m - to), e = __builtin_amdgcn_exp2f(st[0] - to);
-            m = to;
-            l = l * f + st[1] * e;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const f32x2 x = get2(from + at + (8 * d + j) * 128);
-                    acc[d][2 * j] = acc[d][2 * j] * f + x[0] * e;
-                    acc[d][2 * j + 1] = acc[d][2 * j + 1] * f + x[1] * e;
-                }
+            const f32x2 st = get2(from + SUMS + 2 * (rows32 * 32 + l32));
+            take_in(st[0], st[1], [&](int i) { return get2(from + at + i * 128); });
         }
     }
+    if (!keeps) return;
     if (t >= a.T) return;
     const int head = h * a.group + g;
     const bool empty = !valid || l == 0.0f;
@@ -354,12 +376,12 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(
         a.lse[((int64_t)b * a.q_heads + head) * a.T + t] = empty ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <int D>
+template <int D, int KW>
 int launch(KvAttnArgs &a)
 {
-    const int st = cut_keys(a, kRows, kTile, kLeast, kPerCu);
+    const int st = cut_keys(a, 32 * kWaves / KW, kTile, kLeast, kPerCu);
     if (st) return st;
-    hipLaunchKernelGGL(kv_attention_rows_kernel<D>, dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
+    hipLaunchKernelGGL((kv_attention_rows_kernel<D, KW>), dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     return launch_ok("kv_attention_rows") ? EMBER_OK : EMBER_ERR_DEVICE;
 }
 
@@ -367,7 +389,10 @@ int launch(KvAttnArgs &a)
 
 int launch_kv_attention_rows(KvAttnArgs &a)
 {
-    return a.c.D == 128 ? launch<128>(a) : a.c.D == 64 ? launch<64>(a) : launch<32>(a);
+    const bool few = a.T * a.group <= 64;
+    if (a.c.D == 128) return few ? launch<128, 2>(a) : launch<128, 1>(a);
+    if (a.c.D == 64) return few ? launch<64, 2>(a) : launch<64, 1>(a);
+    return few ? launch<32, 2>(a) : launch<32, 1>(a);
 }
 
 }  // namespace ember
