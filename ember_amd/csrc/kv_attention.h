@@ -80,19 +80,6 @@ __device__ __forceinline__ unsigned fp4_bf16(unsigned w, float scale)
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, S));
 }
 
-// The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
-// head h, or -1.  b, h and pos are the same in all lanes, so the table is read
-// through the scalar cache.
-__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
-{
-    typedef const __attribute__((address_space(4))) int32_t *scalar;
-    const int place = pos >> c.page_shift;
-    if (place >= c.max_pages) return -1;
-    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + place];
-    if ((unsigned)page >= (unsigned)c.pages) return -1;
-    return (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
-}
-
 // The upper halves of three floats' parts: hi, mid and lo of x.
 __device__ __forceinline__ void cut3(float x, unsigned &hi, unsigned &mid, unsigned &lo)
 {

@@ -54,15 +54,17 @@ __device__ __forceinline__ Span span_of(const int32_t *start, const int32_t *cou
     return {start ? start[b] : 0, min(max(n, 0), T)};
 }
 
-// The slot of token `pos` (pos >= 0) in units of rows of one head, or -1 where
-// it has no page: rows of head h are at slot + h * page_size.
-__device__ __forceinline__ int64_t slot_of(const KvCache &c, int b, int pos)
+// The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
+// head h, or -1.  b, h and pos are the same in all lanes, so the table is read
+// through the scalar cache.
+__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
 {
+    typedef const __attribute__((address_space(4))) int32_t *scalar;
     const int place = pos >> c.page_shift;
     if (place >= c.max_pages) return -1;
-    const int page = c.table[(int64_t)b * c.max_pages + place];
+    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + place];
     if ((unsigned)page >= (unsigned)c.pages) return -1;
-    return (((int64_t)page * c.heads) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+    return (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
 }
 
 // The scale that a byte stands for.

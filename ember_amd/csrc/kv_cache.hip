@@ -9,9 +9,11 @@
 // integers the sizes of floats sort alike, infinities and NaNs above all), so
 // no NaN is lost in it.
 //
-// A lane holds 8 neighbours (two 16-byte loads, one 4-byte store of codes), so
-// a group is 4 lanes and a row of D = 128 is 16.  HBM-bound: 4 bytes read and
-// 17/32 written per element, and the other way round.
+// A wave takes 16 tokens of a sequence that are on one page (the table is read
+// once, through the scalar cache), of one head, keys or values.  A lane has 4
+// neighbours at a time, so that a wave reads and writes 1 KiB of floats in a row;
+// a group is 8 lanes, and its largest size found in register moves.  HBM-bound: 4
+// bytes read and 17/32 written per element, and the other way round.
 #include "kv_cache.h"
 
 namespace ember {
@@ -54,91 +56,126 @@ __device__ __forceinline__ unsigned size_bits(float x)
     return __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
 }
 
-// A lane's place in the call's rows: grid (blocks of rows, sequences, k or v).
-template <int D>
-struct Place {
-    static constexpr int LPR = D / 8;        // lanes per row
-    static constexpr int RPB = 256 / LPR;    // rows per workgroup
-    unsigned rows;
-    int lane;
-    __device__ __forceinline__ Place(const CopyArgs &a) : rows((unsigned)a.T * a.c.heads), lane(threadIdx.x % LPR) {}
+template <int CTRL>
+__device__ __forceinline__ unsigned max_with(unsigned x)
+{
+    return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, false));
+}
+// The largest of 8 neighbouring lanes.
+__device__ __forceinline__ unsigned max_of_8(unsigned x)
+{
+    x = max_with<0xB1>(x);    // the other of a pair
+    x = max_with<0x4E>(x);    // the other pair of 4
+    return max_with<0x141>(x);  // the other 4, mirrored
+}
+
+// What a wave does: 16 tokens from `pos` on (a multiple of 16) of a sequence.
+struct Task {
+    int b, h, which;  // sequence, head, keys (0) or values (1)
+    Span sp;
+    int64_t pos, at;  // the first token, and its row in the cache or -1
+    bool first;       // of its sequence
 };
 
-template <int D>
-__global__ __launch_bounds__(256) void kv_write_kernel(CopyArgs a)
+// Pieces of 16 tokens that T rows of a sequence may touch, wherever they start.
+__host__ __device__ inline unsigned pieces_of(int T)
 {
-    const Place<D> pl(a);
-    const int b = blockIdx.y;
-    const Span sp = span_of(a.start, a.count, b, a.T);
-    if (a.next && blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.next[b] = sp.start + sp.count;
-    const float *in = a.in[blockIdx.z];
-    uint8_t *codes = blockIdx.z ? a.c.v_codes : a.c.k_codes, *scales = blockIdx.z ? a.c.v_scales : a.c.k_scales;
-    for (unsigned row = blockIdx.x * pl.RPB + threadIdx.x / pl.LPR; row < pl.rows; row += gridDim.x * pl.RPB) {
-        const int t = (int)(row / (unsigned)a.c.heads), h = (int)(row - (unsigned)t * a.c.heads);
-        const int64_t pos = (int64_t)sp.start + t;
-        if (t >= sp.count || pos < 0) continue;
-        const int64_t slot = pos <= 0x7fffffff ? slot_of(a.c, b, (int)pos) : -1;
-        if (slot < 0) continue;
-        const f32x4 *src = (const f32x4 *)(in + b * a.st.sb + h * a.st.sh + t * a.st.ss + 8 * pl.lane);
-        const f32x4 x0 = src[0], x1 = src[1];
-        unsigned top = 0;
+    return ((unsigned)T + 30) >> 4;
+}
+
+// Task i of sequence blockIdx.y; neighbours are of neighbouring heads.
+__device__ __forceinline__ Task task_of(const CopyArgs &a, unsigned i)
+{
+    Task k;
+    k.b = blockIdx.y;
+    const unsigned heads = a.c.heads, pair = i / heads, piece = pair >> 1;
+    k.h = i - pair * heads;
+    k.which = pair & 1;
+    k.sp = span_of(a.start, a.count, k.b, a.T);
+    k.pos = ((int64_t)(k.sp.start >> 4) + piece) << 4;
+    k.at = k.pos >= 0 && k.pos <= 0x7fffffff ? row_of(a.c, k.b, k.h, (int)k.pos) : -1;
+    k.first = i == 0;
+    return k;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void kv_write_kernel(CopyArgs a, unsigned tasks)
+{
+    constexpr int LPR = D / 4, RPI = 64 / LPR, N = 16 / RPI;  // lanes of a row, rows at a time, times
+    const int lane = threadIdx.x & 63, col = lane % LPR;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (unsigned i = blockIdx.x * 4 + wave; i < tasks; i += gridDim.x * 4) {
+        const Task k = task_of(a, i);
+        if (a.next && k.first && lane == 0) a.next[k.b] = k.sp.start + k.sp.count;
+        if (k.at < 0) continue;
+        const float *in = a.in[k.which] + k.b * a.st.sb + k.h * a.st.sh + 4 * col;
+        uint8_t *codes = (k.which ? a.c.v_codes : a.c.k_codes) + k.at * (D / 2);
+        uint8_t *scales = (k.which ? a.c.v_scales : a.c.k_scales) + k.at * (D / 32);
+        f32x4 x[N];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            top = max(top, size_bits(x0[i]));
-            top = max(top, size_bits(x1[i]));
+        for (int j = 0; j < N; ++j) {
+            const int64_t t = k.pos - k.sp.start + RPI * j + lane / LPR;
+            x[j] = t >= 0 && t < k.sp.count ? *(const f32x4 *)(in + t * a.st.ss) : f32x4{0, 0, 0, 0};
         }
-        top = max(top, (unsigned)__shfl_xor((int)top, 1, 64));
-        top = max(top, (unsigned)__shfl_xor((int)top, 2, 64));
-        const bool held = top < 0x7f000000u;
-        unsigned byte = top ? max((int)((top + 0x3FFFFFu) >> 23) - 2, kLeastScale) : 127;
-        byte = held ? byte : 255;
-        const float scale = scale_of(byte);
-        unsigned w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x0[0], x0[1], scale, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x0[2], x0[3], scale, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x1[0], x1[1], scale, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x1[2], x1[3], scale, 3);
-        const int64_t at = slot + ((int64_t)h << a.c.page_shift);
-        *(unsigned *)(codes + at * (D / 2) + 4 * pl.lane) = held ? w : 0u;
-        if (pl.lane % 4 == 0) scales[at * (D / 32) + pl.lane / 4] = (uint8_t)byte;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int row = RPI * j + lane / LPR;
+            const int64_t t = k.pos - k.sp.start + row;
+            const unsigned top = max_of_8(max(max(size_bits(x[j][0]), size_bits(x[j][1])), max(size_bits(x[j][2]), size_bits(x[j][3]))));
+            const bool held = top < 0x7f000000u;
+            unsigned byte = top ? max((int)((top + 0x3FFFFFu) >> 23) - 2, kLeastScale) : 127;
+            byte = held ? byte : 255;
+            const float scale = scale_of(byte);
+            unsigned w = 0;
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[j][0], x[j][1], scale, 0);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[j][2], x[j][3], scale, 1);
+            if (t >= 0 && t < k.sp.count) {
+                *(uint16_t *)(codes + row * (D / 2) + 2 * col) = held ? (uint16_t)w : 0;
+                if (col % 8 == 0) scales[row * (D / 32) + col / 8] = (uint8_t)byte;
+            }
+        }
     }
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void kv_read_kernel(CopyArgs a)
+__global__ __launch_bounds__(256) void kv_read_kernel(CopyArgs a, unsigned tasks)
 {
-    const Place<D> pl(a);
-    const int b = blockIdx.y;
-    const Span sp = span_of(a.start, a.count, b, a.T);
-    float *out = a.out[blockIdx.z];
-    const uint8_t *codes = blockIdx.z ? a.c.v_codes : a.c.k_codes, *scales = blockIdx.z ? a.c.v_scales : a.c.k_scales;
-    for (unsigned row = blockIdx.x * pl.RPB + threadIdx.x / pl.LPR; row < pl.rows; row += gridDim.x * pl.RPB) {
-        const int t = (int)(row / (unsigned)a.c.heads), h = (int)(row - (unsigned)t * a.c.heads);
-        const int64_t pos = (int64_t)sp.start + t;
-        const int64_t slot = t < sp.count && pos >= 0 && pos <= 0x7fffffff ? slot_of(a.c, b, (int)pos) : -1;
-        f32x4 x0 = {0, 0, 0, 0}, x1 = x0;
-        if (slot >= 0) {
-            const int64_t at = slot + ((int64_t)h << a.c.page_shift);
-            const unsigned w = *(const unsigned *)(codes + at * (D / 2) + 4 * pl.lane);
-            const float scale = scale_of(scales[at * (D / 32) + pl.lane / 4]);
-            const f32x2 p0 = fp4_pair<0>(w, scale), p1 = fp4_pair<1>(w, scale);
-            const f32x2 p2 = fp4_pair<2>(w, scale), p3 = fp4_pair<3>(w, scale);
-            x0 = f32x4{p0[0], p0[1], p1[0], p1[1]};
-            x1 = f32x4{p2[0], p2[1], p3[0], p3[1]};
+    constexpr int LPR = D / 4, RPI = 64 / LPR, N = 16 / RPI;
+    const int lane = threadIdx.x & 63, col = lane % LPR;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (unsigned i = blockIdx.x * 4 + wave; i < tasks; i += gridDim.x * 4) {
+        const Task k = task_of(a, i);
+        float *out = a.out[k.which] + k.b * a.st.sb + k.h * a.st.sh + 4 * col;
+        const uint8_t *codes = (k.which ? a.c.v_codes : a.c.k_codes) + k.at * (D / 2);
+        const uint8_t *scales = (k.which ? a.c.v_scales : a.c.k_scales) + k.at * (D / 32);
+        unsigned w[N], byte[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int row = RPI * j + lane / LPR;
+            const int64_t t = k.pos - k.sp.start + row;
+            const bool there = k.at >= 0 && t >= 0 && t < k.sp.count;
+            w[j] = there ? *(const uint16_t *)(codes + row * (D / 2) + 2 * col) : 0;
+            byte[j] = there ? scales[row * (D / 32) + col / 8] : 127;
         }
-        f32x4 *dst = (f32x4 *)(out + b * a.st.sb + h * a.st.sh + t * a.st.ss + 8 * pl.lane);
-        dst[0] = x0;
-        dst[1] = x1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int64_t t = k.pos - k.sp.start + RPI * j + lane / LPR;
+            const f32x2 p0 = fp4_pair<0>(w[j], scale_of(byte[j])), p1 = fp4_pair<1>(w[j], scale_of(byte[j]));
+            if (t >= 0 && t < a.T) *(f32x4 *)(out + t * a.st.ss) = f32x4{p0[0], p0[1], p1[0], p1[1]};
+        }
     }
 }
 
-// Enough workgroups to fill the chip; each takes further rows in strides.
-template <int D>
+// Of a sequence; T * heads is below 2^31 - 2^16.
+unsigned tasks_of(const CopyArgs &a)
+{
+    return pieces_of(a.T) * a.c.heads * 2;
+}
+// Four tasks to a workgroup; beyond 2^18 of them, each takes further ones.
 dim3 copy_grid(const CopyArgs &a)
 {
-    const int64_t blocks = ((int64_t)a.T * a.c.heads + Place<D>::RPB - 1) / Place<D>::RPB;
-    const int64_t most = 8192 / (2 * a.c.sequences) + 1;
-    return dim3((unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), (unsigned)a.c.sequences, 2);
+    const unsigned n = tasks_of(a);
+    return dim3((n < (1 << 20) ? n + 3 : 1 << 20) / 4, a.c.sequences);
 }
 
 int check_copy(const ember_kv_cache *cache, const void *k, const void *v, int64_t T, int64_t sb, int64_t sh, int64_t ss,
@@ -167,9 +204,10 @@ extern "C" int kv_cache_write(const ember_kv_cache *cache, const float *k, const
     if (((uintptr_t)next & 3) || (next && next == start)) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_write");
     if (a.c.sequences == 0 || (T == 0 && !next)) return EMBER_OK;
     a.in[0] = k, a.in[1] = v, a.next = next;
-    if (a.c.D == 128) hipLaunchKernelGGL(kv_write_kernel<128>, copy_grid<128>(a), dim3(256), 0, 0, a);
-    else if (a.c.D == 64) hipLaunchKernelGGL(kv_write_kernel<64>, copy_grid<64>(a), dim3(256), 0, 0, a);
-    else hipLaunchKernelGGL(kv_write_kernel<32>, copy_grid<32>(a), dim3(256), 0, 0, a);
+    const unsigned n = tasks_of(a);
+    if (a.c.D == 128) hipLaunchKernelGGL(kv_write_kernel<128>, copy_grid(a), dim3(256), 0, 0, a, n);
+    else if (a.c.D == 64) hipLaunchKernelGGL(kv_write_kernel<64>, copy_grid(a), dim3(256), 0, 0, a, n);
+    else hipLaunchKernelGGL(kv_write_kernel<32>, copy_grid(a), dim3(256), 0, 0, a, n);
     return launch_ok("kv_cache_write") ? EMBER_OK : EMBER_ERR_DEVICE;
 }
 
@@ -182,8 +220,9 @@ extern "C" int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, in
     if (st) return st;
     if (a.c.sequences == 0 || T == 0) return EMBER_OK;
     a.out[0] = k, a.out[1] = v;
-    if (a.c.D == 128) hipLaunchKernelGGL(kv_read_kernel<128>, copy_grid<128>(a), dim3(256), 0, 0, a);
-    else if (a.c.D == 64) hipLaunchKernelGGL(kv_read_kernel<64>, copy_grid<64>(a), dim3(256), 0, 0, a);
-    else hipLaunchKernelGGL(kv_read_kernel<32>, copy_grid<32>(a), dim3(256), 0, 0, a);
+    const unsigned n = tasks_of(a);
+    if (a.c.D == 128) hipLaunchKernelGGL(kv_read_kernel<128>, copy_grid(a), dim3(256), 0, 0, a, n);
+    else if (a.c.D == 64) hipLaunchKernelGGL(kv_read_kernel<64>, copy_grid(a), dim3(256), 0, 0, a, n);
+    else hipLaunchKernelGGL(kv_read_kernel<32>, copy_grid(a), dim3(256), 0, 0, a, n);
     return launch_ok("kv_cache_read") ? EMBER_OK : EMBER_ERR_DEVICE;
 }
