@@ -137,7 +137,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(CopyArgs a, unsigned task
     }
 }
 
-template <int D>
+// STREAM: past the caches.
+template <int D, bool STREAM>
 __global__ __launch_bounds__(256) void kv_read_kernel(CopyArgs a, unsigned tasks)
 {
     constexpr int LPR = D / 4, RPI = 64 / LPR, N = 16 / RPI;
@@ -161,7 +162,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(CopyArgs a, unsigned tasks
         for (int j = 0; j < N; ++j) {
             const int64_t t = k.pos - k.sp.start + RPI * j + lane / LPR;
             const f32x2 p0 = fp4_pair<0>(w[j], scale_of(byte[j])), p1 = fp4_pair<1>(w[j], scale_of(byte[j]));
-            if (t >= 0 && t < a.T) *(f32x4 *)(out + t * a.st.ss) = f32x4{p0[0], p0[1], p1[0], p1[1]};
+            const f32x4 x = {p0[0], p0[1], p1[0], p1[1]};
+            if (t >= 0 && t < a.T) {
+                f32x4 *to = (f32x4 *)(out + t * a.st.ss);
+                if (STREAM) __builtin_nontemporal_store(x, to);
+                else *to = x;
+            }
         }
     }
 }
@@ -176,6 +182,20 @@ dim3 copy_grid(const CopyArgs &a)
 {
     const unsigned n = tasks_of(a);
     return dim3((n < (1 << 20) ? n + 3 : 1 << 20) / 4, a.c.sequences);
+}
+
+// What the card's last cache (256 MB) cannot hold is better written past it: 268
+// MB read back take 46 us so and 77 through it (with a kernel that reads it next,
+// 148 and 163); 134 MB 25 and 27 (60 and 57), 33 MB 8.6 and 10.9 (24.7 and 24.1).
+constexpr int64_t kStreamBytes = int64_t(192) << 20;
+
+template <int D>
+void launch_read(const CopyArgs &a, unsigned n)
+{
+    if ((int64_t)a.c.sequences * a.T * a.c.heads * D * 8 > kStreamBytes)
+        hipLaunchKernelGGL((kv_read_kernel<D, true>), copy_grid(a), dim3(256), 0, 0, a, n);
+    else
+        hipLaunchKernelGGL((kv_read_kernel<D, false>), copy_grid(a), dim3(256), 0, 0, a, n);
 }
 
 int check_copy(const ember_kv_cache *cache, const void *k, const void *v, int64_t T, int64_t sb, int64_t sh, int64_t ss,
@@ -221,8 +241,8 @@ extern "C" int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, in
     if (a.c.sequences == 0 || T == 0) return EMBER_OK;
     a.out[0] = k, a.out[1] = v;
     const unsigned n = tasks_of(a);
-    if (a.c.D == 128) hipLaunchKernelGGL(kv_read_kernel<128>, copy_grid(a), dim3(256), 0, 0, a, n);
-    else if (a.c.D == 64) hipLaunchKernelGGL(kv_read_kernel<64>, copy_grid(a), dim3(256), 0, 0, a, n);
-    else hipLaunchKernelGGL(kv_read_kernel<32>, copy_grid(a), dim3(256), 0, 0, a, n);
+    if (a.c.D == 128) launch_read<128>(a, n);
+    else if (a.c.D == 64) launch_read<64>(a, n);
+    else launch_read<32>(a, n);
     return launch_ok("kv_cache_read") ? EMBER_OK : EMBER_ERR_DEVICE;
 }

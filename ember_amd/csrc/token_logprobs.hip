@@ -12,7 +12,8 @@
 // A thread takes 16 logits at a time into registers, so that their maximum is
 // known before the sums, and the next 16 are on their way meanwhile; where rows
 // are few, a row is cut over workgroups, and the last of them to be done (by a
-// count that they add to) joins their sums.  HBM-bound: 4 bytes per logit.
+// count that they add to) joins their sums.  HBM-bound: 4 bytes per logit, read
+// past the caches (4096 x 32001: 88 us, 6.0 TB/s; through them 98).
 //
 // The `top` largest: floats are ordered as unsigned integers (all bits turned
 // over where the sign is set, else the sign alone), with the complement of the
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         const int64_t first = (int64_t)chunk * kChunk + 4 * (int)threadIdx.x;
         if ((int64_t)(chunk + 1) * kChunk <= a.classes) {
 #pragma unroll
-            for (int j = 0; j < kPerThread / 4; ++j) to[j] = *(const f4 *)(p + first + 4 * kThreads * j);
+            for (int j = 0; j < kPerThread / 4; ++j) to[j] = __builtin_nontemporal_load((const f4 *)(p + first + 4 * kThreads * j));
         } else {
 #pragma unroll
             for (int j = 0; j < kPerThread / 4; ++j)

@@ -75,6 +75,23 @@ def test_write_and_read_slots(B, T, H, D, page, start, count):
         np.testing.assert_array_equal(got, ref.astype(np.float32))
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_a_large_context_read_back(D):
+    """Over 192 MiB of values at once, as the same tokens read in parts."""
+    rng = np.random.default_rng(D)
+    H, T = 1024 // D, 25000
+    p = filled(rng, 1, H, 256, D, 600)
+    p.table = ints(np.tile(p.host.table, (1, 33)))   # the same tokens over and over
+    p.view.page_table, p.view.max_pages = p.table.ptr, 33 * p.host.table.shape[1]
+    p.host.table = np.tile(p.host.table, (1, 33))
+    k, v = p.read(T, count=[T - 7])
+    assert k.nbytes + v.nbytes > 192 << 20
+    for t0 in (0, 9000, 24500):
+        pk, pv = p.read(500, start=[t0], count=[min(500, T - 7 - t0)])
+        np.testing.assert_array_equal(k[:, t0:t0 + 500], pk)
+        np.testing.assert_array_equal(v[:, t0:t0 + 500], pv)
+
+
 @pytest.mark.parametrize("fault", [-1, 7, 2 ** 31 - 1, -2 ** 31])
 def test_pages_that_are_not_there(fault):
     """Tokens of a page outside the cache are dropped, read as zero and not seen."""
