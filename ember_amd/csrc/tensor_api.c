@@ -993,6 +993,221 @@ static PyObject *py_attention_bwd_packed(PyObject *module, PyObject *args)
     return (PyObject *)g;
 }
 
+/* ---- key/value cache and token log probabilities (no reference counterpart) ----
+ *
+ * A cache is the tuple (k_codes, k_scales, v_codes, v_scales, page_table, pages,
+ * heads, page_size, head_dim, sequences, max_pages), whose arrays are _Tensors
+ * that hold raw bytes (the table and all other integers: int32, a _Tensor element
+ * each). */
+
+typedef struct {
+    ember_kv_cache view;
+    Py_ssize_t rows; /* sequences */
+} CacheArg;
+
+static int parse_cache(PyObject *tuple, CacheArg *c)
+{
+    TensorObject *kc, *ks, *vc, *vs, *table;
+    long long pages, heads, page, D, B, places;
+    if (!PyTuple_Check(tuple)) {
+        PyErr_SetString(PyExc_TypeError, "cache must be a tuple");
+        return -1;
+    }
+    if (!PyArg_ParseTuple(tuple, "O!O!O!O!O!LLLLLL", &TensorType, &kc, &TensorType, &ks, &TensorType, &vc, &TensorType,
+                          &vs, &TensorType, &table, &pages, &heads, &page, &D, &B, &places))
+        return -1;
+    const long long most = 1LL << 31;
+    if (pages < 0 || heads < 1 || page < 1 || D < 32 || B < 0 || places < 0 || pages >= most || heads >= most || page >= most ||
+        D > 1024 || B >= most || places >= most || (double)pages * heads * page * D > 9e18 ||
+        (double)kc->size < (double)pages * heads * page * D / 8 || (double)vc->size < (double)pages * heads * page * D / 8 ||
+        (double)ks->size < (double)pages * heads * page * D / 128 || (double)vs->size < (double)pages * heads * page * D / 128 ||
+        (double)table->size < (double)B * places) {
+        PyErr_SetString(PyExc_ValueError, "cache arrays are smaller than its sizes say");
+        return -1;
+    }
+    c->view = (ember_kv_cache){kc->d_ptr, ks->d_ptr, vc->d_ptr, vs->d_ptr, (const int32_t *)table->d_ptr, pages, heads, page, D,
+                               B, places};
+    c->rows = (Py_ssize_t)B;
+    return 0;
+}
+
+/* Whether rows (B, T, heads, D) with these strides from element `at` on lie in t. */
+static int check_rows(TensorObject *t, long long at, long long B, long long T, long long H, long long D, long long sb,
+                      long long sh, long long ss, const char *name)
+{
+    const double end = (double)at + (double)(B - 1) * sb + (double)(T - 1) * ss + (double)(H - 1) * sh + D;
+    if (at < 0 || B < 0 || T < 0 || H < 1 || sb < 0 || sh < 0 || ss < 0 || (B > 0 && T > 0 && end > (double)t->size)) {
+        PyErr_Format(PyExc_ValueError, "%s does not hold the rows that its sizes and strides say", name);
+        return -1;
+    }
+    return 0;
+}
+
+static int check_ints(TensorObject *t, Py_ssize_t n, const char *name)
+{
+    if (t && t->size < n) {
+        PyErr_Format(PyExc_ValueError, "%s holds %zd elements, expected %zd", name, t->size, n);
+        return -1;
+    }
+    return 0;
+}
+
+/* _kv_cache_write(cache, k, k_at, v, v_at, T, sb, sh, ss, start, count|None, next): k and v from elements k_at and v_at on. */
+static PyObject *py_kv_cache_write(PyObject *module, PyObject *args)
+{
+    PyObject *co, *no;
+    TensorObject *k, *v, *start, *next;
+    long long k_at, v_at, T, sb, sh, ss;
+    CacheArg c;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "OO!LO!LLLLLO!OO!", &co, &TensorType, &k, &k_at, &TensorType, &v, &v_at, &T, &sb, &sh, &ss,
+                          &TensorType, &start, &no, &TensorType, &next) ||
+        parse_cache(co, &c))
+        return NULL;
+    TensorObject *count = opt_tensor(no, "count");
+    if (count == (TensorObject *)-1) return NULL;
+    if (check_rows(k, k_at, c.rows, T, c.view.heads, c.view.head_dim, sb, sh, ss, "k") ||
+        check_rows(v, v_at, c.rows, T, c.view.heads, c.view.head_dim, sb, sh, ss, "v") || check_ints(start, c.rows, "start") ||
+        check_ints(count, c.rows, "count") || check_ints(next, c.rows, "next"))
+        return NULL;
+    int st = kv_cache_write(&c.view, k->d_ptr + k_at, v->d_ptr + v_at, T, sb, sh, ss, (const int32_t *)start->d_ptr,
+                            count ? (const int32_t *)count->d_ptr : NULL, (int32_t *)next->d_ptr);
+    if (raise_status(st, "_kv_cache_write")) return NULL;
+    Py_RETURN_NONE;
+}
+
+/* _kv_cache_read(cache, T, start, count|None) -> (k, v), dense (sequences, T, heads, head_dim). */
+static PyObject *py_kv_cache_read(PyObject *module, PyObject *args)
+{
+    PyObject *co, *no;
+    TensorObject *start;
+    long long T;
+    CacheArg c;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "OLO!O", &co, &T, &TensorType, &start, &no) || parse_cache(co, &c)) return NULL;
+    TensorObject *count = opt_tensor(no, "count");
+    if (count == (TensorObject *)-1 || check_ints(start, c.rows, "start") || check_ints(count, c.rows, "count")) return NULL;
+    const int64_t H = c.view.heads, D = c.view.head_dim;
+    if (T < 0 || (double)T * c.rows * H * D > 9e18) {
+        PyErr_SetString(PyExc_ValueError, "_kv_cache_read: T out of range");
+        return NULL;
+    }
+    TensorObject *k = alloc_tensor((Py_ssize_t)(c.rows * T * H * D)), *v = NULL;
+    if (!k || !(v = alloc_tensor(k->size))) {
+        Py_XDECREF(k);
+        return NULL;
+    }
+    int st = kv_cache_read(&c.view, k->d_ptr, v->d_ptr, T, T * H * D, D, H * D, (const int32_t *)start->d_ptr,
+                           count ? (const int32_t *)count->d_ptr : NULL);
+    if (raise_status(st, "_kv_cache_read")) {
+        Py_DECREF(k);
+        Py_DECREF(v);
+        return NULL;
+    }
+    return Py_BuildValue("(NN)", (PyObject *)k, (PyObject *)v);
+}
+
+/* _kv_cache_attention(cache, q, q_at, T, q_heads, scale, causal, sb, sh, ss, start, count|None) -> (o, lse):
+ * o dense (sequences, T, q_heads, head_dim), lse (sequences, q_heads, T). */
+static PyObject *py_kv_cache_attention(PyObject *module, PyObject *args)
+{
+    PyObject *co, *no;
+    TensorObject *q, *start;
+    long long q_at, T, Hq, sb, sh, ss;
+    float scale;
+    int causal;
+    CacheArg c;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "OO!LLLfpLLLO!O", &co, &TensorType, &q, &q_at, &T, &Hq, &scale, &causal, &sb, &sh, &ss,
+                          &TensorType, &start, &no) ||
+        parse_cache(co, &c))
+        return NULL;
+    TensorObject *count = opt_tensor(no, "count");
+    const int64_t D = c.view.head_dim;
+    if (count == (TensorObject *)-1 || check_rows(q, q_at, c.rows, T, Hq, D, sb, sh, ss, "q") ||
+        check_ints(start, c.rows, "start") || check_ints(count, c.rows, "count"))
+        return NULL;
+    if ((double)c.rows * T * Hq * D > 9e18) {
+        PyErr_SetString(PyExc_ValueError, "_kv_cache_attention: sizes out of range");
+        return NULL;
+    }
+    TensorObject *o = alloc_tensor((Py_ssize_t)(c.rows * T * Hq * D)), *lse = NULL;
+    if (!o || !(lse = alloc_tensor((Py_ssize_t)(c.rows * Hq * T)))) {
+        Py_XDECREF(o);
+        return NULL;
+    }
+    int st = kv_cache_attention(&c.view, q->d_ptr + q_at, o->d_ptr, lse->d_ptr, T, Hq, scale, causal, sb, sh, ss, T * Hq * D, D,
+                                Hq * D, (const int32_t *)start->d_ptr, count ? (const int32_t *)count->d_ptr : NULL);
+    if (raise_status(st, "_kv_cache_attention")) {
+        Py_DECREF(o);
+        Py_DECREF(lse);
+        return NULL;
+    }
+    return Py_BuildValue("(NN)", (PyObject *)o, (PyObject *)lse);
+}
+
+static int check_logits(TensorObject *x, TensorObject *tokens, long long rows, long long classes, const char *what)
+{
+    if (rows < 0 || classes < 1 || (double)rows * classes != (double)x->size || tokens->size != rows) {
+        PyErr_Format(PyExc_ValueError, "%s: logits must hold rows * classes elements and tokens rows", what);
+        return -1;
+    }
+    return 0;
+}
+
+/* _token_logprobs(logits, tokens, rows, classes, top) -> (logp, lse, entropy, top_tokens|None, top_logp|None). */
+static PyObject *py_token_logprobs(PyObject *module, PyObject *args)
+{
+    TensorObject *x, *tokens, *out[5] = {NULL};
+    long long rows, classes;
+    int top;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!O!LLi", &TensorType, &x, &TensorType, &tokens, &rows, &classes, &top)) return NULL;
+    if (check_logits(x, tokens, rows, classes, "_token_logprobs")) return NULL;
+    if (top < 0 || top > 64 || top > classes) {
+        PyErr_SetString(PyExc_ValueError, "_token_logprobs: top must be from 0 to 64 and at most classes");
+        return NULL;
+    }
+    for (int i = 0; i < (top ? 5 : 3); i++)
+        if (!(out[i] = alloc_tensor((Py_ssize_t)(i < 3 ? rows : rows * top)))) goto failed;
+    int st = token_logprobs(x->d_ptr, classes, (const int32_t *)tokens->d_ptr, rows, classes, out[0]->d_ptr, out[1]->d_ptr,
+                            out[2]->d_ptr, top ? (int32_t *)out[3]->d_ptr : NULL, top ? out[4]->d_ptr : NULL, top);
+    if (raise_status(st, "_token_logprobs")) goto failed;
+    if (!top) return Py_BuildValue("(NNNOO)", out[0], out[1], out[2], Py_None, Py_None);
+    return Py_BuildValue("(NNNNN)", out[0], out[1], out[2], out[3], out[4]);
+failed:
+    for (int i = 0; i < 5; i++) Py_XDECREF(out[i]);
+    return NULL;
+}
+
+/* _token_logprobs_bwd(logits, tokens, lse, entropy, d_logp|None, d_entropy|None, rows, classes) -> d_logits. */
+static PyObject *py_token_logprobs_bwd(PyObject *module, PyObject *args)
+{
+    TensorObject *x, *tokens, *lse, *entropy;
+    PyObject *po, *eo;
+    long long rows, classes;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!O!O!O!OOLL", &TensorType, &x, &TensorType, &tokens, &TensorType, &lse, &TensorType, &entropy,
+                          &po, &eo, &rows, &classes))
+        return NULL;
+    TensorObject *dp = opt_tensor(po, "d_logp"), *de = opt_tensor(eo, "d_entropy");
+    if (dp == (TensorObject *)-1 || de == (TensorObject *)-1 || check_logits(x, tokens, rows, classes, "_token_logprobs_bwd"))
+        return NULL;
+    if (lse->size != rows || entropy->size != rows || (dp && dp->size != rows) || (de && de->size != rows)) {
+        PyErr_SetString(PyExc_ValueError, "_token_logprobs_bwd: lse, entropy and gradients must hold rows elements");
+        return NULL;
+    }
+    TensorObject *g = alloc_tensor(x->size);
+    if (!g) return NULL;
+    int st = token_logprobs_bwd(x->d_ptr, classes, (const int32_t *)tokens->d_ptr, lse->d_ptr, entropy->d_ptr,
+                                dp ? dp->d_ptr : NULL, de ? de->d_ptr : NULL, g->d_ptr, classes, rows, classes);
+    if (raise_status(st, "_token_logprobs_bwd")) {
+        Py_DECREF(g);
+        return NULL;
+    }
+    return (PyObject *)g;
+}
+
 /* Fused optimiser steps over lists of _Tensor of matching sizes, updated in
  * place with one launch per 48 tensors:
  *   _adam_step(params, grads, means, variances, lr, beta1, beta2, eps, t)
@@ -1155,6 +1370,11 @@ static PyMethodDef module_methods[] = {
     METHOD("_layernorm_bwd", py_layernorm_bwd, "LayerNorm backward -> (dx, dgamma, dbeta)"),
     METHOD("_attention_fwd_packed", py_attention_fwd_packed, "attention on packed (B,S,3,H,D) qkv"),
     METHOD("_attention_bwd_packed", py_attention_bwd_packed, "backward -> packed dqkv"),
+    METHOD("_kv_cache_write", py_kv_cache_write, "round rows into a 4-bit key/value cache"),
+    METHOD("_kv_cache_read", py_kv_cache_read, "values that a 4-bit cache holds -> (k, v)"),
+    METHOD("_kv_cache_attention", py_kv_cache_attention, "attention over a 4-bit cache -> (o, lse)"),
+    METHOD("_token_logprobs", py_token_logprobs, "log probabilities by token id -> (logp, lse, entropy, top_tokens, top_logp)"),
+    METHOD("_token_logprobs_bwd", py_token_logprobs_bwd, "gradient of log probabilities and entropy"),
     {"_synchronize", (PyCFunction)py_synchronize, METH_NOARGS, "wait for all queued device work"},
     {"_empty_cache", (PyCFunction)py_empty_cache, METH_NOARGS,
      "return the allocator's cached blocks on the current device to HIP"},

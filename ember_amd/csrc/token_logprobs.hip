@@ -401,6 +401,10 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_bwd_kernel(GradArgs a
     const int at = known ? (int)max(min(token - first, (int64_t)kGradSegment), (int64_t)-1) : -1;
     const float lse = a.lse[row], dp = known && a.d_logp ? a.d_logp[row] : 0.0f;
     const float dh = a.d_entropy ? a.d_entropy[row] : 0.0f, h = dh != 0.0f ? a.entropy[row] : 0.0f;
+    if (dp == 0.0f && dh == 0.0f) {  // a padded row: whatever it holds
+        for (int c = threadIdx.x; c < n; c += kThreads) q[c] = 0.0f;
+        return;
+    }
     auto grad = [&](float x, int c) {
         const float logp = x - lse, pr = expf(logp);
         // p ln p is 0 where p is.

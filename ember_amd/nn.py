@@ -16,10 +16,12 @@ from __future__ import annotations
 
 import math
 from abc import ABC, abstractmethod
+from collections.abc import Sequence
 from itertools import chain
 
 from ember_amd import _core as C
 from ember_amd import random as _random
+from ember_amd.kv_cache import KVCache
 from ember_amd.tensor import Tensor, attention_backward, attention_forward
 
 
@@ -380,7 +382,8 @@ class DecoderBlock(Layer):
         y = x2 + GELU(LN2(x2) W1 + b1) W2 + b2
     with causal fused attention reading the packed QKV projection in place.
     Weights Xavier-uniform, biases 0, LayerNorm gamma 1 / beta 0.  ``forward``
-    takes (x, B, S); ``backward`` returns dx and fills ``gradients()``."""
+    takes (x, B, S); ``backward`` returns dx and fills ``gradients()``.
+    ``decode`` runs new tokens against a 4-bit cache of the earlier ones."""
 
     def __init__(self, d_model: int, n_heads: int, mlp_ratio: int = 4, causal: bool = True):
         if d_model % n_heads:
@@ -453,3 +456,34 @@ class DecoderBlock(Layer):
         self._grads = [self.ln1.grad_gamma, self.ln1.grad_beta, g_wqkv, g_bqkv, g_wo, g_bo,
                        self.ln2.grad_gamma, self.ln2.grad_beta, g_w1, g_b1, g_w2, g_b2]
         return dx
+
+    def make_cache(self, sequences: int, tokens: int, page_size: int = 64, pages: int | None = None) -> KVCache:
+        """An empty cache for ``decode``: ``sequences`` of up to ``tokens`` tokens."""
+        return KVCache(sequences, self.h, self.d // self.h, tokens, page_size, pages)
+
+    def decode(self, x: Tensor, cache: KVCache, count: Sequence[int] | None = None) -> Tensor:
+        """The block on rows that follow what ``cache`` holds: x is (sequences *
+        T, d), T new tokens of each sequence (``count[b]`` of them where given,
+        padded behind), which are appended to the cache and attend to it.  Causal
+        blocks only; for inference: what ``backward`` needs stays as it was.
+        In rows past ``count`` the attention gives 0."""
+        if not self.causal:
+            raise ValueError("decode() needs a causal block")
+        rows, d = _rows(x)
+        if (cache.heads, cache.head_dim) != (self.h, self.d // self.h):
+            raise ValueError(f"the cache has {cache.heads} heads of {cache.head_dim}, the block {self.h} of {self.d // self.h}")
+        if d != self.d or rows % cache.sequences:
+            raise ValueError(f"x must be ({cache.sequences} * T, {self.d}), got {x.shape}")
+        T = rows // cache.sequences
+        if rows == 0:
+            return _random.zeros(x.shape)
+        norm = lambda x, ln: Tensor._from_core(  # noqa: E731
+            C._layernorm_fwd(x._core, ln.gamma._core, ln.beta._core, rows, d, ln.eps)[0], x.shape)
+        qkv, _ = linear(norm(x, self.ln1), self.w_qkv, self.b_qkv)
+        D, strides = cache.head_dim, (T * 3 * d, self.d // self.h, 3 * d)
+        cache._append(qkv._core, d, qkv._core, 2 * d, T, strides, count)
+        o, _ = cache._attend(qkv._core, 0, T, self.h, strides, True, float(1.0 / math.sqrt(D)))
+        x2, _ = linear(Tensor._from_core(o, (rows, d)), self.w_o, self.b_o, residual=x)
+        a, _ = linear(norm(x2, self.ln2), self.w_1, self.b_1, gelu=True)
+        y, _ = linear(a, self.w_2, self.b_2, residual=x2)
+        return y

@@ -427,7 +427,8 @@ int token_logprobs(const float *logits, int64_t row_stride, const int32_t *token
  * d_entropy is),
  *   d_logits[r][j] = d_logp * ([j == tokens[r]] - p_j)
  *                    - d_entropy * p_j * (ln p_j + entropy),
- * d_logp taken as 0 where tokens[r] is out of range; row r at d_logits +
+ * d_logp taken as 0 where tokens[r] is out of range, and a row with both
+ * gradients 0 gets zeros whatever its logits hold; row r at d_logits +
  * r*out_stride.  d_logits may be logits itself (with the same stride); it
  * must not overlap it otherwise. */
 int token_logprobs_bwd(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,

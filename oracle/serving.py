@@ -13,7 +13,7 @@ GROUP = 32
 def quantise(x):
     """Codes (..., D/2) and scale bytes (..., D/32), uint8, of float32 x (..., D)."""
     x = np.asarray(x, np.float32)
-    g = x.reshape(*x.shape[:-1], -1, GROUP).astype(np.float64)
+    g = x.reshape(*x.shape[:-1], x.shape[-1] // GROUP, GROUP).astype(np.float64)
     amax = np.abs(g).max(-1)
     held = amax < 2.0 ** 127  # false for NaN
     safe = np.where(held & (amax > 0), amax, 6.0)
@@ -30,7 +30,7 @@ def quantise(x):
 
 def values(codes, scales):
     """float64 (..., D) that codes and scale bytes stand for."""
-    n = np.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], -1)
+    n = np.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], 2 * codes.shape[-1])
     size = E2M1[n & 7] * np.where(n & 8, -1.0, 1.0)
     scale = np.where(scales == 255, np.nan, 2.0 ** (scales.astype(np.float64) - 127))
     return size * np.repeat(scale, GROUP, -1)
