@@ -9,19 +9,23 @@
 //
 // Products run on v_mfma_f32_16x16x32_bf16.  A cached value is a bf16 number,
 // so only the fp32 operand is split (x = hi + mid + lo, 8 bits each, by cutting
-// off: exact for all that is not denormal) and a product is three instructions
-// where two fp32 operands take six.  Operands come straight from the cache:
-//   S^T (16 keys x 16 columns) = K . Q^T.  Lane l holds key l % 16 and, of its
-//     row, the D/4 elements from (l / 16) * D/4 on: one load of D/8 bytes and one
-//     scale, 8 codes to an instruction.  Which 8 elements of D that are is free, as
-//     long as Q's operand has the same.
-//   O^T += V^T . P^T.  Lane l of S^T holds column l % 16 and keys 4*(l/16) .. +3.
-//     P is used from those registers, so V's operand has to hold these four
-//     tokens too, and for each of them a code conversion gives two neighbouring
-//     elements of D.  They are taken as two contraction elements, (token, even)
-//     and (token, odd), and P^T has a column for each: p or 0 for the even one, 0
-//     or p for the odd one.  So a wave has 8 rows in 16 columns, and no value of V
-//     is moved between lanes or within a register.
+// off: exact for all that is not denormal), and with few rows the parts are rows
+// and columns of one instruction.  K and V come straight from the cache:
+//   S (16 x 16 keys) = Q . K^T.  Row 4*a + i of Q's operand is part i of row a
+//     (i = 3: nothing), so that lane l has the parts' products of row l / 16 and
+//     key l % 16 in its registers, and adds them.  Of K, lane l holds key l % 16
+//     and the D/4 elements of its row from (l / 16) * D/4 on: one load of D/8 bytes
+//     and one scale, 8 codes to an operand.  Which 8 elements of D that are is
+//     free, as long as Q's operand has the same.  Each lane has one score of 16
+//     keys (of 32 with two rows, where the two tiles' are shared out).
+//   O^T (D x 16) += V^T . P^T.  P's parts go through LDS (3 halves to a score) to
+//     lanes that hold a column and 4 tokens, 4*(l/16) .. +3.  For each token a code
+//     conversion gives two neighbouring elements of D; they are taken as two
+//     contraction elements, (token, even) and (token, odd), and P^T has a column
+//     for each: p or 0 for the even one, 0 or p for the odd one.  So no value of V
+//     is moved between lanes or within a register.  A column is (row, even or odd,
+//     part): two rows of three parts, four rows of two with the third part in a
+//     second instruction, or eight rows with an instruction a part.
 // A workgroup is 4 waves that take turns at tiles of 32 keys and join at the
 // end.  A unit's keys are cut into pieces, each with a workgroup of its own; the
 // last of them to be done (by a count that they all add to) joins the pieces, in
@@ -36,8 +40,11 @@ namespace ember {
 namespace {
 
 constexpr int kTile = 32;  // keys
-constexpr int kRows = 8;   // rows per workgroup
-constexpr int kPerCu = 3;  // workgroups that a CU holds at once
+// Workgroups that a CU holds at once: by their registers.
+constexpr int per_cu(int D, int rows)
+{
+    return D == 128 && rows == 8 ? 3 : 4;
+}
 constexpr int kLeast = 8;  // tiles of a piece: two for each wave
 constexpr int kFewRows = 40;
 
@@ -104,56 +111,84 @@ struct Values {
     }
 };
 
-template <int D>
-__global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAttnArgs a)
+// ROWS (2, 4 or 8) rows to a workgroup.
+template <int D, int ROWS>
+__global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_kernel(KvAttnArgs a)
 {
     constexpr int KS = D / 32;  // contraction steps of S, and pairs of elements of a lane of O
     constexpr int STR = D + 4;
-    __shared__ float slab[kWaves][kRows * STR];
-    __shared__ float stat[kWaves][kRows][2];
+    constexpr int SETS = ROWS == 8 ? 2 : 1;     // of 4 rows of S
+    constexpr int SC = ROWS == 2 ? 1 : 2;       // scores of a lane in a tile, of each set
+    constexpr int SLOTS = 8 / ROWS;             // columns of O for a row's parts
+    constexpr int OPS = ROWS == 2 ? 1 : ROWS == 4 ? 2 : 3;
+    __shared__ float slab[kWaves][ROWS * STR];
+    __shared__ float stat[kWaves][ROWS][2];
+    __shared__ uint16_t parts[kWaves][3][ROWS][kTile];
     __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, r = lane >> 4, row8 = col >> 1;
-    const bool odd = col & 1;
+    const int col = lane & 15, r = lane >> 4;
     const int units = a.c.heads * a.tiles;
     Plan plan;
     const Place pl = start_block(a, plan);
     if (pl.b < 0) return;
     const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
-    const int h = unit / a.tiles, tile = unit - h * a.tiles;
+    const int h = unit / a.tiles, row0 = (unit - h * a.tiles) * ROWS;
     const Span sp = span_of(a.start, a.count, b, a.T);
     const int len = length_of(a, sp);
 
-    // This lane's row, and the first key that it does not see.
-    const int row = tile * kRows + row8, t = row / a.group, g = row - t * a.group;
-    const bool valid = t < sp.count;
-    const int last_t = min((tile * kRows + kRows - 1) / a.group, sp.count - 1);
-    const int keys = tile * kRows / a.group < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the workgroup's rows see
-    const int limit = valid ? limit_of(a, sp, len, t) : keys;
-    const int sure = keys ? limit_of(a, sp, len, tile * kRows / a.group) : 0;  // every row sees the keys before
+    const int last_t = min((row0 + ROWS - 1) / a.group, sp.count - 1);
+    const int keys = row0 / a.group < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the rows see
+    const int sure = keys ? limit_of(a, sp, len, row0 / a.group) : 0;  // every row sees the keys before
+    auto row_limit = [&](int row) {  // the first key that a row does not see
+        const int t = (row0 + row) / a.group;
+        return t < sp.count ? limit_of(a, sp, len, t) : keys;
+    };
+    // This lane's rows and keys of S, and its row, half and parts of O.
+    const int s_row = ROWS == 2 ? r & 1 : r, s_key = ROWS == 2 ? 16 * (r >> 1) + col : col;
+    const int o_row = col / (2 * SLOTS), slot = col % SLOTS;
+    const bool odd = col / SLOTS & 1;
+    int s_limit[SETS];
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) s_limit[i] = row_limit(s_row + 4 * i);
+    const int o_limit = row_limit(o_row);
 
-    u32x4 q[KS][3];
-    {
+    u32x4 q[SETS][KS];
+#pragma unroll
+    for (int set = 0; set < SETS; ++set) {
+        const int row = row0 + 4 * set + (ROWS == 2 ? col >> 2 & 1 : col >> 2), t = row / a.group, g = row - t * a.group, part = col & 3;
         const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + r * (D / 4);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x2 x = valid ? *(const f32x2 *)(src + 8 * s + 2 * i) : f32x2{0, 0};
+                const f32x2 x = t < sp.count && part < 3 ? *(const f32x2 *)(src + 8 * s + 2 * i) : f32x2{0, 0};
                 unsigned p0[3], p1[3];
                 cut3(x[0], p0[0], p0[1], p0[2]);
                 cut3(x[1], p1[0], p1[1], p1[2]);
-#pragma unroll
-                for (int j = 0; j < 3; ++j) q[s][j][i] = (p0[j] >> 16) | p1[j];
+                const unsigned x0 = part == 0 ? p0[0] : part == 1 ? p0[1] : p0[2], x1 = part == 0 ? p1[0] : part == 1 ? p1[1] : p1[2];
+                q[set][s][i] = (x0 >> 16) | x1;
             }
     }
 
     f32x4 acc[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) acc[s] = f32x4{0, 0, 0, 0};
-    float m = kNone, l = 0.0f;
-    const unsigned half = odd ? 0x03020c0cu : 0x0c0c0302u;  // a float's upper half as the upper or the lower of two
-    const unsigned turn = 8 * (col * D / 512) + 9;          // the byte of the lane's group of 32 to bits 23 .. 30
+    float m[SETS], l[SETS];
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) m[i] = kNone, l[i] = 0.0f;
+    // Where a half goes in a pair (or nowhere: the part that a column has none of).
+    constexpr unsigned kZero = 0x0c0c0c0cu;
+    unsigned low[OPS], high[OPS];
+    int from[OPS];  // the column's part, row and tokens in `parts`
+#pragma unroll
+    for (int i = 0; i < OPS; ++i) {
+        const bool none = ROWS == 2 ? slot == 3 : ROWS == 4 ? i == 1 && slot == 1 : false;
+        low[i] = none ? kZero : odd ? 0x01000c0cu : 0x0c0c0100u;
+        high[i] = none ? kZero : odd ? 0x03020c0cu : 0x0c0c0302u;
+        const int part = ROWS == 2 ? min(slot, 2) : ROWS == 4 ? (i == 1 ? 2 : slot) : i;
+        from[i] = (part * ROWS + o_row) * kTile + 4 * r;
+    }
+    const unsigned turn = 8 * (col * D / 512) + 9;  // the byte of the lane's group of 32 to bits 23 .. 30
 
     const int n = (keys + kTile - 1) / kTile;
     const int end = pl.piece + 1 < pl.pieces ? min(n, (pl.piece + 1) * plan.per) : n;
@@ -164,21 +199,24 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
     // One tile; the next one's keys are loaded as soon as this one's are used,
     // and its values after this one's.
     auto step = [&](auto more) {
-        float s[2][4];
+        float s[SETS][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f32x4 sum = {0, 0, 0, 0};
+            f32x4 sum[SETS];
+#pragma unroll
+            for (int set = 0; set < SETS; ++set) sum[set] = f32x4{0, 0, 0, 0};
             const float scale = scale_of(kk[j].scale);
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
                 const unsigned w = kk[j].code.w[x];
                 const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
 #pragma unroll
-                for (int part = 2; part >= 0; --part) sum = mfma_16x16x32(k, q[x][part], sum);
+                for (int set = 0; set < SETS; ++set) sum[set] = mfma_16x16x32(q[set][x], k, sum[set]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[j][i] = sum[i];
+            for (int set = 0; set < SETS; ++set) s[set][j] = (sum[set][2] + sum[set][1]) + sum[set][0];
         }
+        if (ROWS == 2) s[0][0] = r >> 1 ? s[0][1] : s[0][0];
         if constexpr (more.value) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) kk[j].load(a.c, ahead[j], lane);
@@ -186,39 +224,65 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
         const bool partly = tl * kTile + kTile > sure || at[0] < 0 || at[1] < 0;
         if (partly) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int set = 0; set < SETS; ++set)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (tl * kTile + 16 * j + 4 * r + i >= limit || at[j] < 0) s[j][i] = -INFINITY;
+                for (int j = 0; j < SC; ++j) {
+                    const bool gone = ROWS == 2 ? (r >> 1 ? at[1] : at[0]) < 0 : at[j] < 0;
+                    if (tl * kTile + 16 * j + s_key >= s_limit[set] || gone) s[set][j] = -INFINITY;
+                }
         }
-        float top = s[0][0];
+        float top[SETS];
+        bool raise = false;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int set = 0; set < SETS; ++set) {
+            top[set] = (SC == 1 ? s[set][0] : fmaxf(s[set][0], s[set][1])) * a.scale2;
+            raise |= top[set] > m[set] + kRaise;
+        }
+        if (__any(raise)) {
+            float f[SETS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
-        top *= a.scale2;
-        if (__any(top > m + kRaise)) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= f;
+            for (int set = 0; set < SETS; ++set) {
+                float t = top[set];
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
+                if (ROWS == 2) t = fmaxf(t, __shfl_xor(t, 32, 64));
+                const float to = fmaxf(m[set], t);
+                f[set] = __builtin_amdgcn_exp2f(m[set] - to);
+                m[set] = to;
+                l[set] *= f[set];
+            }
+            float g = __shfl(f[0], 16 * (o_row & 3), 64);
+            if (SETS == 2) {
+                const float g1 = __shfl(f[SETS - 1], 16 * (o_row & 3), 64);
+                g = o_row >> 2 ? g1 : g;
+            }
 #pragma unroll
             for (int x = 0; x < KS; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[x][i] *= f;
+                for (int i = 0; i < 4; ++i) acc[x][i] *= g;
         }
-        auto values = [&](auto J) {
-            constexpr int j = decltype(J)::value;
-            u32x4 p[3];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[j][i], a.scale2, -m));
-                l += e;
+        for (int set = 0; set < SETS; ++set)
+#pragma unroll
+            for (int j = 0; j < SC; ++j) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[set][j], a.scale2, -m[set]));
+                l[set] += e;
                 unsigned hi, mid, lo;
                 cut3(e, hi, mid, lo);
-                p[0][i] = __builtin_amdgcn_perm(0, hi, half), p[1][i] = __builtin_amdgcn_perm(0, mid, half);
-                p[2][i] = __builtin_amdgcn_perm(0, lo, half);
+                const int row = s_row + 4 * set, key = 16 * j + s_key;
+                parts[wave][0][row][key] = (uint16_t)(hi >> 16);
+                parts[wave][1][row][key] = (uint16_t)(mid >> 16);
+                parts[wave][2][row][key] = (uint16_t)(lo >> 16);
+            }
+        wave_sync();
+        auto values = [&](auto J) {
+            constexpr int j = decltype(J)::value;
+            u32x4 p[OPS];
+#pragma unroll
+            for (int i = 0; i < OPS; ++i) {
+                const uint2 w = *(const uint2 *)(&parts[wave][0][0][0] + from[i] + 16 * j);
+                p[i] = u32x4{__builtin_amdgcn_perm(0, w.x, low[i]), __builtin_amdgcn_perm(0, w.x, high[i]),
+                             __builtin_amdgcn_perm(0, w.y, low[i]), __builtin_amdgcn_perm(0, w.y, high[i])};
             }
             // The scale's byte turned to where a float has its exponent: no
             // other bit of it counts.
@@ -238,7 +302,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
                 if (__any(spoilt[0] || spoilt[1] || spoilt[2] || spoilt[3])) {
                     bool mine = false;
                     for (int x = 0; x < 16; ++x)
-                        mine |= at[j] >= 0 && tl * kTile + 16 * j + x < limit &&
+                        mine |= at[j] >= 0 && tl * kTile + 16 * j + x < o_limit &&
                                 a.c.v_scales[(at[j] + x) * (D / 32) + r * D / 128] > kMostScale;
 #pragma unroll
                     for (int x = 0; x < KS; ++x)
@@ -264,12 +328,13 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
                 convert(std::integral_constant<int, 3>{});
             }
 #pragma unroll
-            for (int part = 2; part >= 0; --part)  // the small parts first
+            for (int i = OPS - 1; i >= 0; --i)  // the small parts first
 #pragma unroll
-                for (int x = 0; x < KS; ++x) acc[x] = mfma_16x16x32(v[x], p[part], acc[x]);
+                for (int x = 0; x < KS; ++x) acc[x] = mfma_16x16x32(v[x], p[i], acc[x]);
         };
         values(std::integral_constant<int, 0>{});
         values(std::integral_constant<int, 1>{});
+        wave_sync();
         if constexpr (more.value) {
             tl += kWaves;
 #pragma unroll
@@ -291,18 +356,27 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
         while (tl + kWaves < end) step(std::true_type{});
         step(std::false_type{});
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int set = 0; set < SETS; ++set) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) l[set] += __shfl_xor(l[set], o, 64);
+        if (ROWS == 2) l[set] += __shfl_xor(l[set], 32, 64);
+        if (col == 0 && (ROWS != 2 || r < 2)) stat[wave][s_row + 4 * set][0] = m[set], stat[wave][s_row + 4 * set][1] = l[set];
+    }
 
-    // Join the waves.
-    if (!odd && r == 0) stat[wave][row8][0] = m, stat[wave][row8][1] = l;
+    // Join the parts, and the waves.
 #pragma unroll
     for (int x = 0; x < KS; ++x)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) slab[wave][row8 * STR + (4 * r + i) * (D / 16) + 2 * x + odd] = acc[x][i];
+        for (int i = 0; i < 4; ++i) {
+            float o = acc[x][i];
+#pragma unroll
+            for (int k = 1; k < SLOTS; k <<= 1) o += __shfl_xor(o, k, 64);
+            if (slot == 0) slab[wave][o_row * STR + (4 * r + i) * (D / 16) + 2 * x + odd] = o;
+        }
     __syncthreads();
     const int rw = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-    const bool works = rw < kRows;
+    const bool works = rw < ROWS;
     float top = kNone, sum = 0.0f;
     f32x4 o = {0, 0, 0, 0};
     if (works) {
@@ -316,12 +390,12 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
         }
     }
     if (pl.pieces > 1) {
-        constexpr int PART = kRows * (D + 2);
+        constexpr int PART = ROWS * (D + 2);
         if (works) {
             float *mine = a.part + (int64_t)blockIdx.x * PART;
             put2(mine + rw * D + d, o[0], o[1]);
             put2(mine + rw * D + d + 2, o[2], o[3]);
-            if (d == 0) put2(mine + kRows * D + 2 * rw, top, sum);
+            if (d == 0) put2(mine + ROWS * D + 2 * rw, top, sum);
         }
         wait_vmem();  // the stores have reached memory
         __syncthreads();
@@ -338,7 +412,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
                     const float *one = from + min(i + j, pl.pieces - 1) * step;
-                    st[j] = get2(one + kRows * D + 2 * rw), o0[j] = get2(one + rw * D + d), o1[j] = get2(one + rw * D + d + 2);
+                    st[j] = get2(one + ROWS * D + 2 * rw), o0[j] = get2(one + rw * D + d), o1[j] = get2(one + rw * D + d + 2);
                 }
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
@@ -352,7 +426,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
         }
     }
     if (works) {
-        const int row = tile * kRows + rw, t = row / a.group, head = h * a.group + row - t * a.group;
+        const int row = row0 + rw, t = row / a.group, head = h * a.group + row - t * a.group;
         if (t >= a.T) return;
         const bool empty = t >= sp.count || sum == 0.0f;
         *(f32x4 *)(a.o + b * a.os.sb + head * a.os.sh + t * a.os.ss + d) = empty ? f32x4{0, 0, 0, 0} : o / sum;
@@ -361,13 +435,20 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_kernel(KvAtt
     }
 }
 
-template <int D>
+template <int D, int ROWS>
 int launch(KvAttnArgs &a)
 {
-    const int st = cut_keys(a, kRows, kTile, kLeast, kPerCu);
+    const int st = cut_keys(a, ROWS, kTile, kLeast, per_cu(D, ROWS));
     if (st) return st;
-    hipLaunchKernelGGL(kv_attention_kernel<D>, dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
+    hipLaunchKernelGGL((kv_attention_kernel<D, ROWS>), dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     return launch_ok("kv_attention") ? EMBER_OK : EMBER_ERR_DEVICE;
+}
+
+template <int D>
+int launch_rows(KvAttnArgs &a)
+{
+    const int rows = a.T * a.group;
+    return rows <= 2 ? launch<D, 2>(a) : rows <= 4 ? launch<D, 4>(a) : launch<D, 8>(a);
 }
 
 }  // namespace
@@ -417,5 +498,5 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     // gives scores that differ by nothing.
     a.scale2 = std::max(scale * kLog2e, 1e-37f);
     if (T * a.group > kFewRows) return launch_kv_attention_rows(a);
-    return a.c.D == 128 ? launch<128>(a) : a.c.D == 64 ? launch<64>(a) : launch<32>(a);
+    return a.c.D == 128 ? launch_rows<128>(a) : a.c.D == 64 ? launch_rows<64>(a) : launch_rows<32>(a);
 }

@@ -102,13 +102,6 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane)
            (unsigned)__builtin_amdgcn_readlane((int)(unsigned)k, lane);
 }
 
-// What the lanes of a wave have written to LDS is there for all of them.
-__device__ __forceinline__ void wave_sync()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Appends the lanes' keys above `last` to `found`, which has c; returns how many
 // there are then (those past kFound are not kept).
 constexpr int kFound = 128;

@@ -46,6 +46,13 @@ __device__ __forceinline__ float wave_max(float v)
     return wave_all(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// What the lanes of a wave have written to LDS is there for all of them.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Stores and loads at device scope pass the L2s by: the workgroups of a launch
 // are on XCDs with an L2 each.  What a workgroup has put is there for others once
 // its waves have waited for their stores (wait_vmem) and met at a barrier; a
