@@ -111,6 +111,14 @@ struct Values {
     }
 };
 
+// The value of another lane of four: the other of a pair (0xB1), or of the other
+// pair (0x4E).
+template <int CTRL>
+__device__ __forceinline__ float quad(float x)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+
 // ROWS (2, 4 or 8) rows to a workgroup.
 template <int D, int ROWS>
 __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_kernel(KvAttnArgs a)
@@ -371,7 +379,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         for (int i = 0; i < 4; ++i) {
             float o = acc[x][i];
 #pragma unroll
-            for (int k = 1; k < SLOTS; k <<= 1) o += __shfl_xor(o, k, 64);
+            for (int k = 1; k < SLOTS; k <<= 1) o += k == 1 ? quad<0xB1>(o) : quad<0x4E>(o);
             if (slot == 0) slab[wave][o_row * STR + (4 * r + i) * (D / 16) + 2 * x + odd] = o;
         }
     __syncthreads();
