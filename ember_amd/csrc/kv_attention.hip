@@ -9,23 +9,30 @@
 //
 // Products run on v_mfma_f32_16x16x32_bf16.  A cached value is a bf16 number,
 // so only the fp32 operand is split (x = hi + mid + lo, 8 bits each, by cutting
-// off: exact for all that is not denormal), and with few rows the parts are rows
-// and columns of one instruction.  K and V come straight from the cache:
-//   S (16 x 16 keys) = Q . K^T.  Row 4*a + i of Q's operand is part i of row a
-//     (i = 3: nothing), so that lane l has the parts' products of row l / 16 and
-//     key l % 16 in its registers, and adds them.  Of K, lane l holds key l % 16
-//     and the D/4 elements of its row from (l / 16) * D/4 on: one load of D/8 bytes
-//     and one scale, 8 codes to an operand.  Which 8 elements of D that are is
-//     free, as long as Q's operand has the same.  Each lane has one score of 16
-//     keys (of 32 with two rows, where the two tiles' are shared out).
-//   O^T (D x 16) += V^T . P^T.  P's parts go through LDS (3 halves to a score) to
-//     lanes that hold a column and 4 tokens, 4*(l/16) .. +3.  For each token a code
-//     conversion gives two neighbouring elements of D; they are taken as two
-//     contraction elements, (token, even) and (token, odd), and P^T has a column
-//     for each: p or 0 for the even one, 0 or p for the odd one.  So no value of V
-//     is moved between lanes or within a register.  A column is (row, even or odd,
-//     part): two rows of three parts, four rows of two with the third part in a
-//     second instruction, or eight rows with an instruction a part.
+// off: exact for all that is not denormal).  K and V come straight from the cache:
+//   K's operand: lane l holds key l % 16 and the D/4 elements of its row from
+//     (l / 16) * D/4 on: one load of D/8 bytes and one scale, 8 codes to an operand.
+//     Which 8 elements of D that are is free, as long as Q's operand has the same.
+//   O^T (D x 16) += V^T . P^T.  Of V, lane l holds tokens 4*(l/16) .. +3 of 16.  For
+//     each a code conversion gives two neighbouring elements of D; they are taken
+//     as two contraction elements, (token, even) and (token, odd), and P^T has a
+//     column for each: p or 0 for the even one, 0 or p for the odd one.  So no
+//     value of V is moved between lanes or within a register.
+// Eight rows to a workgroup: S^T (16 keys x 16 columns) = K . Q^T, a column for a row's
+//   even elements and one for its odd ones, and three instructions for a product.
+//   Lane l has column l % 16 and keys 4*(l/16) .. +3, which is what P^T needs: P
+//   stays in registers.
+// Two or four rows: the parts share an instruction.  S (16 x 16 keys) = Q . K^T, and
+//   row 4*a + i of Q's operand is part i of row a (i = 3: nothing), so that lane l
+//   has the parts' products of row l / 16 and key l % 16, and adds them: one score
+//   for 16 keys (for 32 with two rows, where the two tiles' are shared out), where
+//   eight rows' lanes have four each.  P's parts go through LDS to the lanes of
+//   their columns: (row, even or odd, part), three parts of two rows, or two of
+//   four rows with the third in a second instruction.  A tile of 32 keys takes 16 to
+//   24 matrix instructions in place of 48.
+// Measured (us), eight-row scheme and these: 32 sequences of up to 8192, one token of
+// 32 / 8 heads of 128: 41.1 and 37.8; 32 x 2048, 16 heads of 64: 19.7 and 17.2.  With
+// eight rows through LDS: 32 x 16 heads of 64, 24 rows over 2048 46.4 and 50.4.
 // A workgroup is 4 waves that take turns at tiles of 32 keys and join at the
 // end.  A unit's keys are cut into pieces, each with a workgroup of its own; the
 // last of them to be done (by a count that they all add to) joins the pieces, in
@@ -125,13 +132,13 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
 {
     constexpr int KS = D / 32;  // contraction steps of S, and pairs of elements of a lane of O
     constexpr int STR = D + 4;
-    constexpr int SETS = ROWS == 8 ? 2 : 1;     // of 4 rows of S
-    constexpr int SC = ROWS == 2 ? 1 : 2;       // scores of a lane in a tile, of each set
+    constexpr bool SHARED = ROWS < 8;           // the parts share an instruction
+    constexpr int SC = ROWS == 2 ? 1 : ROWS == 4 ? 2 : 8;  // scores of a lane in a tile
     constexpr int SLOTS = 8 / ROWS;             // columns of O for a row's parts
     constexpr int OPS = ROWS == 2 ? 1 : ROWS == 4 ? 2 : 3;
     __shared__ float slab[kWaves][ROWS * STR];
     __shared__ float stat[kWaves][ROWS][2];
-    __shared__ uint16_t parts[kWaves][3][ROWS][kTile];
+    __shared__ uint16_t parts[SHARED ? kWaves : 1][3][ROWS][kTile];
     __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, r = lane >> 4;
@@ -151,19 +158,19 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         const int t = (row0 + row) / a.group;
         return t < sp.count ? limit_of(a, sp, len, t) : keys;
     };
-    // This lane's rows and keys of S, and its row, half and parts of O.
-    const int s_row = ROWS == 2 ? r & 1 : r, s_key = ROWS == 2 ? 16 * (r >> 1) + col : col;
+    // This lane's row, half and parts of O, and its row and keys of S: score x is
+    // of key s_key(x) of the tile.
     const int o_row = col / (2 * SLOTS), slot = col % SLOTS;
     const bool odd = col / SLOTS & 1;
-    int s_limit[SETS];
-#pragma unroll
-    for (int i = 0; i < SETS; ++i) s_limit[i] = row_limit(s_row + 4 * i);
-    const int o_limit = row_limit(o_row);
+    const int s_row = ROWS == 2 ? r & 1 : ROWS == 4 ? r : o_row;
+    auto s_key = [&](int x) { return ROWS == 2 ? 16 * (r >> 1) + col : ROWS == 4 ? 16 * x + col : 16 * (x >> 2) + 4 * r + (x & 3); };
+    const int s_limit = row_limit(s_row), o_limit = row_limit(o_row);
 
-    u32x4 q[SETS][KS];
-#pragma unroll
-    for (int set = 0; set < SETS; ++set) {
-        const int row = row0 + 4 * set + (ROWS == 2 ? col >> 2 & 1 : col >> 2), t = row / a.group, g = row - t * a.group, part = col & 3;
+    // SHARED: the operand's row is (row, part), and a lane has one of the parts.
+    u32x4 q[SHARED ? 1 : 3][KS];
+    {
+        const int row = row0 + (ROWS == 2 ? col >> 2 & 1 : ROWS == 4 ? col >> 2 : o_row), t = row / a.group, g = row - t * a.group;
+        const int part = SHARED ? col & 3 : 0;
         const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + r * (D / 4);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
@@ -173,27 +180,30 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
                 unsigned p0[3], p1[3];
                 cut3(x[0], p0[0], p0[1], p0[2]);
                 cut3(x[1], p1[0], p1[1], p1[2]);
-                const unsigned x0 = part == 0 ? p0[0] : part == 1 ? p0[1] : p0[2], x1 = part == 0 ? p1[0] : part == 1 ? p1[1] : p1[2];
-                q[set][s][i] = (x0 >> 16) | x1;
+                if (SHARED) {
+                    p0[0] = part == 0 ? p0[0] : part == 1 ? p0[1] : p0[2];
+                    p1[0] = part == 0 ? p1[0] : part == 1 ? p1[1] : p1[2];
+                }
+#pragma unroll
+                for (int j = 0; j < (SHARED ? 1 : 3); ++j) q[j][s][i] = (p0[j] >> 16) | p1[j];
             }
     }
 
     f32x4 acc[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) acc[s] = f32x4{0, 0, 0, 0};
-    float m[SETS], l[SETS];
+    float m = kNone, l = 0.0f;
+    // Where a half goes in a pair, by v_perm; nowhere for the part that a column
+    // has none of.
+    const unsigned low_half = odd ? 0x01000c0cu : 0x0c0c0100u, high_half = odd ? 0x03020c0cu : 0x0c0c0302u;
+    unsigned low[2], high[2];
+    int from[2];  // the column's part, row and tokens in `parts`
 #pragma unroll
-    for (int i = 0; i < SETS; ++i) m[i] = kNone, l[i] = 0.0f;
-    // Where a half goes in a pair (or nowhere: the part that a column has none of).
-    constexpr unsigned kZero = 0x0c0c0c0cu;
-    unsigned low[OPS], high[OPS];
-    int from[OPS];  // the column's part, row and tokens in `parts`
-#pragma unroll
-    for (int i = 0; i < OPS; ++i) {
-        const bool none = ROWS == 2 ? slot == 3 : ROWS == 4 ? i == 1 && slot == 1 : false;
-        low[i] = none ? kZero : odd ? 0x01000c0cu : 0x0c0c0100u;
-        high[i] = none ? kZero : odd ? 0x03020c0cu : 0x0c0c0302u;
-        const int part = ROWS == 2 ? min(slot, 2) : ROWS == 4 ? (i == 1 ? 2 : slot) : i;
+    for (int i = 0; i < 2; ++i) {
+        const bool none = ROWS == 2 ? slot == 3 : i == 1 && slot == 1;
+        low[i] = none ? 0x0c0c0c0cu : low_half;
+        high[i] = none ? 0x0c0c0c0cu : high_half;
+        const int part = ROWS == 2 ? min(slot, 2) : i == 1 ? 2 : slot;
         from[i] = (part * ROWS + o_row) * kTile + 4 * r;
     }
     const unsigned turn = 8 * (col * D / 512) + 9;  // the byte of the lane's group of 32 to bits 23 .. 30
@@ -207,24 +217,30 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
     // One tile; the next one's keys are loaded as soon as this one's are used,
     // and its values after this one's.
     auto step = [&](auto more) {
-        float s[SETS][2];
+        float s[8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f32x4 sum[SETS];
-#pragma unroll
-            for (int set = 0; set < SETS; ++set) sum[set] = f32x4{0, 0, 0, 0};
+            f32x4 sum = {0, 0, 0, 0};
             const float scale = scale_of(kk[j].scale);
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
                 const unsigned w = kk[j].code.w[x];
                 const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
+                if constexpr (SHARED) {
+                    sum = mfma_16x16x32(q[0][x], k, sum);
+                } else {
 #pragma unroll
-                for (int set = 0; set < SETS; ++set) sum[set] = mfma_16x16x32(q[set][x], k, sum[set]);
+                    for (int part = 2; part >= 0; --part) sum = mfma_16x16x32(k, q[part][x], sum);
+                }
             }
+            if constexpr (SHARED) {
+                s[j] = (sum[2] + sum[1]) + sum[0];
+            } else {
 #pragma unroll
-            for (int set = 0; set < SETS; ++set) s[set][j] = (sum[set][2] + sum[set][1]) + sum[set][0];
+                for (int i = 0; i < 4; ++i) s[4 * j + i] = sum[i];
+            }
         }
-        if (ROWS == 2) s[0][0] = r >> 1 ? s[0][1] : s[0][0];
+        if (ROWS == 2) s[0] = r >> 1 ? s[1] : s[0];
         if constexpr (more.value) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) kk[j].load(a.c, ahead[j], lane);
@@ -232,65 +248,58 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         const bool partly = tl * kTile + kTile > sure || at[0] < 0 || at[1] < 0;
         if (partly) {
 #pragma unroll
-            for (int set = 0; set < SETS; ++set)
-#pragma unroll
-                for (int j = 0; j < SC; ++j) {
-                    const bool gone = ROWS == 2 ? (r >> 1 ? at[1] : at[0]) < 0 : at[j] < 0;
-                    if (tl * kTile + 16 * j + s_key >= s_limit[set] || gone) s[set][j] = -INFINITY;
-                }
+            for (int x = 0; x < SC; ++x)
+                if (tl * kTile + s_key(x) >= s_limit || (s_key(x) < 16 ? at[0] : at[1]) < 0) s[x] = -INFINITY;
         }
-        float top[SETS];
-        bool raise = false;
+        float top = s[0];
 #pragma unroll
-        for (int set = 0; set < SETS; ++set) {
-            top[set] = (SC == 1 ? s[set][0] : fmaxf(s[set][0], s[set][1])) * a.scale2;
-            raise |= top[set] > m[set] + kRaise;
-        }
-        if (__any(raise)) {
-            float f[SETS];
+        for (int x = 1; x < SC; ++x) top = fmaxf(top, s[x]);
+        top *= a.scale2;
+        if (__any(top > m + kRaise)) {
+            // The lanes of a row: 16 neighbours (and as many 32 on), or those 16 apart.
+            if (SHARED) {
 #pragma unroll
-            for (int set = 0; set < SETS; ++set) {
-                float t = top[set];
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
-                if (ROWS == 2) t = fmaxf(t, __shfl_xor(t, 32, 64));
-                const float to = fmaxf(m[set], t);
-                f[set] = __builtin_amdgcn_exp2f(m[set] - to);
-                m[set] = to;
-                l[set] *= f[set];
+                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            } else {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
             }
-            float g = __shfl(f[0], 16 * (o_row & 3), 64);
-            if (SETS == 2) {
-                const float g1 = __shfl(f[SETS - 1], 16 * (o_row & 3), 64);
-                g = o_row >> 2 ? g1 : g;
-            }
+            if (ROWS != 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float to = fmaxf(m, top);
+            float f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
+            if (SHARED) f = __shfl(f, 16 * o_row, 64);
 #pragma unroll
             for (int x = 0; x < KS; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[x][i] *= g;
+                for (int i = 0; i < 4; ++i) acc[x][i] *= f;
         }
+        unsigned cut[SC][3];
 #pragma unroll
-        for (int set = 0; set < SETS; ++set)
+        for (int x = 0; x < SC; ++x) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale2, -m));
+            l += e;
+            cut3(e, cut[x][0], cut[x][1], cut[x][2]);
+            if (SHARED)
 #pragma unroll
-            for (int j = 0; j < SC; ++j) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[set][j], a.scale2, -m[set]));
-                l[set] += e;
-                unsigned hi, mid, lo;
-                cut3(e, hi, mid, lo);
-                const int row = s_row + 4 * set, key = 16 * j + s_key;
-                parts[wave][0][row][key] = (uint16_t)(hi >> 16);
-                parts[wave][1][row][key] = (uint16_t)(mid >> 16);
-                parts[wave][2][row][key] = (uint16_t)(lo >> 16);
-            }
-        wave_sync();
+                for (int part = 0; part < 3; ++part) parts[wave][part][s_row][s_key(x)] = (uint16_t)(cut[x][part] >> 16);
+        }
+        if (SHARED) wave_sync();
         auto values = [&](auto J) {
             constexpr int j = decltype(J)::value;
             u32x4 p[OPS];
+            if constexpr (SHARED) {
 #pragma unroll
-            for (int i = 0; i < OPS; ++i) {
-                const uint2 w = *(const uint2 *)(&parts[wave][0][0][0] + from[i] + 16 * j);
-                p[i] = u32x4{__builtin_amdgcn_perm(0, w.x, low[i]), __builtin_amdgcn_perm(0, w.x, high[i]),
-                             __builtin_amdgcn_perm(0, w.y, low[i]), __builtin_amdgcn_perm(0, w.y, high[i])};
+                for (int i = 0; i < OPS; ++i) {
+                    const uint2 w = *(const uint2 *)(&parts[wave][0][0][0] + from[i] + 16 * j);
+                    p[i] = u32x4{__builtin_amdgcn_perm(0, w.x, low[i]), __builtin_amdgcn_perm(0, w.x, high[i]),
+                                 __builtin_amdgcn_perm(0, w.y, low[i]), __builtin_amdgcn_perm(0, w.y, high[i])};
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < OPS; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) p[i][x] = __builtin_amdgcn_perm(0, cut[4 * j + x][i], high_half);
             }
             // The scale's byte turned to where a float has its exponent: no
             // other bit of it counts.
@@ -342,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         };
         values(std::integral_constant<int, 0>{});
         values(std::integral_constant<int, 1>{});
-        wave_sync();
+        if (SHARED) wave_sync();
         if constexpr (more.value) {
             tl += kWaves;
 #pragma unroll
@@ -364,13 +373,14 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         while (tl + kWaves < end) step(std::true_type{});
         step(std::false_type{});
     }
+    if (SHARED) {
 #pragma unroll
-    for (int set = 0; set < SETS; ++set) {
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) l[set] += __shfl_xor(l[set], o, 64);
-        if (ROWS == 2) l[set] += __shfl_xor(l[set], 32, 64);
-        if (col == 0 && (ROWS != 2 || r < 2)) stat[wave][s_row + 4 * set][0] = m[set], stat[wave][s_row + 4 * set][1] = l[set];
+        for (int o = 8; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    } else {
+        l += __shfl_xor(l, 16, 64);
     }
+    if (ROWS != 4) l += __shfl_xor(l, 32, 64);
+    if (SHARED ? col == 0 && r < ROWS : !odd && r == 0) stat[wave][s_row][0] = m, stat[wave][s_row][1] = l;
 
     // Join the parts, and the waves.
 #pragma unroll
