@@ -46,25 +46,36 @@ __device__ __forceinline__ int length_of(const KvAttnArgs &a, Span sp)
 // a join is worth.
 struct Plan {
     int per;
+    // Of sequence `lane`, of the first 64: its rows, length and tiles.
+    Span sp;
+    int len, tiles;
     __device__ __forceinline__ int pieces(int tiles) const { return max((tiles + per - 1) / per, 1); }
 };
 
-__device__ __forceinline__ int tiles_of(const KvAttnArgs &a, int b)
+__device__ __forceinline__ int tiles_of(const KvAttnArgs &a, int len)
 {
-    return b < a.c.sequences ? (length_of(a, span_of(a.start, a.count, b, a.T)) + a.keys - 1) / a.keys : 0;
+    return (len + a.keys - 1) / a.keys;
+}
+__device__ __forceinline__ int tiles_of_sequence(const KvAttnArgs &a, int b)
+{
+    return b < a.c.sequences ? tiles_of(a, length_of(a, span_of(a.start, a.count, b, a.T))) : 0;
 }
 
 __device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
 {
     const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles, most = a.blocks / units;
-    const int mine = tiles_of(a, lane);
+    Plan p;
+    p.sp = span_of(a.start, a.count, min(lane, a.c.sequences - 1), a.T);
+    p.len = length_of(a, p.sp);
+    p.tiles = tiles_of(a, p.len);
     auto sum = [&](auto f) {
-        auto n = wave_sum(lane < a.c.sequences ? f(mine) : decltype(f(0))(0));
-        for (int b = 64; b < a.c.sequences; b += 64) n += wave_sum(b + lane < a.c.sequences ? f(tiles_of(a, b + lane)) : decltype(f(0))(0));
+        auto n = wave_sum(lane < a.c.sequences ? f(p.tiles) : decltype(f(0))(0));
+        for (int b = 64; b < a.c.sequences; b += 64)
+            n += wave_sum(b + lane < a.c.sequences ? f(tiles_of_sequence(a, b + lane)) : decltype(f(0))(0));
         return n;
     };
     // The sum of all tiles may pass 32 bits; as a float it is near enough.
-    Plan p = {max((int)(sum([](int n) { return (float)n; }) / most), a.least)};
+    p.per = max((int)(sum([](int n) { return (float)n; }) / most), a.least);
     while (sum([&](int n) { return p.pieces(n); }) > most) p.per += p.per / 8 + 1;
     return p;
 }
@@ -90,30 +101,44 @@ __device__ __forceinline__ void cut3(float x, unsigned &hi, unsigned &mid, unsig
     lo = float_bits(x) & 0xffff0000u;
 }
 
-// Where a workgroup stands: its unit, its piece of the unit's keys, and the
-// unit's first workgroup (its further ones follow `units` apart).
+// Where a workgroup stands: its sequence's rows and length, its unit, its piece of
+// the unit's keys, and the unit's first workgroup (its further ones follow
+// `units` apart).  The same in all lanes.
 struct Place {
     int b, unit, piece, pieces, first;
+    Span sp;
+    int len;
 };
 
 // The place of workgroup `block`; b = -1 where the plan needs fewer.
-__device__ __forceinline__ Place place_of(const KvAttnArgs &a, Plan p, int block)
+__device__ __forceinline__ Place place_of(const KvAttnArgs &a, const Plan &p, int block)
 {
     const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles;
     int before = 0;
     for (int b0 = 0; b0 < a.c.sequences; b0 += 64) {
-        const int n = b0 + lane < a.c.sequences ? p.pieces(tiles_of(a, b0 + lane)) : 0;
+        const int tiles = b0 ? tiles_of_sequence(a, b0 + lane) : p.tiles;
+        const int n = b0 + lane < a.c.sequences ? p.pieces(tiles) : 0;
         const int upto = wave_scan_sum(n);
         const int at = __popcll(__ballot(block >= before + upto * units));  // sequences that end before
         if (at < 64) {
-            const int pieces = __builtin_amdgcn_readlane(n, at);
-            const int from = before + (__builtin_amdgcn_readlane(upto, at) - pieces) * units;
-            const int piece = (block - from) / units, unit = block - from - piece * units;
-            return {b0 + at, unit, piece, pieces, from + unit};
+            Place pl;
+            pl.b = b0 + at;
+            pl.pieces = __builtin_amdgcn_readlane(n, at);
+            const int from = before + (__builtin_amdgcn_readlane(upto, at) - pl.pieces) * units;
+            pl.piece = (block - from) / units, pl.unit = block - from - pl.piece * units;
+            pl.first = from + pl.unit;
+            if (b0) {
+                pl.sp = span_of(a.start, a.count, pl.b, a.T);
+                pl.len = length_of(a, pl.sp);
+            } else {
+                pl.sp = {__builtin_amdgcn_readlane(p.sp.start, at), __builtin_amdgcn_readlane(p.sp.count, at)};
+                pl.len = __builtin_amdgcn_readlane(p.len, at);
+            }
+            return pl;
         }
         before += __builtin_amdgcn_readlane(upto, 63) * units;
     }
-    return {-1, 0, 0, 0, 0};
+    return {-1, 0, 0, 0, 0, {0, 0}, 0};
 }
 
 __device__ __forceinline__ void put2(float *p, float x, float y)
@@ -136,13 +161,14 @@ __device__ __forceinline__ int limit_of(const KvAttnArgs &a, Span sp, int len, i
 __device__ __forceinline__ Place start_block(const KvAttnArgs &a, Plan &plan)
 {
     const int units = a.c.heads * a.tiles;
-    plan = {0x40000000};
     if (a.part) {
         plan = make_plan(a);
         return place_of(a, plan, blockIdx.x);
     }
+    plan.per = 0x40000000;
     const int b = blockIdx.x / units;
-    return {b, (int)blockIdx.x - b * units, 0, 1, 0};
+    const Span sp = span_of(a.start, a.count, b, a.T);
+    return {b, (int)blockIdx.x - b * units, 0, 1, 0, sp, length_of(a, sp)};
 }
 
 // Attention for many rows (kv_attention_rows.hip).

@@ -148,8 +148,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
     if (pl.b < 0) return;
     const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
     const int h = unit / a.tiles, row0 = (unit - h * a.tiles) * ROWS;
-    const Span sp = span_of(a.start, a.count, b, a.T);
-    const int len = length_of(a, sp);
+    const Span sp = pl.sp;
+    const int len = pl.len;
 
     const int last_t = min((row0 + ROWS - 1) / a.group, sp.count - 1);
     const int keys = row0 / a.group < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the rows see

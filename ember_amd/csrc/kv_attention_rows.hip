@@ -173,8 +173,8 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(
     const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
     // The last rows see most keys: they start first.
     const int h = unit / a.tiles, tile = a.tiles - 1 - (unit - h * a.tiles);
-    const Span sp = span_of(a.start, a.count, b, a.T);
-    const int len = length_of(a, sp);
+    const Span sp = pl.sp;
+    const int len = pl.len;
 
     // This lane's row, and the first key that it does not see.
     const int row = tile * kRows + rows32 * 32 + l32, t = row / a.group, g = row - t * a.group;
