@@ -19,6 +19,18 @@ constexpr int kWaves = 4;        // of a workgroup
 constexpr int kMostPlan = 1024;  // sequences that are planned for; with more, a unit is not cut
 constexpr int kMostUnits = 1 << 14;  // that are cut
 
+// Division by a number that the host knows: with inv = floor(2^32 / d) the
+// product's upper half is the quotient or one below it, for every n below 2^32.
+struct Divisor {
+    unsigned d, inv;
+    Divisor(unsigned d = 1) : d(d), inv(d > 1 ? (unsigned)((uint64_t(1) << 32) / d) : 0xffffffffu) {}
+    __device__ __forceinline__ int of(int n) const
+    {
+        const unsigned q = __umulhi((unsigned)n, inv);
+        return (int)(q + ((unsigned)n - q * d >= d));
+    }
+};
+
 struct KvAttnArgs {
     KvCache c;
     const float *q;
@@ -27,8 +39,9 @@ struct KvAttnArgs {
     const int32_t *start, *count;
     float *part;  // of each workgroup: O (rows, D), then m and l of each row; null: units are not cut
     int T, q_heads, group, tiles, blocks, causal;  // tiles: of rows, of a head
-    int keys, least;  // keys of a tile, tiles of a piece at least
+    int key_shift, least;  // of the keys of a tile, tiles of a piece at least
     float scale2;  // scale * log2(e), above 0
+    Divisor by_group, by_tiles, by_units;  // units: of a sequence
 };
 
 // Tokens that a sequence has after the call, as far as its table has room.
@@ -54,7 +67,7 @@ struct Plan {
 
 __device__ __forceinline__ int tiles_of(const KvAttnArgs &a, int len)
 {
-    return (len + a.keys - 1) / a.keys;
+    return (len + (1 << a.key_shift) - 1) >> a.key_shift;
 }
 __device__ __forceinline__ int tiles_of_sequence(const KvAttnArgs &a, int b)
 {
@@ -63,7 +76,7 @@ __device__ __forceinline__ int tiles_of_sequence(const KvAttnArgs &a, int b)
 
 __device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
 {
-    const int lane = threadIdx.x & 63, units = a.c.heads * a.tiles, most = a.blocks / units;
+    const int lane = threadIdx.x & 63, most = a.by_units.of(a.blocks);
     Plan p;
     p.sp = span_of(a.start, a.count, min(lane, a.c.sequences - 1), a.T);
     p.len = length_of(a, p.sp);
@@ -125,7 +138,7 @@ __device__ __forceinline__ Place place_of(const KvAttnArgs &a, const Plan &p, in
             pl.b = b0 + at;
             pl.pieces = __builtin_amdgcn_readlane(n, at);
             const int from = before + (__builtin_amdgcn_readlane(upto, at) - pl.pieces) * units;
-            pl.piece = (block - from) / units, pl.unit = block - from - pl.piece * units;
+            pl.piece = a.by_units.of(block - from), pl.unit = block - from - pl.piece * units;
             pl.first = from + pl.unit;
             if (b0) {
                 pl.sp = span_of(a.start, a.count, pl.b, a.T);
@@ -166,7 +179,7 @@ __device__ __forceinline__ Place start_block(const KvAttnArgs &a, Plan &plan)
         return place_of(a, plan, blockIdx.x);
     }
     plan.per = 0x40000000;
-    const int b = blockIdx.x / units;
+    const int b = a.by_units.of(blockIdx.x);
     const Span sp = span_of(a.start, a.count, b, a.T);
     return {b, (int)blockIdx.x - b * units, 0, 1, 0, sp, length_of(a, sp)};
 }

@@ -147,15 +147,15 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
     const Place pl = start_block(a, plan);
     if (pl.b < 0) return;
     const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
-    const int h = unit / a.tiles, row0 = (unit - h * a.tiles) * ROWS;
+    const int h = a.by_tiles.of(unit), row0 = (unit - h * a.tiles) * ROWS;
     const Span sp = pl.sp;
     const int len = pl.len;
 
-    const int last_t = min((row0 + ROWS - 1) / a.group, sp.count - 1);
-    const int keys = row0 / a.group < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the rows see
-    const int sure = keys ? limit_of(a, sp, len, row0 / a.group) : 0;  // every row sees the keys before
+    const int last_t = min(a.by_group.of(row0 + ROWS - 1), sp.count - 1);
+    const int keys = a.by_group.of(row0) < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the rows see
+    const int sure = keys ? limit_of(a, sp, len, a.by_group.of(row0)) : 0;  // every row sees the keys before
     auto row_limit = [&](int row) {  // the first key that a row does not see
-        const int t = (row0 + row) / a.group;
+        const int t = a.by_group.of(row0 + row);
         return t < sp.count ? limit_of(a, sp, len, t) : keys;
     };
     // This lane's row, half and parts of O, and its row and keys of S: score x is
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
     // SHARED: the operand's row is (row, part), and a lane has one of the parts.
     u32x4 q[SHARED ? 1 : 3][KS];
     {
-        const int row = row0 + (ROWS == 2 ? col >> 2 & 1 : ROWS == 4 ? col >> 2 : o_row), t = row / a.group, g = row - t * a.group;
+        const int row = row0 + (ROWS == 2 ? col >> 2 & 1 : ROWS == 4 ? col >> 2 : o_row), t = a.by_group.of(row), g = row - t * a.group;
         const int part = SHARED ? col & 3 : 0;
         const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + r * (D / 4);
 #pragma unroll
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         }
     }
     if (works) {
-        const int row = row0 + rw, t = row / a.group, head = h * a.group + row - t * a.group;
+        const int row = row0 + rw, t = a.by_group.of(row), head = h * a.group + row - t * a.group;
         if (t >= a.T) return;
         const bool empty = t >= sp.count || sum == 0.0f;
         *(f32x4 *)(a.o + b * a.os.sb + head * a.os.sh + t * a.os.ss + d) = empty ? f32x4{0, 0, 0, 0} : o / sum;
@@ -474,9 +474,10 @@ int launch_rows(KvAttnArgs &a)
 int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
 {
     a.tiles = (int)(((int64_t)a.T * a.group + rows - 1) / rows);
-    a.keys = keys, a.least = least;
+    a.key_shift = __builtin_ctz(keys), a.least = least;
     const int64_t all = (int64_t)a.c.sequences * a.c.heads * a.tiles;  // units
     if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
+    a.by_group = Divisor(a.group), a.by_tiles = Divisor(a.tiles), a.by_units = Divisor(a.c.heads * a.tiles);
     // One round of workgroups over the chip; where the units alone are about as
     // many, two pieces each, so that the longest sequence does not decide.  With
     // many units none is cut.

@@ -172,20 +172,20 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(
     if (pl.b < 0) return;
     const int b = __builtin_amdgcn_readfirstlane(pl.b), unit = __builtin_amdgcn_readfirstlane(pl.unit);
     // The last rows see most keys: they start first.
-    const int h = unit / a.tiles, tile = a.tiles - 1 - (unit - h * a.tiles);
+    const int h = a.by_tiles.of(unit), tile = a.tiles - 1 - (unit - h * a.tiles);
     const Span sp = pl.sp;
     const int len = pl.len;
 
     // This lane's row, and the first key that it does not see.
-    const int row = tile * kRows + rows32 * 32 + l32, t = row / a.group, g = row - t * a.group;
+    const int row = tile * kRows + rows32 * 32 + l32, t = a.by_group.of(row), g = row - t * a.group;
     const bool valid = t < sp.count;
-    const int first_t = tile * kRows / a.group, last_t = min((tile * kRows + kRows - 1) / a.group, sp.count - 1);
+    const int first_t = a.by_group.of(tile * kRows), last_t = min(a.by_group.of(tile * kRows + kRows - 1), sp.count - 1);
     const int keys = first_t < sp.count && a.c.pages ? limit_of(a, sp, len, last_t) : 0;  // all that the workgroup's rows see
     const int limit = valid ? limit_of(a, sp, len, t) : keys;
     // All of the wave's rows see the keys before `sure`, none those from `seen` on.
     const int wave_row = tile * kRows + rows32 * 32;
-    const int sure = min(keys, limit_of(a, sp, len, wave_row / a.group));
-    const int seen = wave_row / a.group < sp.count ? min(keys, limit_of(a, sp, len, (wave_row + 31) / a.group)) : 0;
+    const int sure = min(keys, limit_of(a, sp, len, a.by_group.of(wave_row)));
+    const int seen = a.by_group.of(wave_row) < sp.count ? min(keys, limit_of(a, sp, len, a.by_group.of(wave_row + 31))) : 0;
 
     u32x4 q[KS][3];
     {
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu) void kv_attention_rows_kernel(
             take_in(st[0], st[1], [&](int i) { return part[64 * i]; });
         }
     }
-    const bool keeps = wave % KW == 0 && wave_row / a.group < a.T;  // has rows to write
+    const bool keeps = wave % KW == 0 && a.by_group.of(wave_row) < a.T;  // has rows to write
     if (pl.pieces > 1) {
         constexpr int PART = kRows * (D + 2), SUMS = kRows * D;
         float *mine = a.part + (int64_t)blockIdx.x * PART;
