@@ -166,20 +166,51 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
     auto s_key = [&](int x) { return ROWS == 2 ? 16 * (r >> 1) + col : ROWS == 4 ? 16 * x + col : 16 * (x >> 2) + 4 * r + (x & 3); };
     const int s_limit = row_limit(s_row), o_limit = row_limit(o_row);
 
-    // SHARED: the operand's row is (row, part), and a lane has one of the parts.
-    u32x4 q[SHARED ? 1 : 3][KS];
-    {
-        const int row = row0 + (ROWS == 2 ? col >> 2 & 1 : ROWS == 4 ? col >> 2 : o_row), t = a.by_group.of(row), g = row - t * a.group;
-        const int part = SHARED ? col & 3 : 0;
-        const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + r * (D / 4);
+    f32x4 acc[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) acc[s] = f32x4{0, 0, 0, 0};
+    float m = kNone, l = 0.0f;
+    const int n = (keys + kTile - 1) / kTile;
+    const int end = pl.piece + 1 < pl.pieces ? min(n, (pl.piece + 1) * plan.per) : n;
+    int tl = __builtin_amdgcn_readfirstlane(pl.piece * plan.per) + wave;
+    if (tl < end) {
+        // Q, and the first tile's keys and values on its heels.
+        f32x4 raw[KS][2];
+        bool any;
+        const int part = SHARED ? col & 3 : 0;  // SHARED: the operand's row is (row, part)
+        {
+            const int row = row0 + (ROWS == 2 ? col >> 2 & 1 : ROWS == 4 ? col >> 2 : o_row);
+            // A row that is not there reads another, for nothing: without a branch,
+            // so that waiting for Q is not waiting for what is loaded after it.
+            any = a.by_group.of(row) < sp.count && part < 3;
+            const int t = any ? a.by_group.of(row) : 0, g = any ? row - t * a.group : 0;
+            const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + r * (D / 4);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) raw[s][i] = *(const f32x4 *)(src + 8 * s + 4 * i);
+        }
+        int64_t at[2], ahead[2];
+        Keys<D> kk[2];
+        Values<D> vv[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            at[j] = row_of(a.c, b, h, tl * kTile + 16 * j);
+            ahead[j] = row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) kk[j].load(a.c, at[j], lane);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vv[j].load(a.c, at[j], lane);
+
+        u32x4 q[SHARED ? 1 : 3][KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x2 x = t < sp.count && part < 3 ? *(const f32x2 *)(src + 8 * s + 2 * i) : f32x2{0, 0};
                 unsigned p0[3], p1[3];
-                cut3(x[0], p0[0], p0[1], p0[2]);
-                cut3(x[1], p1[0], p1[1], p1[2]);
+                cut3(any ? raw[s][i >> 1][2 * (i & 1)] : 0.0f, p0[0], p0[1], p0[2]);
+                cut3(any ? raw[s][i >> 1][2 * (i & 1) + 1] : 0.0f, p1[0], p1[1], p1[2]);
                 if (SHARED) {
                     p0[0] = part == 0 ? p0[0] : part == 1 ? p0[1] : p0[2];
                     p1[0] = part == 0 ? p1[0] : part == 1 ? p1[1] : p1[2];
@@ -187,189 +218,170 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
 #pragma unroll
                 for (int j = 0; j < (SHARED ? 1 : 3); ++j) q[j][s][i] = (p0[j] >> 16) | p1[j];
             }
-    }
 
-    f32x4 acc[KS];
+        // Where a half goes in a pair, by v_perm; nowhere for the part that a column
+        // has none of.
+        const unsigned low_half = odd ? 0x01000c0cu : 0x0c0c0100u, high_half = odd ? 0x03020c0cu : 0x0c0c0302u;
+        unsigned low[2], high[2];
+        int from[2];  // the column's part, row and tokens in `parts`
 #pragma unroll
-    for (int s = 0; s < KS; ++s) acc[s] = f32x4{0, 0, 0, 0};
-    float m = kNone, l = 0.0f;
-    // Where a half goes in a pair, by v_perm; nowhere for the part that a column
-    // has none of.
-    const unsigned low_half = odd ? 0x01000c0cu : 0x0c0c0100u, high_half = odd ? 0x03020c0cu : 0x0c0c0302u;
-    unsigned low[2], high[2];
-    int from[2];  // the column's part, row and tokens in `parts`
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const bool none = ROWS == 2 ? slot == 3 : i == 1 && slot == 1;
-        low[i] = none ? 0x0c0c0c0cu : low_half;
-        high[i] = none ? 0x0c0c0c0cu : high_half;
-        const int part = ROWS == 2 ? min(slot, 2) : i == 1 ? 2 : slot;
-        from[i] = (part * ROWS + o_row) * kTile + 4 * r;
-    }
-    const unsigned turn = 8 * (col * D / 512) + 9;  // the byte of the lane's group of 32 to bits 23 .. 30
+        for (int i = 0; i < 2; ++i) {
+            const bool none = ROWS == 2 ? slot == 3 : i == 1 && slot == 1;
+            low[i] = none ? 0x0c0c0c0cu : low_half;
+            high[i] = none ? 0x0c0c0c0cu : high_half;
+            const int part = ROWS == 2 ? min(slot, 2) : i == 1 ? 2 : slot;
+            from[i] = (part * ROWS + o_row) * kTile + 4 * r;
+        }
+        const unsigned turn = 8 * (col * D / 512) + 9;  // the byte of the lane's group of 32 to bits 23 .. 30
 
-    const int n = (keys + kTile - 1) / kTile;
-    const int end = pl.piece + 1 < pl.pieces ? min(n, (pl.piece + 1) * plan.per) : n;
-    int tl = __builtin_amdgcn_readfirstlane(pl.piece * plan.per) + wave;
-    int64_t at[2], ahead[2];
-    Keys<D> kk[2];
-    Values<D> vv[2];
-    // One tile; the next one's keys are loaded as soon as this one's are used,
-    // and its values after this one's.
-    auto step = [&](auto more) {
-        float s[8];
+        // One tile; the next one's keys are loaded as soon as this one's are used,
+        // and its values after this one's.
+        auto step = [&](auto more) {
+            float s[8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            f32x4 sum = {0, 0, 0, 0};
-            const float scale = scale_of(kk[j].scale);
+                f32x4 sum = {0, 0, 0, 0};
+                const float scale = scale_of(kk[j].scale);
 #pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                const unsigned w = kk[j].code.w[x];
-                const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
-                if constexpr (SHARED) {
-                    sum = mfma_16x16x32(q[0][x], k, sum);
-                } else {
+                for (int x = 0; x < KS; ++x) {
+                    const unsigned w = kk[j].code.w[x];
+                    const u32x4 k = {fp4_bf16<0>(w, scale), fp4_bf16<1>(w, scale), fp4_bf16<2>(w, scale), fp4_bf16<3>(w, scale)};
+                    if constexpr (SHARED) {
+                        sum = mfma_16x16x32(q[0][x], k, sum);
+                    } else {
 #pragma unroll
-                    for (int part = 2; part >= 0; --part) sum = mfma_16x16x32(k, q[part][x], sum);
-                }
-            }
-            if constexpr (SHARED) {
-                s[j] = (sum[2] + sum[1]) + sum[0];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * j + i] = sum[i];
-            }
-        }
-        if (ROWS == 2) s[0] = r >> 1 ? s[1] : s[0];
-        if constexpr (more.value) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) kk[j].load(a.c, ahead[j], lane);
-        }
-        const bool partly = tl * kTile + kTile > sure || at[0] < 0 || at[1] < 0;
-        if (partly) {
-#pragma unroll
-            for (int x = 0; x < SC; ++x)
-                if (tl * kTile + s_key(x) >= s_limit || (s_key(x) < 16 ? at[0] : at[1]) < 0) s[x] = -INFINITY;
-        }
-        float top = s[0];
-#pragma unroll
-        for (int x = 1; x < SC; ++x) top = fmaxf(top, s[x]);
-        top *= a.scale2;
-        if (__any(top > m + kRaise)) {
-            // The lanes of a row: 16 neighbours (and as many 32 on), or those 16 apart.
-            if (SHARED) {
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-            } else {
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-            }
-            if (ROWS != 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float to = fmaxf(m, top);
-            float f = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= f;
-            if (SHARED) f = __shfl(f, 16 * o_row, 64);
-#pragma unroll
-            for (int x = 0; x < KS; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[x][i] *= f;
-        }
-        unsigned cut[SC][3];
-#pragma unroll
-        for (int x = 0; x < SC; ++x) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale2, -m));
-            l += e;
-            cut3(e, cut[x][0], cut[x][1], cut[x][2]);
-            if (SHARED)
-#pragma unroll
-                for (int part = 0; part < 3; ++part) parts[wave][part][s_row][s_key(x)] = (uint16_t)(cut[x][part] >> 16);
-        }
-        if (SHARED) wave_sync();
-        auto values = [&](auto J) {
-            constexpr int j = decltype(J)::value;
-            u32x4 p[OPS];
-            if constexpr (SHARED) {
-#pragma unroll
-                for (int i = 0; i < OPS; ++i) {
-                    const uint2 w = *(const uint2 *)(&parts[wave][0][0][0] + from[i] + 16 * j);
-                    p[i] = u32x4{__builtin_amdgcn_perm(0, w.x, low[i]), __builtin_amdgcn_perm(0, w.x, high[i]),
-                                 __builtin_amdgcn_perm(0, w.y, low[i]), __builtin_amdgcn_perm(0, w.y, high[i])};
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < OPS; ++i)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) p[i][x] = __builtin_amdgcn_perm(0, cut[4 * j + x][i], high_half);
-            }
-            // The scale's byte turned to where a float has its exponent: no
-            // other bit of it counts.
-            float vscale[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned w = vv[j].scale.w[i * D / 128];
-                vscale[i] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(w, w, turn + 8 * (i * (D / 32) & 3)));
-            }
-            if (partly) {
-                // Is a value no number, in a place that some rows do not see
-                // (or that was never written)?  Then zero in the product, and
-                // NaN given to the rows that do see it.
-                bool spoilt[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) spoilt[i] = ((float_bits(vscale[i]) >> 23) & 0xff) > kMostScale;
-                if (__any(spoilt[0] || spoilt[1] || spoilt[2] || spoilt[3])) {
-                    bool mine = false;
-                    for (int x = 0; x < 16; ++x)
-                        mine |= at[j] >= 0 && tl * kTile + 16 * j + x < o_limit &&
-                                a.c.v_scales[(at[j] + x) * (D / 32) + r * D / 128] > kMostScale;
-#pragma unroll
-                    for (int x = 0; x < KS; ++x)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[x][i] = mine ? NAN : acc[x][i];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        vscale[i] = spoilt[i] ? 1.0f : vscale[i];
-                        vv[j].code[i].w[0] = spoilt[i] ? 0 : vv[j].code[i].w[0];
+                        for (int part = 2; part >= 0; --part) sum = mfma_16x16x32(k, q[part][x], sum);
                     }
                 }
-            }
-            u32x4 v[KS];
-            auto convert = [&](auto X) {
-                constexpr int x = decltype(X)::value;
+                if constexpr (SHARED) {
+                    s[j] = (sum[2] + sum[1]) + sum[0];
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[x][i] = fp4_bf16<x>(vv[j].code[i].w[0], vscale[i]);
+                    for (int i = 0; i < 4; ++i) s[4 * j + i] = sum[i];
+                }
+            }
+            if (ROWS == 2) s[0] = r >> 1 ? s[1] : s[0];
+            if constexpr (more.value) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) kk[j].load(a.c, ahead[j], lane);
+            }
+            const bool partly = tl * kTile + kTile > sure || at[0] < 0 || at[1] < 0;
+            if (partly) {
+#pragma unroll
+                for (int x = 0; x < SC; ++x)
+                    if (tl * kTile + s_key(x) >= s_limit || (s_key(x) < 16 ? at[0] : at[1]) < 0) s[x] = -INFINITY;
+            }
+            float top = s[0];
+#pragma unroll
+            for (int x = 1; x < SC; ++x) top = fmaxf(top, s[x]);
+            top *= a.scale2;
+            if (__any(top > m + kRaise)) {
+                // The lanes of a row: 16 neighbours (and as many 32 on), or those 16 apart.
+                if (SHARED) {
+#pragma unroll
+                    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+                } else {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                }
+                if (ROWS != 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float to = fmaxf(m, top);
+                float f = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= f;
+                if (SHARED) f = __shfl(f, 16 * o_row, 64);
+#pragma unroll
+                for (int x = 0; x < KS; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[x][i] *= f;
+            }
+            unsigned cut[SC][3];
+#pragma unroll
+            for (int x = 0; x < SC; ++x) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale2, -m));
+                l += e;
+                cut3(e, cut[x][0], cut[x][1], cut[x][2]);
+                if (SHARED)
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) parts[wave][part][s_row][s_key(x)] = (uint16_t)(cut[x][part] >> 16);
+            }
+            if (SHARED) wave_sync();
+            auto values = [&](auto J) {
+                constexpr int j = decltype(J)::value;
+                u32x4 p[OPS];
+                if constexpr (SHARED) {
+#pragma unroll
+                    for (int i = 0; i < OPS; ++i) {
+                        const uint2 w = *(const uint2 *)(&parts[wave][0][0][0] + from[i] + 16 * j);
+                        p[i] = u32x4{__builtin_amdgcn_perm(0, w.x, low[i]), __builtin_amdgcn_perm(0, w.x, high[i]),
+                                     __builtin_amdgcn_perm(0, w.y, low[i]), __builtin_amdgcn_perm(0, w.y, high[i])};
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < OPS; ++i)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) p[i][x] = __builtin_amdgcn_perm(0, cut[4 * j + x][i], high_half);
+                }
+                // The scale's byte turned to where a float has its exponent: no
+                // other bit of it counts.
+                float vscale[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned w = vv[j].scale.w[i * D / 128];
+                    vscale[i] = __builtin_bit_cast(float, __builtin_amdgcn_alignbit(w, w, turn + 8 * (i * (D / 32) & 3)));
+                }
+                if (partly) {
+                    // Is a value no number, in a place that some rows do not see
+                    // (or that was never written)?  Then zero in the product, and
+                    // NaN given to the rows that do see it.
+                    bool spoilt[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) spoilt[i] = ((float_bits(vscale[i]) >> 23) & 0xff) > kMostScale;
+                    if (__any(spoilt[0] || spoilt[1] || spoilt[2] || spoilt[3])) {
+                        bool mine = false;
+                        for (int x = 0; x < 16; ++x)
+                            mine |= at[j] >= 0 && tl * kTile + 16 * j + x < o_limit &&
+                                    a.c.v_scales[(at[j] + x) * (D / 32) + r * D / 128] > kMostScale;
+#pragma unroll
+                        for (int x = 0; x < KS; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[x][i] = mine ? NAN : acc[x][i];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            vscale[i] = spoilt[i] ? 1.0f : vscale[i];
+                            vv[j].code[i].w[0] = spoilt[i] ? 0 : vv[j].code[i].w[0];
+                        }
+                    }
+                }
+                u32x4 v[KS];
+                auto convert = [&](auto X) {
+                    constexpr int x = decltype(X)::value;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[x][i] = fp4_bf16<x>(vv[j].code[i].w[0], vscale[i]);
+                };
+                convert(std::integral_constant<int, 0>{});
+                if constexpr (KS > 1) convert(std::integral_constant<int, 1>{});
+                if constexpr (KS > 2) {
+                    convert(std::integral_constant<int, 2>{});
+                    convert(std::integral_constant<int, 3>{});
+                }
+#pragma unroll
+                for (int i = OPS - 1; i >= 0; --i)  // the small parts first
+#pragma unroll
+                    for (int x = 0; x < KS; ++x) acc[x] = mfma_16x16x32(v[x], p[i], acc[x]);
             };
-            convert(std::integral_constant<int, 0>{});
-            if constexpr (KS > 1) convert(std::integral_constant<int, 1>{});
-            if constexpr (KS > 2) {
-                convert(std::integral_constant<int, 2>{});
-                convert(std::integral_constant<int, 3>{});
+            values(std::integral_constant<int, 0>{});
+            values(std::integral_constant<int, 1>{});
+            if (SHARED) wave_sync();
+            if constexpr (more.value) {
+                tl += kWaves;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    vv[j].load(a.c, ahead[j], lane);
+                    at[j] = ahead[j];
+                    ahead[j] = row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j);  // past the end: not used
+                }
             }
-#pragma unroll
-            for (int i = OPS - 1; i >= 0; --i)  // the small parts first
-#pragma unroll
-                for (int x = 0; x < KS; ++x) acc[x] = mfma_16x16x32(v[x], p[i], acc[x]);
         };
-        values(std::integral_constant<int, 0>{});
-        values(std::integral_constant<int, 1>{});
-        if (SHARED) wave_sync();
-        if constexpr (more.value) {
-            tl += kWaves;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                vv[j].load(a.c, ahead[j], lane);
-                at[j] = ahead[j];
-                ahead[j] = tl + kWaves < end ? row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j) : -1;
-            }
-        }
-    };
-    if (tl < end) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            at[j] = row_of(a.c, b, h, tl * kTile + 16 * j);
-            kk[j].load(a.c, at[j], lane);
-            vv[j].load(a.c, at[j], lane);
-            ahead[j] = tl + kWaves < end ? row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j) : -1;
-        }
         while (tl + kWaves < end) step(std::true_type{});
         step(std::false_type{});
     }

@@ -55,16 +55,17 @@ __device__ __forceinline__ Span span_of(const int32_t *start, const int32_t *cou
 }
 
 // The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
-// head h, or -1.  b, h and pos are the same in all lanes, so the table is read
-// through the scalar cache.
+// head h, or -1; the table has a page at least.  b, h and pos are the same in all
+// lanes, so the table is read through the scalar cache, and without a branch, so
+// that several lookups are on their way together.
 __device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
 {
     typedef const __attribute__((address_space(4))) int32_t *scalar;
     const int place = pos >> c.page_shift;
-    if (place >= c.max_pages) return -1;
-    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + place];
-    if ((unsigned)page >= (unsigned)c.pages) return -1;
-    return (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+    const bool in = (unsigned)place < (unsigned)c.max_pages;
+    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + (in ? place : 0)];
+    const int64_t row = (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+    return in && (unsigned)page < (unsigned)c.pages ? row : -1;
 }
 
 // The scale that a byte stands for.
