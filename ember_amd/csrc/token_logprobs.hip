@@ -38,7 +38,8 @@ constexpr int kThreads = 256;
 constexpr int kPerThread = 16;
 constexpr int kChunk = kThreads * kPerThread;
 constexpr int kMostRows = 1 << 13;  // that are cut
-constexpr int kKeys = 2048;         // of lists that are joined at a time
+constexpr int kKeys = 2048;         // of lists that are joined at a time,
+constexpr int kNear = 8;            // the first ones of each
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows start anywhere
@@ -104,7 +105,7 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane)
 
 // Appends the lanes' keys above `last` to `found`, which has c; returns how many
 // there are then (those past kFound are not kept).
-constexpr int kFound = 128;
+constexpr int kFound = 256;
 __device__ __forceinline__ int gather(uint64_t *found, int c, uint64_t key, uint64_t last)
 {
     const uint64_t some = __ballot(key > last);
@@ -136,52 +137,69 @@ struct Best {
             if (k > last) put(k, top);
         }
     }
-    // Of one key of each lane, at least `top` of which count: the k-th largest,
-    // cut to 16 bits, is a bound (none if fewer lanes have one).
-    __device__ __forceinline__ void raise(unsigned upper, int top)
+    // Of two keys of each lane (their upper halves; 0: none): the k-th largest, cut
+    // to 16 bits, is a bound (none if there are fewer).
+    __device__ __forceinline__ void raise(unsigned u0, unsigned u1, int top)
     {
         unsigned bound = 0;
-        for (unsigned bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-            if (__popcll(__ballot(upper >= (bound | bit))) >= top) bound |= bit;
+        for (unsigned bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+            const unsigned to = bound | bit;
+            if (__popcll(__ballot(u0 >= to)) + __popcll(__ballot(u1 >= to)) >= top) bound = to;
+        }
         const uint64_t l = bound ? ((uint64_t)bound << 32) - 1 : 0;
         last = l > last ? l : last;
     }
-    // The `top` largest of c keys in `found` (c <= kFound), each put where the
+    // The `top` largest of c keys in `found` (c <= 64 * N), each put where the
     // number of larger ones says; `found` is used up.
+    template <int N>
     __device__ __forceinline__ void sort(uint64_t *found, int c, int top)
     {
         const int lane = threadIdx.x & 63;
         wave_sync();
-        const uint64_t k0 = lane < c ? found[lane] : 0, k1 = lane + 64 < c ? found[lane + 64] : 0;
-        int r0 = 0, r1 = 0;
+        uint64_t k[N];
+        int above[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) k[j] = lane + 64 * j < c ? found[lane + 64 * j] : 0, above[j] = 0;
 #pragma unroll 8
         for (int i = 0; i < c; ++i) {
-            const uint64_t k = found[i];
-            r0 += k > k0, r1 += k > k1;
+            const uint64_t other = found[i];
+#pragma unroll
+            for (int j = 0; j < N; ++j) above[j] += other > k[j];
         }
         wave_sync();
-        if (lane < c && r0 < top) found[r0] = k0;
-        if (lane + 64 < c && r1 < top) found[r1] = k1;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (lane + 64 * j < c && above[j] < top) found[above[j]] = k[j];
         wave_sync();
         mine = lane < min(c, top) ? found[lane] : 0;
         const uint64_t l = lane_key(mine, top - 1);
         last = l > last ? l : last;
     }
-    // Takes in n sorted lists of `top` keys, one after the other in `lists`.
-    __device__ __forceinline__ void join(const uint64_t *lists, int n, int top, uint64_t *found)
+    __device__ __forceinline__ void sort(uint64_t *found, int c, int top)
+    {
+        if (c <= 128) sort<2>(found, c, top);
+        else sort<4>(found, c, top);
+    }
+    // Takes in n sorted lists of `top` keys: key(i, at) is list i's `at`-th, and the
+    // first `near` of a list are at hand.
+    template <class F>
+    __device__ __forceinline__ void join(int n, int near, int top, uint64_t *found, F key)
     {
         const int lane = threadIdx.x & 63;
-        uint64_t head = 0;
-        if (n >= 64) {
-            for (int i = lane; i < n; i += 64) head = lists[i * top] > head ? lists[i * top] : head;
-        } else if (lane / n < top) {
-            head = lists[lane % n * top + lane / n];
+        // A bound from the lists' first keys: two places of a list (or lists) to a lane.
+        unsigned head[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = lane + 64 * j, at = n < 128 ? i / n : 0;
+            uint64_t k = at < near ? key(i - at * n, at) : 0;
+            for (int more = i + 128; more < n; more += 128) k = max(k, key(more, 0));
+            head[j] = (unsigned)(k >> 32);
         }
-        raise((unsigned)(head >> 32), top);
+        raise(head[0], head[1], top);
         auto all = [&](auto f) {
             for (int i = lane; i - lane < n; i += 64)
                 for (int at = 0; at < top; ++at) {
-                    const uint64_t k = i < n ? lists[i * top + at] : 0;
+                    const uint64_t k = i < n ? key(i, at) : 0;
                     if (!__any(k > last)) break;  // nor the lists' further ones
                     f(k);
                 }
@@ -277,14 +295,14 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
     Best best;
     load(next, piece * a.per);
     for (int chunk = piece * a.per; chunk < end; ++chunk) {
-        float most = -INFINITY;
+        float half[2] = {-INFINITY, -INFINITY};  // the largest of 8
 #pragma unroll
         for (int j = 0; j < kPerThread / 4; ++j) {
             x[j] = next[j];
-            most = fmaxf(most, fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+            half[j & 1] = fmaxf(half[j & 1], fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
         }
         if (chunk + 1 < end) load(next, chunk + 1);
-        add(t, x, most);
+        add(t, x, fmaxf(half[0], half[1]));
         if (TOP) {
             const int64_t first = (int64_t)chunk * kChunk + 4 * (int)threadIdx.x;
             auto all = [&](auto f) {
@@ -302,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
             };
             auto take = [&](uint64_t k) { best.take(k, a.top); };
             if (chunk == piece * a.per) {
-                best.raise((unsigned)(key_of(most, 0) >> 32), a.top);
+                best.raise((unsigned)(key_of(half[0], 0) >> 32), (unsigned)(key_of(half[1], 0) >> 32), a.top);
                 int c = 0;
                 all([&](uint64_t k) { c = gather(found[wave], c, k, best.last); });
                 if (c <= kFound) best.sort(found[wave], c, a.top);
@@ -340,22 +358,24 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         if (lane == 0) sums[wave] = t;
         if (TOP) {
             best = Best();
-            const int at_once = kKeys / (4 * a.top);  // pieces
+            constexpr int at_once = kKeys / (4 * kNear);  // pieces
             for (int i0 = 0; i0 < a.pieces; i0 += at_once) {
-                const int n = min(at_once, a.pieces - i0), keys = 4 * a.top;
+                const int n = 4 * min(at_once, a.pieces - i0);
+                auto place = [&](int i, int at) { return from + (i0 + (i >> 2)) * size + 16 + 8 * ((i & 3) * a.top + at); };
                 __syncthreads();
-                // All of a thread's loads in flight at once.
+                // The lists' first keys, all of a thread's loads in flight at once.
                 uint64_t k[kKeys / kThreads];
 #pragma unroll
                 for (int j = 0; j < kKeys / kThreads; ++j) {
-                    const int i = min(j * kThreads + (int)threadIdx.x, n * keys - 1), pc = i / keys;
-                    k[j] = get8(from + (i0 + pc) * size + 16 + 8 * (i - pc * keys));
+                    const int i = (j * kThreads + (int)threadIdx.x) / kNear, at = threadIdx.x % kNear;
+                    k[j] = i < n && at < a.top ? get8(place(i, at)) : 0;
                 }
 #pragma unroll
-                for (int j = 0; j < kKeys / kThreads; ++j)
-                    if (j * kThreads + (int)threadIdx.x < n * keys) lists[j * kThreads + threadIdx.x] = k[j];
+                for (int j = 0; j < kKeys / kThreads; ++j) lists[j * kThreads + threadIdx.x] = k[j];
                 __syncthreads();
-                if (wave == 0) best.join(lists, 4 * n, a.top, found[0]);
+                if (wave == 0)
+                    best.join(n, min(kNear, a.top), a.top, found[0],
+                              [&](int i, int at) { return at < kNear ? lists[i * kNear + at] : get8(place(i, at)); });
             }
         }
     } else if (TOP) {
@@ -366,7 +386,8 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
     t = join(join(sums[0], sums[1]), join(sums[2], sums[3]));
     if (TOP && a.pieces == 1) {
         best = Best();
-        best.join(lists, 4, a.top, found[0]);
+        if (4 * a.top <= 128) best.sort<2>(lists, 4 * a.top, a.top);
+        else best.join(4, a.top, a.top, found[0], [&](int i, int at) { return lists[i * a.top + at]; });
     }
     finish(a, row, t, best.mine);
 }
