@@ -18,6 +18,7 @@ constexpr float kRaise = 8.0f;
 constexpr int kWaves = 4;        // of a workgroup
 constexpr int kMostPlan = 1024;  // sequences that are planned for; with more, a unit is not cut
 constexpr int kMostUnits = 1 << 14;  // that are cut
+constexpr int64_t kMostScratch = int64_t(160) << 20;  // bytes of their pieces
 
 // Division by a number that the host knows: with inv = floor(2^32 / d) the
 // product's upper half is the quotient or one below it, for every n below 2^32.

@@ -492,12 +492,13 @@ int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
     a.by_group = Divisor(a.group), a.by_tiles = Divisor(a.tiles), a.by_units = Divisor(a.c.heads * a.tiles);
     // One round of workgroups over the chip; where the units alone are about as
     // many, two pieces each, so that the longest sequence does not decide.  With
-    // many units none is cut.
+    // many units, or where the pieces' results were large, none is cut.
     const int64_t slots = (int64_t)per_cu * std::max(device_cu_count(), 1);
-    const bool cut = a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * slots);
-    a.blocks = (int)(cut ? std::max(slots, 2 * all) : all);
+    const int64_t blocks = std::max(slots, 2 * all), bytes = blocks * rows * (a.c.D + 2) * (int64_t)sizeof(float);
+    const bool cut = a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * slots) && bytes <= kMostScratch;
+    a.blocks = (int)(cut ? blocks : all);
     if (cut) {
-        a.part = (float *)scratch(kScratchKvAttention, (size_t)a.blocks * rows * (a.c.D + 2) * sizeof(float));
+        a.part = (float *)scratch(kScratchKvAttention, (size_t)bytes);
         if (!a.part) return EMBER_ERR_OUT_OF_MEMORY;
     }
     return EMBER_OK;
@@ -527,7 +528,7 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     a.causal = causal != 0;
     // Above 0, so that a masked score stays -infinity under it; a scale of 0 then
     // gives scores that differ by nothing.
-    a.scale2 = std::max(scale * kLog2e, 1e-37f);
+    a.scale2 = std::min(std::max(scale * kLog2e, 1e-37f), 3.4e38f);
     if (T * a.group > kFewRows) return launch_kv_attention_rows(a);
     return a.c.D == 128 ? launch_rows<128>(a) : a.c.D == 64 ? launch_rows<64>(a) : launch_rows<32>(a);
 }

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(CopyArgs a, unsigned task
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (unsigned i = blockIdx.x * 4 + wave; i < tasks; i += gridDim.x * 4) {
         const Task k = task_of(a, i);
-        if (a.next && k.first && lane == 0) a.next[k.b] = k.sp.start + k.sp.count;
+        if (a.next && k.first && lane == 0) a.next[k.b] = (int)((unsigned)k.sp.start + k.sp.count);
         if (k.at < 0) continue;
         const float *in = a.in[k.which] + k.b * a.st.sb + k.h * a.st.sh + 4 * col;
         uint8_t *codes = (k.which ? a.c.v_codes : a.c.k_codes) + k.at * (D / 2);

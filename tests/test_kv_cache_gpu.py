@@ -206,6 +206,52 @@ def test_many_rows_and_splits(D, T):
     p.check_attention(normal(rng, 3, T, 2, D), False, start=[1700 - T, 600, 0], count=[T, 5, T])
 
 
+@pytest.mark.parametrize("B", [65, 150, 1100])
+@pytest.mark.parametrize("T, G_", [(1, 1), (1, 3), (2, 4), (9, 5)])
+def test_many_sequences(B, T, G_):
+    """More sequences than a wave has lanes, and more than are planned for, of all lengths."""
+    rng = np.random.default_rng(B + T)
+    tab, pages = table(rng, B, 3)
+    p = Pair(pages, 1, 16, 32, tab)
+    p.write(normal(rng, B, 48, 1, 32), normal(rng, B, 48, 1, 32))
+    start = rng.integers(-1, 48 - T + 1, B)
+    p.check_attention(normal(rng, B, T, G_, 32), True, start=start, count=rng.integers(0, T + 1, B))
+
+
+def test_sequences_of_very_different_lengths():
+    """One long sequence among many short and empty ones, cut into pieces."""
+    rng = np.random.default_rng(20)
+    B, lengths = 70, np.zeros(70, int)
+    lengths[[3, 66]] = 3000, 900
+    lengths[10:60] = rng.integers(0, 40, 50)
+    tab = np.full((B, 12), -1, np.int32)
+    need, n = -(-lengths // 256), 0
+    for b in range(B):
+        tab[b, :need[b]] = np.arange(n, n + need[b])
+        n += need[b]
+    p = Pair(n, 1, 256, 64, tab)
+    for b in np.nonzero(lengths)[0]:
+        k, v = np.zeros((2, B, lengths[b], 1, 64), np.float32)
+        k[b], v[b] = normal(rng, lengths[b], 1, 64), normal(rng, lengths[b], 1, 64)
+        p.write(k, v, count=np.where(np.arange(B) == b, lengths[b], 0))
+    for T, heads in ((1, 2), (2, 3), (30, 2)):
+        p.check_attention(normal(rng, B, T, heads, 64), True, start=lengths - T)
+
+
+@pytest.mark.parametrize("pages, places", [(0, 2), (3, 0), (0, 0)])
+def test_caches_of_nothing(pages, places):
+    """No pages, or no place for any: nothing is written, read or seen."""
+    rng = np.random.default_rng(21)
+    p = Pair(pages, 2, 16, 64, np.zeros((2, places), np.int32))
+    got, ref = p.write(normal(rng, 2, 5, 2, 64), normal(rng, 2, 5, 2, 64))
+    np.testing.assert_array_equal(got, ref)
+    for x in p.read(5):
+        assert (x == 0).all()
+    for T in (1, 5, 50):
+        o, lse = p.attention(normal(rng, 2, T, 4, 64), True)
+        assert (o == 0).all() and np.isneginf(lse).all()
+
+
 def test_scores_of_all_sizes():
     """Scores from -300 to 300, growing along the keys (the maximum is raised often), and scale 0."""
     rng = np.random.default_rng(8)
