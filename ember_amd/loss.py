@@ -124,7 +124,10 @@ def _token_ids(logits: Tensor, tokens) -> np.ndarray:
     if logits.shape[-1] < 1:
         raise ValueError("logits need at least one class")
     classes = logits.shape[-1]
-    return np.where((ids >= 0) & (ids < classes), ids, -1).astype(np.int32).reshape(-1)
+    known = ((ids >= 0) & (ids < classes)).reshape(-1)
+    out = np.full(ids.size, -1, np.int32)
+    out[known] = ids.reshape(-1)[known]
+    return out
 
 
 def _upload(ids: np.ndarray):

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import ember_amd as em
-from ember_amd import _core
+from ember_amd import _core, loss
 from ember_amd.loss import TokenLoss
 from ember_amd.tensor import Tensor
 
@@ -129,6 +129,12 @@ def test_token_types():
         em.token_logprobs(fake((4, 0)), np.zeros(4, int))
     with pytest.raises(RuntimeError):
         TokenLoss().backward()
+
+
+@pytest.mark.parametrize("kind", [np.uint8, np.uint16, np.uint32, np.uint64, np.int8, np.int16, np.int64])
+def test_ids_out_of_range_are_padded_in_any_type(kind):
+    ids = np.array([[0, 99], [100, np.iinfo(kind).max]], kind)
+    assert loss._token_ids(fake((2, 2, 100)), ids).tolist() == [0, 99, -1, -1]
 
 
 def test_binding_checks_sizes_before_device_work():
