@@ -198,6 +198,13 @@ void launch_read(const CopyArgs &a, unsigned n)
         hipLaunchKernelGGL((kv_read_kernel<D, false>), copy_grid(a), dim3(256), 0, 0, a, n);
 }
 
+// Whether two arrays of n integers have one in common.
+bool share(const int32_t *x, const int32_t *y, int n)
+{
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y, bytes = (uintptr_t)n * sizeof(int32_t);
+    return x && y && (a < b ? b - a : a - b) < bytes;
+}
+
 int check_copy(const ember_kv_cache *cache, const void *k, const void *v, int64_t T, int64_t sb, int64_t sh, int64_t ss,
                const int32_t *start, const int32_t *count, CopyArgs *a, const char *what)
 {
@@ -221,7 +228,9 @@ extern "C" int kv_cache_write(const ember_kv_cache *cache, const float *k, const
     CopyArgs a = {};
     const int st = check_copy(cache, k, v, T, in_sb, in_sh, in_ss, start, count, &a, "kv_cache_write");
     if (st) return st;
-    if (((uintptr_t)next & 3) || (next && next == start)) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_write");
+    // Some workgroups read start and count when others have written next.
+    if (((uintptr_t)next & 3) || share(next, start, a.c.sequences) || share(next, count, a.c.sequences))
+        return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_write");
     if (a.c.sequences == 0 || (T == 0 && !next)) return EMBER_OK;
     a.in[0] = k, a.in[1] = v, a.next = next;
     const unsigned n = tasks_of(a);

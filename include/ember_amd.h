@@ -15,15 +15,16 @@
  * Threads.  Like the reference (single-threaded, every call made under the
  * Python GIL), the library expects one host thread in it at a time per
  * device: operators that use library scratch (attention_bwd's row
- * statistics, split-K and reduction partials) share one buffer per device
- * and operator, and two threads' launches may interleave on the null
- * stream.  The allocator and the error slots are thread-safe.
+ * statistics, split-K and reduction partials, the pieces of kv_cache_attention
+ * and token_logprobs) share one buffer per device and operator, and two threads'
+ * launches may interleave on the null stream.  The allocator and the error slots are thread-safe.
  *
  * Error behaviour.  The reference prints and calls exit() on any device
  * error (src/core/utils_gpu.cuh:13-19).  Here the void entry points keep
  * their signatures but record the first error in a sticky per-thread slot
  * (ember_get_last_error) and print it to stderr; the process is not killed.
- * The attention entry points, which are new, return that status directly.
+ * The entry points that are new (attention, the key/value cache, token log
+ * probabilities and the fused training operators) return that status directly.
  * Argument errors never launch a kernel.
  */
 #ifndef EMBER_AMD_H
@@ -377,7 +378,8 @@ typedef struct ember_kv_cache {
 /* Rounds the valid rows of k and v into the cache.  Two valid rows must not
  * land on the same slot (a page written through two table entries).  next,
  * when not NULL, is an int32 device array that gets start[b] + the number of
- * valid rows, where the sequence's next call starts; it must not be start. */
+ * valid rows, where the sequence's next call starts; it must not overlap start
+ * or count. */
 int kv_cache_write(const ember_kv_cache *cache, const float *k, const float *v, int64_t T,
                    int64_t in_sb, int64_t in_sh, int64_t in_ss, const int32_t *start,
                    const int32_t *count, int32_t *next);
@@ -396,9 +398,9 @@ int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, int64_t T, in
  * fp32: products are those of an fp32 attention over kv_cache_read's values.
  * A row of q that holds an infinity or a NaN gets NaN; keys and values that
  * read back as NaN reach the rows that see them, and no others.  scale is
- * finite and >= 0; T * q_heads / heads is at most 2^30, and sequences * heads *
- * T * q_heads / heads at most 2^24.  Uses library scratch; o must not overlap
- * q. */
+ * finite and >= 0.  With R = T * q_heads / heads rows to a cache head, R is at
+ * most 2^30; calls with sequences * heads * ceil(R / 8) from 2^24 on may be
+ * refused.  Uses library scratch; o must not overlap q. */
 int kv_cache_attention(const ember_kv_cache *cache, const float *q, float *o, float *lse, int64_t T,
                        int64_t q_heads, float scale, int causal, int64_t in_sb, int64_t in_sh,
                        int64_t in_ss, int64_t out_sb, int64_t out_sh, int64_t out_ss,
