@@ -239,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         auto step = [&](auto more) {
             float s[8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 f32x4 sum = {0, 0, 0, 0};
                 const float scale = scale_of(kk[j].scale);
 #pragma unroll

@@ -269,11 +269,16 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                 e0 = lower_part(e0), e1 = lower_part(e1);
                 p[2][i] = upper_halves(e0, e1);
             }
+            constexpr int NP = DB < 2 ? 1 : 2;  // products in turn, so that none waits for the one before
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const uint4 v = at.v[v_place<D>(32 * d + l32, 2 * (2 * kb + st) + half)];
+            for (int d = 0; d < DB; d += NP) {
+                uint4 v[NP];
 #pragma unroll
-                for (int part = 2; part >= 0; --part) acc[d] = mfma32(v, p[part], acc[d]);
+                for (int j = 0; j < NP; ++j) v[j] = at.v[v_place<D>(32 * (d + j) + l32, 2 * (2 * kb + st) + half)];
+#pragma unroll
+                for (int part = 2; part >= 0; --part)
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) acc[d + j] = mfma32(v[j], p[part], acc[d + j]);
             }
         }
     };
