@@ -1,14 +1,28 @@
 // kv_attention_rows.hip -- attention of many query rows over the 4-bit cache: a
 // prompt read in pieces, on what is cached.
 //
-// The same sums as in kv_attention.hip, on v_mfma_f32_32x32x16_bf16: a workgroup
+// The same sums as in kv_attention.hip, on v_mfma_f32_32x32x16_f16: a workgroup
 // has 128 rows, 32 to a wave, and its waves share tiles of 64 keys and values
-// that are converted to bf16 once and laid out in LDS as the matrix core takes
-// them, so that the conversion is a small part of the work:
-//   S^T (32 keys x 32 rows) = K . Q^T, Q's three parts in registers;
-//   O^T (D x 32 rows) += V^T . P^T, P's three parts from S^T's registers: lane l
-//     holds column l % 32 and, of each 16 keys, those of its half h = l / 32: 4h ..
-//     4h+3 and 8+4h .. 8+4h+3.  V^T lies in LDS with its keys in that order.
+// that are converted once and laid out in LDS as the matrix core takes them, so
+// that the conversion is a small part of the work:
+//   S^T (32 keys x 32 rows) = K . Q^T, Q's parts in registers;
+//   O^T (D x 32 rows) += V^T . P^T, P's parts from S^T's registers: lane l holds
+//     column l % 32 and, of each 16 keys, those of its half h = l / 32: 4h .. 4h+3
+//     and 8+4h .. 8+4h+3.  V^T lies in LDS with its keys in that order.
+//
+// Numbers.  In units of a power of two, u, of the workgroup's, fp16 holds exactly
+// each cached value whose scale is from 2^-23 to 2^13 of u (denormals count in
+// full: compared on the device, conversion and product).  The fp32 operands are
+// cut into two fp16 parts, hi = fp16(x) and lo = fp16(x - hi), off by at most 2^-23
+// of x, or by 2^-25 where x is below 1.  A row of Q is shifted so that its largest is
+// in [2^14, 2^15): what is lost there is 2^-39 of it.  Weights are e^(s - m) * 2^7 (at
+// most 2^15, as m lags by 2^8 at most): what is lost is 2^-32 of the largest weight,
+// where the sums' own fp32 loses 2^-25 of theirs.  u is taken near the scales of the
+// piece's first token; where a value that a row sees fits no fp16 (far larger or
+// smaller than that, or no number), the workgroup walks its keys again with bf16
+// values, which hold them all, and three parts.
+//   2 x 1024 rows of 32 / 8 heads of 128 over 8192: two fp16 parts 356 us, three bf16 ones
+//   486, and both, where every piece has such a value, 2.1 times the first's.
 // Two tiles of LDS: while one is worked on, the next is converted into the other
 // and the one after is loaded; one barrier a tile.
 //
@@ -17,7 +31,10 @@
 // neither the 32 rows that a wave reads at once nor the ones that it writes lie
 // in the same banks.
 //
-// Work: 12 * T * keys * D matrix operations a head where 4 are the definition's.
+// Work: 8 * T * keys * D matrix operations a head where 4 are the definition's.
+// Bound by the matrix cores: 2 x 1024 rows of 32 / 8 heads of 128 over 8192 keys, causal,
+// 356 us, 557 TFLOP/s of the definition's and 1.11 PFLOP/s of fp16; 4 x 512 rows of 16
+// heads of 64 over 4096 65 us.
 #include <type_traits>
 
 #include "kv_attention.h"
@@ -27,12 +44,14 @@ namespace ember {
 namespace {
 
 constexpr int kTile = 64;    // keys
-// Workgroups that a CU holds at once: by their registers.
+// Workgroups that a CU holds at once: as many as their registers allow.
 constexpr int per_cu(int D)
 {
     return D == 128 ? 2 : D == 64 ? 3 : 4;
 }
-constexpr int kLeast = 8;    // tiles of a piece
+constexpr int kLeast = 8;    // tiles of a piece: its start and its join cost about two
+// fp16 holds every code times 2^kLeastUnit .. 2^kMostUnit.
+constexpr int kLeastUnit = -23, kMostUnit = 13;
 
 // As in kv_attention.hip.
 __device__ unsigned g_done[kMostUnits];
@@ -58,6 +77,33 @@ template <int D>
 __device__ __forceinline__ int v_place(int d, int c)
 {
     return d * 8 + (c ^ ((d ^ (d / (D / 16))) & 7));
+}
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// HALF: the exponent bytes of the scales that K and V are held in units of.
+struct Units {
+    int k, v;
+};
+
+// The scale that a group is converted with; fits = false if there is none that
+// keeps its values.
+template <bool HALF>
+__device__ __forceinline__ float unit_scale(unsigned byte, int unit, bool &fits)
+{
+    if (!HALF) return scale_of(byte);
+    const int over = (int)byte - unit, to = min(max(over, kLeastUnit), kMostUnit);
+    fits = to == over;
+    return scale_of(to + 127);
+}
+
+// Two neighbouring codes as numbers of 16 bits.
+template <bool HALF, int S>
+__device__ __forceinline__ unsigned fp4_pair16(unsigned w, float scale)
+{
+    if constexpr (HALF) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, S));
+    else return fp4_bf16<S>(w, scale);
 }
 
 // What a thread loads of a tile: a quarter of a key's row, and of 4 tokens' values
@@ -101,15 +147,22 @@ struct Raw {
         }
     }
 
-    // Converts and writes them.
-    __device__ __forceinline__ void put(Lds<D> &lds, int thread) const
+    // Converts and writes them; false if what one of the first `keys` of the tile
+    // holds (of those that are there) does not fit the number type.
+    template <bool HALF>
+    __device__ __forceinline__ bool put(Lds<D> &lds, int thread, Units at, int keys) const
     {
         const int key = thread >> 2, r = thread & 3;
-        const float kscale = scale_of(ks);
+        bool fits = true;
+        const float kscale = unit_scale<HALF>(ks, at.k, fits);
+        unsigned some = 0;  // not zero
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-            lds.k[k_place<D>(key, r * (D / 32) + i)] = uint4{fp4_bf16<0>(k[i], kscale), fp4_bf16<1>(k[i], kscale),
-                                                            fp4_bf16<2>(k[i], kscale), fp4_bf16<3>(k[i], kscale)};
+        for (int i = 0; i < D / 32; ++i) {
+            some |= k[i];
+            lds.k[k_place<D>(key, r * (D / 32) + i)] = uint4{fp4_pair16<HALF, 0>(k[i], kscale), fp4_pair16<HALF, 1>(k[i], kscale),
+                                                            fp4_pair16<HALF, 2>(k[i], kscale), fp4_pair16<HALF, 3>(k[i], kscale)};
+        }
+        bool all = fits || (!(some & 0x77777777) && ks <= kMostScale) || key >= keys;
         const int quad = thread >> 4, col = thread & 15;
         float scale[4];
         unsigned w[4], bad = 0;
@@ -119,7 +172,8 @@ struct Raw {
             const bool spoilt = byte > kMostScale;
             bad |= spoilt ? 1u << (8 * i) : 0;
             w[i] = spoilt ? 0 : v[i];  // zero in the products
-            scale[i] = spoilt ? 1.0f : scale_of(byte);
+            scale[i] = unit_scale<HALF>(spoilt ? 127 : byte, at.v, fits);
+            all &= fits || !(w[i] & 0x77777777) || 4 * quad + i >= keys;
         }
         if (col % (16 / (D / 32)) == 0) lds.flags[16 * (col * D / 512) + quad] = bad;
         if ((thread & 63) == 0) lds.flags[16 * (D / 32) + (thread >> 6)] = there ? 0 : 1;
@@ -129,8 +183,8 @@ struct Raw {
         uint2 *to = (uint2 *)lds.v;
         auto pair = [&](auto X) {
             constexpr int x = decltype(X)::value;
-            const unsigned a = fp4_bf16<x>(w[0], scale[0]), b = fp4_bf16<x>(w[1], scale[1]);
-            const unsigned e = fp4_bf16<x>(w[2], scale[2]), f = fp4_bf16<x>(w[3], scale[3]);
+            const unsigned a = fp4_pair16<HALF, x>(w[0], scale[0]), b = fp4_pair16<HALF, x>(w[1], scale[1]);
+            const unsigned e = fp4_pair16<HALF, x>(w[2], scale[2]), f = fp4_pair16<HALF, x>(w[3], scale[3]);
             const int d = col * (D / 16) + 2 * x;
             to[2 * v_place<D>(d, piece) + half] = uint2{__builtin_amdgcn_perm(b, a, 0x05040100), __builtin_amdgcn_perm(f, e, 0x05040100)};
             to[2 * v_place<D>(d + 1, piece) + half] = uint2{__builtin_amdgcn_perm(b, a, 0x07060302), __builtin_amdgcn_perm(f, e, 0x07060302)};
@@ -141,12 +195,15 @@ struct Raw {
             pair(std::integral_constant<int, 2>{});
             pair(std::integral_constant<int, 3>{});
         }
+        return all || !there;
     }
 };
 
+template <bool HALF>
 __device__ __forceinline__ f32x16 mfma32(uint4 a, u32x4 b, f32x16 c)
 {
-    return mfma_32x32x16(u32x4{a.x, a.y, a.z, a.w}, b, c);
+    if constexpr (HALF) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return mfma_32x32x16(u32x4{a.x, a.y, a.z, a.w}, b, c);
 }
 
 // Two floats' upper halves as a packed pair.
@@ -159,8 +216,44 @@ __device__ __forceinline__ float lower_part(float x)
     return x - __builtin_bit_cast(float, float_bits(x) & 0xffff0000u);
 }
 
-// KW = 1: 128 rows, every wave takes all keys of a tile.  KW = 2: 64 rows, a wave
-// takes 32 keys of a tile, and pairs of waves join at the end.
+// Parts of an fp32 operand, and a pair of its elements cut into them.
+template <bool HALF>
+constexpr int kParts = HALF ? 2 : 3;
+template <bool HALF>
+__device__ __forceinline__ void cut_pair(float x0, float x1, u32x4 (&to)[kParts<HALF>], int i)
+{
+    if constexpr (HALF) {
+        const f16x2 hi = __builtin_convertvector((f32x2{x0, x1}), f16x2);
+        float minus = -1.0f;
+        asm("" : "+s"(minus));  // not seen to be -1: x - hi is one instruction (v_fma_mix), not two
+        const f16x2 lo = __builtin_convertvector((f32x2{fmaf((float)hi[0], minus, x0), fmaf((float)hi[1], minus, x1)}), f16x2);
+        to[0][i] = __builtin_bit_cast(unsigned, hi);
+        to[1][i] = __builtin_bit_cast(unsigned, lo);
+    } else {
+        to[0][i] = upper_halves(x0, x1);
+        x0 = lower_part(x0), x1 = lower_part(x1);
+        to[1][i] = upper_halves(x0, x1);
+        x0 = lower_part(x0), x1 = lower_part(x1);
+        to[2][i] = upper_halves(x0, x1);
+    }
+}
+
+// Units near the scales of a piece's first tokens.
+__device__ __forceinline__ Units units_at(const KvCache &c, int64_t at)
+{
+    typedef const __attribute__((address_space(4))) unsigned *scalar;
+    auto most = [&](const uint8_t *p) {
+        const unsigned w = *(scalar)(uintptr_t)(p + max(at, (int64_t)0) * c.D / 32);
+        const unsigned top = max(max(w & 0xff, w >> 8 & 0xff), max(w >> 16 & 0xff, w >> 24));
+        return (int)(at < 0 || top > kMostScale ? 127 : min(top + 5, (unsigned)kMostScale));
+    };
+    return {most(c.k_scales), most(c.v_scales)};
+}
+
+// KW = 1: 128 rows, every wave takes all keys of a tile.  KW = 2, up to 64 rows: a
+// wave takes 32 keys of a tile, and pairs of waves join at the end (64 rows of 8 x 8
+// heads of 128 over 4096 keys: 42 us, with KW = 1 61; 65 rows and more would convert
+// every tile twice).
 template <int D, int KW>
 __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kernel(KvAttnArgs a)
 {
@@ -191,129 +284,161 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
     const int sure = min(keys, limit_of(a, sp, len, a.by_group.of(wave_row)));
     const int seen = a.by_group.of(wave_row) < sp.count ? min(keys, limit_of(a, sp, len, a.by_group.of(wave_row + 31))) : 0;
 
-    u32x4 q[KS][3];
-    {
-        const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + 8 * half;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const f32x4 x = valid ? *(const f32x4 *)(src + 16 * s + 4 * i) : f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float x0 = x[2 * j], x1 = x[2 * j + 1];
-                    q[s][0][2 * i + j] = upper_halves(x0, x1);
-                    x0 = lower_part(x0), x1 = lower_part(x1);
-                    q[s][1][2 * i + j] = upper_halves(x0, x1);
-                    x0 = lower_part(x0), x1 = lower_part(x1);
-                    q[s][2][2 * i + j] = upper_halves(x0, x1);
-                }
-            }
-    }
-
-    f32x16 acc[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = zero16();
-    float m = kNone, l = 0.0f;
-
     const int n = (keys + kTile - 1) / kTile;
     const int first = __builtin_amdgcn_readfirstlane(pl.piece * plan.per);
     const int end = pl.piece + 1 < pl.pieces ? min(n, first + plan.per) : n;
 
-    auto block = [&](const Lds<D> &at, int key0, auto KB) {
-        constexpr int kb = decltype(KB)::value;
-        f32x16 s = zero16();
-        if (D < 128) __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-        for (int x = 0; x < KS; ++x) {
-            const uint4 k = at.k[k_place<D>(32 * kb + l32, 2 * x + half)];
-#pragma unroll
-            for (int part = 2; part >= 0; --part) s = mfma32(k, q[x][part], s);
+    f32x16 acc[DB];
+    float m, l;
+    auto piece_at = [&](int tl) { return tl < end ? row_of(a.c, b, h, tl * kTile + 16 * wave) : -1; };
+    // The piece's tiles; false if a value does not fit (then the sums are worth nothing).
+    auto walk = [&](auto H) -> bool {
+        constexpr bool HALF = decltype(H)::value;
+        constexpr int P = kParts<HALF>;
+        Raw<D> raw;
+        bool fits = true;
+        Units units16 = {127, 127};
+        if (first < end) {
+            raw.load(a.c, piece_at(first), threadIdx.x);
+            if (HALF) units16 = units_at(a.c, row_of(a.c, b, h, first * kTile));
         }
-        // Vector work goes before other waves' products, which fill the time beside
-        // it (D = 64: 78.0 -> 76.1 us at 512 rows of 4 x 16 heads over 4096; D = 128,
-        // with two waves to choose from: 499 -> 503).
-        if (D < 128) __builtin_amdgcn_s_setprio(1);
-        const bool partly = key0 + 32 > sure || (at.flags[16 * DB + 2 * kb] | at.flags[16 * DB + 2 * kb + 1]);
-        if (__builtin_amdgcn_readfirstlane(partly)) {
+        u32x4 q[KS][P];
+        float scale2 = a.scale2;
+        {
+            const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + 8 * half;
+            f32x4 x[KS][2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (key0 + acc_row(i, half) >= limit || at.flags[16 * DB + 2 * kb + i / 8]) s[i] = -INFINITY;
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) x[s][i] = valid ? *(const f32x4 *)(src + 16 * s + 4 * i) : f32x4{0, 0, 0, 0};
+            int shift = 0;
+            if (HALF) {
+                float most = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
+                shift = 14 + 127 - (int)(float_bits(most) >> 23);
+                scale2 = fminf(fmaxf(ldexpf(scale2, units16.k - 127 - shift), 1e-37f), 3.4e38f);
+            }
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float x0 = x[s][i][2 * j], x1 = x[s][i][2 * j + 1];
+                        cut_pair<HALF>(HALF ? ldexpf(x0, shift) : x0, HALF ? ldexpf(x1, shift) : x1, q[s], 2 * i + j);
+                    }
         }
-        float top = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top *= a.scale2;
-        if (__any(top > m + kRaise)) {
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            l *= f;
+        for (int d = 0; d < DB; ++d) acc[d] = zero16();
+        m = kNone, l = 0.0f;
+        auto block = [&](const Lds<D> &at, int key0, auto KB) {
+            constexpr int kb = decltype(KB)::value;
+            constexpr float up = HALF ? 7.0f : 0.0f;  // the weights' unit: 2^-7
+            f32x16 s = zero16();
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) {
+                const uint4 k = at.k[k_place<D>(32 * kb + l32, 2 * x + half)];
+#pragma unroll
+                for (int part = P - 1; part >= 0; --part) s = mfma32<HALF>(k, q[x][part], s);
+            }
+            // Vector work goes before other waves' products, which fill the time beside
+            // it (D = 64: 66.7 -> 65.2 us at 512 rows of 4 x 16 heads over 4096; D = 128,
+            // 2 x 1024 rows of 32 / 8 heads over 8192: 360.4 -> 357.9).
+            __builtin_amdgcn_s_setprio(1);
+            const bool partly = key0 + 32 > sure || (at.flags[16 * DB + 2 * kb] | at.flags[16 * DB + 2 * kb + 1]);
+            if (__builtin_amdgcn_readfirstlane(partly)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + acc_row(i, half) >= limit || at.flags[16 * DB + 2 * kb + i / 8]) s[i] = -INFINITY;
+            }
+            float top = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+            top *= scale2;
+            if (__any(top > m + kRaise)) {
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                u32x4 p[P];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i], scale2, up - m));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i + 1], scale2, up - m));
+                    l += e0;
+                    l += e1;
+                    cut_pair<HALF>(e0, e1, p, i);
+                }
+                constexpr int NP = DB < 2 ? 1 : 2;  // products in turn, so that none waits for the one before
+#pragma unroll
+                for (int d = 0; d < DB; d += NP) {
+                    uint4 v[NP];
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) v[j] = at.v[v_place<D>(32 * (d + j) + l32, 2 * (2 * kb + st) + half)];
+#pragma unroll
+                    for (int part = P - 1; part >= 0; --part)
+#pragma unroll
+                        for (int j = 0; j < NP; ++j) acc[d + j] = mfma32<HALF>(v[j], p[part], acc[d + j]);
+                }
+            }
+        };
+
+        auto put = [&](int tl) {
+            fits &= raw.template put<HALF>(lds[(tl - first) & 1], threadIdx.x, units16, keys - tl * kTile);
+        };
+        if (first < end) {
+            put(first);
+            if (first + 1 < end) raw.load(a.c, piece_at(first + 1), threadIdx.x);
+            __syncthreads();
+        }
+        for (int tl = first; tl < end; ++tl) {
+            const Lds<D> &at = lds[(tl - first) & 1];
+            if (tl + 1 < end) {
+                put(tl + 1);
+                if (tl + 2 < end) raw.load(a.c, piece_at(tl + 2), threadIdx.x);
+            }
+            const int key0 = tl * kTile;
+            if (key0 < seen) {
+                // Values that are no numbers: NaN for the rows that see them.
+                unsigned bad = lane < 16 * DB ? at.flags[lane] : 0;
+                if (__any(bad)) {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+                        for (int x = 0; x < kTile; ++x)
+                            if ((at.flags[16 * d + x / 4] >> (8 * (x & 3)) & 1) && key0 + x < limit && !at.flags[16 * DB + x / 16])
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) acc[d][i] = NAN;
+                }
+                if (KW == 1 || wave % 2 == 0) block(at, key0, std::integral_constant<int, 0>{});
+                if ((KW == 1 || wave % 2 == 1) && key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
+            }
+            __syncthreads();
+        }
+        if (HALF) {
+            m -= 7.0f;
+            const float unit = scale_of(units16.v);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+                for (int i = 0; i < 16; ++i) acc[d][i] *= unit;
         }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-            u32x4 p[3];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i], a.scale2, -m));
-                float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i + 1], a.scale2, -m));
-                l += e0;
-                l += e1;
-                p[0][i] = upper_halves(e0, e1);
-                e0 = lower_part(e0), e1 = lower_part(e1);
-                p[1][i] = upper_halves(e0, e1);
-                e0 = lower_part(e0), e1 = lower_part(e1);
-                p[2][i] = upper_halves(e0, e1);
-            }
-            constexpr int NP = DB < 2 ? 1 : 2;  // products in turn, so that none waits for the one before
-#pragma unroll
-            for (int d = 0; d < DB; d += NP) {
-                uint4 v[NP];
-#pragma unroll
-                for (int j = 0; j < NP; ++j) v[j] = at.v[v_place<D>(32 * (d + j) + l32, 2 * (2 * kb + st) + half)];
-#pragma unroll
-                for (int part = 2; part >= 0; --part)
-#pragma unroll
-                    for (int j = 0; j < NP; ++j) acc[d + j] = mfma32(v[j], p[part], acc[d + j]);
-            }
-        }
+        return !HALF || __syncthreads_and(fits);
     };
-
-    auto piece_at = [&](int tl) { return tl < end ? row_of(a.c, b, h, tl * kTile + 16 * wave) : -1; };
-    Raw<D> raw;
-    if (first < end) {
-        raw.load(a.c, piece_at(first), threadIdx.x);
-        raw.put(lds[0], threadIdx.x);
-        if (first + 1 < end) raw.load(a.c, piece_at(first + 1), threadIdx.x);
-        __syncthreads();
-    }
-    for (int tl = first; tl < end; ++tl) {
-        const Lds<D> &at = lds[(tl - first) & 1];
-        if (tl + 1 < end) {
-            raw.put(lds[(tl - first + 1) & 1], threadIdx.x);
-            if (tl + 2 < end) raw.load(a.c, piece_at(tl + 2), threadIdx.x);
-        }
-        const int key0 = tl * kTile;
-        if (key0 < seen) {
-            // Values that are no numbers: NaN for the rows that see them.
-            unsigned bad = lane < 16 * DB ? at.flags[lane] : 0;
-            if (__any(bad)) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    for (int x = 0; x < kTile; ++x)
-                        if ((at.flags[16 * d + x / 4] >> (8 * (x & 3)) & 1) && key0 + x < limit && !at.flags[16 * DB + x / 16])
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[d][i] = NAN;
-            }
-            if (KW == 1 || wave % 2 == 0) block(at, key0, std::integral_constant<int, 0>{});
-            if ((KW == 1 || wave % 2 == 1) && key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
-        }
-        __syncthreads();
-    }
+    if (!walk(std::true_type{})) walk(std::false_type{});
     l += __shfl_xor(l, 32, 64);
 
     auto take_in = [&](float m1, float l1, auto value) {  // another part of this wave's rows

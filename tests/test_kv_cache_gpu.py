@@ -267,6 +267,27 @@ def test_scores_of_all_sizes():
     p.check_attention(q, True, scale=0.0, start=[155])
 
 
+@pytest.mark.parametrize("first", [0, -17, -19, -40, 17, 19, 40])
+@pytest.mark.parametrize("D, T", [(32, 21), (64, 50), (128, 50)])
+def test_many_rows_over_scales_far_apart(D, T, first):
+    """Tokens and groups of very different sizes: the first token's keys and values
+    are about 2^first times the others'."""
+    rng = np.random.default_rng(D + first + 40)
+    L = 200
+    tab, pages = table(rng, 2, 13)
+    p = Pair(pages, 2, 16, D, tab)
+    sizes = lambda spread: 2.0 ** rng.integers(-spread, spread + 1, (2, L, 2, D // 32)).repeat(32, -1)  # noqa: E731
+    groups = 2.0 ** rng.integers(-5, 6, D // 32).repeat(32)
+    k, v = normal(rng, 2, L, 2, D) / groups, normal(rng, 2, L, 2, D) * sizes(6)
+    k *= 2.0 ** np.minimum(-first, 0)
+    k[:, 0] *= 2.0 ** first
+    v[:, 0] *= 2.0 ** first
+    k[1, 5:20] = 0
+    v[1, 60:70] = -0.0
+    p.write(k.astype(np.float32), v.astype(np.float32))
+    p.check_attention((normal(rng, 2, T, 6, D) * groups).astype(np.float32), True, start=[L - T, 60])
+
+
 def test_a_row_of_q_that_is_no_number():
     rng = np.random.default_rng(9)
     p = filled(rng, 1, 1, 16, 64, 40)
