@@ -52,8 +52,7 @@ constexpr int per_cu(int D, int rows)
 {
     return D == 128 && rows == 8 ? 3 : 4;
 }
-constexpr int kLeast = 8;  // tiles of a piece: two for each wave
-constexpr int kFewRows = 40;
+constexpr int kLeast = 8;  // tiles of a piece: two for each wave, so that the loads of one run beside the other
 
 // Units that are cut: how many of their workgroups are done.  Zero between
 // calls: the last one, which all the others have added to, clears its unit's.
@@ -481,6 +480,17 @@ int launch_rows(KvAttnArgs &a)
     return rows <= 2 ? launch<D, 2>(a) : rows <= 4 ? launch<D, 4>(a) : launch<D, 8>(a);
 }
 
+// Rows of a cache head beyond which the kernel for many rows takes over: it walks
+// the keys once for 64 rows, this one for 8, but its start is longer, which shows
+// where the sequences' heads do not fill the chip by themselves.  This one and that
+// one (us): 256 heads of 64 over 2048, 32 rows 30.5 and 24.0; of 128, 28 rows 43.3 and
+// 36.3; 512 of 64, 24 rows 43.0 and 44.5.  128 heads of 128, 28 rows 27.0 and 28.2, 40
+// rows 32.3 and 30.8; 16 of 64 over 8192, 40 rows 18.9 and 26.2.
+int few_rows(const KvCache &c)
+{
+    return (int64_t)c.sequences * c.heads >= device_cu_count() ? 24 : 40;
+}
+
 }  // namespace
 
 int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
@@ -529,6 +539,6 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     // Above 0, so that a masked score stays -infinity under it; a scale of 0 then
     // gives scores that differ by nothing.
     a.scale2 = std::min(std::max(scale * kLog2e, 1e-37f), 3.4e38f);
-    if (T * a.group > kFewRows) return launch_kv_attention_rows(a);
+    if (T * a.group > few_rows(a.c)) return launch_kv_attention_rows(a);
     return a.c.D == 128 ? launch_rows<128>(a) : a.c.D == 64 ? launch_rows<64>(a) : launch_rows<32>(a);
 }
