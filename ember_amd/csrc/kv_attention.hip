@@ -501,11 +501,14 @@ int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
     if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
     a.by_group = Divisor(a.group), a.by_tiles = Divisor(a.tiles), a.by_units = Divisor(a.c.heads * a.tiles);
     // One round of workgroups over the chip; where the units alone are about as
-    // many, two pieces each, so that the longest sequence does not decide.  With
-    // many units, or where the pieces' results were large, none is cut.
+    // many, two pieces each, so that the longest sequence does not decide; but no
+    // more than the page table has room for.  With many units, where the pieces'
+    // results were large, or where no sequence can be longer than a piece, none is
+    // cut (and none plans: one token of 4 heads of 64 over 256 5.8 -> 5.0 us).
     const int64_t slots = (int64_t)per_cu * std::max(device_cu_count(), 1);
-    const int64_t blocks = std::max(slots, 2 * all), bytes = blocks * rows * (a.c.D + 2) * (int64_t)sizeof(float);
-    const bool cut = a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * slots) && bytes <= kMostScratch;
+    const int64_t longest = (((int64_t)a.c.max_pages << a.c.page_shift) + keys - 1) / keys, pieces = (longest + least - 1) / least;
+    const int64_t blocks = std::min(std::max(slots, 2 * all), all * pieces), bytes = blocks * rows * (a.c.D + 2) * (int64_t)sizeof(float);
+    const bool cut = pieces > 1 && a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * slots) && bytes <= kMostScratch;
     a.blocks = (int)(cut ? blocks : all);
     if (cut) {
         a.part = (float *)scratch(kScratchKvAttention, (size_t)bytes);
