@@ -21,7 +21,7 @@
 // piece's first token; where a value that a row sees fits no fp16 (far larger or
 // smaller than that, or no number), the workgroup walks its keys again with bf16
 // values, which hold them all, and three parts.
-//   2 x 1024 rows of 32 / 8 heads of 128 over 8192: two fp16 parts 356 us, three bf16 ones
+//   2 x 1024 rows of 32 / 8 heads of 128 over 8192: two fp16 parts 352 us, three bf16 ones
 //   486, and both, where every piece has such a value, 2.1 times the first's.
 // Two tiles of LDS: while one is worked on, the next is converted into the other
 // and the one after is loaded; one barrier a tile.
@@ -32,9 +32,11 @@
 // in the same banks.
 //
 // Work: 8 * T * keys * D matrix operations a head where 4 are the definition's.
-// Bound by the matrix cores: 2 x 1024 rows of 32 / 8 heads of 128 over 8192 keys, causal,
-// 356 us, 557 TFLOP/s of the definition's and 1.11 PFLOP/s of fp16; 4 x 512 rows of 16
-// heads of 64 over 4096 65 us.
+// Bound by power: 2 x 1024 rows of 32 / 8 heads of 128 over 8192 keys, causal, take 352
+// us, 563 TFLOP/s of the definition's and 1.13 PFLOP/s of fp16 at about 1.9 GHz (a large
+// bf16 library product reaches 1.23), the matrix cores busy half of the time and the
+// vector units the other, however the two are mixed; 4 x 512 rows of 16 heads of 64 over
+// 4096 64 us.
 #include <type_traits>
 
 #include "kv_attention.h"
@@ -350,9 +352,12 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
             }
             // Vector work goes before other waves' products, which fill the time beside
             // it (D = 64: 66.7 -> 65.2 us at 512 rows of 4 x 16 heads over 4096; D = 128,
-            // 2 x 1024 rows of 32 / 8 heads over 8192: 360.4 -> 357.9).
+            // 2 x 1024 rows of 32 / 8 heads over 8192: 360.4 -> 357.9).  Both halves'
+            // scores before the weights gave nothing (351 and 357).
             __builtin_amdgcn_s_setprio(1);
-            const bool partly = key0 + 32 > sure || (at.flags[16 * DB + 2 * kb] | at.flags[16 * DB + 2 * kb + 1]);
+            bool partly = key0 + 32 > sure;  // (no branch: the flags are read early)
+            partly |= at.flags[16 * DB + 2 * kb] != 0;
+            partly |= at.flags[16 * DB + 2 * kb + 1] != 0;
             if (__builtin_amdgcn_readfirstlane(partly)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -413,8 +418,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
             }
             const int key0 = tl * kTile;
             if (key0 < seen) {
+                const unsigned bad = lane < 16 * DB ? at.flags[lane] : 0;
+                if (KW == 1 || wave % 2 == 0) block(at, key0, std::integral_constant<int, 0>{});
+                if ((KW == 1 || wave % 2 == 1) && key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
                 // Values that are no numbers: NaN for the rows that see them.
-                unsigned bad = lane < 16 * DB ? at.flags[lane] : 0;
                 if (__any(bad)) {
 #pragma unroll
                     for (int d = 0; d < DB; ++d)
@@ -423,8 +430,6 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) acc[d][i] = NAN;
                 }
-                if (KW == 1 || wave % 2 == 0) block(at, key0, std::integral_constant<int, 0>{});
-                if ((KW == 1 || wave % 2 == 1) && key0 + 32 < seen) block(at, key0 + 32, std::integral_constant<int, 1>{});
             }
             __syncthreads();
         }
