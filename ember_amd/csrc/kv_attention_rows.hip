@@ -94,7 +94,10 @@ struct Units {
 template <bool HALF>
 __device__ __forceinline__ float unit_scale(unsigned byte, int unit, bool &fits)
 {
-    if (!HALF) return scale_of(byte);
+    if (!HALF) {
+        fits = byte <= kMostScale;
+        return scale_of(byte);
+    }
     const int over = (int)byte - unit, to = min(max(over, kLeastUnit), kMostUnit);
     fits = to == over;
     return scale_of(to + 127);
@@ -164,18 +167,25 @@ struct Raw {
             lds.k[k_place<D>(key, r * (D / 32) + i)] = uint4{fp4_pair16<HALF, 0>(k[i], kscale), fp4_pair16<HALF, 1>(k[i], kscale),
                                                             fp4_pair16<HALF, 2>(k[i], kscale), fp4_pair16<HALF, 3>(k[i], kscale)};
         }
-        bool all = fits || (!(some & 0x77777777) && ks <= kMostScale) || key >= keys;
+        bool all = !HALF || fits || (!(some & 0x77777777) && ks <= kMostScale) || key >= keys;
         const int quad = thread >> 4, col = thread & 15;
         float scale[4];
-        unsigned w[4], bad = 0;
+        unsigned w[4], byte[4], bad = 0;
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned byte = (vs[i * D / 128] >> (8 * ((i * (D / 32) & 3) + col * D / 512))) & 0xff;
-            const bool spoilt = byte > kMostScale;
-            bad |= spoilt ? 1u << (8 * i) : 0;
-            w[i] = spoilt ? 0 : v[i];  // zero in the products
-            scale[i] = unit_scale<HALF>(spoilt ? 127 : byte, at.v, fits);
-            all &= fits || !(w[i] & 0x77777777) || 4 * quad + i >= keys;
+            byte[i] = (vs[i * D / 128] >> (8 * ((i * (D / 32) & 3) + col * D / 512))) & 0xff;
+            w[i] = v[i];
+            scale[i] = unit_scale<HALF>(byte[i], at.v, fits);
+            odd |= !fits;
+        }
+        if (odd) {  // seldom
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                unit_scale<HALF>(byte[i], at.v, fits);
+                if (byte[i] > kMostScale) w[i] = 0, scale[i] = 1.0f, bad |= 1u << (8 * i);  // zero in the products
+                else all &= fits || !(w[i] & 0x77777777) || 4 * quad + i >= keys;
+            }
         }
         if (col % (16 / (D / 32)) == 0) lds.flags[16 * (col * D / 512) + quad] = bad;
         if ((thread & 63) == 0) lds.flags[16 * (D / 32) + (thread >> 6)] = there ? 0 : 1;
@@ -240,14 +250,15 @@ __device__ __forceinline__ void cut_pair(float x0, float x1, u32x4 (&to)[kParts<
     }
 }
 
-// Units near the scales of a piece's first tokens.
+// Units near the scales of a piece's first tokens; the bytes past kMostScale, of what
+// is no number, fit none.
 __device__ __forceinline__ Units units_at(const KvCache &c, int64_t at)
 {
     typedef const __attribute__((address_space(4))) unsigned *scalar;
     auto most = [&](const uint8_t *p) {
         const unsigned w = *(scalar)(uintptr_t)(p + max(at, (int64_t)0) * c.D / 32);
         const unsigned top = max(max(w & 0xff, w >> 8 & 0xff), max(w >> 16 & 0xff, w >> 24));
-        return (int)(at < 0 || top > kMostScale ? 127 : min(top + 5, (unsigned)kMostScale));
+        return (int)(at < 0 || top > kMostScale ? 127 : min(top + 5, (unsigned)(kMostScale - kMostUnit)));
     };
     return {most(c.k_scales), most(c.v_scales)};
 }
@@ -402,18 +413,17 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
             }
         };
 
-        auto put = [&](int tl) {
-            fits &= raw.template put<HALF>(lds[(tl - first) & 1], threadIdx.x, units16, keys - tl * kTile);
+        auto put = [&](int tl, Lds<D> &to) {
+            fits &= raw.template put<HALF>(to, threadIdx.x, units16, keys - tl * kTile);
         };
         if (first < end) {
-            put(first);
+            put(first, lds[0]);
             if (first + 1 < end) raw.load(a.c, piece_at(first + 1), threadIdx.x);
             __syncthreads();
         }
-        for (int tl = first; tl < end; ++tl) {
-            const Lds<D> &at = lds[(tl - first) & 1];
+        auto step = [&](int tl, const Lds<D> &at, Lds<D> &other) {
             if (tl + 1 < end) {
-                put(tl + 1);
+                put(tl + 1, other);
                 if (tl + 2 < end) raw.load(a.c, piece_at(tl + 2), threadIdx.x);
             }
             const int key0 = tl * kTile;
@@ -432,6 +442,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                 }
             }
             __syncthreads();
+        };
+        for (int tl = first; tl < end; tl += 2) {  // (so that places in LDS are the same each time)
+            step(tl, lds[0], lds[1]);
+            if (tl + 1 < end) step(tl + 1, lds[1], lds[0]);
         }
         if (HALF) {
             m -= 7.0f;
