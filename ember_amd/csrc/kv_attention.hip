@@ -190,12 +190,13 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
                 for (int i = 0; i < 2; ++i) raw[s][i] = *(const f32x4 *)(src + 8 * s + 4 * i);
         }
         int64_t at[2], ahead[2];
+        int page[2];  // of the next tile: both lookups are on their way together, beside the products
         Keys<D> kk[2];
         Values<D> vv[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             at[j] = row_of(a.c, b, h, tl * kTile + 16 * j);
-            ahead[j] = row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j);
+            page[j] = page_of(a.c, b, (tl + kWaves) * kTile + 16 * j);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) kk[j].load(a.c, at[j], lane);
@@ -262,7 +263,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
             if (ROWS == 2) s[0] = r >> 1 ? s[1] : s[0];
             if constexpr (more.value) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) kk[j].load(a.c, ahead[j], lane);
+                for (int j = 0; j < 2; ++j) {
+                    ahead[j] = row_on(a.c, page[j], h, (tl + kWaves) * kTile + 16 * j);
+                    kk[j].load(a.c, ahead[j], lane);
+                }
             }
             const bool partly = tl * kTile + kTile > sure || at[0] < 0 || at[1] < 0;
             if (partly) {
@@ -276,13 +280,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
             top *= a.scale2;
             if (__any(top > m + kRaise)) {
                 // The lanes of a row: 16 neighbours (and as many 32 on), or those 16 apart.
-                if (SHARED) {
-#pragma unroll
-                    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-                } else {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                }
-                if (ROWS != 4) top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const auto most = [](float x, float y) { return fmaxf(x, y); };
+                top = SHARED ? row_all(top, most) : across_16(top, most);
+                if (ROWS != 4) top = across_32(top, most);
                 const float to = fmaxf(m, top);
                 float f = __builtin_amdgcn_exp2f(m - to);
                 m = to;
@@ -377,20 +377,16 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
                 for (int j = 0; j < 2; ++j) {
                     vv[j].load(a.c, ahead[j], lane);
                     at[j] = ahead[j];
-                    ahead[j] = row_of(a.c, b, h, (tl + kWaves) * kTile + 16 * j);  // past the end: not used
+                    page[j] = page_of(a.c, b, (tl + kWaves) * kTile + 16 * j);  // past the end: not used
                 }
             }
         };
         while (tl + kWaves < end) step(std::true_type{});
         step(std::false_type{});
     }
-    if (SHARED) {
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-    } else {
-        l += __shfl_xor(l, 16, 64);
-    }
-    if (ROWS != 4) l += __shfl_xor(l, 32, 64);
+    const auto sum2 = [](float x, float y) { return x + y; };
+    l = SHARED ? row_all(l, sum2) : across_16(l, sum2);
+    if (ROWS != 4) l = across_32(l, sum2);
     if (SHARED ? col == 0 && r < ROWS : !odd && r == 0) stat[wave][s_row][0] = m, stat[wave][s_row][1] = l;
 
     // Join the parts, and the waves.

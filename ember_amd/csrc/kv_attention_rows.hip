@@ -303,6 +303,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
 
     f32x16 acc[DB];
     float m, l;
+    const auto larger = [](float x, float y) { return fmaxf(x, y); };
     auto piece_at = [&](int tl) { return tl < end ? row_of(a.c, b, h, tl * kTile + 16 * wave) : -1; };
     // The piece's tiles; false if a value does not fit (then the sums are worth nothing).
     auto walk = [&](auto H) -> bool {
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
-                most = fmaxf(most, __shfl_xor(most, 32, 64));
+                most = across_32(most, larger);
                 shift = 14 + 127 - (int)(float_bits(most) >> 23);
                 scale2 = fminf(fmaxf(ldexpf(scale2, units16.k - 127 - shift), 1e-37f), 3.4e38f);
             }
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
             for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
             top *= scale2;
             if (__any(top > m + kRaise)) {
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                top = across_32(top, larger);
                 const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
                 m = to;
                 l *= f;
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
         return !HALF || __syncthreads_and(fits);
     };
     if (!walk(std::true_type{})) walk(std::false_type{});
-    l += __shfl_xor(l, 32, 64);
+    l = across_32(l, [](float x, float y) { return x + y; });
 
     auto take_in = [&](float m1, float l1, auto value) {  // another part of this wave's rows
         const float to = fmaxf(m, m1), f = __builtin_amdgcn_exp2f(m - to), e = __builtin_amdgcn_exp2f(m1 - to);

@@ -54,18 +54,24 @@ __device__ __forceinline__ Span span_of(const int32_t *start, const int32_t *cou
     return {start ? start[b] : 0, min(max(n, 0), T)};
 }
 
-// The first row of 16 tokens (pos a multiple of 16: pages hold them whole) of
-// head h, or -1; the table has a page at least.  b, h and pos are the same in all
-// lanes, so the table is read through the scalar cache, and without a branch, so
-// that several lookups are on their way together.
-__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
+// The page that the table names for 16 tokens of a sequence (pos a multiple of 16:
+// pages hold them whole; the table has a page at least, and the last one stands
+// for those past it).  b and pos are the same in all lanes, so the table is read
+// through the scalar cache.
+__device__ __forceinline__ int page_of(const KvCache &c, int b, int pos)
 {
     typedef const __attribute__((address_space(4))) int32_t *scalar;
-    const int place = pos >> c.page_shift;
-    const bool in = (unsigned)place < (unsigned)c.max_pages;
-    const int page = ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + (in ? place : 0)];
+    return ((scalar)(uintptr_t)c.table)[(int64_t)b * c.max_pages + min(pos >> c.page_shift, c.max_pages - 1)];
+}
+// Their first row of head h, or -1 where there is no such page.
+__device__ __forceinline__ int64_t row_on(const KvCache &c, int page, int h, int pos)
+{
     const int64_t row = (((int64_t)page * c.heads + h) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
-    return in && (unsigned)page < (unsigned)c.pages ? row : -1;
+    return (unsigned)page < (unsigned)c.pages ? row : -1;
+}
+__device__ __forceinline__ int64_t row_of(const KvCache &c, int b, int h, int pos)
+{
+    return row_on(c, page_of(c, b, pos), h, pos);
 }
 
 // The scale that a byte stands for.

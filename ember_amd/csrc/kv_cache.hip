@@ -93,7 +93,7 @@ __device__ __forceinline__ Task task_of(const CopyArgs &a, unsigned i)
     k.which = pair & 1;
     k.sp = span_of(a.start, a.count, k.b, a.T);
     k.pos = ((int64_t)(k.sp.start >> 4) + piece) << 4;
-    k.at = k.pos >= 0 && k.pos <= 0x7fffffff && a.c.max_pages ? row_of(a.c, k.b, k.h, (int)k.pos) : -1;
+    k.at = k.pos >= 0 && k.pos >> a.c.page_shift < a.c.max_pages ? row_of(a.c, k.b, k.h, (int)k.pos) : -1;
     k.first = i == 0;
     return k;
 }

@@ -46,6 +46,29 @@ __device__ __forceinline__ float wave_max(float v)
     return wave_all(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// f over the 16 neighbouring lanes that a lane is of, the same in each of them.
+template <class F>
+__device__ __forceinline__ float row_all(float v, F f)
+{
+    v = f(v, lane_below<0x121, 0xf>(v, v));  // from 1, 2, 4 and 8 lanes below, around the 16
+    v = f(v, lane_below<0x122, 0xf>(v, v));
+    v = f(v, lane_below<0x124, 0xf>(v, v));
+    return f(v, lane_below<0x128, 0xf>(v, v));
+}
+// f of a lane's value and that of the lane 16 (32) from it, in both.
+template <class F>
+__device__ __forceinline__ float across_16(float v, F f)
+{
+    const auto x = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    return f(__builtin_bit_cast(float, (unsigned)x[0]), __builtin_bit_cast(float, (unsigned)x[1]));
+}
+template <class F>
+__device__ __forceinline__ float across_32(float v, F f)
+{
+    const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    return f(__builtin_bit_cast(float, (unsigned)x[0]), __builtin_bit_cast(float, (unsigned)x[1]));
+}
+
 // What the lanes of a wave have written to LDS is there for all of them.
 __device__ __forceinline__ void wave_sync()
 {
