@@ -30,13 +30,20 @@
 //   their columns: (row, even or odd, part), three parts of two rows, or two of
 //   four rows with the third in a second instruction.  A tile of 32 keys takes 16 to
 //   24 matrix instructions in place of 48.
-// Measured (us), eight-row scheme and these: 32 sequences of up to 8192, one token of
-// 32 / 8 heads of 128: 41.1 and 37.8; 32 x 2048, 16 heads of 64: 19.7 and 17.2.  With
-// eight rows through LDS: 32 x 16 heads of 64, 24 rows over 2048 46.4 and 50.4.
+// Which is taken goes by a head's rows (2, 4 or more).  Measured (us), the eight-row
+// scheme and these: 32 sequences of up to 8192, one token of 32 / 8 heads of 128: 41.1
+// and 37.8; 32 x 2048, 16 heads of 64: 19.7 and 17.2.  With eight rows through LDS: 32
+// x 16 heads of 64, 24 rows over 2048 46.4 and 50.4.
 // A workgroup is 4 waves that take turns at tiles of 32 keys and join at the
 // end.  A unit's keys are cut into pieces, each with a workgroup of its own; the
 // last of them to be done (by a count that they all add to) joins the pieces, in
 // their order.
+//
+// HBM-bound where contexts are long: 17/32 byte of K and V per element.  32 sequences
+// of up to 8192, 32 / 8 heads of 128 (148 MB) take 36.5 us, 4 of up to 32768, 16 heads
+// of 128 (178 MB) 46.5, of which about 9 are the launch, the plan, the first loads and
+// the join; what is between runs at 5.5 TB/s.  16 x 5 rows over 3001, 16 heads of 64 (28
+// MB) 14.6.
 #include <algorithm>
 #include <type_traits>
 
@@ -47,7 +54,7 @@ namespace ember {
 namespace {
 
 constexpr int kTile = 32;  // keys
-// Workgroups that a CU holds at once: by their registers.
+// Workgroups that a CU holds at once: as many as their registers allow.
 constexpr int per_cu(int D, int rows)
 {
     return D == 128 && rows == 8 ? 3 : 4;
@@ -479,9 +486,10 @@ int launch_rows(KvAttnArgs &a)
 // Rows of a cache head beyond which the kernel for many rows takes over: it walks
 // the keys once for 64 rows, this one for 8, but its start is longer, which shows
 // where the sequences' heads do not fill the chip by themselves.  This one and that
-// one (us): 256 heads of 64 over 2048, 32 rows 30.5 and 24.0; of 128, 28 rows 43.3 and
-// 36.3; 512 of 64, 24 rows 43.0 and 44.5.  128 heads of 128, 28 rows 27.0 and 28.2, 40
-// rows 32.3 and 30.8; 16 of 64 over 8192, 40 rows 18.9 and 26.2.
+// one (us, over 2048 keys): 256 heads of 64, 24 rows 24.9 and 21.4, 32 rows 30.5 and
+// 24.0; 512 of 64, 16 rows 28.6 and 38.2, 24 rows 39.0 and 38.7; 512 of 128, 24 rows 60
+// and 64.  128 heads of 128, 28 rows 26.4 and 27.0, 40 rows 31.2 and 29.8; 16 of 64
+// over 8192, 40 rows 17.6 and 26.0.
 int few_rows(const KvCache &c)
 {
     return (int64_t)c.sequences * c.heads >= device_cu_count() ? 24 : 40;
