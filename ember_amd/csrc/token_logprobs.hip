@@ -217,14 +217,14 @@ __device__ __forceinline__ Sums wave_join(Sums a)
     return {a.m, wave_sum(a.s), wave_sum(a.w)};
 }
 
-// The row's results, from its sums; `best` is lane i's i-th key.  One wave.
-__device__ __forceinline__ void finish(const ScoreArgs &a, int row, Sums t, uint64_t best)
+// The row's results, from its sums and its token's logit; `best` is lane i's i-th
+// key.  One wave.
+__device__ __forceinline__ void finish(const ScoreArgs &a, int row, Sums t, bool known, float of_token, uint64_t best)
 {
     const int lane = threadIdx.x & 63;
     const float logs = logf(t.s);
     if (lane == 0) {
-        const int tok = a.tokens[row];
-        a.logp[row] = tok >= 0 && tok < a.classes ? (a.x[row * a.stride + tok] - t.m) - logs : 0.0f;
+        a.logp[row] = known ? (of_token - t.m) - logs : 0.0f;
         if (a.lse) a.lse[row] = t.m + logs;
         if (a.entropy) a.entropy[row] = logs - t.w / t.s;
     }
@@ -294,6 +294,10 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
     Sums t = {-INFINITY, 0.0f, 0.0f};
     Best best;
     load(next, piece * a.per);
+    // Beside the first chunk, not at the end, where nothing hides two loads in turn.
+    const int token = a.tokens[row];
+    const bool known = token >= 0 && token < a.classes;
+    const float of_token = p[known ? token : 0];
     for (int chunk = piece * a.per; chunk < end; ++chunk) {
         float half[2] = {-INFINITY, -INFINITY};  // the largest of 8
 #pragma unroll
@@ -348,6 +352,18 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         __syncthreads();
         if (!last) return;
         const char *from = a.part + (int64_t)index * a.pieces * size;
+        constexpr int at_once = kKeys / (4 * kNear);  // pieces
+        uint64_t k[kKeys / kThreads];
+        auto place = [&](int i, int at) { return from + (i >> 2) * size + 16 + 8 * ((i & 3) * a.top + at); };
+        // The first keys of the lists of pieces i0 .., a thread's loads on their way together.
+        auto heads = [&](int i0) {
+#pragma unroll
+            for (int j = 0; j < kKeys / kThreads; ++j) {
+                const int i = 4 * i0 + (j * kThreads + (int)threadIdx.x) / kNear, at = threadIdx.x % kNear;
+                k[j] = i < 4 * a.pieces && at < a.top ? get8(place(i, at)) : 0;
+            }
+        };
+        if (TOP) heads(0);
         t = {-INFINITY, 0.0f, 0.0f};
         for (int i = threadIdx.x; i < a.pieces; i += kThreads) {
             const uint64_t ms = get8(from + i * size), w = get8(from + i * size + 8);
@@ -358,24 +374,17 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         if (lane == 0) sums[wave] = t;
         if (TOP) {
             best = Best();
-            constexpr int at_once = kKeys / (4 * kNear);  // pieces
             for (int i0 = 0; i0 < a.pieces; i0 += at_once) {
-                const int n = 4 * min(at_once, a.pieces - i0);
-                auto place = [&](int i, int at) { return from + (i0 + (i >> 2)) * size + 16 + 8 * ((i & 3) * a.top + at); };
-                __syncthreads();
-                // The lists' first keys, all of a thread's loads in flight at once.
-                uint64_t k[kKeys / kThreads];
-#pragma unroll
-                for (int j = 0; j < kKeys / kThreads; ++j) {
-                    const int i = (j * kThreads + (int)threadIdx.x) / kNear, at = threadIdx.x % kNear;
-                    k[j] = i < n && at < a.top ? get8(place(i, at)) : 0;
+                if (i0) {
+                    __syncthreads();
+                    heads(i0);
                 }
 #pragma unroll
                 for (int j = 0; j < kKeys / kThreads; ++j) lists[j * kThreads + threadIdx.x] = k[j];
                 __syncthreads();
                 if (wave == 0)
-                    best.join(n, min(kNear, a.top), a.top, found[0],
-                              [&](int i, int at) { return at < kNear ? lists[i * kNear + at] : get8(place(i, at)); });
+                    best.join(4 * min(at_once, a.pieces - i0), min(kNear, a.top), a.top, found[0],
+                              [&](int i, int at) { return at < kNear ? lists[i * kNear + at] : get8(place(4 * i0 + i, at)); });
             }
         }
     } else if (TOP) {
@@ -389,7 +398,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
         if (4 * a.top <= 128) best.sort<2>(lists, 4 * a.top, a.top);
         else best.join(4, a.top, a.top, found[0], [&](int i, int at) { return lists[i * a.top + at]; });
     }
-    finish(a, row, t, best.mine);
+    finish(a, row, t, known, of_token, best.mine);
 }
 
 // The gradient: each logit read once and each result written once, 8 bytes an element
