@@ -10,11 +10,12 @@
 //     column l % 32 and, of each 16 keys, those of its half h = l / 32: 4h .. 4h+3
 //     and 8+4h .. 8+4h+3.  V^T lies in LDS with its keys in that order.
 //
-// Numbers.  In units of a power of two, u, of the workgroup's, fp16 holds exactly
-// each cached value whose scale is from 2^-23 to 2^13 of u (denormals count in
-// full: compared on the device, conversion and product).  The fp32 operands are
-// cut into two fp16 parts, hi = fp16(x) and lo = fp16(x - hi), off by at most 2^-23
-// of x, or by 2^-25 where x is below 1.  A row of Q is shifted so that its largest is
+// Numbers.  In units of a power of two, u, of the workgroup's, each cached value whose
+// scale is from 2^-13 to 2^13 of u is a normal fp16 number.  (Denormal ones, to 2^-23,
+// would be exact too, but the matrix cores add their products as those of unnormalized
+// numbers: off by up to 2^-16 of themselves.)  The fp32 operands are cut into two fp16
+// parts, hi = fp16(x) and lo = fp16(x - hi), off by at most 2^-23 of x, or by 2^-25
+// where x is below 1.  A row of Q is shifted so that its largest is
 // in [2^14, 2^15): what is lost there is 2^-39 of it.  Weights are e^(s - m) * 2^7 (at
 // most 2^15, as m lags by 2^8 at most): what is lost is 2^-32 of the largest weight,
 // where the sums' own fp32 loses 2^-25 of theirs.  u is taken near the scales of the
@@ -52,8 +53,8 @@ constexpr int per_cu(int D)
     return D == 128 ? 2 : D == 64 ? 3 : 4;
 }
 constexpr int kLeast = 8;    // tiles of a piece: its start and its join cost about two
-// fp16 holds every code times 2^kLeastUnit .. 2^kMostUnit.
-constexpr int kLeastUnit = -23, kMostUnit = 13;
+// Every code but 0 times 2^kLeastUnit .. 2^kMostUnit is a normal fp16 number.
+constexpr int kLeastUnit = -13, kMostUnit = 13;
 
 // As in kv_attention.hip.
 __device__ unsigned g_done[kMostUnits];
@@ -258,7 +259,7 @@ __device__ __forceinline__ Units units_at(const KvCache &c, int64_t at)
     auto most = [&](const uint8_t *p) {
         const unsigned w = *(scalar)(uintptr_t)(p + max(at, (int64_t)0) * c.D / 32);
         const unsigned top = max(max(w & 0xff, w >> 8 & 0xff), max(w >> 16 & 0xff, w >> 24));
-        return (int)(at < 0 || top > kMostScale ? 127 : min(top + 5, (unsigned)(kMostScale - kMostUnit)));
+        return (int)(at < 0 || top > kMostScale ? 127 : min(top, (unsigned)(kMostScale - kMostUnit)));
     };
     return {most(c.k_scales), most(c.v_scales)};
 }

@@ -288,6 +288,23 @@ def test_many_rows_over_scales_far_apart(D, T, first):
     p.check_attention((normal(rng, 2, T, 6, D) * groups).astype(np.float32), True, start=[L - T, 60])
 
 
+@pytest.mark.parametrize("D, T", [(64, 50), (128, 140)])
+@pytest.mark.parametrize("less", [0, 6, 11, 13, 14, 17, 19, 24])
+def test_many_rows_over_values_below_the_first(D, T, less):
+    """Columns in which only the first token has none, and the others' are 2^-less
+    of its size elsewhere; few keys and flat weights, so that the bound is near the
+    roundings' own size."""
+    rng = np.random.default_rng(less)
+    L = 5
+    tab, pages = table(rng, 1, 1)
+    p = Pair(pages, 1, 16, D, tab)
+    k, v = normal(rng, 1, L, 1, D) * np.float32(0.01), normal(rng, 1, L, 1, D) * np.float32(2.0 ** (20 - less))
+    v[0, 0, 0] = 0
+    v[0, 0, 0, :32] = 2.0 ** 20
+    p.write(k, v)
+    p.check_attention(normal(rng, 1, T, 1, D), False, start=[0], count=[L])
+
+
 def test_a_row_of_q_that_is_no_number():
     rng = np.random.default_rng(9)
     p = filled(rng, 1, 1, 16, 64, 40)
