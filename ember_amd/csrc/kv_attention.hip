@@ -41,9 +41,9 @@
 //
 // HBM-bound where contexts are long: 17/32 byte of K and V per element.  32 sequences
 // of up to 8192, 32 / 8 heads of 128 (148 MB) take 36.5 us, 4 of up to 32768, 16 heads
-// of 128 (178 MB) 46.5, of which about 9 are the launch, the plan, the first loads and
-// the join; what is between runs at 5.5 TB/s.  16 x 5 rows over 3001, 16 heads of 64 (28
-// MB) 14.6.
+// of 128 (178 MB) 42.6, of which about 8 are the launch, the plan, the first loads and
+// the join; what is between runs at 5.2 to 5.5 TB/s.  16 x 5 rows over 3001, 16 heads of
+// 64 (28 MB) 14.8.
 #include <algorithm>
 #include <type_traits>
 
@@ -59,7 +59,20 @@ constexpr int per_cu(int D, int rows)
 {
     return D == 128 && rows == 8 ? 3 : 4;
 }
-constexpr int kLeast = 8;  // tiles of a piece: two for each wave, so that the loads of one run beside the other
+// Workgroups that the keys are cut for, to a CU: fewer than fit, as every further piece
+// of a unit is joined by one workgroup in the end, and more of them stream no faster.
+// As many as fit and these (us): D = 128, 4 x 1 token, 16 heads over up to 32768 46.4
+// and 42.6, 4 tokens of 16 / 4 heads over 16384 23.2 and 17.6, 8 rows of 8 x 8 heads over
+// 4096 15.0 and 13.2; D = 64, 4 x 4 tokens of 16 heads over up to 16384 18.4 and 17.7; 16
+// x 5 rows over 3001 14.8 and 15.0, with two 16.3.
+constexpr int cut_for(int D, int rows)
+{
+    return D == 128 ? (rows == 8 ? 1 : 2) : 3;
+}
+// Tiles of a piece at least: five for each wave.  With 8, 16, 20 and 24: 32 / 8 heads of
+// 128 over 8192 14.2, 12.8, 12.5, 12.5; 8 x 8 heads of 128 over 4096 10.9, 10.4, 10.6, 10.6;
+// 16 x 5 rows over 3001, 16 heads of 64, 14.6, 14.8, 14.9, 15.4.
+constexpr int kLeast = 20;
 
 // Units that are cut: how many of their workgroups are done.  Zero between
 // calls: the last one, which all the others have added to, clears its unit's.
@@ -470,7 +483,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
 template <int D, int ROWS>
 int launch(KvAttnArgs &a)
 {
-    const int st = cut_keys(a, ROWS, kTile, kLeast, per_cu(D, ROWS));
+    const int st = cut_keys(a, ROWS, kTile, kLeast, cut_for(D, ROWS));
     if (st) return st;
     hipLaunchKernelGGL((kv_attention_kernel<D, ROWS>), dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     return launch_ok("kv_attention") ? EMBER_OK : EMBER_ERR_DEVICE;
@@ -504,7 +517,7 @@ int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
     const int64_t all = (int64_t)a.c.sequences * a.c.heads * a.tiles;  // units
     if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
     a.by_group = Divisor(a.group), a.by_tiles = Divisor(a.tiles), a.by_units = Divisor(a.c.heads * a.tiles);
-    // One round of workgroups over the chip; where the units alone are about as
+    // per_cu workgroups to a CU; where the units alone are about as
     // many, two pieces each, so that the longest sequence does not decide; but no
     // more than the page table has room for.  With many units, where the pieces'
     // results were large, or where no sequence can be longer than a piece, none is

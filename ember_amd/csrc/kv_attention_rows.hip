@@ -52,7 +52,11 @@ constexpr int per_cu(int D)
 {
     return D == 128 ? 2 : D == 64 ? 3 : 4;
 }
-constexpr int kLeast = 8;    // tiles of a piece: its start and its join cost about two
+// Tiles of a piece at least.  With 4, 6, 8 and 16 (us): 300 rows of 16 / 4 heads of 128
+// over 2000 38.8, 39.3, 35.3, 50.2; 64 rows of 16 heads of 64 over 8192 30.3, 27.0, 25.4,
+// 29.4; 64 rows of 8 x 8 heads of 128 over 4096 33.3, 32.7, 33.2, 37.3; 1000 rows of 4
+// heads of 128 over 1000 24.7, 27.8, 31.0, 43.7.
+constexpr int kLeast = 8;
 // Every code but 0 times 2^kLeastUnit .. 2^kMostUnit is a normal fp16 number.
 constexpr int kLeastUnit = -13, kMostUnit = 13;
 
@@ -265,9 +269,9 @@ __device__ __forceinline__ Units units_at(const KvCache &c, int64_t at)
 }
 
 // KW = 1: 128 rows, every wave takes all keys of a tile.  KW = 2, up to 64 rows: a
-// wave takes 32 keys of a tile, and pairs of waves join at the end (64 rows of 8 x 8
-// heads of 128 over 4096 keys: 42 us, with KW = 1 61; 65 rows and more would convert
-// every tile twice).
+// wave takes 32 keys of a tile, and pairs of waves join at the end (when both took
+// three bf16 parts, 64 rows of 8 x 8 heads of 128 over 4096 keys 42 us, with KW = 1 61;
+// 65 rows and more would convert every tile twice).
 template <int D, int KW>
 __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kernel(KvAttnArgs a)
 {
