@@ -41,7 +41,11 @@ struct KvAttnArgs {
     float *part;  // of each workgroup: O (rows, D), then m and l of each row; null: units are not cut
     int T, q_heads, group, tiles, blocks, causal;  // tiles: of rows, of a head
     int key_shift, least;  // of the keys of a tile, tiles of a piece at least
-    float scale2;  // scale * log2(e), above 0
+    // scale * log2(e) = q_scale * scale2, and scale2 a power of two: Q is multiplied by
+    // q_scale (from 0.5 to 1, or 0) as it is read, so that a score, a sum of products times
+    // scale2, has no rounding but the sum's.  Rounded, the largest of a row and the same
+    // score under an fma would differ by half a step: 32 from 2^29 on, a factor of 2^32.
+    float q_scale, scale2;
     Divisor by_group, by_tiles, by_units;  // units: of a sequence
 };
 
@@ -103,6 +107,13 @@ template <int S>
 __device__ __forceinline__ unsigned fp4_bf16(unsigned w, float scale)
 {
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, S));
+}
+
+// x * f, rounded to 24 bits before its parts are taken (not kept in an fma).
+__device__ __forceinline__ float product(float x, float f)
+{
+#pragma clang fp contract(off)
+    return x * f;
 }
 
 // The upper halves of three floats' parts: hi, mid and lo of x.

@@ -229,8 +229,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 unsigned p0[3], p1[3];
-                cut3(any ? raw[s][i >> 1][2 * (i & 1)] : 0.0f, p0[0], p0[1], p0[2]);
-                cut3(any ? raw[s][i >> 1][2 * (i & 1) + 1] : 0.0f, p1[0], p1[1], p1[2]);
+                cut3(any ? product(raw[s][i >> 1][2 * (i & 1)], a.q_scale) : 0.0f, p0[0], p0[1], p0[2]);
+                cut3(any ? product(raw[s][i >> 1][2 * (i & 1) + 1], a.q_scale) : 0.0f, p1[0], p1[1], p1[2]);
                 if (SHARED) {
                     p0[0] = part == 0 ? p0[0] : part == 1 ? p0[1] : p0[2];
                     p1[0] = part == 0 ? p1[0] : part == 1 ? p1[1] : p1[2];
@@ -556,9 +556,11 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     a.start = start, a.count = count;
     a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / a.c.heads);
     a.causal = causal != 0;
-    // Above 0, so that a masked score stays -infinity under it; a scale of 0 then
-    // gives scores that differ by nothing.
-    a.scale2 = std::min(std::max(scale * kLog2e, 1e-37f), 3.4e38f);
+    const float all = std::min(scale * kLog2e, 3.402823466e38f);
+    int e;
+    frexpf(all, &e);
+    e = std::min(std::max(e, -126), 127);  // scale2 is a normal number: a masked score stays -infinity under it
+    a.q_scale = ldexpf(all, -e), a.scale2 = ldexpf(1.0f, e);
     if (T * a.group > few_rows(a.c)) return launch_kv_attention_rows(a);
     return a.c.D == 128 ? launch_rows<128>(a) : a.c.D == 64 ? launch_rows<64>(a) : launch_rows<32>(a);
 }

@@ -255,6 +255,15 @@ __device__ __forceinline__ void cut_pair(float x0, float x1, u32x4 (&to)[kParts<
     }
 }
 
+// Two fp16 parts of x0 * f and x1 * f, the lower one from the exact products.
+__device__ __forceinline__ void cut_scaled(float x0, float x1, float f, u32x4 (&to)[2], int i)
+{
+    const f16x2 hi = __builtin_convertvector((f32x2{product(x0, f), product(x1, f)}), f16x2);
+    const f16x2 lo = __builtin_convertvector((f32x2{fmaf(x0, f, -(float)hi[0]), fmaf(x1, f, -(float)hi[1])}), f16x2);
+    to[0][i] = __builtin_bit_cast(unsigned, hi);
+    to[1][i] = __builtin_bit_cast(unsigned, lo);
+}
+
 // Units near the scales of a piece's first tokens; the bytes past kMostScale, of what
 // is no number, fit none.
 __device__ __forceinline__ Units units_at(const KvCache &c, int64_t at)
@@ -307,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
     const int end = pl.piece + 1 < pl.pieces ? min(n, first + plan.per) : n;
 
     f32x16 acc[DB];
-    float m, l;
+    float m, l;  // the weights' unit (their maximum, in the end), and their sum
     const auto larger = [](float x, float y) { return fmaxf(x, y); };
     auto piece_at = [&](int tl) { return tl < end ? row_of(a.c, b, h, tl * kTile + 16 * wave) : -1; };
     // The piece's tiles; false if a value does not fit (then the sums are worth nothing).
@@ -339,9 +348,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
-                most = across_32(most, larger);
+                most = across_32(most, larger) * fmaxf(a.q_scale, 0.5f);  // (0: any shift that Q can take)
                 shift = 14 + 127 - (int)(float_bits(most) >> 23);
-                scale2 = fminf(fmaxf(ldexpf(scale2, units16.k - 127 - shift), 1e-37f), 3.4e38f);
+                scale2 = fminf(fmaxf(ldexpf(scale2, units16.k - 127 - shift), 0x1p-126f), 0x1p127f);
             }
 #pragma unroll
             for (int s = 0; s < KS; ++s)
@@ -350,15 +359,19 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const float x0 = x[s][i][2 * j], x1 = x[s][i][2 * j + 1];
-                        cut_pair<HALF>(HALF ? ldexpf(x0, shift) : x0, HALF ? ldexpf(x1, shift) : x1, q[s], 2 * i + j);
+                        if constexpr (HALF) cut_scaled(ldexpf(x0, shift), ldexpf(x1, shift), a.q_scale, q[s], 2 * i + j);
+                        else cut_pair<false>(product(x0, a.q_scale), product(x1, a.q_scale), q[s], 2 * i + j);
                     }
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[d] = zero16();
-        m = kNone, l = 0.0f;
+        // A weight is 2^(s + c), c = up - m: with the same c for all of a row's weights,
+        // whatever m's size, and at most 2^(up + kRaise).
+        constexpr float up = HALF ? 7.0f : 0.0f;
+        float c = -kNone;
+        l = 0.0f;
         auto block = [&](const Lds<D> &at, int key0, auto KB) {
             constexpr int kb = decltype(KB)::value;
-            constexpr float up = HALF ? 7.0f : 0.0f;  // the weights' unit: 2^-7
             f32x16 s = zero16();
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
@@ -384,10 +397,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
 #pragma unroll
             for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
             top *= scale2;
-            if (__any(top > m + kRaise)) {
+            if (__any(top + c > up + kRaise)) {
                 top = across_32(top, larger);
-                const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
-                m = to;
+                const float to = fminf(c, up - top), f = __builtin_amdgcn_exp2f(to - c);
+                c = to;
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -399,8 +412,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                 u32x4 p[P];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i], scale2, up - m));
-                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i + 1], scale2, up - m));
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i], scale2, c));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[8 * st + 2 * i + 1], scale2, c));
                     l += e0;
                     l += e1;
                     cut_pair<HALF>(e0, e1, p, i);
@@ -453,8 +466,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
             step(tl, lds[0], lds[1]);
             if (tl + 1 < end) step(tl + 1, lds[1], lds[0]);
         }
+        m = -c;
         if (HALF) {
-            m -= 7.0f;
             const float unit = scale_of(units16.v);
 #pragma unroll
             for (int d = 0; d < DB; ++d)

@@ -267,6 +267,32 @@ def test_scores_of_all_sizes():
     p.check_attention(q, True, scale=0.0, start=[155])
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("T", [1, 3, 7, 50, 140])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e12, 1e20])
+def test_large_scores(size, T, D):
+    """Scores of `size` times 1, 1.5, 2, 3, ... 12, 16 keys of each, some rows' all
+    negative.  A row's largest are equal to the bit (keys alike) and all others
+    further below than the scores' roundings reach, 2 (D + 8) half steps of 12
+    sizes and less than 0.01 of `size`: o is the mean of the largest ones' values,
+    off by the roundings of its sum."""
+    rng = np.random.default_rng(D + T)
+    L, q_heads = 128, 1
+    tab, pages = table(rng, 2, 8)
+    p = Pair(pages, 1, 16, D, tab)
+    level = np.array([1, 1.5, 2, 3, 4, 6, 8, 12], np.float32).repeat(16)
+    k = np.broadcast_to(level[None, :, None, None], (2, L, 1, D)).copy()
+    p.write(k, normal(rng, 2, L, 1, D))
+    q = size / (D * G.scale_for(D)) * rng.uniform(0.5, 1.5, (2, T, q_heads, D))
+    q[:, 1::2] *= -1
+    q = q.astype(np.float32)
+    start = [max(L - T, 0), 0]
+    o, lse = p.attention(q, True, start=start)
+    ro, rl, weight, reach = p.host.attention(q, True, G.scale_for(D), start, None)
+    assert (np.abs(o - ro) <= 2 * 2.0 ** -24 * (L + 16) * weight).all()
+    assert (np.abs(lse - rl) <= 2.0 ** -23 * ((D + 8) * reach + np.abs(rl) + 16)).all()
+
+
 @pytest.mark.parametrize("first", [0, -17, -19, -40, 17, 19, 40])
 @pytest.mark.parametrize("D, T", [(32, 21), (64, 50), (128, 50)])
 def test_many_rows_over_scales_far_apart(D, T, first):
