@@ -47,6 +47,8 @@ struct KvAttnArgs {
     // score under an fma would differ by half a step: 32 from 2^29 on, a factor of 2^32.
     float q_scale, scale2;
     Divisor by_group, by_tiles, by_units;  // units: of a sequence
+    int most;      // pieces of a unit of each sequence, together
+    float shares;  // a piece is not less than all sequences' tiles over this, either
 };
 
 // Tokens that a sequence has after the call, as far as its table has room.
@@ -81,7 +83,7 @@ __device__ __forceinline__ int tiles_of_sequence(const KvAttnArgs &a, int b)
 
 __device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
 {
-    const int lane = threadIdx.x & 63, most = a.by_units.of(a.blocks);
+    const int lane = threadIdx.x & 63, most = a.most;
     Plan p;
     p.sp = span_of(a.start, a.count, min(lane, a.c.sequences - 1), a.T);
     p.len = length_of(a, p.sp);
@@ -93,7 +95,7 @@ __device__ __forceinline__ Plan make_plan(const KvAttnArgs &a)
         return n;
     };
     // The sum of all tiles may pass 32 bits; as a float it is near enough.
-    p.per = max((int)(sum([](int n) { return (float)n; }) / most), a.least);
+    p.per = max((int)(sum([](int n) { return (float)n; }) / a.shares), a.least);
     while (sum([&](int n) { return p.pieces(n); }) > most) p.per += p.per / 8 + 1;
     return p;
 }
@@ -199,7 +201,8 @@ __device__ __forceinline__ Place start_block(const KvAttnArgs &a, Plan &plan)
 // Attention for many rows (kv_attention_rows.hip).
 int launch_kv_attention_rows(KvAttnArgs &a);
 // Fills in how the keys are cut, for workgroups of `rows` rows of which a CU
-// holds per_cu, and tiles of `keys` keys; records and returns a status.
-int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu);
+// holds per_cu and is to be given cut_for, and tiles of `keys` keys; records and
+// returns a status.
+int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu, int cut_for);
 
 }  // namespace ember

@@ -483,7 +483,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
 template <int D, int ROWS>
 int launch(KvAttnArgs &a)
 {
-    const int st = cut_keys(a, ROWS, kTile, kLeast, cut_for(D, ROWS));
+    const int st = cut_keys(a, ROWS, kTile, kLeast, per_cu(D, ROWS), cut_for(D, ROWS));
     if (st) return st;
     hipLaunchKernelGGL((kv_attention_kernel<D, ROWS>), dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     return launch_ok("kv_attention") ? EMBER_OK : EMBER_ERR_DEVICE;
@@ -510,23 +510,30 @@ int few_rows(const KvCache &c)
 
 }  // namespace
 
-int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu)
+int cut_keys(KvAttnArgs &a, int rows, int keys, int least, int per_cu, int cut_for)
 {
     a.tiles = (int)(((int64_t)a.T * a.group + rows - 1) / rows);
     a.key_shift = __builtin_ctz(keys), a.least = least;
     const int64_t all = (int64_t)a.c.sequences * a.c.heads * a.tiles;  // units
     if (all * 64 * kWaves > 0xffffffff) return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_attention");
     a.by_group = Divisor(a.group), a.by_tiles = Divisor(a.tiles), a.by_units = Divisor(a.c.heads * a.tiles);
-    // per_cu workgroups to a CU; where the units alone are about as
+    // cut_for workgroups to a CU; where the units alone are about as
     // many, two pieces each, so that the longest sequence does not decide; but no
-    // more than the page table has room for.  With many units, where the pieces'
-    // results were large, or where no sequence can be longer than a piece, none is
-    // cut (and none plans: one token of 4 heads of 64 over 256 5.8 -> 5.0 us).
-    const int64_t slots = (int64_t)per_cu * std::max(device_cu_count(), 1);
+    // more than the page table has room for.  With units of several rounds (beyond 4 *
+    // slots) only what is longer than two sequences of the mean length is cut: one
+    // token of 80 x 32 heads of 128, one sequence of 32768 and 79 of 500, 189 us uncut
+    // and 63 so; all of 2000 119 uncut, 134 in two pieces each and 120 so.  With more units
+    // yet, where the pieces' results were large, or where no sequence can be longer than
+    // a piece, none is cut (and none plans: one token of 4 heads of 64 over 256 5.8 ->
+    // 5.0 us).
+    const int64_t cus = std::max(device_cu_count(), 1), slots = cut_for * cus;
     const int64_t longest = (((int64_t)a.c.max_pages << a.c.page_shift) + keys - 1) / keys, pieces = (longest + least - 1) / least;
-    const int64_t blocks = std::min(std::max(slots, 2 * all), all * pieces), bytes = blocks * rows * (a.c.D + 2) * (int64_t)sizeof(float);
-    const bool cut = pieces > 1 && a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * slots) && bytes <= kMostScratch;
+    const bool rounds = all > 4 * slots;
+    const int64_t blocks = std::min(rounds ? all + all / 2 : std::max(slots, 2 * all), all * pieces), bytes = blocks * rows * (a.c.D + 2) * (int64_t)sizeof(float);
+    const bool cut = pieces > 1 && a.c.sequences <= kMostPlan && all <= std::min<int64_t>(kMostUnits, 4 * per_cu * cus) && bytes <= kMostScratch;
     a.blocks = (int)(cut ? blocks : all);
+    a.most = a.blocks / (a.c.heads * a.tiles);
+    a.shares = rounds ? 0.5f * a.c.sequences : (float)a.most;
     if (cut) {
         a.part = (float *)scratch(kScratchKvAttention, (size_t)bytes);
         if (!a.part) return EMBER_ERR_OUT_OF_MEMORY;

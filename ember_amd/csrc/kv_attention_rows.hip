@@ -556,7 +556,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
 template <int D, int KW>
 int launch(KvAttnArgs &a)
 {
-    const int st = cut_keys(a, 32 * kWaves / KW, kTile, kLeast, per_cu(D));
+    const int st = cut_keys(a, 32 * kWaves / KW, kTile, kLeast, per_cu(D), per_cu(D));
     if (st) return st;
     hipLaunchKernelGGL((kv_attention_rows_kernel<D, KW>), dim3((unsigned)a.blocks), dim3(64 * kWaves), 0, 0, a);
     return launch_ok("kv_attention_rows") ? EMBER_OK : EMBER_ERR_DEVICE;

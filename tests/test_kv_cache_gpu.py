@@ -3,11 +3,14 @@ right to the bit, at the right slots and nowhere else; what is read back is the
 same; attention over it agrees with float64 for one row and many, page ends,
 padded batches, rows that see nothing, and slots that hold no numbers."""
 
+import time
+
 import numpy as np
 import pytest
 
 import gpu_helpers as G
 from ember_amd import capi
+from ember_amd.capi import DeviceArray
 from oracle import serving
 from serving_helpers import Bytes, Pair, ints, table
 
@@ -236,6 +239,50 @@ def test_sequences_of_very_different_lengths():
         p.write(k, v, count=np.where(np.arange(B) == b, lengths[b], 0))
     for T, heads in ((1, 2), (2, 3), (30, 2)):
         p.check_attention(normal(rng, B, T, heads, 64), True, start=lengths - T)
+
+
+@pytest.mark.parametrize("T, G_, heads", [(1, 1, 32), (3, 1, 32), (5, 1, 16), (24, 1, 6)])
+def test_long_sequences_among_units_of_several_rounds(T, G_, heads):
+    """More units than the chip takes in four rounds: the long sequences are cut all the same."""
+    rng = np.random.default_rng(T)
+    B, page, D = 70, 64, 128
+    lengths = rng.integers(0, 40, B)
+    lengths[[2, 68]] = 2500, 1400
+    need, n = -(-lengths // page), 0
+    tab = np.full((B, need.max()), -1, np.int32)
+    for b in range(B):
+        tab[b, :need[b]] = np.arange(n, n + need[b])
+        n += need[b]
+    p = Pair(n, heads, page, D, tab)
+    for a, b in zip((*p.host.codes, *p.host.scales), (*p.codes, *p.scales)):
+        a[...] = rng.integers(120, 126, a.shape) if a is p.host.scales[0] or a is p.host.scales[1] else rng.integers(0, 256, a.shape)
+        b.dev = Bytes(a).dev
+    p.view.k_codes, p.view.v_codes, p.view.k_scales, p.view.v_scales = (x.ptr for x in (*p.codes, *p.scales))
+    o, lse = p.check_attention(normal(rng, B, T, heads * G_, D), True, start=lengths - T)
+
+
+def test_a_long_sequence_does_not_decide():
+    """One of 32768 tokens among 79 of 500 takes less than 80 of 2000, twice as many tokens in all."""
+    B, heads, page, D = 80, 32, 256, 128
+    p = Pair(8, heads, page, D, np.arange(128)[None].repeat(B, 0) % 8, fill=0x77)
+    q, o = (DeviceArray.from_numpy(np.ones((B, 1, heads, D), np.float32)) for _ in range(2))
+
+    def seconds(lengths):
+        start = ints(np.array(lengths) - 1)
+        st = (heads * D, D, heads * D)
+        best = np.inf
+        for _ in range(5):
+            start.numpy()  # waits
+            t0 = time.perf_counter()
+            for _ in range(20):
+                rc = capi.lib().kv_cache_attention(p.view, q.ptr, o.ptr, None, 1, heads, G.scale_for(D), 1, *st, *st, start.ptr, None)
+                capi.check(rc, "kv_cache_attention")
+            start.numpy()  # waits
+            best = min(best, time.perf_counter() - t0)
+        return best
+
+    G.say("kv_cache_attention B=80 heads=32 D=128, 32768 and 79 x 500, and 80 x 2000")
+    assert seconds([32768] + 79 * [500]) < seconds(80 * [2000])
 
 
 @pytest.mark.parametrize("pages, places", [(0, 2), (3, 0), (0, 0)])
