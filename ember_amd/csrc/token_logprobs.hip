@@ -411,14 +411,14 @@ struct GradArgs {
     const float *lse, *entropy, *d_logp, *d_entropy;
     float *dx;
     int64_t stride, out_stride;
-    int rows, classes, segments;
+    int classes, segments, row0;
 };
 
 constexpr int kGradSegment = kThreads * 16;
 
 __global__ __launch_bounds__(kThreads) void token_logprobs_bwd_kernel(GradArgs a)
 {
-    const int row = blockIdx.x / a.segments, seg = blockIdx.x - row * a.segments;
+    const int index = blockIdx.x / a.segments, seg = blockIdx.x - index * a.segments, row = a.row0 + index;
     const int64_t first = (int64_t)seg * kGradSegment;
     const float *p = a.x + row * a.stride + first;
     float *q = a.dx + row * a.out_stride + first;
@@ -456,6 +456,15 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_bwd_kernel(GradArgs a
 
 constexpr int64_t kMostClasses = 0x7fffffff - 65535;
 constexpr int64_t kMostBlocks = (int64_t(1) << 32) / kThreads - 1;  // a grid's threads are counted in 32 bits
+
+// Whether two arrays of `rows` rows of `classes` floats, both `stride` apart, have
+// an element in common, the same rows aside.
+bool rows_meet(const float *x, const float *y, int64_t stride, int64_t rows, int64_t classes)
+{
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    const int64_t apart = (int64_t)((a < b ? b - a : a - b) / sizeof(float)), over = apart / stride, left = apart - over * stride;
+    return apart && ((over < rows && left < classes) || (over + 1 < rows && stride - left < classes));
+}
 
 }  // namespace
 }  // namespace ember
@@ -502,13 +511,19 @@ extern "C" int token_logprobs_bwd(const float *logits, int64_t row_stride, const
     using namespace ember;
     const char *what = "token_logprobs_bwd";
     const int64_t segments = (classes + kGradSegment - 1) / kGradSegment;
-    if (rows < 0 || classes < 1 || classes > kMostClasses || row_stride < classes || out_stride < classes || rows > kMostBlocks / segments)
+    if (rows < 0 || rows > 0x7fffffff || classes < 1 || classes > kMostClasses || row_stride < classes || out_stride < classes)
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
     if (rows == 0) return EMBER_OK;
     if (!logits || !tokens || !lse || !d_logits || (d_entropy && !entropy) || (logits == d_logits && row_stride != out_stride) ||
+        (row_stride == out_stride && rows_meet(logits, d_logits, row_stride, rows, classes)) ||
         (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)d_logp | (uintptr_t)d_entropy | (uintptr_t)d_logits) & 3))
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
-    const GradArgs a = {logits, tokens, lse, entropy, d_logp, d_entropy, d_logits, row_stride, out_stride, (int)rows, (int)classes, (int)segments};
-    hipLaunchKernelGGL(token_logprobs_bwd_kernel, dim3((unsigned)(rows * segments)), dim3(kThreads), 0, 0, a);
-    return launch_ok(what) ? EMBER_OK : EMBER_ERR_DEVICE;
+    GradArgs a = {logits, tokens, lse, entropy, d_logp, d_entropy, d_logits, row_stride, out_stride, (int)classes, (int)segments};
+    const int64_t most = kMostBlocks / segments;
+    for (int64_t row = 0; row < rows; row += most) {
+        a.row0 = (int)row;
+        hipLaunchKernelGGL(token_logprobs_bwd_kernel, dim3((unsigned)(std::min(most, rows - row) * segments)), dim3(kThreads), 0, 0, a);
+        if (!launch_ok(what)) return EMBER_ERR_DEVICE;
+    }
+    return EMBER_OK;
 }

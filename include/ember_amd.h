@@ -434,7 +434,7 @@ int token_logprobs(const float *logits, int64_t row_stride, const int32_t *token
  * d_logp taken as 0 where tokens[r] is out of range, and a row with both
  * gradients 0 gets zeros whatever its logits hold; row r at d_logits +
  * r*out_stride.  d_logits may be logits itself (with the same stride); it
- * must not overlap it otherwise. */
+ * must not overlap it otherwise.  Rows and classes as in token_logprobs. */
 int token_logprobs_bwd(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
                        const float *entropy, const float *d_logp, const float *d_entropy, float *d_logits,
                        int64_t out_stride, int64_t rows, int64_t classes);

@@ -260,3 +260,15 @@ def test_answering_token_by_token():
             np.testing.assert_allclose(logits.to_np(), whole.to_np(), rtol=1e-3, atol=2e-4)
         else:  # a projection's last bit turned a code: one step of the grid in one element
             assert np.abs(logits.to_np() - whole.to_np()).max() <= 0.1 * np.abs(whole.to_np()).max()
+
+
+def test_token_loss_of_more_rows_than_one_grid_takes():
+    """2^24 rows and one: every row's gradient, (p - one-hot) / rows."""
+    rows = (1 << 24) + 1
+    pred = np.zeros((rows, 2), np.float32)
+    loss = TokenLoss()
+    G.say(f"TokenLoss of {rows} rows")
+    assert abs(loss.forward(em.Tensor(pred), np.arange(rows) % 2) - np.log(2)) <= 256 * U  # a sum of 2^24 terms
+    got = loss.backward().to_np()
+    want = np.where(np.arange(2) == (np.arange(rows) % 2)[:, None], -0.5, 0.5) / rows
+    assert (np.abs(got - want) <= 8 * U / rows).all()

@@ -125,3 +125,11 @@ def grad(x=P, stride=100, tokens=P, lse=P, ent=P, d_logp=P, d_ent=P, out=8192, o
 ])
 def test_gradients(change):
     refused(grad(**change))
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=P + 4), dict(out=P + 400), dict(out=P + 404), dict(out=P + 1596), dict(x=8192, out=8192 - 4), dict(x=8192, out=8192 - 1596),
+    dict(stride=150, out_stride=150, out=P + 396), dict(stride=150, out_stride=150, out=P + 204), dict(stride=150, out_stride=150, out=P + 996),
+])
+def test_gradients_partly_over_the_logits(change):
+    refused(grad(**change))

@@ -213,3 +213,17 @@ def test_gradient_of_masked_logits():
     ref = serving.token_logprobs_bwd(np.where(np.isinf(x), -1e30, x), tokens, one, one)
     np.testing.assert_allclose(got, ref, rtol=0, atol=4e-6)
     assert (got[0, 100:] == 0).all() and (got[1, 3:] == 0).all()
+
+
+def test_gradient_of_more_rows_than_one_grid_takes():
+    """2^24 rows and a few: each block of 4099 rows, alike, gets the same gradient."""
+    rng = np.random.default_rng(8)
+    rows, classes, block = (1 << 24) + 11, 3, 4099
+    x = rng.standard_normal((block, classes)).astype(np.float32)
+    tokens = rng.integers(-1, classes, block)
+    _, lse, ent, _, _ = serving.token_logprobs(x, tokens, 1)
+    d_logp, d_ent = rng.standard_normal(block).astype(np.float32), rng.standard_normal(block).astype(np.float32)
+    one = gradient(x, tokens, lse.astype(np.float32), ent.astype(np.float32), d_logp, d_ent)
+    many = lambda a: np.resize(a, (rows, *a.shape[1:]))  # noqa: E731
+    got = gradient(many(x), many(tokens), many(lse.astype(np.float32)), many(ent.astype(np.float32)), many(d_logp), many(d_ent))
+    np.testing.assert_array_equal(got, many(one))
