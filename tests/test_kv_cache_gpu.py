@@ -340,6 +340,16 @@ def test_large_scores(size, T, D):
     assert (np.abs(lse - rl) <= 2.0 ** -23 * ((D + 8) * reach + np.abs(rl) + 16)).all()
 
 
+@pytest.mark.parametrize("T", [1, 3, 7, 50, 140])
+def test_scale_zero_whatever_the_products(T):
+    """Products of 10^37 with a scale of 0: every key that a row sees weighs the same."""
+    rng = np.random.default_rng(T)
+    tab, pages = table(rng, 1, 10)
+    p = Pair(pages, 1, 16, 64, tab)
+    p.write(normal(rng, 1, 160, 1, 64) * np.float32(2.0 ** 60), normal(rng, 1, 160, 1, 64))
+    p.check_attention(normal(rng, 1, T, 1, 64) * np.float32(2.0 ** 60), True, scale=0.0, start=[160 - T])
+
+
 @pytest.mark.parametrize("first", [0, -17, -19, -40, 17, 19, 40])
 @pytest.mark.parametrize("D, T", [(32, 21), (64, 50), (128, 50)])
 def test_many_rows_over_scales_far_apart(D, T, first):
