@@ -200,11 +200,11 @@ void launch_read(const CopyArgs &a, unsigned n)
         hipLaunchKernelGGL((kv_read_kernel<D, false>), copy_grid(a), dim3(256), 0, 0, a, n);
 }
 
-// Whether two arrays of n integers have one in common.
-bool share(const int32_t *x, const int32_t *y, int n)
+// Whether arrays of nx and ny integers have one in common.
+bool share(const int32_t *x, int64_t nx, const int32_t *y, int64_t ny)
 {
-    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y, bytes = (uintptr_t)n * sizeof(int32_t);
-    return x && y && (a < b ? b - a : a - b) < bytes;
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    return x && y && (a < b ? b - a < nx * sizeof(int32_t) : a - b < ny * sizeof(int32_t));
 }
 
 int check_copy(const ember_kv_cache *cache, const void *k, const void *v, int64_t T, int64_t sb, int64_t sh, int64_t ss,
@@ -230,8 +230,9 @@ extern "C" int kv_cache_write(const ember_kv_cache *cache, const float *k, const
     CopyArgs a = {};
     const int st = check_copy(cache, k, v, T, in_sb, in_sh, in_ss, start, count, &a, "kv_cache_write");
     if (st) return st;
-    // Some workgroups read start and count when others have written next.
-    if (((uintptr_t)next & 3) || share(next, start, a.c.sequences) || share(next, count, a.c.sequences))
+    // Some workgroups read start, count and the table when others have written next.
+    const int64_t B = a.c.sequences;
+    if (((uintptr_t)next & 3) || share(next, B, start, B) || share(next, B, count, B) || share(next, B, a.c.table, B * a.c.max_pages))
         return record_error(EMBER_ERR_INVALID_ARGUMENT, "kv_cache_write");
     if (a.c.sequences == 0 || (T == 0 && !next)) return EMBER_OK;
     a.in[0] = k, a.in[1] = v, a.next = next;

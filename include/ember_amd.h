@@ -378,8 +378,8 @@ typedef struct ember_kv_cache {
 /* Rounds the valid rows of k and v into the cache.  Two valid rows must not
  * land on the same slot (a page written through two table entries).  next,
  * when not NULL, is an int32 device array that gets start[b] + the number of
- * valid rows, where the sequence's next call starts; it must not overlap start
- * or count. */
+ * valid rows, where the sequence's next call starts; it must not overlap start,
+ * count or the page table. */
 int kv_cache_write(const ember_kv_cache *cache, const float *k, const float *v, int64_t T,
                    int64_t in_sb, int64_t in_sh, int64_t in_ss, const int32_t *start,
                    const int32_t *count, int32_t *next);

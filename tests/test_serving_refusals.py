@@ -75,6 +75,11 @@ def test_next_overlaps_no_input(nxt):
     refused(write(nxt=nxt, start=8192))
 
 
+@pytest.mark.parametrize("nxt", [P, P + 20, P - 8])
+def test_next_does_not_overlap_the_page_table(nxt):
+    refused(write(nxt=nxt, start=16384, count=None))
+
+
 @pytest.mark.parametrize("change", [
     dict(T=-1), dict(Hq=0), dict(Hq=3), dict(Hq=65536), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None),
     dict(o=None), dict(o=P), dict(q=P + 4), dict(o=8200), dict(lse=P + 2), dict(st=(510, 64, 256)), dict(st=(512, 64, 1 << 24)),
