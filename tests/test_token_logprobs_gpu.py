@@ -227,3 +227,72 @@ def test_gradient_of_more_rows_than_one_grid_takes():
     many = lambda a: np.resize(a, (rows, *a.shape[1:]))  # noqa: E731
     got = gradient(many(x), many(tokens), many(lse.astype(np.float32)), many(ent.astype(np.float32)), many(d_logp), many(d_ent))
     np.testing.assert_array_equal(got, many(one))
+
+
+def check_long(x, tokens, top, **more):
+    """As check, for threads that take many chunks of 4096 logits (16 of each) in
+    turn: n chunks add 16 n roundings and, where the maximum rises, 3 each (the
+    factor's exp, two steps, and its product).  Only logits within 104 of the
+    maximum count (e^-104 is 0 in fp32)."""
+    rows, classes = x.shape
+    logp, lse, ent, ids, best = score(x, tokens, top, **more)
+    rp, rl, re, ri, rb = serving.token_logprobs(x, tokens, top)
+    r = np.minimum(np.where(np.isinf(x), 0, x.max(-1, keepdims=True).astype(np.float64) - x).max(-1), 104)
+    off = U * (r + 19 * -(-classes // 4096) + 64 + 2 * np.log2(classes + 1))
+    with np.errstate(invalid="ignore"):  # of a logit of -infinity both are
+        assert ((logp == rp) | (np.abs(logp - rp) <= off + 2 * U * np.abs(rp))).all()
+    assert (np.abs(lse - rl) <= off + 2 * U * (np.abs(rl) + np.abs(x.max(-1)))).all()
+    assert (np.abs(ent - re) <= 2 * off * (1 + np.minimum(r, 40))).all()
+    if top:
+        np.testing.assert_array_equal(ids, ri)
+        with np.errstate(invalid="ignore"):
+            assert ((best == rb) | (np.abs(best - rb) <= off[:, None] + 2 * U * np.abs(rb))).all()
+
+
+def rows_of_all_kinds(rng, rows, classes):
+    """Rows in turn: normal, rising and falling (every chunk has new alternatives, or
+    none), ties that pass the chunks' ends, whole chunks of -infinity (the first, the
+    last, all but one), and the largest ones in a late chunk."""
+    x = (3 * rng.standard_normal((rows, classes))).astype(np.float32)
+    x[1::7].sort(-1)
+    x[2::7] = -np.sort(-x[2::7])
+    x[3::7] = np.round(x[3::7])
+    x[4::7, :4096] = -np.inf
+    x[5::7, 4096:] = -np.inf
+    x[5::7, -1] = 1
+    x[6::7, classes - 700:] += 9
+    return x
+
+
+@pytest.mark.parametrize("top", [0, 1, 5, 20, 64])
+@pytest.mark.parametrize("rows, classes", [(1100, 9001), (2100, 4097), (1030, 16384), (600, 20001), (700, 12289), (300, 32001)])
+def test_rows_of_several_chunks(rows, classes, top):
+    """More rows than half of what fills the chip (256 CUs): a workgroup walks a row's
+    chunks in turn (the first three), or some of them (two or more pieces a row)."""
+    rng = np.random.default_rng(rows + top)
+    check_long(rows_of_all_kinds(rng, rows, classes), rng.integers(-1, classes + 1, rows), top, pad=top % 3)
+
+
+@pytest.mark.parametrize("top", [0, 5, 20, 64])
+@pytest.mark.parametrize("rows, classes", [(8, 131072), (3, 151936), (8, 151936), (2, 256000), (1, 262145), (7, 300000), (1, 1100000)])
+def test_large_vocabularies(rows, classes, top):
+    """Rows in more pieces than a wave has lanes, and than are joined at a time (64)."""
+    rng = np.random.default_rng(rows + classes + top)
+    check_long(rows_of_all_kinds(rng, rows, classes), rng.integers(0, classes, rows), top)
+
+
+@pytest.mark.parametrize("rows", [1, 1100])
+def test_no_numbers_in_a_late_chunk(rows):
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, 9001)).astype(np.float32)
+    tokens = rng.integers(0, 9001, rows)
+    clean = score(x, tokens, 6)
+    bad = x.copy()
+    bad[0::5, 8999], bad[1::5, 5000] = np.nan, np.inf
+    logp, lse, ent, ids, best = score(bad, tokens, 6)
+    for n in range(2):
+        assert all(np.isnan(a[n::5]).all() for a in (logp, lse, ent, best))
+    assert ((ids >= 0) & (ids < 9001)).all()
+    others = np.arange(rows) % 5 > 1
+    for a, b in zip(clean, (logp, lse, ent, ids, best)):
+        np.testing.assert_array_equal(a[others], b[others])
