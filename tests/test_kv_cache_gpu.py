@@ -221,6 +221,29 @@ def test_many_sequences(B, T, G_):
     p.check_attention(normal(rng, B, T, G_, 32), True, start=start, count=rng.integers(0, T + 1, B))
 
 
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("T, G_", [(1, 1), (2, 1), (1, 2), (1, 3), (3, 1), (1, 4), (2, 2), (5, 1), (1, 8), (4, 5)])
+def test_few_rows_and_splits(D, T, G_):
+    """Two, four and eight rows to a workgroup, with keys cut into pieces (of 640 at
+    least): lengths, counts, NaN in one piece and pages that are not there."""
+    rng = np.random.default_rng(D * T + G_)
+    L, page = 1900, 64
+    tab, pages = table(rng, 4, 30)
+    p = Pair(pages, 2, page, D, tab)
+    k, v = normal(rng, 4, L, 2, D), normal(rng, 4, L, 2, D)
+    v[0, 1400, 1, D - 1] = np.nan
+    k[0, L - 1, 0, 3] = np.inf
+    p.write(k, v, count=[L, 900, 500, L])
+    p.host.table[3, 12:23] = -1
+    p.table = ints(p.host.table)
+    p.view.page_table = p.table.ptr
+    q = normal(rng, 4, T, 2 * G_, D)
+    start = [L - T, 900 - T, 40, L - T - 11]
+    o, _ = p.check_attention(q, True, start=start)
+    assert np.isnan(o[0, :, G_:, D - 32:]).all() and np.isfinite(o[1:]).all()
+    p.check_attention(q, False, start=start, count=[T, 1, 0, T])
+
+
 def test_sequences_of_very_different_lengths():
     """One long sequence among many short and empty ones, cut into pieces."""
     rng = np.random.default_rng(20)
@@ -369,6 +392,55 @@ def test_many_rows_over_scales_far_apart(D, T, first):
     v[1, 60:70] = -0.0
     p.write(k.astype(np.float32), v.astype(np.float32))
     p.check_attention((normal(rng, 2, T, 6, D) * groups).astype(np.float32), True, start=[L - T, 60])
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("T", [50, 140])
+@pytest.mark.parametrize("odd", ["large values", "small values", "small keys", "no number", "no key", "all"])
+def test_many_rows_with_one_piece_far_apart(odd, T, D):
+    """Keys cut into pieces (of 512 at least), one of which holds what fp16 cannot in
+    its first token's units: done again in bf16, and joined with those that were not."""
+    rng = np.random.default_rng(D + T)
+    L = 2300
+    tab, pages = table(rng, 2, 36)
+    p = Pair(pages, 1, 64, D, tab)
+    k, v = normal(rng, 2, L, 1, D), normal(rng, 2, L, 1, D)
+    if odd in ("large values", "all"):
+        v[:, 1300:1310] *= np.float32(2.0 ** 18)
+    if odd in ("small values", "all"):
+        v[:, 1320:1400] *= np.float32(2.0 ** -25)
+    if odd in ("small keys", "all"):
+        k[:, 1350:1420] *= np.float32(2.0 ** -30)
+    if odd in ("no number", "all"):
+        v[0, 1290, 0, 5] = np.nan
+    if odd in ("no key", "all"):
+        k[1, L - 30, 0, 7] = np.inf
+    p.write(k, v)
+    q = normal(rng, 2, T, 1, D)
+    o, lse = p.check_attention(q, True, start=[L - T, L - T])
+    assert np.isnan(lse[1, :, -30:]).all() == (odd in ("no key", "all")) and np.isfinite(lse[1, :, :-30]).all()
+    p.check_attention(q, True, start=[700, 1380 - T], count=[T, T])
+
+
+@pytest.mark.parametrize("D, T", [(32, 15), (64, 15), (128, 40), (64, 60)])
+def test_many_rows_over_scores_of_all_sizes(D, T):
+    """test_scores_of_all_sizes for more than 40 rows, and with pieces.  Weights there
+    are two fp16 parts in a unit of 2^-7 of the largest, whose last step is 2^-24:
+    each is off by 2^-25 * 2^-7 of the largest at most, where that is more than its
+    roundings (columns in which the keys of large weights hold zeros)."""
+    rng = np.random.default_rng(T)
+    for L in (160, 1300):
+        tab, pages = table(rng, 1, -(-L // 16))
+        p = Pair(pages, 1, 16, D, tab)
+        k = normal(rng, 1, L, 1, D) * np.linspace(0.01, 40, L, dtype=np.float32)[None, :, None, None]
+        p.write(k, normal(rng, 1, L, 1, D))
+        q = normal(rng, 1, T, 4, D)
+        o, lse = p.attention(q, True, start=[L - T])
+        ro, rl, weight, reach = p.host.attention(q, True, G.scale_for(D), [L - T], None)
+        off = 2 * 2.0 ** -24 * (D + 8) * reach
+        floor = 2.0 ** -32 * np.abs(p.host.read(L)[1]).sum(1)[:, None]
+        assert (np.abs(o - ro) <= (2 * off.transpose(0, 2, 1)[..., None] + 2.0 ** -23 * (L + 16)) * weight + floor).all()
+        assert (np.abs(lse - rl) <= off + 2.0 ** -23 * (np.abs(rl) + L + 16)).all()
 
 
 @pytest.mark.parametrize("D, T", [(64, 50), (128, 140)])
