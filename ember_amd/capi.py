@@ -119,6 +119,10 @@ def lib() -> C.CDLL:
     L.token_logprobs.argtypes = [_vp, _i64, _vp, _i64, _i64] + [_vp] * 5 + [C.c_int]
     L.token_logprobs_bwd.restype = C.c_int
     L.token_logprobs_bwd.argtypes = [_vp, _i64] + [_vp] * 6 + [_i64] * 3
+    L.token_logprobs_ex.restype = C.c_int
+    L.token_logprobs_ex.argtypes = [_vp, _i64, _vp, _i64, _i64] + [_vp] * 6 + [C.c_int]
+    L.token_logprobs_bwd_ex.restype = C.c_int
+    L.token_logprobs_bwd_ex.argtypes = [_vp, _i64] + [_vp] * 7 + [_i64] * 3
     _lib = L
     return L
 

@@ -1155,10 +1155,10 @@ static int check_logits(TensorObject *x, TensorObject *tokens, long long rows, l
     return 0;
 }
 
-/* _token_logprobs(logits, tokens, rows, classes, top) -> (logp, lse, entropy, top_tokens|None, top_logp|None). */
+/* _token_logprobs(logits, tokens, rows, classes, top) -> (logp, lse, lse_rest, entropy, top_tokens|None, top_logp|None). */
 static PyObject *py_token_logprobs(PyObject *module, PyObject *args)
 {
-    TensorObject *x, *tokens, *out[5] = {NULL};
+    TensorObject *x, *tokens, *out[6] = {NULL};
     long long rows, classes;
     int top;
     (void)module;
@@ -1168,39 +1168,39 @@ static PyObject *py_token_logprobs(PyObject *module, PyObject *args)
         PyErr_SetString(PyExc_ValueError, "_token_logprobs: top must be from 0 to 64 and at most classes");
         return NULL;
     }
-    for (int i = 0; i < (top ? 5 : 3); i++)
-        if (!(out[i] = alloc_tensor((Py_ssize_t)(i < 3 ? rows : rows * top)))) goto failed;
-    int st = token_logprobs(x->d_ptr, classes, (const int32_t *)tokens->d_ptr, rows, classes, out[0]->d_ptr, out[1]->d_ptr,
-                            out[2]->d_ptr, top ? (int32_t *)out[3]->d_ptr : NULL, top ? out[4]->d_ptr : NULL, top);
+    for (int i = 0; i < (top ? 6 : 4); i++)
+        if (!(out[i] = alloc_tensor((Py_ssize_t)(i < 4 ? rows : rows * top)))) goto failed;
+    int st = token_logprobs_ex(x->d_ptr, classes, (const int32_t *)tokens->d_ptr, rows, classes, out[0]->d_ptr, out[1]->d_ptr,
+                               out[2]->d_ptr, out[3]->d_ptr, top ? (int32_t *)out[4]->d_ptr : NULL, top ? out[5]->d_ptr : NULL, top);
     if (raise_status(st, "_token_logprobs")) goto failed;
-    if (!top) return Py_BuildValue("(NNNOO)", out[0], out[1], out[2], Py_None, Py_None);
-    return Py_BuildValue("(NNNNN)", out[0], out[1], out[2], out[3], out[4]);
+    if (!top) return Py_BuildValue("(NNNNOO)", out[0], out[1], out[2], out[3], Py_None, Py_None);
+    return Py_BuildValue("(NNNNNN)", out[0], out[1], out[2], out[3], out[4], out[5]);
 failed:
-    for (int i = 0; i < 5; i++) Py_XDECREF(out[i]);
+    for (int i = 0; i < 6; i++) Py_XDECREF(out[i]);
     return NULL;
 }
 
-/* _token_logprobs_bwd(logits, tokens, lse, entropy, d_logp|None, d_entropy|None, rows, classes) -> d_logits. */
+/* _token_logprobs_bwd(logits, tokens, lse, lse_rest, entropy, d_logp|None, d_entropy|None, rows, classes) -> d_logits. */
 static PyObject *py_token_logprobs_bwd(PyObject *module, PyObject *args)
 {
-    TensorObject *x, *tokens, *lse, *entropy;
+    TensorObject *x, *tokens, *lse, *rest, *entropy;
     PyObject *po, *eo;
     long long rows, classes;
     (void)module;
-    if (!PyArg_ParseTuple(args, "O!O!O!O!OOLL", &TensorType, &x, &TensorType, &tokens, &TensorType, &lse, &TensorType, &entropy,
+    if (!PyArg_ParseTuple(args, "O!O!O!O!O!OOLL", &TensorType, &x, &TensorType, &tokens, &TensorType, &lse, &TensorType, &rest, &TensorType, &entropy,
                           &po, &eo, &rows, &classes))
         return NULL;
     TensorObject *dp = opt_tensor(po, "d_logp"), *de = opt_tensor(eo, "d_entropy");
     if (dp == (TensorObject *)-1 || de == (TensorObject *)-1 || check_logits(x, tokens, rows, classes, "_token_logprobs_bwd"))
         return NULL;
-    if (lse->size != rows || entropy->size != rows || (dp && dp->size != rows) || (de && de->size != rows)) {
+    if (lse->size != rows || rest->size != rows || entropy->size != rows || (dp && dp->size != rows) || (de && de->size != rows)) {
         PyErr_SetString(PyExc_ValueError, "_token_logprobs_bwd: lse, entropy and gradients must hold rows elements");
         return NULL;
     }
     TensorObject *g = alloc_tensor(x->size);
     if (!g) return NULL;
-    int st = token_logprobs_bwd(x->d_ptr, classes, (const int32_t *)tokens->d_ptr, lse->d_ptr, entropy->d_ptr,
-                                dp ? dp->d_ptr : NULL, de ? de->d_ptr : NULL, g->d_ptr, classes, rows, classes);
+    int st = token_logprobs_bwd_ex(x->d_ptr, classes, (const int32_t *)tokens->d_ptr, lse->d_ptr, rest->d_ptr, entropy->d_ptr,
+                                   dp ? dp->d_ptr : NULL, de ? de->d_ptr : NULL, g->d_ptr, classes, rows, classes);
     if (raise_status(st, "_token_logprobs_bwd")) {
         Py_DECREF(g);
         return NULL;
@@ -1373,7 +1373,7 @@ static PyMethodDef module_methods[] = {
     METHOD("_kv_cache_write", py_kv_cache_write, "round rows into a 4-bit key/value cache"),
     METHOD("_kv_cache_read", py_kv_cache_read, "values that a 4-bit cache holds -> (k, v)"),
     METHOD("_kv_cache_attention", py_kv_cache_attention, "attention over a 4-bit cache -> (o, lse)"),
-    METHOD("_token_logprobs", py_token_logprobs, "log probabilities by token id -> (logp, lse, entropy, top_tokens, top_logp)"),
+    METHOD("_token_logprobs", py_token_logprobs, "log probabilities by token id -> (logp, lse, lse_rest, entropy, top_tokens, top_logp)"),
     METHOD("_token_logprobs_bwd", py_token_logprobs_bwd, "gradient of log probabilities and entropy"),
     {"_synchronize", (PyCFunction)py_synchronize, METH_NOARGS, "wait for all queued device work"},
     {"_empty_cache", (PyCFunction)py_empty_cache, METH_NOARGS,

@@ -6,6 +6,8 @@
 // probabilities.  Here a row is read once and nothing of its size is written:
 //   m = max x,  s = sum e^(x - m),  w = sum (x - m) e^(x - m)
 //   lse = m + ln s,  logp = (x_tok - m) - ln s,  entropy = ln s - w / s
+// (and what rounding lse leaves out, for the gradient: where m is far from 0, ln s
+// has few bits left in lse.)
 // Sums over parts of a row join by
 //   s = sum s_i f_i,  w = sum (w_i + (m_i - m) s_i) f_i,  f_i = e^(m_i - m).
 //
@@ -47,7 +49,7 @@ typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows start
 struct ScoreArgs {
     const float *x;
     const int32_t *tokens;
-    float *logp, *lse, *entropy;
+    float *logp, *lse, *rest, *entropy;
     int32_t *top_tokens;
     float *top_logp;
     char *part;  // of each workgroup: m, s, w, and its waves' best (`top` keys each); null: rows are not cut
@@ -225,7 +227,9 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, int row, Sums t, bool
     const float logs = logf(t.s);
     if (lane == 0) {
         a.logp[row] = known ? (of_token - t.m) - logs : 0.0f;
-        if (a.lse) a.lse[row] = t.m + logs;
+        const float lse = t.m + logs, moved = lse - t.m;
+        if (a.lse) a.lse[row] = lse;
+        if (a.rest) a.rest[row] = fabsf(lse) < INFINITY ? (t.m - (lse - moved)) + (logs - moved) : 0.0f;
         if (a.entropy) a.entropy[row] = logs - t.w / t.s;
     }
     if (lane < a.top) {
@@ -408,7 +412,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
 struct GradArgs {
     const float *x;
     const int32_t *tokens;
-    const float *lse, *entropy, *d_logp, *d_entropy;
+    const float *lse, *rest, *entropy, *d_logp, *d_entropy;
     float *dx;
     int64_t stride, out_stride;
     int classes, segments, row0;
@@ -426,14 +430,14 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_bwd_kernel(GradArgs a
     const int token = a.tokens[row];
     const bool known = token >= 0 && token < a.classes;
     const int at = known ? (int)max(min(token - first, (int64_t)kGradSegment), (int64_t)-1) : -1;
-    const float lse = a.lse[row], dp = known && a.d_logp ? a.d_logp[row] : 0.0f;
+    const float lse = a.lse[row], rest = a.rest ? a.rest[row] : 0.0f, dp = known && a.d_logp ? a.d_logp[row] : 0.0f;
     const float dh = a.d_entropy ? a.d_entropy[row] : 0.0f, h = dh != 0.0f ? a.entropy[row] : 0.0f;
     if (dp == 0.0f && dh == 0.0f) {  // a padded row: whatever it holds
         for (int c = threadIdx.x; c < n; c += kThreads) q[c] = 0.0f;
         return;
     }
     auto grad = [&](float x, int c) {
-        const float logp = x - lse, pr = expf(logp);
+        const float logp = (x - lse) - rest, pr = expf(logp);
         // p ln p is 0 where p is.
         const float g = -pr * (dp + (pr == 0.0f ? 0.0f : dh * (logp + h)));
         return c == at ? g + dp : g;
@@ -469,8 +473,9 @@ bool rows_meet(const float *x, const float *y, int64_t stride, int64_t rows, int
 }  // namespace
 }  // namespace ember
 
-extern "C" int token_logprobs(const float *logits, int64_t row_stride, const int32_t *tokens, int64_t rows, int64_t classes,
-                              float *logp, float *lse, float *entropy, int32_t *top_tokens, float *top_logp, int top)
+extern "C" int token_logprobs_ex(const float *logits, int64_t row_stride, const int32_t *tokens, int64_t rows, int64_t classes,
+                                 float *logp, float *lse, float *lse_rest, float *entropy, int32_t *top_tokens, float *top_logp,
+                                 int top)
 {
     using namespace ember;
     const char *what = "token_logprobs";
@@ -479,9 +484,9 @@ extern "C" int token_logprobs(const float *logits, int64_t row_stride, const int
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
     if (rows == 0) return EMBER_OK;
     if (!logits || !tokens || !logp || (top && (!top_tokens || !top_logp)) ||
-        (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)logp | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)top_tokens | (uintptr_t)top_logp) & 3))
+        (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)logp | (uintptr_t)lse | (uintptr_t)lse_rest | (uintptr_t)entropy | (uintptr_t)top_tokens | (uintptr_t)top_logp) & 3))
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
-    ScoreArgs a = {logits, tokens, logp, lse, entropy, top_tokens, top_logp, nullptr, row_stride, (int)rows, (int)classes};
+    ScoreArgs a = {logits, tokens, logp, lse, lse_rest, entropy, top_tokens, top_logp, nullptr, row_stride, (int)rows, (int)classes};
     a.chunks = (int)((classes + kChunk - 1) / kChunk), a.top = top;
     // A row to a workgroup, unless there are too few for the chip (8 of them fit
     // on a CU): then pieces, but of a chunk at least.
@@ -504,9 +509,15 @@ extern "C" int token_logprobs(const float *logits, int64_t row_stride, const int
     return EMBER_OK;
 }
 
-extern "C" int token_logprobs_bwd(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
-                                  const float *entropy, const float *d_logp, const float *d_entropy, float *d_logits,
-                                  int64_t out_stride, int64_t rows, int64_t classes)
+extern "C" int token_logprobs(const float *logits, int64_t row_stride, const int32_t *tokens, int64_t rows, int64_t classes,
+                              float *logp, float *lse, float *entropy, int32_t *top_tokens, float *top_logp, int top)
+{
+    return token_logprobs_ex(logits, row_stride, tokens, rows, classes, logp, lse, nullptr, entropy, top_tokens, top_logp, top);
+}
+
+extern "C" int token_logprobs_bwd_ex(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
+                                     const float *lse_rest, const float *entropy, const float *d_logp, const float *d_entropy,
+                                     float *d_logits, int64_t out_stride, int64_t rows, int64_t classes)
 {
     using namespace ember;
     const char *what = "token_logprobs_bwd";
@@ -516,9 +527,9 @@ extern "C" int token_logprobs_bwd(const float *logits, int64_t row_stride, const
     if (rows == 0) return EMBER_OK;
     if (!logits || !tokens || !lse || !d_logits || (d_entropy && !entropy) || (logits == d_logits && row_stride != out_stride) ||
         (row_stride == out_stride && rows_meet(logits, d_logits, row_stride, rows, classes)) ||
-        (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)lse | (uintptr_t)entropy | (uintptr_t)d_logp | (uintptr_t)d_entropy | (uintptr_t)d_logits) & 3))
+        (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)lse | (uintptr_t)lse_rest | (uintptr_t)entropy | (uintptr_t)d_logp | (uintptr_t)d_entropy | (uintptr_t)d_logits) & 3))
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
-    GradArgs a = {logits, tokens, lse, entropy, d_logp, d_entropy, d_logits, row_stride, out_stride, (int)classes, (int)segments};
+    GradArgs a = {logits, tokens, lse, lse_rest, entropy, d_logp, d_entropy, d_logits, row_stride, out_stride, (int)classes, (int)segments};
     const int64_t most = kMostBlocks / segments;
     for (int64_t row = 0; row < rows; row += most) {
         a.row0 = (int)row;
@@ -526,4 +537,11 @@ extern "C" int token_logprobs_bwd(const float *logits, int64_t row_stride, const
         if (!launch_ok(what)) return EMBER_ERR_DEVICE;
     }
     return EMBER_OK;
+}
+
+extern "C" int token_logprobs_bwd(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
+                                  const float *entropy, const float *d_logp, const float *d_entropy, float *d_logits,
+                                  int64_t out_stride, int64_t rows, int64_t classes)
+{
+    return token_logprobs_bwd_ex(logits, row_stride, tokens, lse, nullptr, entropy, d_logp, d_entropy, d_logits, out_stride, rows, classes);
 }

@@ -147,7 +147,7 @@ def token_logprobs(logits: Tensor, tokens, top: int = 0) -> TokenLogProbs:
     if not 0 <= top <= min(64, logits.shape[-1]):
         raise ValueError(f"top must be from 0 to {min(64, logits.shape[-1])}, not {top}")
     lead = logits.shape[:-1]
-    logp, lse, entropy, ids_core, best = C._token_logprobs(logits._core, _upload(ids), ids.size, logits.shape[-1], top)
+    logp, lse, _, entropy, ids_core, best = C._token_logprobs(logits._core, _upload(ids), ids.size, logits.shape[-1], top)
     rows = [Tensor._from_core(x, lead) for x in (logp, entropy, lse)]
     if not top:
         return TokenLogProbs(*rows, None, None)
@@ -171,9 +171,9 @@ class TokenLoss(Loss):
         ids = _token_ids(pred, target)
         tokens, known = _upload(ids), ids >= 0
         n = int(known.sum())
-        logp, lse, entropy, _, _ = C._token_logprobs(pred._core, tokens, ids.size, pred.shape[-1], 0)
+        logp, lse, rest, entropy, _, _ = C._token_logprobs(pred._core, tokens, ids.size, pred.shape[-1], 0)
         # The caller's Tensor may adopt another buffer before backward().
-        self.saved = (Tensor._from_core(pred._core, pred.shape), tokens, known, n, lse, entropy)
+        self.saved = (Tensor._from_core(pred._core, pred.shape), tokens, known, n, lse, rest, entropy)
         if n == 0:
             return 0.0
         loss = -_sum(Tensor._from_core(logp, (ids.size,))) / n
@@ -184,12 +184,12 @@ class TokenLoss(Loss):
     def backward(self) -> Tensor:
         if self.saved is None:
             raise RuntimeError("forward() must run before backward()")
-        pred, tokens, known, n, lse, entropy = self.saved
+        pred, tokens, known, n, lse, rest, entropy = self.saved
         if n == 0:
             return _random.zeros(pred.shape)
         d_logp = _random.constant(-1.0 / n, (known.size,))
         d_entropy = Tensor(np.where(known, -self.entropy_bonus / n, 0.0)) if self.entropy_bonus else None
-        grad = C._token_logprobs_bwd(pred._core, tokens, lse, entropy, d_logp._core,
+        grad = C._token_logprobs_bwd(pred._core, tokens, lse, rest, entropy, d_logp._core,
                                      None if d_entropy is None else d_entropy._core, known.size, pred.shape[-1])
         return Tensor._from_core(grad, pred.shape)
 

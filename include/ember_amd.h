@@ -434,10 +434,21 @@ int token_logprobs(const float *logits, int64_t row_stride, const int32_t *token
  * d_logp taken as 0 where tokens[r] is out of range, and a row with both
  * gradients 0 gets zeros whatever its logits hold; row r at d_logits +
  * r*out_stride.  d_logits may be logits itself (with the same stride); it
- * must not overlap it otherwise.  Rows and classes as in token_logprobs. */
+ * must not overlap it otherwise.  Rows and classes as in token_logprobs.  p_j is
+ * formed as exp(x_j - lse): off by the rounding of lse, up to 2^-24 |lse| of p_j. */
 int token_logprobs_bwd(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
                        const float *entropy, const float *d_logp, const float *d_entropy, float *d_logits,
                        int64_t out_stride, int64_t rows, int64_t classes);
+/* The same with lse in two floats, lse and what its rounding leaves out (lse_rest,
+ * rows; may be NULL), from which the gradient's p_j is exp((x_j - lse) - lse_rest):
+ * for logits that are far from 0, where lse itself keeps few bits of ln sum. */
+int token_logprobs_ex(const float *logits, int64_t row_stride, const int32_t *tokens, int64_t rows,
+                      int64_t classes, float *logp, float *lse, float *lse_rest, float *entropy,
+                      int32_t *top_tokens, float *top_logp, int top);
+int token_logprobs_bwd_ex(const float *logits, int64_t row_stride, const int32_t *tokens, const float *lse,
+                          const float *lse_rest, const float *entropy, const float *d_logp,
+                          const float *d_entropy, float *d_logits, int64_t out_stride, int64_t rows,
+                          int64_t classes);
 
 #undef EMBER_BINARY_OP
 #undef EMBER_SCALAR_OP

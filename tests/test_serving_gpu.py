@@ -272,3 +272,28 @@ def test_token_loss_of_more_rows_than_one_grid_takes():
     got = loss.backward().to_np()
     want = np.where(np.arange(2) == (np.arange(rows) % 2)[:, None], -0.5, 0.5) / rows
     assert (np.abs(got - want) <= 8 * U / rows).all()
+
+
+@pytest.mark.parametrize("offset", [0.0, -1000.0, 3e4, 1e6])
+@pytest.mark.parametrize("bonus", [0.0, 0.3])
+def test_token_loss_of_logits_far_from_zero(offset, bonus):
+    """Logits with an offset as those without: x - lse is exact where p is not tiny,
+    so p is off by the steps of ln s and exp, 16 and 2 |ln p| half steps at most."""
+    rng = np.random.default_rng(11)
+    rows, classes = 40, 5000
+    x = (3 * normal(rng, rows, classes) + np.float32(offset)).astype(np.float32)
+    tokens = rng.integers(0, classes, rows)
+    loss = TokenLoss(entropy_bonus=bonus)
+    loss.forward(em.Tensor(x), tokens)
+    grad = loss.backward().to_np()
+    m = x.max(-1, keepdims=True).astype(np.float64)
+    logp = x - m - np.log(np.exp(x - m).sum(-1, keepdims=True))
+    p, entropy = np.exp(logp), -(np.exp(logp) * logp).sum(-1, keepdims=True)
+    hot = np.eye(classes)[tokens]
+    want = (p - hot + bonus * p * (logp + entropy)) / rows
+    size = p + hot + bonus * p * (np.abs(logp) + entropy)
+    assert (np.abs(grad - want) <= U * (16 + 4 * np.abs(logp)) * size / rows).all()
+    if not bonus:
+        dense = CrossEntropyLoss()
+        dense.forward(em.Tensor(x), em.Tensor(hot.astype(np.float32)))
+        assert (np.abs(dense.backward().to_np() - want) <= U * (32 + 4 * np.abs(logp)) * size / rows).all()

@@ -138,3 +138,9 @@ def test_gradients(change):
 ])
 def test_gradients_partly_over_the_logits(change):
     refused(grad(**change))
+
+
+def test_the_rest_of_lse_is_aligned():
+    L = capi.lib()
+    refused(L.token_logprobs_ex(P, 100, P, 4, 100, P, P, P + 2, P, None, None, 0))
+    refused(L.token_logprobs_bwd_ex(P, 100, P, P, P + 1, P, P, P, 8192, 100, 4, 100))

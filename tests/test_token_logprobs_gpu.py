@@ -296,3 +296,27 @@ def test_no_numbers_in_a_late_chunk(rows):
     others = np.arange(rows) % 5 > 1
     for a, b in zip(clean, (logp, lse, ent, ids, best)):
         np.testing.assert_array_equal(a[others], b[others])
+
+
+@pytest.mark.parametrize("rows, classes", [(5, 1000), (3, 20000), (1100, 5000)])
+def test_lse_in_two_floats(rows, classes):
+    """lse + lse_rest has ln s to its own roundings, however far the logits are from
+    0; the other outputs are those of token_logprobs, and rows that are no numbers
+    have no rest."""
+    rng = np.random.default_rng(rows)
+    x = (2 * rng.standard_normal((rows, classes)) + 10.0 ** rng.integers(0, 7, (rows, 1))).astype(np.float32)
+    x[1], x[2, 3] = -np.inf, np.inf
+    G.say(f"token_logprobs_ex rows={rows} classes={classes}")
+    dx, tk = DeviceArray.from_numpy(x), ints(np.zeros(rows))
+    logp, lse, rest, ent = (DeviceArray((rows,)) for _ in range(4))
+    capi.check(capi.lib().token_logprobs_ex(dx.ptr, classes, tk.ptr, rows, classes, logp.ptr, lse.ptr, rest.ptr, ent.ptr, None, None, 0),
+               "token_logprobs_ex")
+    for a, b in zip((logp, lse, ent), score(x, np.zeros(rows, int), 0)):
+        np.testing.assert_array_equal(a.numpy(), b)
+    good = np.ones(rows, bool)
+    good[1:3] = False
+    assert (rest.numpy()[1:3] == 0).all()
+    m = x[good].max(-1).astype(np.float64)
+    logs = np.log(np.exp(x[good] - m[:, None]).sum(-1))
+    got = (lse.numpy()[good].astype(np.float64) - m) + rest.numpy()[good]
+    assert (np.abs(got - logs) <= U * (64 + 19 * 2 + np.ptp(x[good], -1) + 4 * logs)).all()
