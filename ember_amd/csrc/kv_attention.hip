@@ -100,11 +100,6 @@ struct Words {
             w[0] = *p;
         }
     }
-    __device__ __forceinline__ void zero()
-    {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0;
-    }
 };
 
 // What a lane holds of 16 keys, and of 16 values.  Where there are none (at < 0)

@@ -27,7 +27,7 @@
 // Two tiles of LDS: while one is worked on, the next is converted into the other
 // and the one after is loaded; one barrier a tile.
 //
-// LDS: K rows are D bf16 long, V^T rows 64, cut into pieces of 16 bytes whose
+// LDS: K rows are D numbers of 16 bits long (fp16, or bf16 in the second walk), V^T rows 64, cut into pieces of 16 bytes whose
 // place in the row is turned by the row's number (k_place, v_place), so that
 // neither the 32 rows that a wave reads at once nor the ones that it writes lie
 // in the same banks.
@@ -65,7 +65,7 @@ __device__ unsigned g_done[kMostUnits];
 
 template <int D>
 struct Lds {
-    uint4 k[kTile * D / 8], v[kTile * D / 8];  // bf16
+    uint4 k[kTile * D / 8], v[kTile * D / 8];  // fp16, or bf16 in the second walk
     // Of the tile's 64 tokens and each group of 32, whether the values are no
     // numbers (bytes: token within the group of D); then, of each 16 tokens,
     // whether they are not there.

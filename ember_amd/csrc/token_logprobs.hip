@@ -316,7 +316,8 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(ScoreArgs a)
             auto all = [&](auto f) {
 #pragma unroll
                 for (int j = 0; j < kPerThread / 4; ++j) {
-                    // Below the last that is kept?  (A NaN is never below.)
+                    // Below the last that is kept?  (A NaN goes with the others of its
+                    // four; its place in the order is not specified.)
                     const float least = value_of(best.last + 1);
                     if (!__any(!(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) < least))) continue;
 #pragma unroll
@@ -488,8 +489,9 @@ extern "C" int token_logprobs_ex(const float *logits, int64_t row_stride, const 
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
     ScoreArgs a = {logits, tokens, logp, lse, lse_rest, entropy, top_tokens, top_logp, nullptr, row_stride, (int)rows, (int)classes};
     a.chunks = (int)((classes + kChunk - 1) / kChunk), a.top = top;
-    // A row to a workgroup, unless there are too few for the chip (8 of them fit
-    // on a CU): then pieces, but of a chunk at least.
+    // A row to a workgroup, unless there are too few for the chip: then pieces, 8 to
+    // a CU (which holds 8 at once without alternatives; with them 5, by their 86
+    // registers and 24.6 KB), but of a chunk at least.
     const int64_t slots = std::min<int64_t>(8 * (int64_t)std::max(device_cu_count(), 1), kMostRows);
     a.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, slots / rows));
     a.per = (a.chunks + a.pieces - 1) / a.pieces;

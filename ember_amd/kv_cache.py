@@ -7,8 +7,8 @@ format: 32 neighbours of a head row share a power of two and are rounded to
 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times it).  ``write`` appends rows, ``attention``
 is the causal attention of the rows last appended over all that their
 sequences hold, ``read`` gives the values back.  Lengths and the page table
-are kept on the host and, for the kernels, on the device; a step that needs
-no new page uploads nothing.
+are kept on the host and, for the kernels, on the device; a step uploads the
+table where a sequence gets a new page, and its counts where they are given.
 """
 
 from __future__ import annotations

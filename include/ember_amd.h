@@ -341,11 +341,14 @@ int layernorm_bwd(const float *x, const float *gamma, const float *mean, const f
  * Keys and values of tokens already seen, for decoding.  A token's head row of
  * D elements is cut into groups of 32 neighbours; a group is held as 32 E2M1
  * codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign bit, 8) that share one scale
- * 2^e, stored as the byte e + 127 (the OCP MXFP4 format).  e is the smallest
- * number with amax <= 6 * 2^e, but at least -119; each element is rounded to
- * the nearest code times 2^e, ties to the even code.  A group of zeros has the
- * scale byte 127; one that holds a NaN or a size from 2^127 on has the byte 255
- * and reads back as NaN.
+ * 2^e, stored as the byte e + 127: the OCP MXFP4 format.  The scale's rule is not
+ * that of OCP's conversion (floor(log2 amax) - 2, sizes past 6 * 2^e cut to it): e
+ * is the smallest number with amax <= 6 * 2^e, but at least -119, so that nothing
+ * is cut; each element is rounded to the nearest code times 2^e, ties to the
+ * even code.  A group of zeros has the scale byte 127; one that holds a NaN or a
+ * size from 2^127 on has the byte 255 and reads back as NaN.  Caches that were
+ * filled otherwise may hold any codes, and the bytes 8 to 252 and 255; what
+ * attention makes of others is not specified.
  *
  * Codes are (pages, heads, page_size, D/2) bytes, element 2i of a row in the
  * low nibble of byte i and 2i+1 in the high one; scales are (pages, heads,
@@ -395,9 +398,10 @@ int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, int64_t T, in
  * o_t = softmax_j(s[t][.]) v, lse_t = ln sum_j exp(s[t][j]) (may be NULL),
  * dense (sequences, q_heads, T).  A row that is not valid, or sees no key,
  * gets o = 0 and lse = -infinity.  Keys and values enter exactly, and q, times
- * scale's significand, to 24 bits; where a cache head has more than 24 rows, to 23 bits or to 2^-39 of its
- * row's largest element, whichever is coarser, and weights to 23 bits or to 2^-32
- * of the row's largest: an fp32 attention over kv_cache_read's values.
+ * scale's significand, to 24 bits; where a cache head has more than 24 rows, to 23
+ * bits or to 2^-39 of its row's largest element, whichever is coarser, and weights
+ * to 23 bits or to 2^-32 of the row's largest: an fp32 attention over
+ * kv_cache_read's values.
  * A row of q that holds an infinity or a NaN gets NaN; keys and values that
  * read back as NaN reach the rows that see them, and no others.  scale is
  * finite and >= 0.  With R = T * q_heads / heads rows to a cache head, R is at
