@@ -44,6 +44,12 @@
 // of 128 (178 MB) 42.6, of which about 8 are the launch, the plan, the first loads and
 // the join; what is between runs at 5.2 to 5.5 TB/s.  16 x 5 rows over 3001, 16 heads of
 // 64 (28 MB) 14.8.
+//
+// Compiled with blocks that are only jumped to at multiples of 32 bytes: how the loop's
+// blocks fall on what is fetched at once decides short calls, and any edit before them
+// moved it.  One token of 2 x 5 heads of 64 over up to 20206 12.8 us so, 12.8 to 14.5
+// by the place of the loop without; of 32 / 8 heads of 128 over 131072 36.0, and to
+// 39.2; long calls alike.
 #include <algorithm>
 #include <type_traits>
 
@@ -396,11 +402,6 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
                 }
             }
         };
-        // Where the loop begins in a line of the instruction cache (64 bytes) decides how
-        // its blocks fall on further ones: one token of 2 x 5 heads of 64 over up to 20206
-        // 12.8 us from byte 48 on, 13.8 from 32 on, 14.4 before; 2 x 56 / 8 heads over up to
-        // 14943 12.5, 13.1 and 13.3 to 13.8; long calls alike.
-        asm volatile(".p2align 6\n.rept 14\ns_nop 0\n.endr");
         while (tl + kWaves < end) step(std::true_type{});
         step(std::false_type{});
     }
