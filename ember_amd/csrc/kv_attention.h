@@ -41,11 +41,12 @@ struct KvAttnArgs {
     float *part;  // of each workgroup: O (rows, D), then m and l of each row; null: units are not cut
     int T, q_heads, group, tiles, blocks, causal;  // tiles: of rows, of a head
     int key_shift, least;  // of the keys of a tile, tiles of a piece at least
-    // scale * log2(e) = q_scale * scale2, and scale2 a power of two: Q is multiplied by
-    // q_scale (from 0.5 to 1, or 0) as it is read, so that a score, a sum of products times
-    // scale2, has no rounding but the sum's.  Rounded, the largest of a row and the same
-    // score under an fma would differ by half a step: 32 from 2^29 on, a factor of 2^32.
-    float q_scale, scale2;
+    // scale * log2(e): Q is multiplied by it as it is read, and a score is the sum of
+    // products.  (Scaled then and rounded, the largest of a row and the same score under an
+    // fma would differ by half a step: 32 from 2^29 on, a factor of 2^32.)  Where Q is
+    // shifted to its row's size, by q_scale (from 0.5 to 1, or 0), and what is left,
+    // scale2, is a power of two.
+    float scale, q_scale, scale2;
     Divisor by_group, by_tiles, by_units;  // units: of a sequence
     int most;      // pieces of a unit of each sequence, together
     float shares;  // a piece is not less than all sequences' tiles over this, either

@@ -223,6 +223,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
         for (int j = 0; j < 2; ++j) kk[j].load(a.c, at[j], lane);
 #pragma unroll
         for (int j = 0; j < 2; ++j) vv[j].load(a.c, at[j], lane);
+        // No use of Q, and so no wait for it, between the loads, which the compiler mixes
+        // (8 rows of 8 x 8 heads of 128 over 4096 13.1 -> 11.9 us; with four rows 12.7 ->
+        // 13.3, and with heads of 64 12.5 -> 12.7).
+        if (D == 128 && ROWS == 8) __builtin_amdgcn_sched_barrier(0);
 
         u32x4 q[SHARED ? 1 : 3][KS];
 #pragma unroll
@@ -230,8 +234,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 unsigned p0[3], p1[3];
-                cut3(any ? product(raw[s][i >> 1][2 * (i & 1)], a.q_scale) : 0.0f, p0[0], p0[1], p0[2]);
-                cut3(any ? product(raw[s][i >> 1][2 * (i & 1) + 1], a.q_scale) : 0.0f, p1[0], p1[1], p1[2]);
+                cut3(any ? product(raw[s][i >> 1][2 * (i & 1)], a.scale) : 0.0f, p0[0], p0[1], p0[2]);
+                cut3(any ? product(raw[s][i >> 1][2 * (i & 1) + 1], a.scale) : 0.0f, p1[0], p1[1], p1[2]);
                 if (SHARED) {
                     p0[0] = part == 0 ? p0[0] : part == 1 ? p0[1] : p0[2];
                     p1[0] = part == 0 ? p1[0] : part == 1 ? p1[1] : p1[2];
@@ -298,7 +302,6 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
             float top = s[0];
 #pragma unroll
             for (int x = 1; x < SC; ++x) top = fmaxf(top, s[x]);
-            top *= a.scale2;
             if (__any(top > m + kRaise)) {
                 // The lanes of a row: 16 neighbours (and as many 32 on), or those 16 apart.
                 const auto most = [](float x, float y) { return fmaxf(x, y); };
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D, ROWS)) void kv_attention_ker
             unsigned cut[SC][3];
 #pragma unroll
             for (int x = 0; x < SC; ++x) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[x], a.scale2, -m));
+                const float e = __builtin_amdgcn_exp2f(s[x] - m);
                 l += e;
                 cut3(e, cut[x][0], cut[x][1], cut[x][2]);
                 if (SHARED)
@@ -564,11 +567,11 @@ extern "C" int kv_cache_attention(const ember_kv_cache *cache, const float *q, f
     a.start = start, a.count = count;
     a.T = (int)T, a.q_heads = (int)q_heads, a.group = (int)(q_heads / a.c.heads);
     a.causal = causal != 0;
-    const float all = std::min(scale * kLog2e, 3.402823466e38f);
+    a.scale = std::min(scale * kLog2e, 3.402823466e38f);
     int e;
-    frexpf(all, &e);
+    frexpf(a.scale, &e);
     e = std::min(std::max(e, -126), 127);  // scale2 is a normal number: a masked score stays -infinity under it
-    a.q_scale = ldexpf(all, -e), a.scale2 = ldexpf(1.0f, e);
+    a.q_scale = ldexpf(a.scale, -e), a.scale2 = ldexpf(1.0f, e);
     if (T * a.group > few_rows(a.c)) return launch_kv_attention_rows(a);
     return a.c.D == 128 ? launch_rows<128>(a) : a.c.D == 64 ? launch_rows<64>(a) : launch_rows<32>(a);
 }

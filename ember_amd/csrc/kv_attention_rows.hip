@@ -331,7 +331,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
             if (HALF) units16 = units_at(a.c, row_of(a.c, b, h, first * kTile));
         }
         u32x4 q[KS][P];
-        float scale2 = a.scale2;
+        float scale2 = 1.0f;
         {
             const float *src = a.q + b * a.qs.sb + (int64_t)(h * a.group + g) * a.qs.sh + t * a.qs.ss + 8 * half;
             f32x4 x[KS][2];
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                         for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
                 most = across_32(most, larger) * fmaxf(a.q_scale, 0.5f);  // (0: any shift that Q can take)
                 shift = 14 + 127 - (int)(float_bits(most) >> 23);
-                scale2 = fminf(fmaxf(ldexpf(scale2, units16.k - 127 - shift), 0x1p-126f), 0x1p127f);
+                scale2 = fminf(fmaxf(ldexpf(a.scale2, units16.k - 127 - shift), 0x1p-126f), 0x1p127f);
             }
 #pragma unroll
             for (int s = 0; s < KS; ++s)
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void kv_attention_rows_kern
                     for (int j = 0; j < 2; ++j) {
                         const float x0 = x[s][i][2 * j], x1 = x[s][i][2 * j + 1];
                         if constexpr (HALF) cut_scaled(ldexpf(x0, shift), ldexpf(x1, shift), a.q_scale, q[s], 2 * i + j);
-                        else cut_pair<false>(product(x0, a.q_scale), product(x1, a.q_scale), q[s], 2 * i + j);
+                        else cut_pair<false>(product(x0, a.scale), product(x1, a.scale), q[s], 2 * i + j);
                     }
         }
 #pragma unroll

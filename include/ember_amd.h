@@ -397,8 +397,8 @@ int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, int64_t T, in
  * the valid row t iff j < start + count and, when causal, j <= start + t;
  * o_t = softmax_j(s[t][.]) v, lse_t = ln sum_j exp(s[t][j]) (may be NULL),
  * dense (sequences, q_heads, T).  A row that is not valid, or sees no key,
- * gets o = 0 and lse = -infinity.  Keys and values enter exactly, and q, times
- * scale's significand, to 24 bits; where a cache head has more than 24 rows, to 23
+ * gets o = 0 and lse = -infinity.  Keys and values enter exactly, and q * scale to
+ * 24 bits (below 2^-110 to fewer); where a cache head has more than 24 rows, to 23
  * bits or to 2^-39 of its row's largest element, whichever is coarser, and weights
  * to 23 bits or to 2^-32 of the row's largest: an fp32 attention over
  * kv_cache_read's values.

@@ -364,6 +364,17 @@ def test_large_scores(size, T, D):
 
 
 @pytest.mark.parametrize("T", [1, 3, 7, 50, 140])
+@pytest.mark.parametrize("scale", [1e-40, 1e-30, 0.7, 1.3 * 2.0 ** 100, 1e38])
+def test_scales_of_all_sizes(scale, T):
+    """A scale and queries whose product is of ordinary size, to the ends of fp32's range."""
+    rng = np.random.default_rng(T)
+    scale = float(np.float32(scale))
+    p = filled(rng, 1, 1, 16, 64, 150)
+    q = (normal(rng, 1, T, 1, 64) * min(0.125 / scale, 2.0 ** 120)).astype(np.float32)
+    p.check_attention(q, True, scale=scale, start=[150 - T])
+
+
+@pytest.mark.parametrize("T", [1, 3, 7, 50, 140])
 def test_scale_zero_whatever_the_products(T):
     """Products of 10^37 with a scale of 0: every key that a row sees weighs the same."""
     rng = np.random.default_rng(T)
