@@ -67,10 +67,10 @@ constexpr int per_cu(int D, int rows)
 }
 // Workgroups that the keys are cut for, to a CU: fewer than fit, as every further piece
 // of a unit is joined by one workgroup in the end, and more of them stream no faster.
-// As many as fit and these (us): D = 128, 4 x 1 token, 16 heads over up to 32768 46.4
-// and 42.6, 4 tokens of 16 / 4 heads over 16384 23.2 and 17.6, 8 rows of 8 x 8 heads over
-// 4096 15.0 and 13.2; D = 64, 4 x 4 tokens of 16 heads over up to 16384 18.4 and 17.7; 16
-// x 5 rows over 3001 14.8 and 15.0, with two 16.3.
+// As many as fit and these (us): D = 128, 4 x 1 token, 16 heads over up to 32768 46.5
+// and 42.8, 4 tokens of 16 / 4 heads over 16384 18.0 and 16.3, 8 rows of 8 x 8 heads over
+// 4096 13.2 and 11.9; D = 64, 4 x 4 tokens of 16 heads over up to 16384 19.1 and 17.9; 16
+// x 5 rows over 3001 14.8 and 14.8, with two 16.1.
 constexpr int cut_for(int D, int rows)
 {
     return D == 128 ? (rows == 8 ? 1 : 2) : 3;

@@ -22,21 +22,22 @@
 // piece's first token; where a value that a row sees fits no fp16 (far larger or
 // smaller than that, or no number), the workgroup walks its keys again with bf16
 // values, which hold them all, and three parts.
-//   2 x 1024 rows of 32 / 8 heads of 128 over 8192: two fp16 parts 345 us, three bf16 ones
-//   486, and both, where every piece has such a value, 2.1 times the first's.
+//   2 x 1024 rows of 32 / 8 heads of 128 over up to 8192 (186 GFLOP): two fp16 parts 345
+//   us, three bf16 ones 486, and both, where every piece has such a value, 2.1 times the
+//   first's.
 // Two tiles of LDS: while one is worked on, the next is converted into the other
 // and the one after is loaded; one barrier a tile.
 //
-// LDS: K rows are D numbers of 16 bits long (fp16, or bf16 in the second walk), V^T rows 64, cut into pieces of 16 bytes whose
-// place in the row is turned by the row's number (k_place, v_place), so that
-// neither the 32 rows that a wave reads at once nor the ones that it writes lie
-// in the same banks.
+// LDS: K rows are D numbers of 16 bits long (fp16, or bf16 in the second walk), V^T
+// rows 64, cut into pieces of 16 bytes whose place in the row is turned by the row's
+// number (k_place, v_place), so that neither the 32 rows that a wave reads at once
+// nor the ones that it writes lie in the same banks.
 //
 // Work: 8 * T * keys * D matrix operations a head where 4 are the definition's.
-// Bound by power: 2 x 1024 rows of 32 / 8 heads of 128 over 8192 keys, causal, take 345
-// us, 574 TFLOP/s of the definition's and 1.15 PFLOP/s of fp16 at about 1.9 GHz (a large
-// bf16 library product reaches 1.23; before the clock falls, 279 us), the matrix cores
-// busy 51 % of the time and the vector units 43 %, however the two are mixed; 4 x 512
+// Bound by power: 2 x 1024 rows of 32 / 8 heads of 128 over 8192 keys each, causal, take
+// 490 us, 526 TFLOP/s of the definition's and 1.05 PFLOP/s of fp16 at about 1.9 GHz (a
+// large bf16 library product reaches 1.23), the matrix cores busy 51 % of the time and
+// the vector units 43 %, however the two are mixed; 4 x 512
 // rows of 16 heads of 64 over 4096 61 us.
 #include <type_traits>
 
