@@ -402,7 +402,8 @@ int kv_cache_read(const ember_kv_cache *cache, float *k, float *v, int64_t T, in
  * bits or to 2^-39 of its row's largest element, whichever is coarser, and weights
  * to 23 bits or to 2^-32 of the row's largest: an fp32 attention over
  * kv_cache_read's values.
- * A row of q that holds an infinity or a NaN gets NaN; keys and values that
+ * A row of q that holds an infinity or a NaN gets NaN, and may where q * scale *
+ * log2(e) passes fp32's range; keys and values that
  * read back as NaN reach the rows that see them, and no others.  scale is
  * finite and >= 0.  With R = T * q_heads / heads rows to a cache head, R is at
  * most 2^30; calls with sequences * heads * ceil(R / 8) from 2^24 on may be
