@@ -375,6 +375,22 @@ def test_scales_of_all_sizes(scale, T):
 
 
 @pytest.mark.parametrize("T", [1, 3, 7, 50, 140])
+@pytest.mark.parametrize("sizes", [(-100, 100), (100, -100), (120, -115), (-140, 20), (20, -60)])
+def test_queries_and_keys_of_all_sizes(sizes, T):
+    """Queries about 2^a, other rows up to 2^40 smaller, and keys about 2^b, under a
+    scale that makes scores of ordinary size."""
+    rng = np.random.default_rng(T)
+    a, b = sizes
+    tab, pages = table(rng, 1, 10)
+    p = Pair(pages, 1, 16, 64, tab)
+    p.write(normal(rng, 1, 150, 1, 64) * np.float32(2.0 ** b), normal(rng, 1, 150, 1, 64))
+    apart = 2.0 ** -rng.integers(0, 41, (1, T, 2, 1))
+    apart[0, 0] = 1
+    q = (normal(rng, 1, T, 2, 64) * apart * 2.0 ** a).astype(np.float32)
+    p.check_attention(q, True, scale=float(np.float32(0.1 * 2.0 ** -(a + b))), start=[150 - T])
+
+
+@pytest.mark.parametrize("T", [1, 3, 7, 50, 140])
 def test_scale_zero_whatever_the_products(T):
     """Products of 10^37 with a scale of 0: every key that a row sees weighs the same."""
     rng = np.random.default_rng(T)
