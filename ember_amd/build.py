@@ -29,7 +29,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 # (source, extra hipcc flags).  -amdgpu-mfma-vgpr-form=1 keeps MFMA
 # accumulators in VGPRs; attention_bwd.hip explains which instantiations use
-# which form and why.  -align-all-nofallthru-blocks=5: kv_attention.hip says why.
+# which form and why.  -align-all-nofallthru-blocks=6: kv_attention.hip says why.
 HIP_SOURCES = [
     ("runtime.hip", []),
     ("elementwise.hip", []),
@@ -46,7 +46,7 @@ HIP_SOURCES = [
     ("softmax.hip", []),
     ("distributions.hip", []),
     ("kv_cache.hip", []),
-    ("kv_attention.hip", ["-mllvm", "-align-all-nofallthru-blocks=5"]),
+    ("kv_attention.hip", ["-mllvm", "-align-all-nofallthru-blocks=6"]),
     ("kv_attention_rows.hip", []),
     ("token_logprobs.hip", []),
 ]

@@ -45,11 +45,11 @@
 // the join; what is between runs at 5.2 to 5.5 TB/s.  16 x 5 rows over 3001, 16 heads of
 // 64 (28 MB) 14.8.
 //
-// Compiled with blocks that are only jumped to at multiples of 32 bytes: how the loop's
-// blocks fall on what is fetched at once decides short calls, and any edit before them
-// moved it.  One token of 2 x 5 heads of 64 over up to 20206 12.8 us so, 12.8 to 14.5
-// by the place of the loop without; of 32 / 8 heads of 128 over 131072 36.0, and to
-// 39.2; long calls alike.
+// Compiled with blocks that are only jumped to at multiples of 64 bytes, a line of the
+// instruction cache: how the loop's blocks fall on lines decides short calls, and any
+// edit before them moved it.  One token of 2 x 5 heads of 64 over up to 20206 12.9 us
+// so, 12.8 to 14.5 by the place of the loop without (with 32 bytes 12.8, and after an edit
+// 14.7); of 32 / 8 heads of 128 over 131072 36.0, and to 39.2; other long calls alike.
 #include <algorithm>
 #include <type_traits>
 
