@@ -49,6 +49,10 @@ HIP_SOURCES = [
     ("kv_attention.hip", ["-mllvm", "-align-all-nofallthru-blocks=6"]),
     ("kv_attention_rows.hip", []),
     ("token_logprobs.hip", []),
+    ("rmsnorm.hip", []),
+    ("rows8.hip", []),
+    ("linear8.hip", []),
+    ("gated.hip", []),
 ]
 
 HIP_FLAGS = [

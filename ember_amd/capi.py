@@ -37,6 +37,13 @@ class KVCacheView(C.Structure):
                 ("sequences", _i64), ("max_pages", _i64)]
 
 
+class Rows8View(C.Structure):
+    """ember_rows8: where a matrix in 8 bits lies (addresses of device memory),
+    and its size."""
+
+    _fields_ = [("codes", _vp), ("scales", _vp), ("rows", _i64), ("cols", _i64)]
+
+
 def exported_symbols() -> list[str]:
     """Every function name include/ember_amd.h declares (operators.def expanded)."""
     names: list[str] = []
@@ -92,6 +99,20 @@ def lib() -> C.CDLL:
     L.cross_entropy_loss.argtypes = [_vp] * 4 + [C.c_int, C.c_int, C.c_float, C.POINTER(C.c_float)]
     L.gemm_ex.restype = C.c_int
     L.gemm_ex.argtypes = [_vp] * 3 + [C.c_int] * 6 + [_vp] * 3 + [C.c_int]
+    L.linear_fwd.restype = C.c_int
+    L.linear_fwd.argtypes = [_vp] * 6 + [C.c_int] * 4
+    L.gelu_bwd.restype = C.c_int
+    L.gelu_bwd.argtypes = [_vp] * 4 + [_i64]
+    L.col_sum.restype = C.c_int
+    L.col_sum.argtypes = [_vp] * 2 + [_i64] * 2
+    L.gelu_bwd_col_sum.restype = C.c_int
+    L.gelu_bwd_col_sum.argtypes = [_vp] * 4 + [_i64] * 2
+    L.layernorm_fwd.restype = C.c_int
+    L.layernorm_fwd.argtypes = [_vp] * 6 + [_i64] * 2 + [C.c_float]
+    L.layernorm_bwd.restype = C.c_int
+    L.layernorm_bwd.argtypes = [_vp] * 9 + [_i64] * 2
+    L.mse_loss.restype = C.c_int
+    L.mse_loss.argtypes = [_vp] * 3 + [C.c_int, C.c_float, C.POINTER(C.c_float)]
     L.ember_set_deterministic.argtypes = [C.c_int]
     L.ember_set_deterministic.restype = None
     L.ember_get_deterministic.argtypes = []
@@ -123,6 +144,25 @@ def lib() -> C.CDLL:
     L.token_logprobs_ex.argtypes = [_vp, _i64, _vp, _i64, _i64] + [_vp] * 6 + [C.c_int]
     L.token_logprobs_bwd_ex.restype = C.c_int
     L.token_logprobs_bwd_ex.argtypes = [_vp, _i64] + [_vp] * 7 + [_i64] * 3
+    rows8 = C.POINTER(Rows8View)
+    L.rmsnorm_fwd.restype = C.c_int
+    L.rmsnorm_fwd.argtypes = [_vp] * 6 + [_i64] * 2 + [C.c_float]
+    L.rmsnorm_bwd.restype = C.c_int
+    L.rmsnorm_bwd.argtypes = [_vp] * 7 + [_i64] * 2
+    L.rmsnorm_fwd8.restype = C.c_int
+    L.rmsnorm_fwd8.argtypes = [_vp] * 4 + [rows8, C.c_float]
+    L.rows8_write.restype = C.c_int
+    L.rows8_write.argtypes = [rows8, _vp, _i64, C.c_int]
+    L.rows8_read.restype = C.c_int
+    L.rows8_read.argtypes = [rows8, _vp, _i64]
+    L.linear8_fwd.restype = C.c_int
+    L.linear8_fwd.argtypes = [rows8, rows8] + [_vp] * 3 + [C.c_int]
+    L.gated_fwd.restype = C.c_int
+    L.gated_fwd.argtypes = [_vp] * 5 + [C.c_int] * 4
+    L.gated_bwd.restype = C.c_int
+    L.gated_bwd.argtypes = [_vp] * 4 + [C.c_int] * 4
+    L.gated8_fwd.restype = C.c_int
+    L.gated8_fwd.argtypes = [rows8, rows8, _vp, rows8, C.c_int]
     _lib = L
     return L
 

@@ -41,7 +41,10 @@ enum ScratchSlot {
     kScratchAttnOrder = 5,
     kScratchKvAttention = 6,
     kScratchLogprobs = 7,
-    kScratchSlots = 8
+    kScratchRmsNorm = 8,
+    kScratchLinear8 = 9,
+    kScratchGated = 10,
+    kScratchSlots = 11
 };
 
 // The library-wide switch set by ember_set_deterministic.

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "activation.h"
 #include "common.h"
 #include "gemm_shape.h"
 #include "mfma.h"
@@ -42,14 +43,6 @@ struct GemmArgs {
     float *pre;
     int act;  // 0 none, 1 Ember's GELU
 };
-
-// Ember's GELU, 0.5*x*(1 + tanh(0.8*x)) (ember/nn/activations.py:58), in the
-// order Ember's element-wise operators evaluate it.
-__device__ __forceinline__ float gelu08(float x)
-{
-#pragma clang fp contract(off)
-    return (x * 0.5f) * (tanhf(x * 0.8f) + 1.0f);
-}
 
 __device__ __forceinline__ float epilogue(const GemmArgs &g, float v, int64_t off, int col)
 {

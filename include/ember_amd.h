@@ -16,7 +16,7 @@
  * Python GIL), the library expects one host thread in it at a time per
  * device: operators that use library scratch (attention_bwd's row
  * statistics, split-K and reduction partials, the pieces of kv_cache_attention
- * and token_logprobs) share one buffer per device and operator, and two threads'
+ * and token_logprobs, a gated layer's sums) share one buffer per device and operator, and two threads'
  * launches may interleave on the null stream.  The allocator and the error slots are thread-safe.
  *
  * Error behaviour.  The reference prints and calls exit() on any device
@@ -24,7 +24,7 @@
  * their signatures but record the first error in a sticky per-thread slot
  * (ember_get_last_error) and print it to stderr; the process is not killed.
  * The entry points that are new (attention, the key/value cache, token log
- * probabilities and the fused training operators) return that status directly.
+ * probabilities, 8-bit matrices, gated layers and the fused training operators) return that status directly.
  * Argument errors never launch a kernel.
  */
 #ifndef EMBER_AMD_H
@@ -454,6 +454,85 @@ int token_logprobs_bwd_ex(const float *logits, int64_t row_stride, const int32_t
                           const float *lse_rest, const float *entropy, const float *d_logp,
                           const float *d_entropy, float *d_logits, int64_t out_stride, int64_t rows,
                           int64_t classes);
+
+/* ---- RMS norm, 8-bit matrices and gated layers (new; no reference counterpart) ----
+ *
+ * RMS norm over the last dimension d (d % 4 == 0, d <= 16384; at most 2^31 - 1
+ * rows; pointers 16-byte aligned, rstd 4), the residual's addition before it:
+ *   s = x + residual (x alone where residual is NULL), stored to sum where that
+ *   is not NULL;  rstd = 1/sqrt(sum(s^2)/d + eps), kept for the backward where
+ *   rstd is not NULL;  y = s*rstd*gamma.
+ * The mean and y are formed in double precision and rounded once.  sum and y may
+ * each be x or residual, not both the same.  eps is finite and >= 0. */
+int rmsnorm_fwd(const float *x, const float *residual, const float *gamma, float *sum, float *y, float *rstd,
+                int64_t rows, int64_t d, float eps);
+/* Its gradient, from the forward's sums s and rstd: with xhat = s*rstd and g =
+ * dy*gamma, dx = rstd*(g - xhat*mean(g*xhat)) (plus dres where that is not NULL:
+ * the gradient that reaches s past the norm; dx may be dres), the gradient of x
+ * and of residual alike, and dgamma = sum_rows(dy*xhat), added in a fixed order.
+ * dx overlaps no other input, dgamma nothing.  Uses library scratch. */
+int rmsnorm_bwd(const float *s, const float *gamma, const float *rstd, const float *dy, const float *dres,
+                float *dx, float *dgamma, int64_t rows, int64_t d);
+
+/* A matrix (rows, cols) in 8 bits.  A row is cut into groups of 128 neighbours,
+ * the last one shorter; a group is held as E4M3 codes (OCP's format without
+ * infinities: 4 bits of exponent, 3 of fraction, largest 448) that share one scale
+ * 2^e, stored as the byte e + 127.  e is the smallest number with amax <= 448 *
+ * 2^e, but at least -119, so that nothing is cut; each element is rounded to the
+ * nearest code times 2^e, ties to the even code.  A group of zeros has the scale
+ * byte 127; one that holds a NaN or a size from 2^127 on has the byte 255 and
+ * reads back as NaN.  Matrices that were filled otherwise may hold any codes
+ * (127 and 255 are NaN) and the bytes 8 to 246 and 255; others' results are not
+ * specified.
+ *
+ * codes is (rows, ceil(cols/128)*128) bytes, zero behind a row's end, and scales
+ * (rows, ceil(cols/512)*4) bytes, 127 behind a row's last group: device memory of
+ * the caller's, 16-byte aligned.  The entry points that write a matrix write these
+ * too, and those that read one count on them.  At most 2^31 - 1 rows; cols from 1
+ * to 2^30.  The struct itself is host memory, read during the call only. */
+typedef struct ember_rows8 {
+    void *codes, *scales;
+    int64_t rows, cols;
+} ember_rows8;
+
+/* Rounds x: element (r, c) is x[r*ld + c], or with trans (a Linear layer's
+ * weight, stored in x out) x[c*ld + r]; ld at least a stored row's length, at most
+ * 2^40. */
+int rows8_write(const ember_rows8 *to, const float *x, int64_t ld, int trans);
+/* The values held, to out[r*ld + c]. */
+int rows8_read(const ember_rows8 *from, float *out, int64_t ld);
+/* rmsnorm_fwd with y rounded as rows8_write rounds it: rows and d are y's, and
+ * what y reads back is the same as if rmsnorm_fwd's y had been written. */
+int rmsnorm_fwd8(const float *x, const float *residual, const float *gamma, float *sum, const ember_rows8 *y,
+                 float eps);
+
+/* out(n x m) = act(a w^T + bias) + residual for a (n x k) and w (m x k, a Linear
+ * layer's weight written with trans), both in 8 bits; bias (m) and residual (n x
+ * m) may be NULL, act as in linear_fwd.  Codes and scales enter exactly, products
+ * are exact and added in fp32.  A NaN reaches every element that it is a term of.
+ * out may be residual. */
+int linear8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, const float *residual, float *out,
+                int act);
+
+/* A gated layer, h(n x hidden) = act(x wg + bg) * (x wu + bu): x (n x d), w =
+ * [wg | wu] (d x 2 hidden), bias = [bg | bu] or NULL, act 1 = Ember's GELU, 2 =
+ * SiLU, g / (1 + exp(-g)).  pre (n x 2 hidden), where not NULL, gets both sums,
+ * [x wg + bg | x wu + bu], for the backward.  hidden and d from 1, hidden below
+ * 2^30.  Uses library scratch. */
+int gated_fwd(const float *x, const float *w, const float *bias, float *h, float *pre, int n, int hidden, int d,
+              int act);
+/* The gradient with respect to pre of what follows a gated layer, y = h w_down:
+ * with dh = dy w_down^T for dy (n x d) and w_down (hidden x d),
+ *   dpre = [dh * up * act'(gate) | dh * act(gate)],  pre = [gate | up].
+ * The rest of the layer's backward is products with it: dx = dpre w^T, dw = x^T
+ * dpre, dw_down = h^T dy (gemm_ex) and the bias' gradient col_sum(dpre).  dpre
+ * overlaps no input.  Uses library scratch. */
+int gated_bwd(const float *dy, const float *w_down, const float *pre, float *dpre, int n, int hidden, int d,
+              int act);
+/* A gated layer in 8 bits: a (n x k), w (2 hidden x k: wg's rows, then wu's), both
+ * sums and h in fp32, h (n x hidden) then rounded as rows8_write rounds.  h
+ * overlaps neither a nor w.  Uses library scratch. */
+int gated8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, const ember_rows8 *h, int act);
 
 #undef EMBER_BINARY_OP
 #undef EMBER_SCALAR_OP

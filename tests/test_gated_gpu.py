@@ -1,0 +1,164 @@
+"""Gated layers in fp32 (gated_fwd, gated_bwd) against float64, and the whole
+backward of one against differences."""
+
+import numpy as np
+import pytest
+
+import gpu_helpers as G
+from ember_amd import capi
+from ember_amd.capi import DeviceArray
+from feedforward_helpers import ACT, U, arr, ff, gate_error
+from serving_helpers import ptr
+from tolerance import gemm_error_bound
+
+pytestmark = pytest.mark.gpu
+
+# (n, hidden, d): one row, odd sizes, whole tiles of each size, k that is cut among workgroups.
+SIZES = [(1, 1, 1), (1, 64, 64), (3, 5, 7), (17, 33, 100), (64, 64, 32), (65, 129, 31), (100, 680, 256), (128, 128, 128), (200, 685, 257),
+         (256, 256, 64), (300, 1000, 513), (16, 512, 4096), (1024, 512, 512), (1025, 770, 300)]
+
+
+def forward(x, w, bias, act, want_pre=True, log=None):
+    n, d = x.shape
+    hidden = w.shape[1] // 2
+    G.say(f"gated_fwd n={n} hidden={hidden} d={d} bias={bias is not None} act={act}")
+    dx, dw, b = arr(x), arr(w), arr(bias)
+    h = DeviceArray.from_numpy(np.full((n, hidden), G.SENTINEL))
+    pre = DeviceArray.from_numpy(np.full((n, 2 * hidden), G.SENTINEL)) if want_pre else None
+    capi.launch_log_reset()
+    rc = capi.lib().gated_fwd(dx.ptr, dw.ptr, ptr(b), h.ptr, ptr(pre), n, hidden, d, ACT[act])
+    if log is not None:
+        log.extend(capi.launch_log())
+    capi.check(rc, "gated_fwd")
+    return h.numpy(), None if pre is None else pre.numpy()
+
+
+def backward(dy, w_down, pre, act):
+    n, d = dy.shape
+    hidden = w_down.shape[0]
+    G.say(f"gated_bwd n={n} hidden={hidden} d={d} act={act}")
+    dev = [arr(a) for a in (dy, w_down, pre)]
+    dpre = DeviceArray.from_numpy(np.full((n, 2 * hidden), G.SENTINEL))
+    capi.check(capi.lib().gated_bwd(*(a.ptr for a in dev), dpre.ptr, n, hidden, d, ACT[act]), "gated_bwd")
+    return dpre.numpy()
+
+
+def inputs(n, hidden, d, seed=0):
+    rng = np.random.default_rng(n * 7 + hidden * 3 + d + seed)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    return f(n, d), f(d, 2 * hidden) / np.float32(np.sqrt(d)), f(2 * hidden), f(hidden, d) / np.float32(np.sqrt(hidden)), f(n, d)
+
+
+@pytest.mark.parametrize("act", list(ACT))
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("n,hidden,d", SIZES)
+def test_forward(n, hidden, d, bias, act):
+    x, w, b, _, _ = inputs(n, hidden, d)
+    b = b if bias else None
+    h, pre = forward(x, w, b, act)
+    exact = x.astype(np.float64) @ w + (0 if b is None else b)
+    off = gemm_error_bound(x, w) + 2 * U * np.abs(exact)
+    assert (np.abs(pre - exact) <= off).all()
+    assert np.linalg.norm(pre - exact) <= 32 * U * np.linalg.norm(exact) + 32 * U * np.linalg.norm(np.abs(x).astype(np.float64) @ np.abs(w)) / np.sqrt(d)
+    # h is formed of the sums that are kept.
+    kept = ff.gate(act, pre.astype(np.float64))
+    assert (np.abs(h - kept) <= gate_error(act, pre.astype(np.float64), 0 * off) + 2.0 ** -148).all()
+    assert (np.abs(h - ff.gate(act, exact)) <= gate_error(act, exact, off) + 2.0 ** -148).all()
+    np.testing.assert_array_equal(forward(x, w, b, act, want_pre=False)[0], h)
+
+
+def slope_error(act, gate):
+    """How far an activation's slope may be off: a few half steps of its terms, of
+    which x times the slope of tanh or the logistic function is at most |x|."""
+    return 8 * U * (1 + np.abs(gate))
+
+
+@pytest.mark.parametrize("act", list(ACT))
+@pytest.mark.parametrize("n,hidden,d", SIZES)
+def test_backward(n, hidden, d, act):
+    x, w, b, w_down, dy = inputs(n, hidden, d, 1)
+    pre = (x.astype(np.float64) @ w + b).astype(np.float32)
+    got = backward(dy, w_down, pre, act)
+    wide = pre.astype(np.float64)
+    dh = dy.astype(np.float64) @ w_down.T.astype(np.float64)
+    exact = ff.gate_bwd(act, dh, wide)
+    off = gemm_error_bound(dy, np.ascontiguousarray(w_down.T))
+    value, slope = ff.activate(act, wide[:, :hidden])
+    up = wide[:, hidden:]
+    tol = np.concatenate(((np.abs(slope) + slope_error(act, wide[:, :hidden])) * np.abs(up) * off + slope_error(act, wide[:, :hidden]) * np.abs(dh * up),
+                          (np.abs(value) + 8 * U * np.abs(wide[:, :hidden])) * off + 8 * U * np.abs(wide[:, :hidden] * dh)), 1)
+    assert (np.abs(got - exact) <= tol + 4 * U * np.abs(exact) + 2.0 ** -148).all()
+    np.testing.assert_array_equal(backward(dy, w_down, pre, act), got)
+
+
+@pytest.mark.parametrize("act", list(ACT))
+def test_far_gates(act):
+    """Gates far from zero on both sides, zeros, infinities and NaN."""
+    gate = np.float32([0, -0.0, 30, -30, 90, -90, 200, -200, 1e30, -1e30, np.inf, np.nan, 1e-30, 3e38])
+    hidden = gate.size
+    x, w = np.ones((1, 1), np.float32), np.concatenate((gate, np.full(hidden, 2, np.float32)))[None]
+    with np.errstate(all="ignore"):
+        h, pre = forward(x, w, None, act)
+        want = ff.gate(act, w.astype(np.float64)).astype(np.float32)
+        np.testing.assert_array_equal(np.isnan(h[0]), np.isnan(want[0]))
+        fine = np.isfinite(want[0])
+        assert (h[0][~fine & ~np.isnan(want[0])] == np.inf).all()
+        assert (np.abs(h[0] - want[0])[fine] <= 32 * U * np.abs(gate[fine])).all()
+        finite = np.isfinite(gate)
+        dpre = backward(np.ones((1, 1), np.float32), np.ones((hidden, 1), np.float32), np.where(np.isfinite(w), w, 0), act)[0]
+        want = ff.gate_bwd(act, np.ones((1, hidden)), np.where(np.isfinite(w), w, 0).astype(np.float64))[0]
+        for half in (dpre[:hidden] - want[:hidden], dpre[hidden:] - want[hidden:]):
+            assert (np.abs(half[finite]) <= 32 * U * (1 + np.abs(gate[finite]))).all()
+
+
+def test_infinite_and_huge_operands():
+    """What the split products cannot carry is formed again in fp32."""
+    x, w, b, _, _ = inputs(70, 90, 40)
+    x[3, 5], x[9, 0], w[7, 100] = np.inf, 1e36, 1e30
+    h, pre = forward(x, w, b, "silu")
+    with np.errstate(all="ignore"):
+        exact = (x.astype(np.float64) @ w + b)
+        bad = ~np.isfinite(exact) | (np.abs(exact) > 3e38)
+        rest = ~bad
+        assert (~np.isfinite(pre[bad])).all()
+        wide = np.where(np.isfinite(x), x, 0)
+        tol = gemm_error_bound(wide, w) + 2 * U * np.abs(np.where(rest, exact, 0))
+        assert (np.abs(pre - exact)[rest] <= tol[rest]).all()
+    other = np.ones(70, bool)
+    other[[3, 9]] = False
+    assert np.isfinite(h[other][:, np.arange(90) != 10]).all()
+
+
+def test_whole_backward_against_differences():
+    """dx, dw, dbias and dw_down of sum(y * dy) for y = h w_down, formed of gated_bwd,
+    gemm_ex and col_sum, against central differences of the float64 forward."""
+    n, hidden, d, act = 6, 9, 5, "silu"
+    x, w, b, w_down, dy = inputs(n, hidden, d, 3)
+    h, pre = forward(x, w, b, act)
+    L = capi.lib()
+    dev = {k: arr(v) for k, v in dict(x=x, w=w, w_down=w_down, dy=dy, pre=pre, h=h).items()}
+    new = {k: DeviceArray(s) for k, s in dict(dpre=(n, 2 * hidden), dx=(n, d), dw=(d, 2 * hidden), dw_down=(hidden, d), db=(2 * hidden,)).items()}
+    p = lambda k: (dev.get(k) or new[k]).ptr  # noqa: E731
+    capi.check(L.gated_bwd(p("dy"), p("w_down"), p("pre"), p("dpre"), n, hidden, d, ACT[act]), "gated_bwd")
+    capi.check(L.gemm_ex(p("dpre"), p("w"), p("dx"), 1, n, d, 2 * hidden, 0, 1, None, None, None, 0), "gemm_ex")
+    capi.check(L.gemm_ex(p("x"), p("dpre"), p("dw"), 1, d, 2 * hidden, n, 1, 0, None, None, None, 0), "gemm_ex")
+    capi.check(L.gemm_ex(p("h"), p("dy"), p("dw_down"), 1, hidden, d, n, 1, 0, None, None, None, 0), "gemm_ex")
+    capi.check(L.col_sum(p("dpre"), p("db"), n, 2 * hidden), "col_sum")
+    at = dict(x=x, w=w, b=b, w_down=w_down)
+    at = {k: v.astype(np.float64) for k, v in at.items()}
+    loss = lambda v: (ff.gate(act, v["x"] @ v["w"] + v["b"]) @ v["w_down"] * dy).sum()  # noqa: E731
+    for name, grad in (("x", "dx"), ("w", "dw"), ("b", "db"), ("w_down", "dw_down")):
+        got = new[grad].numpy()
+        for i in np.ndindex(got.shape):
+            up, down = dict(at), dict(at)
+            up[name], down[name] = at[name].copy(), at[name].copy()
+            up[name][i] += 1e-5
+            down[name][i] -= 1e-5
+            want = (loss(up) - loss(down)) / 2e-5
+            assert abs(got[i] - want) <= 2e-5 * (1 + abs(want)), (name, i)
+
+
+def test_no_rows():
+    p = DeviceArray((64,)).ptr
+    capi.check(capi.lib().gated_fwd(p, p, None, p, None, 0, 4, 4, 1), "gated_fwd")
+    capi.check(capi.lib().gated_bwd(p, p, p, p, 0, 4, 4, 1), "gated_bwd")
