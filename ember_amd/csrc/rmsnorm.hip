@@ -201,17 +201,28 @@ int norm_args(const void *const *ptrs, int n, const void *const *optional, int m
 }
 
 template <bool TO8>
-int norm_launch(const NormArgs &a, const char *who)
+int norm_launch(const NormArgs &all, const char *who)
 {
-    if (!(a.eps >= 0.0f) || isinf(a.eps)) return record_error(EMBER_ERR_INVALID_ARGUMENT, who);
-    if (a.rows == 0) return EMBER_OK;
-    const unsigned rows = (unsigned)a.rows;
-    if (a.d <= 1024)
-        hipLaunchKernelGGL((rms_fwd_kernel<1, TO8>), dim3(rows / 4 + (rows % 4 != 0)), dim3(256), 0, 0, a);
-    else if (a.d <= 4096)
-        hipLaunchKernelGGL((rms_fwd_kernel<4, TO8>), dim3(rows), dim3(256), 0, 0, a);
-    else
-        hipLaunchKernelGGL((rms_fwd_kernel<16, TO8>), dim3(rows), dim3(1024), 0, 0, a);
+    if (!(all.eps >= 0.0f) || isinf(all.eps)) return record_error(EMBER_ERR_INVALID_ARGUMENT, who);
+    // A grid holds fewer than 2^32 threads.
+    constexpr int64_t kRowsPerLaunch = 1 << 21;
+    for (int64_t row = 0; row < all.rows; row += kRowsPerLaunch) {
+        NormArgs a = all;
+        a.rows = std::min(all.rows - row, kRowsPerLaunch);
+        a.x += row * a.d;
+        if (a.residual) a.residual += row * a.d;
+        if (a.sum) a.sum += row * a.d;
+        if (a.y) a.y += row * a.d;
+        if (a.rstd) a.rstd += row;
+        if (TO8) a.y8.codes += row * a.y8.pitch(), a.y8.scales += row * a.y8.scale_pitch;
+        const unsigned rows = (unsigned)a.rows;
+        if (a.d <= 1024)
+            hipLaunchKernelGGL((rms_fwd_kernel<1, TO8>), dim3((rows + 3) / 4), dim3(256), 0, 0, a);
+        else if (a.d <= 4096)
+            hipLaunchKernelGGL((rms_fwd_kernel<4, TO8>), dim3(rows), dim3(256), 0, 0, a);
+        else
+            hipLaunchKernelGGL((rms_fwd_kernel<16, TO8>), dim3(rows), dim3(1024), 0, 0, a);
+    }
     return launch_ok(who) ? EMBER_OK : EMBER_ERR_DEVICE;
 }
 

@@ -72,14 +72,19 @@ __device__ __forceinline__ float scale8(unsigned byte)
 {
     return __builtin_bit_cast(float, byte << 23);
 }
+// Two neighbouring codes, pair i of lo (0, 1) and hi (2, 3), as packed bf16.
+__device__ __forceinline__ unsigned bf16_pair8(unsigned lo, unsigned hi, int i, float scale)
+{
+    const unsigned w = i < 2 ? lo : hi;
+    return i & 1 ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))
+                 : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+}
 // Eight codes as one bf16 operand of a matrix instruction.
 __device__ __forceinline__ u32x4 bf16_of8(unsigned lo, unsigned hi, float scale)
 {
     u32x4 v;
-    v[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
-    v[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
-    v[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
-    v[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = bf16_pair8(lo, hi, i, scale);
     return v;
 }
 

@@ -15,7 +15,7 @@ namespace ember {
 
 int rows8_view(const ember_rows8 *m, Rows8 *out, const char *what)
 {
-    if (!m || m->rows < 0 || m->rows > 0x7fffffff || m->cols < 1 || m->cols > (1 << 30) || !m->codes || !m->scales ||
+    if (!m || m->rows < 0 || m->rows > (1 << 26) || m->cols < 1 || m->cols > (1 << 23) || !m->codes || !m->scales ||
         (((uintptr_t)m->codes | (uintptr_t)m->scales) & 15))
         return record_error(EMBER_ERR_INVALID_ARGUMENT, what);
     const int groups = (int)((m->cols + kGroup8 - 1) / kGroup8);

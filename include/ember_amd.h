@@ -488,8 +488,8 @@ int rmsnorm_bwd(const float *s, const float *gamma, const float *rstd, const flo
  * codes is (rows, ceil(cols/128)*128) bytes, zero behind a row's end, and scales
  * (rows, ceil(cols/512)*4) bytes, 127 behind a row's last group: device memory of
  * the caller's, 16-byte aligned.  The entry points that write a matrix write these
- * too, and those that read one count on them.  At most 2^31 - 1 rows; cols from 1
- * to 2^30.  The struct itself is host memory, read during the call only. */
+ * too, and those that read one count on them.  At most 2^26 rows; cols from 1 to
+ * 2^23.  The struct itself is host memory, read during the call only. */
 typedef struct ember_rows8 {
     void *codes, *scales;
     int64_t rows, cols;

@@ -21,8 +21,8 @@ def rows8(codes=P, scales=Q, rows=3, cols=200):
     return capi.Rows8View(codes, scales, rows, cols)
 
 
-BAD_MATRICES = [dict(codes=None), dict(scales=None), dict(codes=P + 8), dict(scales=Q + 4), dict(rows=-1), dict(rows=2 ** 31), dict(cols=0),
-                dict(cols=-5), dict(cols=2 ** 30 + 1)]
+BAD_MATRICES = [dict(codes=None), dict(scales=None), dict(codes=P + 8), dict(scales=Q + 4), dict(rows=-1), dict(rows=2 ** 26 + 1), dict(cols=0),
+                dict(cols=-5), dict(cols=2 ** 23 + 1)]
 
 
 def write(m=None, x=R, ld=200, trans=0):
