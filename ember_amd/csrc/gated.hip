@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void gate_fwd_kernel(const float *__restrict__
 {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t at = i + i / hidden * hidden;
-        h[i] = gated(act, pre[at], pre[at + hidden]);
+        h[i] = gated(steepness(act), pre[at], pre[at + hidden]);
     }
 }
 
@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void gate_bwd_kernel(const float *__restrict__
 {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t at = i + i / hidden * hidden;
-        const Activated a = activate(act, pre[at]);
+        const Activated a = activate(steepness(act), pre[at]);
         const float up = pre[at + hidden], g = dh[i];
         dpre[at] = g * up * a.slope;
         dpre[at + hidden] = g * a.value;

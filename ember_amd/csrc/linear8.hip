@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * W) void linear8_few(Linear8Args g)
             const bool in = col + i < g.m;
             float o = v[0][i] + (g.bias && in ? g.bias[col + i] : 0.0f);
             if (GATED)
-                o = gated(g.act, o, v[NB - 1][i] + (g.bias && in ? g.bias[g.m + col + i] : 0.0f));
+                o = gated(steepness(g.act), o, v[NB - 1][i] + (g.bias && in ? g.bias[g.m + col + i] : 0.0f));
             else if (g.act == kActGelu)
                 o = gelu08(o);
             v[0][i] = o + more[i];
@@ -234,7 +234,7 @@ __device__ __forceinline__ void meet()
 //     branches: past the last stage requests read nothing, and what is read of them
 //     is not used.
 template <int TM, int TN, int WR, int WC, int NBUF, bool GATED>
-__global__ __launch_bounds__(64 * WR * WC, TM == 128 && NBUF == 2 ? 2 : 1) void linear8_tiles(Linear8Args g)
+__global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && NBUF == 2 ? 2 : 1) void linear8_tiles(Linear8Args g)
 {
     constexpr int NW = WR * WC, RB = TM / WR / 32, CB = TN / WC / 32, CBH = CB / 2;
     constexpr int CA = TM / 8 / NW, CW = TN / 8 / NW;  // copies of 8 rows to a wave
@@ -403,8 +403,8 @@ __global__ __launch_bounds__(64 * WR * WC, TM == 128 && NBUF == 2 ? 2 : 1) void 
     // one over registers would be unrolled to many times the main loop's code.  32
     // columns are swapped in every other four rows, so that the two halves of a
     // wave write to different banks.
-    static_assert(TM * 8 * 16 >= 32 * TN * 4 && WR <= 4, "32 rows fit a buffer");
-    float *const rows = (float *)(wr == 0 ? A0 : wr == 1 ? A1 : wr == 2 ? B0 : B1);
+    static_assert(WR <= 2 || (WR <= 4 && TM >= TN), "32 rows fit a buffer");
+    float *const rows = (float *)(wr == 0 ? B0 : wr == 1 || WR <= 2 ? B1 : wr == 2 ? A0 : A1);
     auto at = [](int r, int col) { return r * TN + (col ^ (r & 4) << 3); };
     // at(acc_row(i, half), l32 + a block's column) of even and of odd blocks.
     float *const put[2] = {rows + 4 * half * TN + l32 + 32 * half, rows + 4 * half * TN + l32 - 32 * half};
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(64 * WR * WC, TM == 128 && NBUF == 2 ? 2 : 1) void 
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) put[cb & 1][acc_row(i, 0) * TN + brow(cb) - l32] = acc[rb][cb][i];
+            for (int i = 0; i < 16; ++i) put[(brow(cb) - l32) / 32 & 1][acc_row(i, 0) * TN + brow(cb) - l32] = acc[rb][cb][i];
         __syncthreads();
         const int row1 = row0 + 32 * (RB * wr + rb);
         if constexpr (!GATED) {
@@ -474,17 +474,28 @@ __global__ __launch_bounds__(64 * WR * WC, TM == 128 && NBUF == 2 ? 2 : 1) void 
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (col + i < g.m) bg[i] = g.bias[col + i], bu[i] = g.bias[g.m + col + i];
-            for (int r = t / 32; r < 32; r += 2 * WC) {
-                const f32x4 x = *(const f32x4 *)&rows[at(r, 4 * q)] + bg, u = *(const f32x4 *)&rows[at(r, TN / 2 + 4 * q)] + bu;
-                f32x4 v;
+            const float c = steepness(g.act);
+            constexpr int STEP = 2 * WC, N = 4;  // rows at a time, and times taken together
+            for (int r0 = t / 32; r0 < 32; r0 += N * STEP) {
+                f32x4 x[N], u[N];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = col + i < g.m ? gated(g.act, x[i], u[i]) : 0.0f;
-                const unsigned byte = scale_byte8(max_of_32(max(max(size_bits8(v[0]), size_bits8(v[1])), max(size_bits8(v[2]), size_bits8(v[3])))));
-                if (row1 + r >= g.n) continue;
-                *(unsigned *)(g.h.codes + (row1 + r) * g.h.pitch() + col) = byte == 255 ? 0 : codes8(v[0], v[1], v[2], v[3], inverse_scale8(byte));
-                uint8_t *const to = g.h.scales + (int64_t)(row1 + r) * g.h.scale_pitch;
-                if (q == 0) to[group] = (uint8_t)byte;
-                if (group == g.h.groups - 1 && q > 0 && group + q < g.h.scale_pitch) to[group + q] = 127;
+                for (int k = 0; k < N; ++k) {
+                    x[k] = *(const f32x4 *)&rows[at(r0 + k * STEP, 4 * q)] + bg;
+                    u[k] = *(const f32x4 *)&rows[at(r0 + k * STEP, TN / 2 + 4 * q)] + bu;
+                }
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int64_t row = row1 + r0 + k * STEP;
+                    f32x4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = col + i < g.m ? gated(c, x[k][i], u[k][i]) : 0.0f;
+                    const unsigned byte = scale_byte8(max_of_32(max(max(size_bits8(v[0]), size_bits8(v[1])), max(size_bits8(v[2]), size_bits8(v[3])))));
+                    if (row >= g.n) continue;
+                    *(unsigned *)(g.h.codes + row * g.h.pitch() + col) = byte == 255 ? 0 : codes8(v[0], v[1], v[2], v[3], inverse_scale8(byte));
+                    uint8_t *const to = g.h.scales + row * g.h.scale_pitch;
+                    if (q == 0) to[group] = (uint8_t)byte;
+                    if (group == g.h.groups - 1 && q > 0 && group + q < g.h.scale_pitch) to[group + q] = 127;
+                }
             }
         }
     }
@@ -522,7 +533,7 @@ __global__ __launch_bounds__(256) void gated8_reduce(Linear8Args g, int splits, 
                 float a = p[0], b = p[hidden];
                 for (int z = 1; z < splits; ++z) a += p[z * total], b += p[z * total + hidden];
                 if (g.bias) a += g.bias[col + j], b += g.bias[hidden + col + j];
-                v[j] = gated(g.act, a, b);
+                v[j] = gated(steepness(g.act), a, b);
             }
             top = max(top, size_bits8(v[j]));
         }
@@ -604,14 +615,15 @@ bool launch_few(const Linear8Args &g, const char *who)
     return launch_ok(who);
 }
 
-// What a call costs with each kernel, in us, fitted to measured times of 24 sizes
-// from 65 x 4096 x 4096 to 8192 x 8192 x 8192 with every kernel and 1 to 16 splits
-// of k: the choice by it is within 5 % of the fastest for each, 0.7 % on average.
+// What a call costs with each kernel, in us, fitted to measured times of 24 products
+// (65 x 4096 x 4096 to 8192 x 8192 x 8192) and 18 gated layers with every kernel and
+// 1 to 16 splits of k: the choice by it is within 5 % of the fastest for nearly all.
 // Few rows: a launch, and what a CU's workgroups read (13 bytes a cycle).  Tiles: a
-// launch with the ends of a tile, a stage's time with the chip nearly empty (one
-// workgroup's latency) and full, the sums' way to memory, and for splits the launch
-// and bytes that add them.
-enum Kernel { kFew, kSmallTiles, kLargeTiles };
+// launch, and for each round over the CUs the ends of a tile and its stages, whose
+// time is one workgroup's latency with the chip nearly empty and throughput with it
+// full; the sums' way to memory; and for sums that are added or gated in a launch of
+// their own, that and its bytes.
+enum Kernel { kFew, kSmallTiles, kMidTiles, kLargeTiles };
 struct Choice {
     Kernel kernel;
     int splits, chunk;
@@ -629,9 +641,14 @@ Choice choose(int64_t n, int64_t m, int groups, bool gated)
     const auto consider = [&](Kernel kernel, int splits, int chunk, double us) {
         if (us < least) least = us, best = {kernel, splits, chunk};
     };
-    {
-        const double tiles = over(n, 256) * over(m, gated ? 128 : 256), full = std::min(1.0, tiles / 256);
-        consider(kLargeTiles, 1, groups, 9 + over((int64_t)tiles, 256) * groups * (2.25 + 0.6 * full) + (gated ? 0 : 0.5 * moved));
+    const auto rounds = [&](double tiles, double ends, double empty, double full) {
+        return 3 + over((int64_t)tiles, 256) * (ends + groups * (empty + (full - empty) * std::min(1.0, tiles / 256)));
+    };
+    if (gated) {
+        consider(kLargeTiles, 1, groups, rounds(over(n, 256) * over(m, 128), 9, 2.25, 3.05));
+        consider(kMidTiles, 1, groups, rounds(over(n, 128) * over(m, 128), 8, 1.35, 1.7));
+    } else {
+        consider(kLargeTiles, 1, groups, rounds(over(n, 256) * over(m, 256), 6, 2.25, 2.95) + 0.5 * moved);
     }
     for (int want = 1; want <= kMostSplits; want *= 2) {
         const int chunk = want == 1 ? groups : ((groups + want - 1) / want + 3) / 4 * 4, splits = (groups + chunk - 1) / chunk;
@@ -697,8 +714,9 @@ int gated8_launch(const Linear8Args &all, const char *who)
         Linear8Args g = rows_from(all, row);
         const Choice c = choose(g.n, g.m, g.w.groups, true);
         g.chunk = c.chunk;
-        if (c.kernel == kLargeTiles) {
-            if (!launch_tiles<256, 256, 4, 2, 2, true>(g, 1, who)) return EMBER_ERR_DEVICE;
+        if (c.kernel == kLargeTiles || c.kernel == kMidTiles) {
+            if (!(c.kernel == kMidTiles ? launch_tiles<128, 256, 2, 4, 2, true>(g, 1, who) : launch_tiles<256, 256, 4, 2, 2, true>(g, 1, who)))
+                return EMBER_ERR_DEVICE;
         } else if (c.kernel == kFew) {
             g.out = (float *)scratch(kScratchLinear8, (size_t)g.n * g.m * sizeof(float));
             if (!g.out) return EMBER_ERR_OUT_OF_MEMORY;
