@@ -35,9 +35,10 @@ __device__ __forceinline__ float sigmoid(float x)
 // The activations of gated layers: x * sigmoid(c x), with c = 1 SiLU and with c =
 // 1.6 Ember's GELU, as (1 + tanh z) / 2 = sigmoid(2 z).  An x of -infinity gives NaN
 // and far ones below 0 -0, as the formulas do.
+constexpr float kSteepGelu = 1.6f, kSteepSilu = 1.0f;
 __device__ __forceinline__ float steepness(int act)
 {
-    return act == kActGelu ? 1.6f : 1.0f;
+    return act == kActGelu ? kSteepGelu : kSteepSilu;
 }
 // Value and slope.
 struct Activated {
@@ -48,10 +49,18 @@ __device__ __forceinline__ Activated activate(float c, float x)
     const float s = sigmoid(c * x), v = x * s;
     return {v, s + c * (v * (1.0f - s))};  // c x alone may pass fp32's range
 }
-// A gated layer's output.
+// A gated layer's output, and its gradient with respect to both sums.
 __device__ __forceinline__ float gated(float c, float gate, float up)
 {
     return gate * sigmoid(c * gate) * up;
+}
+struct GateGrad {
+    float gate, up;
+};
+__device__ __forceinline__ GateGrad gate_grad(float c, float gate, float up, float dh)
+{
+    const Activated a = activate(c, gate);
+    return {dh * up * a.slope, dh * a.value};
 }
 
 }  // namespace ember

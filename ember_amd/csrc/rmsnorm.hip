@@ -161,29 +161,37 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void rms_bwd_kernel(const flo
         }
 }
 
-// dgamma = the sum of n rows of `part`: a workgroup owns 16 quads of columns, a
-// sixteenth of it every sixteenth row, and adds the sixteenths in order.
-__global__ __launch_bounds__(256) void rms_param_grad_kernel(const float *__restrict__ part, float *__restrict__ dgamma, int n, int d)
+// dgamma = the sum of n rows of `part`: a workgroup owns 16 quads of columns, and
+// its 64 groups of threads every 64th row each; the groups' sums are added in order.
+constexpr int kGroups = 64;
+__global__ __launch_bounds__(16 * kGroups) void rms_param_grad_kernel(const float *__restrict__ part, float *__restrict__ dgamma, int n, int d)
 {
-    __shared__ f32x4 red[16][16];
+    __shared__ f32x4 red[kGroups][16];
     const int q = threadIdx.x % 16, g = threadIdx.x / 16, col = 4 * (blockIdx.x * 16 + q);
     f32x4 s = {0, 0, 0, 0};
     if (col < d) {
         int b = g;
-        for (; b + 7 * 16 < n; b += 8 * 16) {  // eight loads in flight
+        for (; b + 7 * kGroups < n; b += 8 * kGroups) {  // eight loads in flight
             f32x4 v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = *(const f32x4 *)(part + (int64_t)(b + 16 * u) * d + col);
+            for (int u = 0; u < 8; ++u) v[u] = *(const f32x4 *)(part + (int64_t)(b + kGroups * u) * d + col);
 #pragma unroll
             for (int u = 0; u < 8; ++u) s += v[u];
         }
-        for (; b < n; b += 16) s += *(const f32x4 *)(part + (int64_t)b * d + col);
+        for (; b < n; b += kGroups) s += *(const f32x4 *)(part + (int64_t)b * d + col);
     }
     red[g][q] = s;
     __syncthreads();
+    // Eight groups' sums by eight groups of threads, then those by the first.
+    if (g < 8) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += red[g + 8 * i][q];
+        red[g][q] = s;
+    }
+    __syncthreads();
     if (g == 0 && col < d) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][q];
+        for (int i = 1; i < 8; ++i) s += red[i][q];
         *(f32x4 *)(dgamma + col) = s;
     }
 }
@@ -262,11 +270,15 @@ extern "C" int rmsnorm_bwd(const float *s, const float *gamma, const float *rstd
     if (!rstd || ((uintptr_t)rstd & 3)) return record_error(EMBER_ERR_INVALID_ARGUMENT, "rmsnorm_bwd");
     const dim3 quads((unsigned)((d / 4 + 15) / 16));
     if (rows == 0) {  // a sum over no rows
-        hipLaunchKernelGGL(rms_param_grad_kernel, quads, dim3(256), 0, 0, (const float *)nullptr, dgamma, 0, (int)d);
+        hipLaunchKernelGGL(rms_param_grad_kernel, quads, dim3(16 * kGroups), 0, 0, (const float *)nullptr, dgamma, 0, (int)d);
         return launch_ok("rmsnorm_bwd") ? EMBER_OK : EMBER_ERR_DEVICE;
     }
-    // Runs of eight rows; from 2^18 rows on longer ones, so that part has at most 2^15.
-    const int64_t run = std::max<int64_t>(8, (rows + 32767) / 32768);
+    // A run of rows to a workgroup: as many workgroups as fill the chip (four to a CU;
+    // of sixteen waves one), and no more, for each writes a row of partial sums.
+    // (8192 x 1024 in runs of 8: 32 us, of 32: 35; 64 x 4096 in runs of 1: 6.6, of 8: 19;
+    // 1000 x 16384 in runs of 4: 64, of 1: 76.)
+    const int64_t most = d <= 4096 ? 1024 : 256, at_once = d <= 1024 ? 4 : 1;
+    const int64_t run = std::max<int64_t>(at_once, (rows + most - 1) / most + at_once - 1) / at_once * at_once;
     const int blocks = (int)((rows + run - 1) / run);
     float *part = (float *)scratch(kScratchRmsNorm, (size_t)blocks * d * sizeof(float));
     if (!part) return EMBER_ERR_OUT_OF_MEMORY;
@@ -277,6 +289,6 @@ extern "C" int rmsnorm_bwd(const float *s, const float *gamma, const float *rstd
     else
         hipLaunchKernelGGL(rms_bwd_kernel<16>, dim3(blocks), dim3(1024), 0, 0, s, gamma, rstd, dy, dres, dx, part, rows, (int)d, (int)run);
     if (!launch_ok("rmsnorm_bwd")) return EMBER_ERR_DEVICE;
-    hipLaunchKernelGGL(rms_param_grad_kernel, quads, dim3(256), 0, 0, part, dgamma, blocks, (int)d);
+    hipLaunchKernelGGL(rms_param_grad_kernel, quads, dim3(16 * kGroups), 0, 0, part, dgamma, blocks, (int)d);
     return launch_ok("rms_param_grad_kernel") ? EMBER_OK : EMBER_ERR_DEVICE;
 }

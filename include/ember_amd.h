@@ -518,7 +518,7 @@ int linear8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, c
  * [wg | wu] (d x 2 hidden), bias = [bg | bu] or NULL, act 1 = Ember's GELU, 2 =
  * SiLU, g / (1 + exp(-g)).  pre (n x 2 hidden), where not NULL, gets both sums,
  * [x wg + bg | x wu + bu], for the backward.  hidden and d from 1, hidden below
- * 2^30.  Uses library scratch. */
+ * 2^29.  Uses library scratch. */
 int gated_fwd(const float *x, const float *w, const float *bias, float *h, float *pre, int n, int hidden, int d,
               int act);
 /* The gradient with respect to pre of what follows a gated layer, y = h w_down:
