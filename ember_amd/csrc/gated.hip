@@ -59,7 +59,7 @@ void launch_shape(GemmArgs &g, int ksplit, int shape)
 // g's product as choose_gemm has it: gated by its own kernel, or in parts that
 // `reduce` adds and gates.
 template <bool TB, Gate GATE, class R>
-int gated_launch(GemmArgs &g, R reduce, const char *who)
+int gated_launch(GemmArgs &g, R reduce, const char *who, const char *joined)
 {
     const GemmChoice choice = choose_gemm(g.n, g.m, g.k, 1, num_cus());
     if (choice.ksplit > 1) {
@@ -71,7 +71,7 @@ int gated_launch(GemmArgs &g, R reduce, const char *who)
             if (!launch_ok(who)) return EMBER_ERR_DEVICE;
             const int64_t elements = (int64_t)g.n * g.hidden;
             hipLaunchKernelGGL(reduce, dim3((unsigned)std::min<int64_t>((elements + 255) / 256, 8 * num_cus())), dim3(256), 0, 0, g, choice.ksplit, elements);
-            return launch_ok(who) ? EMBER_OK : EMBER_ERR_DEVICE;
+            return launch_ok(joined) ? EMBER_OK : EMBER_ERR_DEVICE;
         }
     }
     launch_shape<TB, GATE>(g, 1, choice.shape);
@@ -113,7 +113,7 @@ extern "C" int gated_fwd(const float *x, const float *w, const float *bias, floa
     if (n == 0) return EMBER_OK;
     GemmArgs g = gated_product(x, w, n, 2 * hidden, d, 2 * hidden, hidden, act);
     g.c = h, g.pre = pre, g.bias = bias;
-    return gated_launch<false, kGateForward>(g, gate_fwd_reduce, "gated_fwd");
+    return gated_launch<false, kGateForward>(g, gate_fwd_reduce, "gated_fwd", "gate_fwd_reduce");
 }
 
 extern "C" int gated_bwd(const float *dy, const float *w_down, const float *pre, float *dpre, int n, int hidden, int d, int act)
@@ -124,5 +124,5 @@ extern "C" int gated_bwd(const float *dy, const float *w_down, const float *pre,
     if (n == 0) return EMBER_OK;
     GemmArgs g = gated_product(dy, w_down, n, hidden, d, d, hidden, act);
     g.sums = pre, g.dsums = dpre;
-    return gated_launch<true, kGateBackward>(g, gate_bwd_reduce, "gated_bwd");
+    return gated_launch<true, kGateBackward>(g, gate_bwd_reduce, "gated_bwd", "gate_bwd_reduce");
 }

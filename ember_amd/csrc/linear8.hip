@@ -545,19 +545,20 @@ __global__ __launch_bounds__(256) void gated8_reduce(Linear8Args g, int splits, 
 }
 
 template <int TM, int TN, int WR, int WC, int NBUF, bool GATED>
-bool launch_tiles(const Linear8Args &g, int splits, const char *who)
+bool launch_tiles(const Linear8Args &g, int splits, const char *kernel)
 {
     const int64_t tiles = (((int64_t)g.n + TM - 1) / TM) * (((int64_t)g.m + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN));
     hipLaunchKernelGGL((linear8_tiles<TM, TN, WR, WC, NBUF, GATED>), dim3((unsigned)tiles, splits), dim3(64 * WR * WC), 0, 0, g);
-    return launch_ok(who);
+    return launch_ok(kernel);
 }
 
 // 128 x 128 tiles: four buffers, which leave room for one workgroup on a CU, where
 // there are no more than CUs.
-bool launch_small(const Linear8Args &g, int splits, const char *who)
+bool launch_small(const Linear8Args &g, int splits)
 {
     const int64_t tiles = (((int64_t)g.n + 127) / 128) * (((int64_t)g.m + 127) / 128);
-    return tiles * splits <= 256 ? launch_tiles<128, 128, 2, 2, 4, false>(g, splits, who) : launch_tiles<128, 128, 2, 2, 2, false>(g, splits, who);
+    return tiles * splits <= 256 ? launch_tiles<128, 128, 2, 2, 4, false>(g, splits, "linear8_tiles128_ahead")
+                                 : launch_tiles<128, 128, 2, 2, 2, false>(g, splits, "linear8_tiles128");
 }
 
 // Rows of a few-rows workgroup, in sixteens.
@@ -604,7 +605,7 @@ void launch_few_rows(const Linear8Args &g)
 }
 
 template <bool GATED>
-bool launch_few(const Linear8Args &g, const char *who)
+bool launch_few(const Linear8Args &g)
 {
     switch (few_rows(g.n)) {
         case 1: launch_few_rows<1, GATED>(g); break;
@@ -612,7 +613,7 @@ bool launch_few(const Linear8Args &g, const char *who)
         case 3: launch_few_rows<3, GATED>(g); break;
         default: launch_few_rows<4, GATED>(g);
     }
-    return launch_ok(who);
+    return launch_ok(GATED ? "gated8_few" : "linear8_few");
 }
 
 // What a call costs with each kernel, in us, fitted to measured times of 24 products
@@ -684,7 +685,7 @@ Linear8Args rows_from(const Linear8Args &g, int64_t row)
     return p;
 }
 
-int linear8_launch(const Linear8Args &all, const char *who)
+int linear8_launch(const Linear8Args &all)
 {
     for (int64_t row = 0; row < all.n; row += kRowsPerLaunch) {
         Linear8Args g = rows_from(all, row);
@@ -696,33 +697,34 @@ int linear8_launch(const Linear8Args &all, const char *who)
             g.part = (float *)scratch(kScratchLinear8, (size_t)c.splits * total * sizeof(float));
             if (!g.part) return EMBER_ERR_OUT_OF_MEMORY;
         }
-        if (!(c.kernel == kFew ? launch_few<false>(g, who)
-              : c.kernel == kLargeTiles ? launch_tiles<256, 256, 4, 2, 2, false>(g, 1, who)
-                                        : launch_small(g, c.splits, who)))
+        if (!(c.kernel == kFew ? launch_few<false>(g)
+              : c.kernel == kLargeTiles ? launch_tiles<256, 256, 4, 2, 2, false>(g, 1, "linear8_tiles256")
+                                        : launch_small(g, c.splits)))
             return EMBER_ERR_DEVICE;
         if (c.splits > 1) {
             hipLaunchKernelGGL(linear8_reduce, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 1 << 13)), dim3(256), 0, 0, g, c.splits, total);
-            if (!launch_ok(who)) return EMBER_ERR_DEVICE;
+            if (!launch_ok("linear8_reduce")) return EMBER_ERR_DEVICE;
         }
     }
     return EMBER_OK;
 }
 
-int gated8_launch(const Linear8Args &all, const char *who)
+int gated8_launch(const Linear8Args &all)
 {
     for (int64_t row = 0; row < all.n; row += kRowsPerLaunch) {
         Linear8Args g = rows_from(all, row);
         const Choice c = choose(g.n, g.m, g.w.groups, true);
         g.chunk = c.chunk;
         if (c.kernel == kLargeTiles || c.kernel == kMidTiles) {
-            if (!(c.kernel == kMidTiles ? launch_tiles<128, 256, 2, 4, 2, true>(g, 1, who) : launch_tiles<256, 256, 4, 2, 2, true>(g, 1, who)))
+            if (!(c.kernel == kMidTiles ? launch_tiles<128, 256, 2, 4, 2, true>(g, 1, "gated8_tiles128")
+                                        : launch_tiles<256, 256, 4, 2, 2, true>(g, 1, "gated8_tiles256")))
                 return EMBER_ERR_DEVICE;
         } else if (c.kernel == kFew) {
             g.out = (float *)scratch(kScratchLinear8, (size_t)g.n * g.m * sizeof(float));
             if (!g.out) return EMBER_ERR_OUT_OF_MEMORY;
             g.aligned = aligned_rows(g);
-            if (!launch_few<true>(g, who)) return EMBER_ERR_DEVICE;
-            const int st = rows8_write_launch(g.h, g.out, g.m, 0, who);
+            if (!launch_few<true>(g)) return EMBER_ERR_DEVICE;
+            const int st = rows8_write_launch(g.h, g.out, g.m, 0, "rows8_write");
             if (st) return st;
         } else {
             const int64_t tasks = (int64_t)g.n * g.h.scale_pitch;
@@ -730,9 +732,9 @@ int gated8_launch(const Linear8Args &all, const char *who)
             g.aligned = g.m % 4 == 0;
             g.part = (float *)scratch(kScratchLinear8, (size_t)c.splits * g.n * g.m * sizeof(float));
             if (!g.part) return EMBER_ERR_OUT_OF_MEMORY;
-            if (!launch_small(g, c.splits, who)) return EMBER_ERR_DEVICE;
+            if (!launch_small(g, c.splits)) return EMBER_ERR_DEVICE;
             hipLaunchKernelGGL(gated8_reduce, dim3((unsigned)std::min<int64_t>((tasks + 7) / 8, 1 << 13)), dim3(256), 0, 0, g, c.splits, tasks);
-            if (!launch_ok(who)) return EMBER_ERR_DEVICE;
+            if (!launch_ok("gated8_reduce")) return EMBER_ERR_DEVICE;
         }
     }
     return EMBER_OK;
@@ -760,7 +762,7 @@ extern "C" int linear8_fwd(const ember_rows8 *a, const ember_rows8 *w, const flo
     if (!out || (((uintptr_t)out | (uintptr_t)bias | (uintptr_t)residual) & 3) || act < kActNone || act > kActGelu)
         return record_error(EMBER_ERR_INVALID_ARGUMENT, "linear8_fwd");
     g.bias = bias, g.residual = residual, g.out = out, g.n = g.a.rows, g.m = g.w.rows, g.act = act;
-    return g.n && g.m ? linear8_launch(g, "linear8_fwd") : EMBER_OK;
+    return g.n && g.m ? linear8_launch(g) : EMBER_OK;
 }
 
 extern "C" int gated8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, const ember_rows8 *h, int act)
@@ -775,5 +777,5 @@ extern "C" int gated8_fwd(const ember_rows8 *a, const ember_rows8 *w, const floa
         return record_error(EMBER_ERR_INVALID_ARGUMENT, "gated8_fwd");
     if (to.rows == 0) return EMBER_OK;
     g.bias = bias, g.h = to, g.n = to.rows, g.m = to.cols, g.act = act;
-    return gated8_launch(g, "gated8_fwd");
+    return gated8_launch(g);
 }

@@ -33,13 +33,17 @@ def forward(x, w, bias, act, want_pre=True, log=None):
     return h.numpy(), None if pre is None else pre.numpy()
 
 
-def backward(dy, w_down, pre, act):
+def backward(dy, w_down, pre, act, log=None):
     n, d = dy.shape
     hidden = w_down.shape[0]
     G.say(f"gated_bwd n={n} hidden={hidden} d={d} act={act}")
     dev = [arr(a) for a in (dy, w_down, pre)]
     dpre = DeviceArray.from_numpy(np.full((n, 2 * hidden), G.SENTINEL))
-    capi.check(capi.lib().gated_bwd(*(a.ptr for a in dev), dpre.ptr, n, hidden, d, ACT[act]), "gated_bwd")
+    capi.launch_log_reset()
+    rc = capi.lib().gated_bwd(*(a.ptr for a in dev), dpre.ptr, n, hidden, d, ACT[act])
+    if log is not None:
+        log.extend(capi.launch_log())
+    capi.check(rc, "gated_bwd")
     return dpre.numpy()
 
 
