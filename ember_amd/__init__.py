@@ -3,7 +3,8 @@
 ``libember_amd.so`` is the C ABI (``include/ember_amd.h``); ``ember_amd._core``
 binds it for Python; this package mirrors the reference's ``ember`` front-end
 on top (``Tensor``, the element-wise and reduction functions, ``softmax``,
-``T``) and adds ``attention``, a 4-bit ``KVCache`` and ``token_logprobs``.  Names resolve lazily so that
+``T``) and adds ``attention``, a 4-bit ``KVCache``, ``token_logprobs`` and matrices
+in 8 bits with their products.  Names resolve lazily so that
 ``ember_amd.build`` can run before anything is built.
 """
 
@@ -16,9 +17,10 @@ _TENSOR_NAMES = (
     "tanh", "ctgh", "T", "sum", "softmax", "sqrt", "attention", "attention_forward",
     "attention_backward", "synchronize", "empty_cache", "memory_stats",
 )
-_SERVING_NAMES = {"KVCache": "kv_cache", "token_logprobs": "loss"}
+_SERVING_NAMES = {"KVCache": "kv_cache", "token_logprobs": "loss",
+                  **dict.fromkeys(("Rows8", "quantize8", "linear8", "gated8", "rms_norm8"), "rows8")}
 _CAPI_NAMES = ("set_deterministic", "is_deterministic")
-_SUBMODULES = ("nn", "optim", "loss", "random", "kv_cache", "capi", "build")
+_SUBMODULES = ("nn", "optim", "loss", "random", "kv_cache", "rows8", "capi", "build")
 
 __all__ = list(_TENSOR_NAMES) + list(_SERVING_NAMES) + list(_CAPI_NAMES) + ["nn", "optim", "loss", "random"]
 

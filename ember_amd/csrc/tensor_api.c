@@ -1336,6 +1336,286 @@ static PyObject *py_memory_stats(PyObject *module, PyObject *unused)
                          (unsigned long long)cached, "peak", (unsigned long long)peak);
 }
 
+/* ---- RMS norm, 8-bit matrices and gated layers ---- */
+
+static TensorObject *opt_sized(PyObject *o, Py_ssize_t size, const char *name)
+{
+    TensorObject *t = opt_tensor(o, name);
+    if (t && t != (TensorObject *)-1 && t->size != size) {
+        PyErr_Format(PyExc_ValueError, "%s has %zd elements, expected %zd", name, t->size, size);
+        return (TensorObject *)-1;
+    }
+    return t;
+}
+
+static float *opt_ptr(const TensorObject *t)
+{
+    return t ? t->d_ptr : NULL;
+}
+
+/* Elements of the buffers that hold the codes and scales of (rows, cols) in 8 bits;
+ * -1 and ValueError where there are no such. */
+static int rows8_sizes(long long rows, long long cols, Py_ssize_t *codes, Py_ssize_t *scales)
+{
+    if (rows < 0 || rows > (1 << 26) || cols < 1 || cols > (1 << 23)) {
+        PyErr_SetString(PyExc_ValueError, "a matrix in 8 bits has up to 2^26 rows and from 1 to 2^23 columns");
+        return -1;
+    }
+    *codes = (Py_ssize_t)(rows * ((cols + 127) / 128 * 32));
+    *scales = (Py_ssize_t)(rows * ((cols + 511) / 512));
+    return 0;
+}
+
+/* (codes, scales, rows, cols) */
+static int parse_rows8(PyObject *tuple, ember_rows8 *m)
+{
+    TensorObject *codes, *scales;
+    long long rows, cols;
+    Py_ssize_t nc, ns;
+    if (!PyTuple_Check(tuple)) {
+        PyErr_SetString(PyExc_TypeError, "a matrix in 8 bits must be a tuple");
+        return -1;
+    }
+    if (!PyArg_ParseTuple(tuple, "O!O!LL", &TensorType, &codes, &TensorType, &scales, &rows, &cols) || rows8_sizes(rows, cols, &nc, &ns))
+        return -1;
+    if (codes->size != nc || scales->size != ns) {
+        PyErr_SetString(PyExc_ValueError, "a matrix in 8 bits has buffers of other sizes than its own");
+        return -1;
+    }
+    *m = (ember_rows8){codes->d_ptr, scales->d_ptr, rows, cols};
+    return 0;
+}
+
+static int new_rows8(long long rows, long long cols, ember_rows8 *m, TensorObject **codes, TensorObject **scales)
+{
+    Py_ssize_t nc, ns;
+    if (rows8_sizes(rows, cols, &nc, &ns)) return -1;
+    if (!(*codes = alloc_tensor(nc))) return -1;
+    if (!(*scales = alloc_tensor(ns))) {
+        Py_DECREF(*codes);
+        return -1;
+    }
+    *m = (ember_rows8){(*codes)->d_ptr, (*scales)->d_ptr, rows, cols};
+    return 0;
+}
+
+static PyObject *give_rows8(int status, const char *what, TensorObject *codes, TensorObject *scales)
+{
+    if (raise_status(status, what)) {
+        Py_DECREF(codes);
+        Py_DECREF(scales);
+        return NULL;
+    }
+    return Py_BuildValue("(NN)", (PyObject *)codes, (PyObject *)scales);
+}
+
+/* _rows8_write(x, rows, cols, trans) -> (codes, scales): x is (rows, cols), or with trans (cols, rows). */
+static PyObject *py_rows8_write(PyObject *module, PyObject *args)
+{
+    TensorObject *x, *codes, *scales;
+    long long rows, cols;
+    int trans;
+    ember_rows8 m;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!LLp", &TensorType, &x, &rows, &cols, &trans) || new_rows8(rows, cols, &m, &codes, &scales)) return NULL;
+    if (x->size != (Py_ssize_t)(rows * cols)) {
+        PyErr_SetString(PyExc_ValueError, "_rows8_write: size mismatch");
+        Py_DECREF(codes);
+        Py_DECREF(scales);
+        return NULL;
+    }
+    return give_rows8(rows8_write(&m, x->d_ptr, trans ? rows : cols, trans), "_rows8_write", codes, scales);
+}
+
+/* _rows8_read(m) -> (rows, cols) */
+static PyObject *py_rows8_read(PyObject *module, PyObject *args)
+{
+    PyObject *mo;
+    ember_rows8 m;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O", &mo) || parse_rows8(mo, &m)) return NULL;
+    TensorObject *x = alloc_tensor((Py_ssize_t)(m.rows * m.cols));
+    if (!x) return NULL;
+    if (raise_status(rows8_read(&m, x->d_ptr, m.cols), "_rows8_read")) {
+        Py_DECREF(x);
+        return NULL;
+    }
+    return (PyObject *)x;
+}
+
+/* _rmsnorm_fwd(x, residual|None, gamma, rows, d, eps) -> (y, x + residual|None, rstd) */
+static PyObject *py_rmsnorm_fwd(PyObject *module, PyObject *args)
+{
+    TensorObject *x, *gamma;
+    PyObject *ro;
+    long long rows, d;
+    float eps;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!OO!LLf", &TensorType, &x, &ro, &TensorType, &gamma, &rows, &d, &eps)) return NULL;
+    if (rows < 0 || rows >= 1LL << 31 || d <= 0 || d >= 1LL << 31 || x->size != (Py_ssize_t)(rows * d) || gamma->size != d) {
+        PyErr_SetString(PyExc_ValueError, "_rmsnorm_fwd: size mismatch");
+        return NULL;
+    }
+    TensorObject *res = opt_sized(ro, x->size, "residual");
+    if (res == (TensorObject *)-1) return NULL;
+    TensorObject *y = alloc_tensor(x->size), *rstd = NULL, *sum = NULL;
+    if (!y || !(rstd = alloc_tensor((Py_ssize_t)rows)) || (res && !(sum = alloc_tensor(x->size))) ||
+        raise_status(rmsnorm_fwd(x->d_ptr, opt_ptr(res), gamma->d_ptr, opt_ptr(sum), y->d_ptr, rstd->d_ptr, rows, d, eps), "_rmsnorm_fwd")) {
+        Py_XDECREF(y);
+        Py_XDECREF(rstd);
+        Py_XDECREF(sum);
+        return NULL;
+    }
+    if (!sum) return Py_BuildValue("(NON)", (PyObject *)y, Py_None, (PyObject *)rstd);
+    return Py_BuildValue("(NNN)", (PyObject *)y, (PyObject *)sum, (PyObject *)rstd);
+}
+
+/* _rmsnorm_fwd8(x, residual|None, gamma, rows, d, eps) -> ((codes, scales) of y, x + residual|None) */
+static PyObject *py_rmsnorm_fwd8(PyObject *module, PyObject *args)
+{
+    TensorObject *x, *gamma, *codes, *scales, *sum = NULL;
+    PyObject *ro;
+    long long rows, d;
+    float eps;
+    ember_rows8 m;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!OO!LLf", &TensorType, &x, &ro, &TensorType, &gamma, &rows, &d, &eps)) return NULL;
+    if (rows < 0 || rows >= 1LL << 31 || d <= 0 || d >= 1LL << 31 || x->size != (Py_ssize_t)(rows * d) || gamma->size != d) {
+        PyErr_SetString(PyExc_ValueError, "_rmsnorm_fwd8: size mismatch");
+        return NULL;
+    }
+    TensorObject *res = opt_sized(ro, x->size, "residual");
+    if (res == (TensorObject *)-1 || new_rows8(rows, d, &m, &codes, &scales)) return NULL;
+    PyObject *y = NULL;
+    if (!res || (sum = alloc_tensor(x->size)))
+        y = give_rows8(rmsnorm_fwd8(x->d_ptr, opt_ptr(res), gamma->d_ptr, opt_ptr(sum), &m, eps), "_rmsnorm_fwd8", codes, scales);
+    else {
+        Py_DECREF(codes);
+        Py_DECREF(scales);
+    }
+    if (!y) {
+        Py_XDECREF(sum);
+        return NULL;
+    }
+    if (!sum) return Py_BuildValue("(NO)", y, Py_None);
+    return Py_BuildValue("(NN)", y, (PyObject *)sum);
+}
+
+/* _rmsnorm_bwd(s, gamma, rstd, dy, dres|None, rows, d) -> (dx, dgamma) */
+static PyObject *py_rmsnorm_bwd(PyObject *module, PyObject *args)
+{
+    TensorObject *s, *gamma, *rstd, *dy;
+    PyObject *ro;
+    long long rows, d;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!O!O!O!OLL", &TensorType, &s, &TensorType, &gamma, &TensorType, &rstd, &TensorType, &dy, &ro, &rows, &d))
+        return NULL;
+    if (rows < 0 || rows >= 1LL << 31 || d <= 0 || d >= 1LL << 31 || s->size != (Py_ssize_t)(rows * d) || dy->size != s->size ||
+        gamma->size != d || rstd->size != rows) {
+        PyErr_SetString(PyExc_ValueError, "_rmsnorm_bwd: size mismatch");
+        return NULL;
+    }
+    TensorObject *res = opt_sized(ro, s->size, "dres");
+    if (res == (TensorObject *)-1) return NULL;
+    TensorObject *dx = alloc_tensor(s->size), *dgamma = NULL;
+    if (!dx || !(dgamma = alloc_tensor((Py_ssize_t)d)) ||
+        raise_status(rmsnorm_bwd(s->d_ptr, gamma->d_ptr, rstd->d_ptr, dy->d_ptr, opt_ptr(res), dx->d_ptr, dgamma->d_ptr, rows, d), "_rmsnorm_bwd")) {
+        Py_XDECREF(dx);
+        Py_XDECREF(dgamma);
+        return NULL;
+    }
+    return Py_BuildValue("(NN)", (PyObject *)dx, (PyObject *)dgamma);
+}
+
+/* _linear8(a, w, bias|None, residual|None, act) -> act(a w^T + bias) + residual, a and w in 8 bits. */
+static PyObject *py_linear8(PyObject *module, PyObject *args)
+{
+    PyObject *ao, *wo, *bo, *ro;
+    int act;
+    ember_rows8 a, w;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "OOOOi", &ao, &wo, &bo, &ro, &act) || parse_rows8(ao, &a) || parse_rows8(wo, &w)) return NULL;
+    if (a.cols != w.cols) {
+        PyErr_SetString(PyExc_ValueError, "_linear8: a and w have different numbers of columns");
+        return NULL;
+    }
+    TensorObject *bias = opt_sized(bo, (Py_ssize_t)w.rows, "bias");
+    if (bias == (TensorObject *)-1) return NULL;
+    TensorObject *res = opt_sized(ro, (Py_ssize_t)(a.rows * w.rows), "residual");
+    if (res == (TensorObject *)-1) return NULL;
+    TensorObject *out = alloc_tensor((Py_ssize_t)(a.rows * w.rows));
+    if (!out) return NULL;
+    if (raise_status(linear8_fwd(&a, &w, opt_ptr(bias), opt_ptr(res), out->d_ptr, act), "_linear8")) {
+        Py_DECREF(out);
+        return NULL;
+    }
+    return (PyObject *)out;
+}
+
+/* _gated_fwd(x, w, bias|None, n, hidden, d, act, want_pre) -> (h, pre|None) */
+static PyObject *py_gated_fwd(PyObject *module, PyObject *args)
+{
+    TensorObject *x, *w;
+    PyObject *bo;
+    int n, hidden, d, act, want_pre;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!O!Oiiiip", &TensorType, &x, &TensorType, &w, &bo, &n, &hidden, &d, &act, &want_pre)) return NULL;
+    if (n < 0 || hidden < 1 || d < 1 || x->size != (Py_ssize_t)n * d || w->size != (Py_ssize_t)d * hidden * 2) {
+        PyErr_SetString(PyExc_ValueError, "_gated_fwd: operand sizes do not match (n, hidden, d)");
+        return NULL;
+    }
+    TensorObject *bias = opt_sized(bo, 2 * (Py_ssize_t)hidden, "bias");
+    if (bias == (TensorObject *)-1) return NULL;
+    TensorObject *h = alloc_tensor((Py_ssize_t)n * hidden), *pre = NULL;
+    if (!h || (want_pre && !(pre = alloc_tensor(2 * (Py_ssize_t)n * hidden))) ||
+        raise_status(gated_fwd(x->d_ptr, w->d_ptr, opt_ptr(bias), h->d_ptr, opt_ptr(pre), n, hidden, d, act), "_gated_fwd")) {
+        Py_XDECREF(h);
+        Py_XDECREF(pre);
+        return NULL;
+    }
+    if (!pre) return Py_BuildValue("(NO)", (PyObject *)h, Py_None);
+    return Py_BuildValue("(NN)", (PyObject *)h, (PyObject *)pre);
+}
+
+/* _gated_bwd(dy, w_down, pre, n, hidden, d, act) -> the gradient with respect to pre */
+static PyObject *py_gated_bwd(PyObject *module, PyObject *args)
+{
+    TensorObject *dy, *w, *pre;
+    int n, hidden, d, act;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "O!O!O!iiii", &TensorType, &dy, &TensorType, &w, &TensorType, &pre, &n, &hidden, &d, &act)) return NULL;
+    if (n < 0 || hidden < 1 || d < 1 || dy->size != (Py_ssize_t)n * d || w->size != (Py_ssize_t)hidden * d ||
+        pre->size != 2 * (Py_ssize_t)n * hidden) {
+        PyErr_SetString(PyExc_ValueError, "_gated_bwd: operand sizes do not match (n, hidden, d)");
+        return NULL;
+    }
+    TensorObject *dpre = alloc_tensor(pre->size);
+    if (!dpre) return NULL;
+    if (raise_status(gated_bwd(dy->d_ptr, w->d_ptr, pre->d_ptr, dpre->d_ptr, n, hidden, d, act), "_gated_bwd")) {
+        Py_DECREF(dpre);
+        return NULL;
+    }
+    return (PyObject *)dpre;
+}
+
+/* _gated8(a, w, bias|None, act) -> (codes, scales) of h, a and w in 8 bits. */
+static PyObject *py_gated8(PyObject *module, PyObject *args)
+{
+    PyObject *ao, *wo, *bo;
+    int act;
+    ember_rows8 a, w, h;
+    TensorObject *codes, *scales;
+    (void)module;
+    if (!PyArg_ParseTuple(args, "OOOi", &ao, &wo, &bo, &act) || parse_rows8(ao, &a) || parse_rows8(wo, &w)) return NULL;
+    if (a.cols != w.cols || w.rows < 2 || w.rows % 2) {
+        PyErr_SetString(PyExc_ValueError, "_gated8: w must have as many columns as a, and a row for each of both projections");
+        return NULL;
+    }
+    TensorObject *bias = opt_sized(bo, (Py_ssize_t)w.rows, "bias");
+    if (bias == (TensorObject *)-1 || new_rows8(a.rows, w.rows / 2, &h, &codes, &scales)) return NULL;
+    return give_rows8(gated8_fwd(&a, &w, opt_ptr(bias), &h, act), "_gated8", codes, scales);
+}
+
 /* ---- module ---- */
 
 #define METHOD(pyname, fn, doc) {pyname, (PyCFunction)fn, METH_VARARGS, doc}
@@ -1375,6 +1655,15 @@ static PyMethodDef module_methods[] = {
     METHOD("_kv_cache_attention", py_kv_cache_attention, "attention over a 4-bit cache -> (o, lse)"),
     METHOD("_token_logprobs", py_token_logprobs, "log probabilities by token id -> (logp, lse, lse_rest, entropy, top_tokens, top_logp)"),
     METHOD("_token_logprobs_bwd", py_token_logprobs_bwd, "gradient of log probabilities and entropy"),
+    METHOD("_rows8_write", py_rows8_write, "round a matrix to 8 bits -> (codes, scales)"),
+    METHOD("_rows8_read", py_rows8_read, "values that a matrix in 8 bits holds"),
+    METHOD("_rmsnorm_fwd", py_rmsnorm_fwd, "RMS norm -> (y, x + residual, rstd)"),
+    METHOD("_rmsnorm_fwd8", py_rmsnorm_fwd8, "RMS norm rounded to 8 bits -> ((codes, scales), x + residual)"),
+    METHOD("_rmsnorm_bwd", py_rmsnorm_bwd, "RMS norm backward -> (dx, dgamma)"),
+    METHOD("_linear8", py_linear8, "act(a @ w^T + bias) + residual of matrices in 8 bits"),
+    METHOD("_gated_fwd", py_gated_fwd, "gated layer -> (h, pre)"),
+    METHOD("_gated_bwd", py_gated_bwd, "gated layer backward -> the gradient of pre"),
+    METHOD("_gated8", py_gated8, "gated layer of matrices in 8 bits -> (codes, scales)"),
     {"_synchronize", (PyCFunction)py_synchronize, METH_NOARGS, "wait for all queued device work"},
     {"_empty_cache", (PyCFunction)py_empty_cache, METH_NOARGS,
      "return the allocator's cached blocks on the current device to HIP"},

@@ -22,6 +22,7 @@ from itertools import chain
 from ember_amd import _core as C
 from ember_amd import random as _random
 from ember_amd.kv_cache import KVCache
+from ember_amd.rows8 import activation_code, gated8, linear8, quantize8, rms_norm8
 from ember_amd.tensor import Tensor, attention_backward, attention_forward
 
 
@@ -159,6 +160,32 @@ def col_sum(x: Tensor) -> Tensor:
     """Column sums of a 2-D Tensor (a Linear layer's bias gradient)."""
     n, m = _rows(x)
     return Tensor._from_core(C._col_sum(x._core, n, m), (m,))
+
+
+def gated(x: Tensor, w: Tensor, b: Tensor | None = None, activation: str = "silu",
+          training: bool = True) -> tuple[Tensor, Tensor | None]:
+    """``act(x @ wg + bg) * (x @ wu + bu)`` in one GEMM with the gate in its
+    epilogue, for w = [wg | wu] (in, 2 * hidden) and b = [bg | bu]; act is "silu",
+    x / (1 + exp(-x)), or "gelu", Ember's.  Returns (h, pre), pre = x @ w + b being
+    kept where ``training`` (``gated_grad`` needs it)."""
+    n, d = _rows(x)
+    d2, m = _rows(w)
+    if d != d2 or m < 2 or m % 2:
+        raise ValueError(f"Shape mismatch: {x.shape} takes a weight of ({d}, 2 * hidden), got {w.shape}")
+    if b is not None and b.shape != (m,):
+        raise ValueError(f"b must be ({m},), got {b.shape}")
+    h, pre = C._gated_fwd(x._core, w._core, None if b is None else b._core, n, m // 2, d, activation_code(activation), training)
+    return Tensor._from_core(h, (n, m // 2)), (Tensor._from_core(pre, (n, m)) if pre is not None else None)
+
+
+def gated_grad(grad_y: Tensor, w_down: Tensor, pre: Tensor, activation: str = "silu") -> Tensor:
+    """The gradient with respect to ``pre`` of y = gated(...) @ w_down, from y's:
+    ``[dh * up * act'(gate) | dh * act(gate)]`` with dh = grad_y @ w_down^T, in one GEMM."""
+    n, d = _rows(grad_y)
+    hidden, d2 = _rows(w_down)
+    if d != d2 or pre.shape != (n, 2 * hidden):
+        raise ValueError(f"Shape mismatch: {grad_y.shape}, {w_down.shape} and {pre.shape}")
+    return Tensor._from_core(C._gated_bwd(grad_y._core, w_down._core, pre._core, n, hidden, d, activation_code(activation)), pre.shape)
 
 
 class Linear(Layer):
@@ -371,41 +398,150 @@ class LayerNorm(Layer):
         return Tensor._from_core(dx, self.x.shape)
 
 
+class RMSNorm(Layer):
+    """RMS norm over the last dimension: s / sqrt(mean(s^2) + eps) * gamma with s = x,
+    or x + residual where ``forward`` is given one (the sum is kept as ``sum``, and
+    the gradient that ``backward`` returns is that of either); gamma = 1 at reset."""
+
+    def __init__(self, features: int, eps: float = 1e-5):
+        self.features = features
+        self.eps = eps
+        self.reset()
+
+    def reset(self) -> None:
+        self.x = self.y = self.sum = None
+        self.gamma = _random.ones((self.features,))
+        self.grad_gamma = None
+        self._saved = None
+
+    def parameters(self) -> list[Tensor]:
+        return [self.gamma]
+
+    def gradients(self) -> list[Tensor | None]:
+        return [self.grad_gamma]
+
+    def forward(self, x: Tensor, training: bool = True, residual: Tensor | None = None) -> Tensor:
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError(f"residual must be {x.shape}, got {residual.shape}")
+        d = x.shape[-1]
+        y, s, rstd = C._rmsnorm_fwd(x._core, None if residual is None else residual._core, self.gamma._core, x.size // d, d, self.eps)
+        self.sum = x if s is None else Tensor._from_core(s, x.shape)
+        self._saved = (self.sum, rstd)
+        return Tensor._from_core(y, x.shape)
+
+    def backward(self, grad_y: Tensor, residual: Tensor | None = None) -> Tensor:
+        """Gradient with respect to x; ``residual`` (the gradient reaching the
+        sum through a skip connection) is added in the same pass."""
+        if self._saved is None:
+            raise RuntimeError("forward() must run before backward()")
+        s, rstd = self._saved
+        d = s.shape[-1]
+        dx, dgamma = C._rmsnorm_bwd(s._core, self.gamma._core, rstd, grad_y._core, None if residual is None else residual._core,
+                                    s.size // d, d)
+        self.grad_gamma = Tensor._from_core(dgamma, (d,))
+        return Tensor._from_core(dx, s.shape)
+
+
 def _xavier(fan_in: int, fan_out: int) -> Tensor:
     a = math.sqrt(6.0 / (fan_in + fan_out))
     return _random.uniform(-a, a, (fan_in, fan_out))
 
 
-class DecoderBlock(Layer):
-    """One pre-LN transformer decoder block on (B*S, d) token rows:
-        h = LN1(x);  x2 = x + Attention(h Wqkv + bqkv) Wo + bo
-        y = x2 + GELU(LN2(x2) W1 + b1) W2 + b2
-    with causal fused attention reading the packed QKV projection in place.
-    Weights Xavier-uniform, biases 0, LayerNorm gamma 1 / beta 0.  ``forward``
-    takes (x, B, S); ``backward`` returns dx and fills ``gradients()``.
-    ``decode`` runs new tokens against a 4-bit cache of the earlier ones."""
+def _gate_weights(d: int, hidden: int) -> Tensor:
+    """Both projections of a gated layer side by side, each as ``_xavier``'s."""
+    a = math.sqrt(6.0 / (d + hidden))
+    return _random.uniform(-a, a, (d, 2 * hidden))
 
-    def __init__(self, d_model: int, n_heads: int, mlp_ratio: int = 4, causal: bool = True):
-        if d_model % n_heads:
-            raise ValueError("d_model must be a multiple of n_heads")
-        self.d, self.h, self.r, self.causal = d_model, n_heads, mlp_ratio, causal
+
+class GatedFeedForward(Layer):
+    """(act(x wg + bg) * (x wu + bu)) w_out + b_out on (rows, features), with
+    ``hidden`` columns between; ``activation`` is "silu" or "gelu" (Ember's).  w_in =
+    [wg | wu] and b_in are one matrix and one vector; without ``bias`` there are only
+    the weights.  Weights Xavier-uniform, biases 0."""
+
+    def __init__(self, features: int, hidden: int, activation: str = "silu", bias: bool = True):
+        activation_code(activation)
+        if features < 1 or hidden < 1:
+            raise ValueError(f"features and hidden must be positive, got {features} and {hidden}")
+        self.features, self.hidden, self.activation, self.bias = features, hidden, activation, bias
         self.reset()
 
     def reset(self) -> None:
-        d, r = self.d, self.r
-        self.ln1 = LayerNorm(d)
-        self.ln2 = LayerNorm(d)
-        self.w_qkv, self.b_qkv = _xavier(d, 3 * d), _random.zeros((3 * d,))
-        self.w_o, self.b_o = _xavier(d, d), _random.zeros((d,))
-        self.w_1, self.b_1 = _xavier(d, r * d), _random.zeros((r * d,))
-        self.w_2, self.b_2 = _xavier(r * d, d), _random.zeros((d,))
-        self._grads: list[Tensor | None] = [None] * 12
+        d, hidden = self.features, self.hidden
+        self.w_in, self.w_out = _gate_weights(d, hidden), _xavier(hidden, d)
+        self.b_in = _random.zeros((2 * hidden,)) if self.bias else None
+        self.b_out = _random.zeros((d,)) if self.bias else None
+        self._grads: list[Tensor | None] = [None] * (4 if self.bias else 2)
         self.x = self.y = None
         self._saved = None
 
     def parameters(self) -> list[Tensor]:
-        return [self.ln1.gamma, self.ln1.beta, self.w_qkv, self.b_qkv, self.w_o, self.b_o,
-                self.ln2.gamma, self.ln2.beta, self.w_1, self.b_1, self.w_2, self.b_2]
+        return [self.w_in, self.b_in, self.w_out, self.b_out] if self.bias else [self.w_in, self.w_out]
+
+    def gradients(self) -> list[Tensor | None]:
+        return list(self._grads)
+
+    def forward(self, x: Tensor, training: bool = True, residual: Tensor | None = None) -> Tensor:
+        h, pre = gated(x, self.w_in, self.b_in, self.activation, training)
+        y, _ = linear(h, self.w_out, self.b_out, residual)
+        self._saved = (x, h, pre) if training else None
+        return y
+
+    def backward(self, grad_y: Tensor) -> Tensor:
+        if self._saved is None:
+            raise RuntimeError("forward(training=True) must run before backward()")
+        x, h, pre = self._saved
+        dpre = gated_grad(grad_y, self.w_out, pre, self.activation)
+        g_in, g_out = weight_grad(x, dpre), weight_grad(h, grad_y)
+        self._grads = [g_in, col_sum(dpre), g_out, col_sum(grad_y)] if self.bias else [g_in, g_out]
+        return input_grad(dpre, self.w_in)
+
+
+class DecoderBlock(Layer):
+    """One pre-norm transformer decoder block on (B*S, d) token rows:
+        h = N1(x);  x2 = x + Attention(h Wqkv + bqkv) Wo + bo
+        y = x2 + GELU(N2(x2) W1 + b1) W2 + b2
+    with causal fused attention reading the packed QKV projection in place.  N1 and
+    N2 are LayerNorm, or with ``norm="rms"`` RMSNorm.  ``gated`` "silu" or "gelu"
+    makes the feed-forward layer (act(N2(x2) wg + bg) * (N2(x2) wu + bu)) W2 + b2 with
+    W1 = [wg | wu].  Its width is ``hidden``, ``mlp_ratio * d_model`` without.
+    Weights Xavier-uniform, biases 0, norms' gamma 1 / beta 0.  ``forward``
+    takes (x, B, S); ``backward`` returns dx and fills ``gradients()``.
+    ``decode`` runs new tokens against a 4-bit cache of the earlier ones, and
+    ``quantize8`` gives a block that does so with its matrices in 8 bits."""
+
+    def __init__(self, d_model: int, n_heads: int, mlp_ratio: int = 4, causal: bool = True, norm: str = "layer",
+                 gated: str | None = None, hidden: int | None = None):
+        if d_model % n_heads:
+            raise ValueError("d_model must be a multiple of n_heads")
+        if norm not in ("layer", "rms"):
+            raise ValueError(f"norm must be 'layer' or 'rms', not {norm!r}")
+        if gated is not None:
+            activation_code(gated)
+        if hidden is not None and hidden < 1:
+            raise ValueError(f"hidden must be positive, not {hidden}")
+        self.d, self.h, self.r, self.causal = d_model, n_heads, mlp_ratio, causal
+        self.norm, self.gated = norm, gated
+        self.hidden = mlp_ratio * d_model if hidden is None else hidden
+        self.reset()
+
+    def reset(self) -> None:
+        d, hidden = self.d, self.hidden
+        norm = RMSNorm if self.norm == "rms" else LayerNorm
+        self.ln1 = norm(d)
+        self.ln2 = norm(d)
+        self.w_qkv, self.b_qkv = _xavier(d, 3 * d), _random.zeros((3 * d,))
+        self.w_o, self.b_o = _xavier(d, d), _random.zeros((d,))
+        self.w_1 = _gate_weights(d, hidden) if self.gated else _xavier(d, hidden)
+        self.b_1 = _random.zeros((self.w_1.shape[1],))
+        self.w_2, self.b_2 = _xavier(hidden, d), _random.zeros((d,))
+        self._grads: list[Tensor | None] = [None] * len(self.parameters())
+        self.x = self.y = None
+        self._saved = None
+
+    def parameters(self) -> list[Tensor]:
+        return [*self.ln1.parameters(), self.w_qkv, self.b_qkv, self.w_o, self.b_o,
+                *self.ln2.parameters(), self.w_1, self.b_1, self.w_2, self.b_2]
 
     def gradients(self) -> list[Tensor | None]:
         return list(self._grads)
@@ -427,7 +563,10 @@ class DecoderBlock(Layer):
         x2, _ = linear(o, self.w_o, self.b_o, residual=x)
         self.ln2.x = x2
         h2 = self.ln2.forward(x2)
-        a, u = linear(h2, self.w_1, self.b_1, gelu=True)
+        if self.gated:
+            a, u = gated(h2, self.w_1, self.b_1, self.gated)
+        else:
+            a, u = linear(h2, self.w_1, self.b_1, gelu=True)
         y, _ = linear(a, self.w_2, self.b_2, residual=x2)
         self._saved = (B, S, scale, h1, qkv, o, lse, x2, h2, a, u)
         return y
@@ -437,12 +576,16 @@ class DecoderBlock(Layer):
             raise RuntimeError("forward() must run before backward()")
         B, S, scale, h1, qkv, o, lse, x2, h2, a, u = self._saved
         D = self.d // self.h
-        # MLP: y = x2 + GELU(h2 W1 + b1) W2 + b2
+        # MLP: y = x2 + GELU(h2 W1 + b1) W2 + b2, or with the gate in GELU's place
         g_w2, g_b2 = weight_grad(a, grad_y), col_sum(grad_y)
-        da = input_grad(grad_y, self.w_2)
-        n, m = _rows(da)
-        du_core, g_b1_core = C._gelu_bwd_col_sum(da._core, u._core, n, m)  # a recomputed from u
-        du, g_b1 = Tensor._from_core(du_core, da.shape), Tensor._from_core(g_b1_core, (m,))
+        if self.gated:
+            du = gated_grad(grad_y, self.w_2, u, self.gated)
+            g_b1 = col_sum(du)
+        else:
+            da = input_grad(grad_y, self.w_2)
+            n, m = _rows(da)
+            du_core, g_b1_core = C._gelu_bwd_col_sum(da._core, u._core, n, m)  # a recomputed from u
+            du, g_b1 = Tensor._from_core(du_core, da.shape), Tensor._from_core(g_b1_core, (m,))
         g_w1 = weight_grad(h2, du)
         dx2 = self.ln2.backward(input_grad(du, self.w_1), residual=grad_y)
         # attention: x2 = x + O Wo + bo
@@ -453,8 +596,7 @@ class DecoderBlock(Layer):
                                     self.causal), qkv.shape)
         g_wqkv, g_bqkv = weight_grad(h1, dqkv), col_sum(dqkv)
         dx = self.ln1.backward(input_grad(dqkv, self.w_qkv), residual=dx2)
-        self._grads = [self.ln1.grad_gamma, self.ln1.grad_beta, g_wqkv, g_bqkv, g_wo, g_bo,
-                       self.ln2.grad_gamma, self.ln2.grad_beta, g_w1, g_b1, g_w2, g_b2]
+        self._grads = [*self.ln1.gradients(), g_wqkv, g_bqkv, g_wo, g_bo, *self.ln2.gradients(), g_w1, g_b1, g_w2, g_b2]
         return dx
 
     def make_cache(self, sequences: int, tokens: int, page_size: int = 64, pages: int | None = None) -> KVCache:
@@ -467,6 +609,21 @@ class DecoderBlock(Layer):
         padded behind), which are appended to the cache and attend to it.  Causal
         blocks only; for inference: what ``backward`` needs stays as it was.
         In rows past ``count`` the attention gives 0."""
+        T = self._new_tokens(x, cache)
+        if T == 0:
+            return _random.zeros(x.shape)
+        qkv, _ = linear(self._normed(x, self.ln1), self.w_qkv, self.b_qkv)
+        x2, _ = linear(self._attend(qkv, cache, T, count), self.w_o, self.b_o, residual=x)
+        h2 = self._normed(x2, self.ln2)
+        if self.gated:
+            a, _ = gated(h2, self.w_1, self.b_1, self.gated, training=False)
+        else:
+            a, _ = linear(h2, self.w_1, self.b_1, gelu=True)
+        y, _ = linear(a, self.w_2, self.b_2, residual=x2)
+        return y
+
+    def _new_tokens(self, x: Tensor, cache: KVCache) -> int:
+        """T of ``decode``'s arguments, which it checks."""
         if not self.causal:
             raise ValueError("decode() needs a causal block")
         rows, d = _rows(x)
@@ -474,16 +631,67 @@ class DecoderBlock(Layer):
             raise ValueError(f"the cache has {cache.heads} heads of {cache.head_dim}, the block {self.h} of {self.d // self.h}")
         if d != self.d or rows % cache.sequences:
             raise ValueError(f"x must be ({cache.sequences} * T, {self.d}), got {x.shape}")
-        T = rows // cache.sequences
-        if rows == 0:
-            return _random.zeros(x.shape)
-        norm = lambda x, ln: Tensor._from_core(  # noqa: E731
-            C._layernorm_fwd(x._core, ln.gamma._core, ln.beta._core, rows, d, ln.eps)[0], x.shape)
-        qkv, _ = linear(norm(x, self.ln1), self.w_qkv, self.b_qkv)
-        D, strides = cache.head_dim, (T * 3 * d, self.d // self.h, 3 * d)
+        return rows // cache.sequences
+
+    def _normed(self, x: Tensor, norm: LayerNorm | RMSNorm) -> Tensor:
+        rows, d = _rows(x)
+        if self.norm == "rms":
+            y = C._rmsnorm_fwd(x._core, None, norm.gamma._core, rows, d, norm.eps)[0]
+        else:
+            y = C._layernorm_fwd(x._core, norm.gamma._core, norm.beta._core, rows, d, norm.eps)[0]
+        return Tensor._from_core(y, x.shape)
+
+    def _attend(self, qkv: Tensor, cache: KVCache, T: int, count: Sequence[int] | None) -> Tensor:
+        """Appends the keys and values of qkv (rows, 3 d) and attends to the cache."""
+        d, D = self.d, cache.head_dim
+        strides = (T * 3 * d, D, 3 * d)
         cache._append(qkv._core, d, qkv._core, 2 * d, T, strides, count)
         o, _ = cache._attend(qkv._core, 0, T, self.h, strides, True, float(1.0 / math.sqrt(D)))
-        x2, _ = linear(Tensor._from_core(o, (rows, d)), self.w_o, self.b_o, residual=x)
-        a, _ = linear(norm(x2, self.ln2), self.w_1, self.b_1, gelu=True)
-        y, _ = linear(a, self.w_2, self.b_2, residual=x2)
-        return y
+        return Tensor._from_core(o, (qkv.shape[0], d))
+
+    def quantize8(self) -> DecoderBlock8:
+        """This causal block for decoding with its four matrices in 8 bits, as they are now."""
+        return DecoderBlock8(self)
+
+
+class DecoderBlock8:
+    """A ``DecoderBlock`` for inference whose matrices are held in 8 bits, 33/32 byte
+    per element; what enters a product is rounded to 8 bits too, by the norm and the
+    gate as they write it.  Norms, biases, attention and all sums stay float32.
+    ``block.quantize8()`` makes one: a copy of the block's weights at that time (its
+    norms' and biases' Tensors are shared)."""
+
+    def __init__(self, block: DecoderBlock):
+        if not block.causal:
+            raise ValueError("decode() needs a causal block")
+        self.block = block
+        self.w_qkv, self.w_o, self.w_1, self.w_2 = (quantize8(w, trans=True) for w in (block.w_qkv, block.w_o, block.w_1, block.w_2))
+
+    @property
+    def nbytes(self) -> int:
+        """Device memory of the matrices."""
+        return sum(w.nbytes for w in (self.w_qkv, self.w_o, self.w_1, self.w_2))
+
+    def make_cache(self, sequences: int, tokens: int, page_size: int = 64, pages: int | None = None) -> KVCache:
+        """An empty cache for ``decode``: ``sequences`` of up to ``tokens`` tokens."""
+        return self.block.make_cache(sequences, tokens, page_size, pages)
+
+    def _normed(self, x: Tensor, norm: LayerNorm | RMSNorm):
+        if self.block.norm == "rms":
+            return rms_norm8(x, norm.gamma, norm.eps)[0]
+        return quantize8(self.block._normed(x, norm))
+
+    def decode(self, x: Tensor, cache: KVCache, count: Sequence[int] | None = None) -> Tensor:
+        """``DecoderBlock.decode`` with the matrices in 8 bits."""
+        b = self.block
+        T = b._new_tokens(x, cache)
+        if T == 0:
+            return _random.zeros(x.shape)
+        qkv = linear8(self._normed(x, b.ln1), self.w_qkv, b.b_qkv)
+        x2 = linear8(quantize8(b._attend(qkv, cache, T, count)), self.w_o, b.b_o, residual=x)
+        h2 = self._normed(x2, b.ln2)
+        if b.gated:
+            a = gated8(h2, self.w_1, b.b_1, b.gated)
+        else:
+            a = quantize8(linear8(h2, self.w_1, b.b_1, gelu=True))
+        return linear8(a, self.w_2, b.b_2, residual=x2)

@@ -1,0 +1,264 @@
+"""nn.RMSNorm, nn.GatedFeedForward and decoder blocks made of them, in training and
+decoding with and without matrices in 8 bits, against float64."""
+
+import numpy as np
+import pytest
+import torch
+
+import ember_amd as em
+import gpu_helpers as G
+from ember_amd import _core, capi, nn, optim
+from feedforward_helpers import ff
+from test_serving_gpu import cached_attention
+from tolerance import assert_north_star
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(rng, *shape):
+    return rng.standard_normal(shape).astype(np.float32)
+
+
+def wide(t, grad=True):
+    return torch.tensor(t.to_np().astype(np.float64), requires_grad=grad)
+
+
+def act64(name, x):
+    return 0.5 * x * (1 + torch.tanh(0.8 * x)) if name == "gelu" else x * torch.sigmoid(x)
+
+
+def rms64(x, gamma, eps):
+    return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps) * gamma
+
+
+def test_quantize8_round_trip():
+    x = normal(np.random.default_rng(0), 7, 300)
+    for trans in (False, True):
+        m = em.quantize8(em.Tensor(x), trans)
+        want = np.ascontiguousarray(x.T) if trans else x
+        codes, scales = ff.quantise8(want)
+        np.testing.assert_array_equal(m.to_tensor().to_np(), ff.values8(codes, scales, want.shape[1]))
+        assert m.nbytes == codes.size + scales.size
+    assert em.quantize8(em.Tensor._from_core(_core._Tensor(0), (0, 5))).to_tensor().shape == (0, 5)
+
+
+def test_functions_of_8_bit_matrices():
+    """Small whole numbers, on which every step but the gate is exact."""
+    rng = np.random.default_rng(1)
+    x, w = rng.integers(-15, 16, (5, 200)).astype(np.float32), rng.integers(-15, 16, (200, 12)).astype(np.float32)
+    b, r = rng.integers(-9, 9, 12).astype(np.float32), rng.integers(-9, 9, (5, 12)).astype(np.float32)
+    x8, w8 = em.quantize8(em.Tensor(x)), em.quantize8(em.Tensor(w), trans=True)
+    np.testing.assert_array_equal(em.linear8(x8, w8, em.Tensor(b), em.Tensor(r)).to_np(), x @ w + b + r)
+    far = np.float32([4096] * 6 + [-1, 0, 1, 2, 3, -4])  # gates of 4096 pass what they gate unchanged
+    h = em.gated8(em.quantize8(em.Tensor(np.ones((3, 200), np.float32))), em.quantize8(em.Tensor(np.zeros((12, 200), np.float32))), em.Tensor(far), "silu")
+    np.testing.assert_array_equal(h.to_tensor().to_np(), np.tile(4096 * far[6:], (3, 1)))
+    y, s = em.rms_norm8(em.Tensor(np.full((2, 64), 3, np.float32)), em.Tensor(np.full(64, 2, np.float32)), 0.0, em.Tensor(np.full((2, 64), -1, np.float32)))
+    np.testing.assert_array_equal(s.to_np(), 2)
+    np.testing.assert_array_equal(y.to_tensor().to_np(), 2)
+
+
+@pytest.mark.parametrize("shape", [(5, 64), (2, 9, 1028)])
+def test_rms_norm_layer(shape):
+    rng = np.random.default_rng(2)
+    x, r, g, past = (normal(rng, *shape) for _ in range(4))
+    layer = nn.RMSNorm(shape[-1])
+    layer.gamma = em.Tensor(normal(rng, shape[-1]))
+    y = layer.forward(em.Tensor(x), residual=em.Tensor(r))
+    np.testing.assert_array_equal(layer.sum.to_np(), x + r)
+    s, gamma = wide(layer.sum), wide(layer.gamma)
+    ref = rms64(s, gamma, layer.eps)
+    (ref * torch.tensor(g.astype(np.float64))).sum().backward()
+    dx = layer.backward(em.Tensor(g), em.Tensor(past))
+    assert_north_star(y.to_np(), ref.detach().numpy())
+    assert_north_star(dx.to_np(), s.grad.numpy() + past)
+    assert_north_star(layer.gradients()[0].to_np(), gamma.grad.numpy())
+    plain = layer(em.Tensor(x))
+    assert_north_star(plain.to_np(), rms64(torch.tensor(x.astype(np.float64)), gamma.detach(), layer.eps).numpy())
+    with pytest.raises(ValueError):
+        layer(em.Tensor(normal(rng, 2, shape[-1] + 4)))
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("n, d, hidden", [(1, 64, 170), (50, 96, 100), (300, 128, 341)])
+def test_gated_feed_forward(n, d, hidden, bias, activation):
+    rng = np.random.default_rng(n + hidden)
+    em.random.seed(n)
+    layer = nn.GatedFeedForward(d, hidden, activation, bias)
+    if bias:
+        layer.b_in, layer.b_out = em.Tensor(normal(rng, 2 * hidden)), em.Tensor(normal(rng, d))
+    x, g = em.Tensor(normal(rng, n, d)), em.Tensor(normal(rng, n, d))
+    y = layer(x)
+    dx = layer.backward(g)
+    at = [wide(t) for t in [x, *layer.parameters()]]
+    w_in, w_out = at[1], at[3 if bias else 2]
+    pre = at[0] @ w_in + (at[2] if bias else 0)
+    ref = act64(activation, pre[:, :hidden]) * pre[:, hidden:] @ w_out + (at[4] if bias else 0)
+    (ref * torch.tensor(g.to_np().astype(np.float64))).sum().backward()
+    assert_north_star(y.to_np(), ref.detach().numpy())
+    for i, (got, t) in enumerate(zip([dx, *layer.gradients()], at)):
+        assert_north_star(got.to_np(), t.grad.numpy(), f"gradient {i}")
+    np.testing.assert_array_equal(layer(x, training=False).to_np(), y.to_np())
+
+
+def block64(block, x, B, S):
+    """The block in float64 on torch, and its leaves: x and the parameters."""
+    leaves = [wide(x), *(wide(p) for p in block.parameters())]
+    x64, rest = leaves[0], list(leaves[1:])
+    take = lambda: rest.pop(0)  # noqa: E731
+
+    def norm(t):
+        gamma = take()
+        if block.norm == "rms":
+            return rms64(t, gamma, 1e-5)
+        return torch.nn.functional.layer_norm(t, (block.d,), gamma, take(), 1e-5)
+    qkv = (norm(x64) @ take() + take()).reshape(B, S, 3, block.h, -1).permute(2, 0, 3, 1, 4)
+    scores = qkv[0] @ qkv[1].transpose(-1, -2) / np.sqrt(block.d // block.h)
+    if block.causal:
+        scores = scores.masked_fill(torch.ones(S, S).triu(1).bool(), -np.inf)
+    o = (torch.softmax(scores, -1) @ qkv[2]).permute(0, 2, 1, 3).reshape(B * S, block.d)
+    x2 = x64 + o @ take() + take()
+    u = norm(x2) @ take() + take()
+    h = act64(block.gated, u[:, :block.hidden]) * u[:, block.hidden:] if block.gated else act64("gelu", u)
+    return x2 + h @ take() + take(), leaves
+
+
+@pytest.mark.parametrize("kind", [dict(norm="rms", gated="silu", hidden=171), dict(norm="rms", gated="gelu"), dict(norm="rms"), dict(gated="silu"), {}])
+@pytest.mark.parametrize("causal", [True, False])
+def test_decoder_block(kind, causal):
+    B, S, H, d = 2, 40, 2, 64
+    rng = np.random.default_rng(3)
+    em.random.seed(4)
+    block = nn.DecoderBlock(d, H, 4, causal, **kind)
+    for p in block.parameters():  # no zeros or ones
+        p._adopt(em.Tensor(p.to_np() + 0.1 * normal(rng, *p.shape)))
+    x, g = em.Tensor(normal(rng, B * S, d)), em.Tensor(normal(rng, B * S, d))
+    G.say(f"decoder block {kind} causal={causal}")
+    y = block(x, B, S)
+    dx = block.backward(g)
+    ref, leaves = block64(block, x, B, S)
+    (ref * torch.tensor(g.to_np().astype(np.float64))).sum().backward()
+    assert_north_star(y.to_np(), ref.detach().numpy(), "y")
+    for i, (got, t) in enumerate(zip([dx, *block.gradients()], leaves)):
+        assert_north_star(got.to_np(), t.grad.numpy(), f"gradient {i}")
+
+
+def test_training_steps():
+    """A few steps of a block of both: every parameter moves, and stays finite."""
+    em.random.seed(5)
+    rng = np.random.default_rng(5)
+    block = nn.DecoderBlock(64, 2, norm="rms", gated="silu", hidden=170)
+    before = [p.to_np() for p in block.parameters()]
+    opt, mse = optim.Adam(block.parameters(), lr=1e-3), em.loss.MSELoss()
+    x, target = em.Tensor(normal(rng, 60, 64)), em.Tensor(normal(rng, 60, 64))
+    for _ in range(3):
+        mse(block(x, 2, 30), target)
+        block.backward(mse.backward())
+        opt.apply(block.gradients())
+    for p, b in zip(block.parameters(), before):
+        assert np.isfinite(p.to_np()).all() and (p.to_np() != b).any()
+
+
+def decode64(block, weights, x, start, count, cached, T):
+    """decode in float64 with the given matrices, its attention over what the cache holds."""
+    val = lambda t: t.to_np().astype(np.float64)  # noqa: E731
+    w_qkv, w_o, w_1, w_2 = weights
+
+    def norm(x, n):
+        if block.norm == "rms":
+            return x / np.sqrt((x * x).mean(-1, keepdims=True) + n.eps) * val(n.gamma)
+        return (x - x.mean(-1, keepdims=True)) / np.sqrt(x.var(-1, keepdims=True) + n.eps) * val(n.gamma) + val(n.beta)
+    x = x.astype(np.float64)
+    qkv = (norm(x, block.ln1) @ w_qkv + val(block.b_qkv)).reshape(len(start), T, 3, block.h, block.d // block.h)
+    o = cached_attention(qkv[:, :, 0], *cached, start, count).reshape(x.shape)
+    x2 = x + o @ w_o + val(block.b_o)
+    u = norm(x2, block.ln2) @ w_1 + val(block.b_1)
+    return x2 + (ff.gate(block.gated, u) if block.gated else ff.activate("gelu", u)[0]) @ w_2 + val(block.b_2)
+
+
+KINDS = [dict(norm="rms", gated="silu", hidden=200), dict(norm="rms", gated="gelu"), dict(gated="silu"), {}]
+STEPS = ((21, [21, 9]), (1, None), (1, None), (3, [3, 0]))
+
+
+def some_block(kind, d=128, heads=2):
+    em.random.seed(6)
+    rng = np.random.default_rng(7)
+    block = nn.DecoderBlock(d, heads, **kind)
+    for p in block.parameters():
+        p._adopt(em.Tensor(p.to_np() + 0.05 * normal(rng, *p.shape)))
+    return block, rng
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_decode(kind):
+    block, rng = some_block(kind)
+    cache = block.make_cache(2, 64, page_size=16)
+    for T, count in STEPS:
+        start = cache.lengths
+        x = normal(rng, 2 * T, 128)
+        y = block.decode(em.Tensor(x), cache, count).to_np()
+        weights = [getattr(block, n).to_np().astype(np.float64) for n in ("w_qkv", "w_o", "w_1", "w_2")]
+        assert_north_star(y, decode64(block, weights, x, start, count or [T, T], [t.to_np() for t in cache.read()], T))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_decode_in_8_bits(kind):
+    """Bit for bit the public functions in turn, and near float64 with the weights
+    that the 8-bit matrices hold: what is left is the rounding of four inputs of
+    products to at most 2^-4 of each element, which passes on to the branches' sums
+    with signs of its own; four times 2^-4 of the branches' size covers it."""
+    block, rng = some_block(kind)
+    block8 = block.quantize8()
+    assert block8.nbytes < 0.27 * sum(4 * np.prod(w.shape) for w in (block.w_qkv, block.w_o, block.w_1, block.w_2))
+    cache, twin = block8.make_cache(2, 64, page_size=16), block8.make_cache(2, 64, page_size=16)
+    w = [em.quantize8(getattr(block, n), trans=True) for n in ("w_qkv", "w_o", "w_1", "w_2")]
+    weights = [m.to_tensor().to_np().astype(np.float64).T for m in w]
+    for T, count in STEPS:
+        start = cache.lengths
+        x = normal(rng, 2 * T, 128)
+        G.say(f"DecoderBlock8.decode {kind} T={T}")
+        y = block8.decode(em.Tensor(x), cache, count).to_np()
+        tx = em.Tensor(x)
+
+        def normed(t, n):
+            if block.norm == "rms":
+                return em.rms_norm8(t, n.gamma, n.eps)[0]
+            return em.quantize8(n.forward(t))
+        qkv = em.linear8(normed(tx, block.ln1), w[0], block.b_qkv).to_np().reshape(2, T, 3, 2, 64)
+        q, k, v = (em.Tensor(np.ascontiguousarray(qkv[:, :, i])) for i in range(3))
+        twin.write(k, v, count)
+        o = twin.attention(q)[0].to_np().reshape(2 * T, 128)
+        x2 = em.linear8(em.quantize8(em.Tensor(o)), w[1], block.b_o, tx)
+        h2 = normed(x2, block.ln2)
+        a = em.gated8(h2, w[2], block.b_1, block.gated) if block.gated else em.quantize8(em.linear8(h2, w[2], block.b_1, gelu=True))
+        np.testing.assert_array_equal(y, em.linear8(a, w[3], block.b_2, x2).to_np())
+        ref = decode64(block, weights, x, start, count or [T, T], [t.to_np() for t in cache.read()], T)
+        assert np.linalg.norm(y - ref) <= 4 * 2.0 ** -4 * np.linalg.norm(ref - x)
+    assert block8.decode(em.Tensor._from_core(_core._Tensor(0), (0, 128)), cache).shape == (0, 128)
+
+
+def test_8_bit_block_keeps_its_weights():
+    """A block8 is of the block's matrices when it was made, whatever becomes of them."""
+    block, rng = some_block(KINDS[0])
+    block8 = block.quantize8()
+    x = em.Tensor(normal(rng, 3, 128))
+    y = block8.decode(x, block8.make_cache(3, 4)).to_np()
+    for w in (block.w_qkv, block.w_o, block.w_1, block.w_2):
+        w._adopt(em.Tensor(np.zeros(w.shape, np.float32)))
+    np.testing.assert_array_equal(block8.decode(x, block8.make_cache(3, 4)).to_np(), y)
+
+
+def test_decode_leaves_training_alone():
+    block, rng = some_block(KINDS[0], 64, 2)
+    x, g = em.Tensor(normal(rng, 60, 64)), em.Tensor(normal(rng, 60, 64))
+    capi.set_deterministic(True)
+    try:
+        block(x, 2, 30)
+        grads = [block.backward(g).to_np(), *(t.to_np() for t in block.gradients())]
+        block(x, 2, 30)
+        for b in (block, block.quantize8()):
+            b.decode(em.Tensor(normal(rng, 6, 64)), block.make_cache(2, 10))
+        for a, b in zip([block.backward(g), *block.gradients()], grads):
+            np.testing.assert_array_equal(a.to_np(), b)
+    finally:
+        capi.set_deterministic(False)
