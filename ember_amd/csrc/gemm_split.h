@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * WR * WC, PER_CU) void gemm_split_kernel(GemmAr
     constexpr int RB = TM / WR / 32, CB = TN / WC / 32;
     typedef Operand<TM, BK, NT, !TA> OA;
     typedef Operand<TN, BK, NT, TB> OB;
-    
+
     __shared__ u32x4 As0[3 * OA::kPlane], As1[3 * OA::kPlane];
     __shared__ u32x4 Bs0[3 * OB::kPlane], Bs1[3 * OB::kPlane];
 

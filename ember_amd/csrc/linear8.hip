@@ -50,7 +50,7 @@ __device__ __forceinline__ unsigned load4(__amdgpu_buffer_rsrc_t rsrc, unsigned 
 }
 
 // Few rows: bound by w's bytes.  A workgroup has 16*MB columns of out (a gated
-// layer: of the gate, and the same of the other projection) and 16*NT rows.  Its 8
+// layer: of the gate, and the same of the other projection) and 16*NT rows.  Its W
 // waves share k, each a run of groups, read straight from memory into registers up
 // to three groups ahead, and add their sums in wave order.  a comes out of the L2
 // once for each workgroup, so columns are many where there are enough of them to
@@ -676,7 +676,7 @@ constexpr int64_t kRowsPerLaunch = 1 << 20;
 Linear8Args rows_from(const Linear8Args &g, int64_t row)
 {
     Linear8Args p = g;
-    p.n = (int)std::min<int64_t>(g.n - row, kRowsPerLaunch);
+    p.n = p.a.rows = p.h.rows = (int)std::min<int64_t>(g.n - row, kRowsPerLaunch);
     p.a.codes += row * g.a.pitch();
     p.a.scales += row * g.a.scale_pitch;
     if (p.out) p.out += row * g.m;

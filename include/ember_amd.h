@@ -510,7 +510,7 @@ int rmsnorm_fwd8(const float *x, const float *residual, const float *gamma, floa
  * layer's weight written with trans), both in 8 bits; bias (m) and residual (n x
  * m) may be NULL, act as in linear_fwd.  Codes and scales enter exactly, products
  * are exact and added in fp32.  A NaN reaches every element that it is a term of.
- * out may be residual. */
+ * out may be residual, and overlaps no other input.  Uses library scratch. */
 int linear8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, const float *residual, float *out,
                 int act);
 
@@ -518,7 +518,7 @@ int linear8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, c
  * [wg | wu] (d x 2 hidden), bias = [bg | bu] or NULL, act 1 = Ember's GELU, 2 =
  * SiLU, g / (1 + exp(-g)).  pre (n x 2 hidden), where not NULL, gets both sums,
  * [x wg + bg | x wu + bu], for the backward.  hidden and d from 1, hidden below
- * 2^29.  Uses library scratch. */
+ * 2^29.  h and pre overlap no input.  Uses library scratch. */
 int gated_fwd(const float *x, const float *w, const float *bias, float *h, float *pre, int n, int hidden, int d,
               int act);
 /* The gradient with respect to pre of what follows a gated layer, y = h w_down:

@@ -162,6 +162,24 @@ def test_whole_backward_against_differences():
             assert abs(got[i] - want) <= 2e-5 * (1 + abs(want)), (name, i)
 
 
+@pytest.mark.parametrize("n,hidden,d", [(5, 12, 8), (70, 200, 36), (300, 260, 2052)])
+def test_unaligned(n, hidden, d):
+    """Everything 4 bytes off what allocations are aligned to."""
+    x, w, b, w_down, dy = inputs(n, hidden, d)
+    h, pre = forward(x, w, b, "silu")
+    dpre = backward(dy, w_down, pre, "silu")
+    off = {k: DeviceArray.from_numpy(np.concatenate(([7.0], v.reshape(-1)))) for k, v in
+           dict(x=x, w=w, b=b, w_down=w_down, dy=dy, h=np.zeros_like(h), pre=np.zeros_like(pre), dpre=np.zeros_like(pre)).items()}
+    p = {k: v.ptr + 4 for k, v in off.items()}
+    G.say(f"gated_fwd, gated_bwd unaligned n={n} hidden={hidden} d={d}")
+    capi.check(capi.lib().gated_fwd(p["x"], p["w"], p["b"], p["h"], p["pre"], n, hidden, d, 2), "gated_fwd")
+    capi.check(capi.lib().gated_bwd(p["dy"], p["w_down"], p["pre"], p["dpre"], n, hidden, d, 2), "gated_bwd")
+    for k, want in (("h", h), ("pre", pre), ("dpre", dpre)):
+        got = off[k].numpy()
+        assert got[0] == 7
+        np.testing.assert_array_equal(got[1:].reshape(want.shape), want)
+
+
 def test_no_rows():
     p = DeviceArray((64,)).ptr
     capi.check(capi.lib().gated_fwd(p, p, None, p, None, 0, 4, 4, 1), "gated_fwd")

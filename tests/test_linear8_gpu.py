@@ -82,6 +82,23 @@ def test_all_codes_and_scales(n):
     check_product(linear8(a, w), *product(a, w), 512)
 
 
+@pytest.mark.parametrize("n", [2, 40, 150])
+def test_smallest_and_largest_scales(n):
+    """Values down to 2^-128, below fp32's smallest normal number, times ones near
+    its largest, and the other way round."""
+    rng = np.random.default_rng(n + 7)
+    codes = lambda r: rng.integers(0, 127, (r, 256)).astype(np.uint8)  # noqa: E731
+    low = lambda r: rng.integers(8, 11, (r, 4)).astype(np.uint8)  # noqa: E731
+    high = lambda r: rng.integers(240, 246, (r, 4)).astype(np.uint8)  # noqa: E731
+    for x, y in ((low, high), (high, low)):
+        a, w = Rows8(n, 256, codes=codes(n), scales=x(n)), Rows8(70, 256, codes=codes(70), scales=y(70))
+        check_product(linear8(a, w), *product(a, w), 256)
+    # The smallest codes alone: 2^-9 of the smallest scale.
+    one, ones = np.ones((n, 128), np.uint8), np.full((33, 128), 0x38, np.uint8)  # 2^-9 and 1
+    a, w = Rows8(n, 128, codes=one, scales=np.full((n, 4), 8, np.uint8)), Rows8(33, 128, codes=ones, scales=np.full((33, 4), 246, np.uint8))
+    np.testing.assert_array_equal(linear8(a, w), 128 * 2.0 ** -9)
+
+
 @pytest.mark.parametrize("n", [4, 50, 260])
 def test_nan_reaches_its_row_and_column_only(n):
     a, w, _ = operands(n, 40, 300)
