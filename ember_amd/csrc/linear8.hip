@@ -588,7 +588,8 @@ void launch_few_as(Linear8Args g)
 
 // Two waves to a workgroup, so that several share a CU and none waits for the last;
 // four where a long k is all that there is to share out (1 x 16384 x 4096: 13.9 us,
-// with two 20.3).
+// with two 20.3), and for 64 columns, of which a CU has one workgroup (37 x 4096 x
+// 16384: 18.3 and 19.1, 16 x 8192 x 16384: 27.6 and 35.8).
 template <int NT, bool GATED>
 void launch_few_rows(const Linear8Args &g)
 {
@@ -597,7 +598,7 @@ void launch_few_rows(const Linear8Args &g)
         if (NT > 2 && mb == 2) launch_few_as<NT, (NT > 2 ? 2 : 1), 2, true>(g);
         else launch_few_as<NT, 1, 2, true>(g);
     } else {
-        if (mb == 4) launch_few_as<NT, 4, 2, false>(g);
+        if (mb == 4) launch_few_as<NT, 4, 4, false>(g);
         else if (mb == 2) launch_few_as<NT, 2, 2, false>(g);
         else if (NT == 1 && g.m <= 4096 && g.w.groups >= 32) launch_few_as<NT, 1, (NT == 1 ? 4 : 2), false>(g);
         else launch_few_as<NT, 1, 2, false>(g);
