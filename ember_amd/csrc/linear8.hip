@@ -229,12 +229,19 @@ __device__ __forceinline__ void meet()
 //     holds half the bytes, and a code is converted by the WC (WR) waves that read
 //     it.
 //   * Three quarters through a stage all of it is in registers: there is the
-//     barrier, behind which the next stage's operands are read beside the last
-//     quarter's products and its buffer's next stage is requested.  There are no
-//     branches: past the last stage requests read nothing, and what is read of them
+//     barrier, behind which the next stage's first operands are read and its
+//     buffer's next stage is requested, a copy at a time between products.  There are
+//     no branches: past the last stage requests read nothing, and what is read of them
 //     is not used.
+//   * A product occupies the matrix cores for 32 cycles and a conversion the vector
+//     unit for 4: each product is followed by three conversions for later ones, in this
+//     order in the code (all conversions of a quarter before its products: 8192 x
+//     8192 x 8192 798 us, in turn 772, copies too 761, the four stages that share a
+//     load of scales in a row 748).  Then power bounds it: at 4096 x 4096 x 16384
+//     1.90 GHz with 68 % of cycles busy, before 1.94 GHz and 65 %; four waves of 128 x
+//     128 convert and read a third less and reach the same there.
 template <int TM, int TN, int WR, int WC, int NBUF, bool GATED>
-__global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && NBUF == 2 ? 2 : 1) void linear8_tiles(Linear8Args g)
+__global__ __launch_bounds__(64 * WR * WC, TM * TN == 128 * 128 && NBUF == 2 ? 2 : 1) void linear8_tiles(Linear8Args g)
 {
     constexpr int NW = WR * WC, RB = TM / WR / 32, CB = TN / WC / 32, CBH = CB / 2;
     constexpr int CA = TM / 8 / NW, CW = TN / 8 / NW;  // copies of 8 rows to a wave
@@ -275,12 +282,15 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && NBUF == 2 ? 2 : 1) vo
         const int r = (c * NW + w) * 8 + lane / 8;
         woff[c] = (unsigned)min(r % COLS, g.m - 1 - col0) * (unsigned)pitch + 16 * (lane % 8 ^ r / 2 % 8);
     }
-    auto request = [&](int s, u32x4 *as, u32x4 *bs) {
+    // Copies `from` to `to` (of CA + CW) of stage s.
+    auto request = [&](int s, u32x4 *as, u32x4 *bs, int from, int to) {
         const unsigned at = s < stages ? (unsigned)s * kGroup8 : kPastAll;
 #pragma unroll
-        for (int c = 0; c < CA; ++c) dma16_at(ra, aoff[c], at, as + (c * NW + w) * 64);
-#pragma unroll
-        for (int c = 0; c < CW; ++c) dma16_at(c < CW / 2 ? rw : ru, woff[c], at, bs + (c * NW + w) * 64);
+        for (int c = from; c < to; ++c)
+            if (c < CA)
+                dma16_at(ra, aoff[c], at, as + (c * NW + w) * 64);
+            else
+                dma16_at(c - CA < CW / 2 ? rw : ru, woff[c - CA], at, bs + ((c - CA) * NW + w) * 64);
     };
 
     // This lane's rows of both tiles, 32 apart, and their scales.
@@ -314,89 +324,107 @@ __global__ __launch_bounds__(64 * WR * WC, WR * WC == 4 && NBUF == 2 ? 2 : 1) vo
         for (int cb = 0; cb < CB; ++cb) acc[rb][cb] = zero16();
 
     // Quarter j of a stage is 32 k: a lane reads unit 2j + half of its rows, of
-    // which either 8 codes go to one instruction.
-    u32x4 fa[2][RB], fb[2][CB];
-    const int at0 = half ^ (l32 >> 1 & 7);
-    auto read = [&](const u32x4 *as, const u32x4 *bs, int j, u32x4 (&a)[RB], u32x4 (&b)[CB]) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) a[rb] = as[8 * (arow + 32 * rb) + (at0 ^ 2 * j)];
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) b[cb] = bs[8 * brow(cb) + (at0 ^ 2 * j)];
-    };
+    // which either 8 codes (t = 0, 1) go to one instruction.  Products and conversions
+    // are issued in turn: beside a product run the conversions of the operands of the
+    // next one (of w) and of the next t (of a).  What a conversion has read is
+    // requested for the next quarter at once.
+    u32x4 fa[2][RB], fb[CB], x[2][RB], y[2];
     float fsa[RB], fsw[CB];
-    auto multiply = [&](const u32x4 (&a)[RB], const u32x4 (&b)[CB]) {
+    const int at0 = half ^ (l32 >> 1 & 7);
+    auto read_a = [&](const u32x4 *as, int j, u32x4 (&to)[RB]) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            u32x4 x[RB];
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) x[rb] = bf16_of8(a[rb][2 * t], a[rb][2 * t + 1], fsa[rb]);
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                const u32x4 y = bf16_of8(b[cb][2 * t], b[cb][2 * t + 1], fsw[cb]);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) acc[rb][cb] = mfma_32x32x16(x[rb], y, acc[rb][cb]);
-            }
-        }
+        for (int rb = 0; rb < RB; ++rb) to[rb] = as[8 * (arow + 32 * rb) + (at0 ^ 2 * j)];
     };
-    // Stage s in as, bs, the next one in an, bn; with NBUF > 2, s % 4 is U.
+    auto read_b = [&](const u32x4 *bs, int j, int cb) { fb[cb] = bs[8 * brow(cb) + (at0 ^ 2 * j)]; };
+    auto scales_a = [&](int shift) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) fsa[rb] = scale8(xa[rb] >> shift & 255);
+    };
+    auto scales_w = [&](int shift) {
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) fsw[cb] = scale8(xw[cb] >> shift & 255);
+    };
+    // Stage s, s % 4 = U, in as, bs, the next one in an, bn.  Its first operands and its
+    // scales are there already, and it leaves the next one's.
     auto stage = [&](auto unrolled, int s, u32x4 *as, u32x4 *bs, u32x4 *an, u32x4 *bn) {
         constexpr int U = decltype(unrolled)::value;
         if (AHEAD && U == 0) load_scales(min(s + 4, stages - 1) & ~3, na, nw);
-        const int shift = AHEAD ? 8 * U : 8 * (s % 4);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) fsa[rb] = scale8(xa[rb] >> shift & 255);
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) fsw[cb] = scale8(xw[cb] >> shift & 255);
         if (AHEAD && U == 3) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) xa[rb] = na[rb];
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) xw[cb] = nw[cb];
         }
-        if (!AHEAD && s % 4 == 3) load_scales(min(s + 1, stages - 1) & ~3, xa, xw);
+        if (!AHEAD && U == 3) load_scales(min(s + 1, stages - 1) & ~3, xa, xw);
+        const int shift = 8 * ((U + 1) % 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (j < 3) {
-                read(as, bs, j + 1, fa[(j + 1) & 1], fb[(j + 1) & 1]);
-            } else {
+            const u32x4 *const ar = j < 3 ? as : an, *const br = j < 3 ? bs : bn;
+            const int next = (j + 1) % 4;
+            if (j == 3) {
                 wait_vmem_n<(NBUF - 2) * (CA + CW)>();  // this wave's copies of the next stage, not those of later ones
                 meet();
-                request(s + NBUF, as, bs);
-                read(an, bn, 0, fa[0], fb[0]);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(fa[j & 1], fb[j & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+            read_a(ar, next, fa[next & 1]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (j == 3 && t == 1) scales_a(shift);
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+                    if (j == 3 && t == 1 && cb == CB - 1) scales_w(shift);
+                    const int u = t * CB + cb, ncb = (cb + 1) % CB, nt = cb + 1 == CB ? t ^ 1 : t;
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        acc[rb][cb] = mfma_32x32x16(x[t][rb], y[u & 1], acc[rb][cb]);
+#pragma unroll
+                        for (int i = 4 * rb / RB; i < 4 * (rb + 1) / RB; ++i)
+                            y[(u + 1) & 1][i] = bf16_pair8(fb[ncb][2 * nt], fb[ncb][2 * nt + 1], i, fsw[ncb]);
+                        constexpr int SLOTS = 2 * CB * RB;
+                        if (j == 3) request(s + NBUF, as, bs, (u * RB + rb) * (CA + CW) / SLOTS, (u * RB + rb + 1) * (CA + CW) / SLOTS);
+                        const auto &a = fa[(t ? next : j) & 1];
+#pragma unroll
+                        for (int q = (cb * RB + rb) * 4 / CB; q < (cb * RB + rb + 1) * 4 / CB; ++q)
+                            x[t ^ 1][q / 4][q % 4] = bf16_pair8(a[q / 4][2 * (t ^ 1)], a[q / 4][2 * (t ^ 1) + 1], q % 4, fsa[q / 4]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (nt == 1) read_b(br, next, ncb);
+                }
+            }
         }
     };
     load_scales(0, xa, xw);
-    request(0, A0, B0);
-    request(1, A1, B1);
+    request(0, A0, B0, 0, CA + CW);
+    request(1, A1, B1, 0, CA + CW);
     if constexpr (AHEAD) {
-        request(2, A2, B2);
-        request(3, A3, B3);
+        request(2, A2, B2, 0, CA + CW);
+        request(3, A3, B3, 0, CA + CW);
     }
     wait_vmem_n<(NBUF - 1) * (CA + CW)>();
     meet();
-    read(A0, B0, 0, fa[0], fb[0]);
+    read_a(A0, 0, fa[0]);
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) read_b(B0, 0, cb);
+    scales_a(0);
+    scales_w(0);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) x[0][rb] = bf16_of8(fa[0][rb][0], fa[0][rb][1], fsa[rb]);
+    y[0] = bf16_of8(fb[0][0], fb[0][1], fsw[0]);
     std::integral_constant<int, 0> u0;
     std::integral_constant<int, 1> u1;
     std::integral_constant<int, 2> u2;
     std::integral_constant<int, 3> u3;
     int s = 0;
-    for (; s + NBUF <= stages; s += NBUF) {
+    constexpr bool FOUR = NBUF > 2;
+    for (; s + 4 <= stages; s += 4) {
         stage(u0, s, A0, B0, A1, B1);
-        if constexpr (NBUF == 2) {
-            stage(u1, s + 1, A1, B1, A0, B0);
-        } else {
-            stage(u1, s + 1, A1, B1, A2, B2);
-            stage(u2, s + 2, A2, B2, A3, B3);
-            stage(u3, s + 3, A3, B3, A0, B0);
-        }
+        stage(u1, s + 1, A1, B1, FOUR ? A2 : A0, FOUR ? B2 : B0);
+        stage(u2, s + 2, FOUR ? A2 : A0, FOUR ? B2 : B0, FOUR ? A3 : A1, FOUR ? B3 : B1);
+        stage(u3, s + 3, FOUR ? A3 : A1, FOUR ? B3 : B1, A0, B0);
     }
     if (s < stages) stage(u0, s, A0, B0, A1, B1);
-    if (NBUF > 2 && s + 1 < stages) stage(u1, s + 1, A1, B1, A2, B2);
-    if (NBUF > 2 && s + 2 < stages) stage(u2, s + 2, A2, B2, A3, B3);
+    if (s + 1 < stages) stage(u1, s + 1, A1, B1, FOUR ? A2 : A0, FOUR ? B2 : B0);
+    if (s + 2 < stages) stage(u2, s + 2, FOUR ? A2 : A0, FOUR ? B2 : B0, FOUR ? A3 : A1, FOUR ? B3 : B1);
 
     // The sums go through LDS, 32 rows of the waves that share rows at a time (each
     // such set has a buffer), and leave in rows: a loop of few instructions, where
