@@ -16,15 +16,17 @@
  * Python GIL), the library expects one host thread in it at a time per
  * device: operators that use library scratch (attention_bwd's row
  * statistics, split-K and reduction partials, the pieces of kv_cache_attention
- * and token_logprobs, a gated layer's sums) share one buffer per device and operator, and two threads'
- * launches may interleave on the null stream.  The allocator and the error slots are thread-safe.
+ * and token_logprobs, a gated layer's sums) share one buffer per device and
+ * operator, and two threads' launches may interleave on the null stream.  The
+ * allocator and the error slots are thread-safe.
  *
  * Error behaviour.  The reference prints and calls exit() on any device
  * error (src/core/utils_gpu.cuh:13-19).  Here the void entry points keep
  * their signatures but record the first error in a sticky per-thread slot
  * (ember_get_last_error) and print it to stderr; the process is not killed.
  * The entry points that are new (attention, the key/value cache, token log
- * probabilities, 8-bit matrices, gated layers and the fused training operators) return that status directly.
+ * probabilities, RMS norm, 8-bit matrices, gated layers and the fused training
+ * operators) return that status directly.
  * Argument errors never launch a kernel.
  */
 #ifndef EMBER_AMD_H
