@@ -491,7 +491,8 @@ int rmsnorm_bwd(const float *s, const float *gamma, const float *rstd, const flo
  * (rows, ceil(cols/512)*4) bytes, 127 behind a row's last group: device memory of
  * the caller's, 16-byte aligned.  The entry points that write a matrix write these
  * too, and those that read one count on them.  At most 2^26 rows; cols from 1 to
- * 2^23.  The struct itself is host memory, read during the call only. */
+ * 2^23.  The struct itself is host memory, read during the call only.  What a call
+ * writes overlaps nothing that it reads, but where its comment allows it. */
 typedef struct ember_rows8 {
     void *codes, *scales;
     int64_t rows, cols;

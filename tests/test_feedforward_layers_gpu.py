@@ -3,12 +3,12 @@ decoding with and without matrices in 8 bits, against float64."""
 
 import numpy as np
 import pytest
-import torch
 
 import ember_amd as em
 import gpu_helpers as G
 from ember_amd import _core, capi, nn, optim
 from feedforward_helpers import ff
+from oracle import decoder
 from test_serving_gpu import cached_attention
 from tolerance import assert_north_star
 
@@ -19,16 +19,8 @@ def normal(rng, *shape):
     return rng.standard_normal(shape).astype(np.float32)
 
 
-def wide(t, grad=True):
-    return torch.tensor(t.to_np().astype(np.float64), requires_grad=grad)
-
-
-def act64(name, x):
-    return 0.5 * x * (1 + torch.tanh(0.8 * x)) if name == "gelu" else x * torch.sigmoid(x)
-
-
-def rms64(x, gamma, eps):
-    return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + eps) * gamma
+def wide(t):
+    return t.to_np().astype(np.float64)
 
 
 def test_quantize8_round_trip():
@@ -60,22 +52,23 @@ def test_functions_of_8_bit_matrices():
 @pytest.mark.parametrize("shape", [(5, 64), (2, 9, 1028)])
 def test_rms_norm_layer(shape):
     rng = np.random.default_rng(2)
+    d = shape[-1]
     x, r, g, past = (normal(rng, *shape) for _ in range(4))
-    layer = nn.RMSNorm(shape[-1])
-    layer.gamma = em.Tensor(normal(rng, shape[-1]))
+    layer = nn.RMSNorm(d)
+    layer.gamma = em.Tensor(normal(rng, d))
     y = layer.forward(em.Tensor(x), residual=em.Tensor(r))
     np.testing.assert_array_equal(layer.sum.to_np(), x + r)
-    s, gamma = wide(layer.sum), wide(layer.gamma)
-    ref = rms64(s, gamma, layer.eps)
-    (ref * torch.tensor(g.astype(np.float64))).sum().backward()
+    gamma, rows = layer.gamma.to_np(), lambda a: a.reshape(-1, d)
+    ref, rstd = ff.rmsnorm_fwd(rows(x + r), gamma, layer.eps)
+    ref_dx, ref_dgamma = ff.rmsnorm_bwd(rows(x + r), gamma, rstd, rows(g), rows(past))
     dx = layer.backward(em.Tensor(g), em.Tensor(past))
-    assert_north_star(y.to_np(), ref.detach().numpy())
-    assert_north_star(dx.to_np(), s.grad.numpy() + past)
-    assert_north_star(layer.gradients()[0].to_np(), gamma.grad.numpy())
-    plain = layer(em.Tensor(x))
-    assert_north_star(plain.to_np(), rms64(torch.tensor(x.astype(np.float64)), gamma.detach(), layer.eps).numpy())
+    assert y.shape == dx.shape == shape
+    assert_north_star(rows(y.to_np()), ref)
+    assert_north_star(rows(dx.to_np()), ref_dx)
+    assert_north_star(layer.gradients()[0].to_np(), ref_dgamma)
+    assert_north_star(rows(layer(em.Tensor(x)).to_np()), ff.rmsnorm_fwd(rows(x), gamma, layer.eps)[0])
     with pytest.raises(ValueError):
-        layer(em.Tensor(normal(rng, 2, shape[-1] + 4)))
+        layer(em.Tensor(normal(rng, 2, d + 4)))
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
@@ -90,37 +83,48 @@ def test_gated_feed_forward(n, d, hidden, bias, activation):
     x, g = em.Tensor(normal(rng, n, d)), em.Tensor(normal(rng, n, d))
     y = layer(x)
     dx = layer.backward(g)
-    at = [wide(t) for t in [x, *layer.parameters()]]
-    w_in, w_out = at[1], at[3 if bias else 2]
-    pre = at[0] @ w_in + (at[2] if bias else 0)
-    ref = act64(activation, pre[:, :hidden]) * pre[:, hidden:] @ w_out + (at[4] if bias else 0)
-    (ref * torch.tensor(g.to_np().astype(np.float64))).sum().backward()
-    assert_north_star(y.to_np(), ref.detach().numpy())
-    for i, (got, t) in enumerate(zip([dx, *layer.gradients()], at)):
-        assert_north_star(got.to_np(), t.grad.numpy(), f"gradient {i}")
+    at = [wide(p) for p in layer.parameters()]
+    w_in, b_in, w_out, b_out = at if bias else (at[0], 0, at[1], 0)
+    x64, g64 = wide(x), wide(g)
+    pre = x64 @ w_in + b_in
+    h = ff.gate(activation, pre)
+    dpre = ff.gate_bwd(activation, g64 @ w_out.T, pre)
+    assert_north_star(y.to_np(), h @ w_out + b_out)
+    grads = [x64.T @ dpre, dpre.sum(0), h.T @ g64, g64.sum(0)]
+    for i, (got, want) in enumerate(zip([dx, *layer.gradients()], [dpre @ w_in.T, *(grads if bias else grads[::2])])):
+        assert_north_star(got.to_np(), want, f"gradient {i}")
     np.testing.assert_array_equal(layer(x, training=False).to_np(), y.to_np())
 
 
-def block64(block, x, B, S):
-    """The block in float64 on torch, and its leaves: x and the parameters."""
-    leaves = [wide(x), *(wide(p) for p in block.parameters())]
-    x64, rest = leaves[0], list(leaves[1:])
-    take = lambda: rest.pop(0)  # noqa: E731
+def block64(block, x, dy, B, S):
+    """The block in float64: y, and the gradients of x and of the parameters."""
+    rest = [wide(p) for p in block.parameters()]
+    x, dy = wide(x), wide(dy)
 
     def norm(t):
-        gamma = take()
+        gamma = rest.pop(0)
         if block.norm == "rms":
-            return rms64(t, gamma, 1e-5)
-        return torch.nn.functional.layer_norm(t, (block.d,), gamma, take(), 1e-5)
-    qkv = (norm(x64) @ take() + take()).reshape(B, S, 3, block.h, -1).permute(2, 0, 3, 1, 4)
-    scores = qkv[0] @ qkv[1].transpose(-1, -2) / np.sqrt(block.d // block.h)
-    if block.causal:
-        scores = scores.masked_fill(torch.ones(S, S).triu(1).bool(), -np.inf)
-    o = (torch.softmax(scores, -1) @ qkv[2]).permute(0, 2, 1, 3).reshape(B * S, block.d)
-    x2 = x64 + o @ take() + take()
-    u = norm(x2) @ take() + take()
-    h = act64(block.gated, u[:, :block.hidden]) * u[:, block.hidden:] if block.gated else act64("gelu", u)
-    return x2 + h @ take() + take(), leaves
+            y, rstd = ff.rmsnorm_fwd(t, gamma, 1e-5)
+            return y, lambda g: ff.rmsnorm_bwd(t, gamma, rstd, g)
+        y, kept = decoder._ln(t, gamma, rest.pop(0))
+        return y, lambda g: decoder._ln_bwd(g, gamma, kept)
+    h1, back1 = norm(x)
+    w_qkv, b_qkv, w_o, b_o = rest[:4]
+    del rest[:4]
+    o, kept = decoder._attn(h1 @ w_qkv + b_qkv, B, S, block.h, block.causal)
+    x2 = x + o @ w_o + b_o
+    h2, back2 = norm(x2)
+    w_1, b_1, w_2, b_2 = rest
+    u = h2 @ w_1 + b_1
+    a = ff.gate(block.gated, u) if block.gated else ff.activate("gelu", u)[0]
+    da = dy @ w_2.T
+    du = ff.gate_bwd(block.gated, da, u) if block.gated else da * ff.activate("gelu", u)[1]
+    dh2, *norm2 = back2(du @ w_1.T)
+    dx2 = dy + dh2
+    dqkv = decoder._attn_bwd(dx2 @ w_o.T, kept, B, S, block.h)
+    dh1, *norm1 = back1(dqkv @ w_qkv.T)
+    return x2 + a @ w_2 + b_2, [dx2 + dh1, *norm1, h1.T @ dqkv, dqkv.sum(0), o.T @ dx2, dx2.sum(0),
+                                *norm2, h2.T @ du, du.sum(0), a.T @ dy, dy.sum(0)]
 
 
 @pytest.mark.parametrize("kind", [dict(norm="rms", gated="silu", hidden=171), dict(norm="rms", gated="gelu"), dict(norm="rms"), dict(gated="silu"), {}])
@@ -136,11 +140,11 @@ def test_decoder_block(kind, causal):
     G.say(f"decoder block {kind} causal={causal}")
     y = block(x, B, S)
     dx = block.backward(g)
-    ref, leaves = block64(block, x, B, S)
-    (ref * torch.tensor(g.to_np().astype(np.float64))).sum().backward()
-    assert_north_star(y.to_np(), ref.detach().numpy(), "y")
-    for i, (got, t) in enumerate(zip([dx, *block.gradients()], leaves)):
-        assert_north_star(got.to_np(), t.grad.numpy(), f"gradient {i}")
+    ref, grads = block64(block, x, g, B, S)
+    assert_north_star(y.to_np(), ref, "y")
+    assert len(grads) == 1 + len(block.gradients())
+    for i, (got, want) in enumerate(zip([dx, *block.gradients()], grads)):
+        assert_north_star(got.to_np(), want, f"gradient {i}")
 
 
 def test_training_steps():
@@ -161,19 +165,18 @@ def test_training_steps():
 
 def decode64(block, weights, x, start, count, cached, T):
     """decode in float64 with the given matrices, its attention over what the cache holds."""
-    val = lambda t: t.to_np().astype(np.float64)  # noqa: E731
     w_qkv, w_o, w_1, w_2 = weights
 
     def norm(x, n):
         if block.norm == "rms":
-            return x / np.sqrt((x * x).mean(-1, keepdims=True) + n.eps) * val(n.gamma)
-        return (x - x.mean(-1, keepdims=True)) / np.sqrt(x.var(-1, keepdims=True) + n.eps) * val(n.gamma) + val(n.beta)
+            return x / np.sqrt((x * x).mean(-1, keepdims=True) + n.eps) * wide(n.gamma)
+        return (x - x.mean(-1, keepdims=True)) / np.sqrt(x.var(-1, keepdims=True) + n.eps) * wide(n.gamma) + wide(n.beta)
     x = x.astype(np.float64)
-    qkv = (norm(x, block.ln1) @ w_qkv + val(block.b_qkv)).reshape(len(start), T, 3, block.h, block.d // block.h)
+    qkv = (norm(x, block.ln1) @ w_qkv + wide(block.b_qkv)).reshape(len(start), T, 3, block.h, block.d // block.h)
     o = cached_attention(qkv[:, :, 0], *cached, start, count).reshape(x.shape)
-    x2 = x + o @ w_o + val(block.b_o)
-    u = norm(x2, block.ln2) @ w_1 + val(block.b_1)
-    return x2 + (ff.gate(block.gated, u) if block.gated else ff.activate("gelu", u)[0]) @ w_2 + val(block.b_2)
+    x2 = x + o @ w_o + wide(block.b_o)
+    u = norm(x2, block.ln2) @ w_1 + wide(block.b_1)
+    return x2 + (ff.gate(block.gated, u) if block.gated else ff.activate("gelu", u)[0]) @ w_2 + wide(block.b_2)
 
 
 KINDS = [dict(norm="rms", gated="silu", hidden=200), dict(norm="rms", gated="gelu"), dict(gated="silu"), {}]
