@@ -647,12 +647,14 @@ bool launch_few(const Linear8Args &g)
 
 // What a call costs with each kernel, in us, fitted to measured times of 24 products
 // (65 x 4096 x 4096 to 8192 x 8192 x 8192) and 18 gated layers with every kernel and
-// 1 to 16 splits of k: the choice by it is within 5 % of the fastest for nearly all.
-// Few rows: a launch, and what a CU's workgroups read (13 bytes a cycle).  Tiles: a
-// launch, and for each round over the CUs the ends of a tile and its stages, whose
-// time is one workgroup's latency with the chip nearly empty and throughput with it
-// full; the sums' way to memory; and for sums that are added or gated in a launch of
-// their own, that and its bytes.
+// 1 to 16 splits of k, and of 56 and 66 with 1 to 128 rows and 2730 to 50000 columns:
+// the choice by it is within 9 % of the fastest for all of those, within 5 % for nearly
+// all.  Few rows: a launch, and what a CU's workgroups read (13 bytes a cycle); the
+// largest workgroups, of which a CU has one (a gated layer's: two), in whole rounds
+// with their ends.  Tiles: a launch, and for each round over the CUs the ends of a tile
+// and its stages, whose time is one workgroup's latency with the chip nearly empty and
+// throughput with it full; the sums' way to memory; and for sums that are added or
+// gated in a launch of their own, that and its bytes.
 enum Kernel { kFew, kSmallTiles, kMidTiles, kLargeTiles };
 struct Choice {
     Kernel kernel;
@@ -667,7 +669,11 @@ Choice choose(int64_t n, int64_t m, int groups, bool gated)
     Choice best = {kFew, 1, groups};
     const int nt = few_rows(n), mb = few_columns(n, m, gated);
     const double units = over(n, 16 * nt) * over(m, 16 * mb);
-    double least = 2.6 + std::max(1.0, units / 256) * groups * 0.0656 * (nt + (gated ? 2 : 1) * mb) + (gated ? 4 + moved : 0);
+    const int blocks = (gated ? 2 : 1) * mb;  // of 16 rows of w
+    double few_rounds = std::max(1.0, units / 256), few_ends = 0.07 * nt * blocks * blocks;
+    if (blocks == 4) few_rounds = gated ? 2 * over((int64_t)units, 512) : over((int64_t)units, 256);
+    if (blocks == 4 && gated) few_ends = 0.5;
+    double least = 2.2 + few_rounds * (few_ends + groups * 0.0656 * (nt + blocks)) + (gated ? 2.5 + moved : 0);
     const auto consider = [&](Kernel kernel, int splits, int chunk, double us) {
         if (us < least) least = us, best = {kernel, splits, chunk};
     };

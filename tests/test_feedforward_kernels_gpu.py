@@ -19,7 +19,7 @@ PRODUCTS = [
     ([AHEAD], 500, 4000, 896), ([AHEAD], 500, 4001, 1024), ([AHEAD], 512, 4000, 1100),
     ([AHEAD, REDUCE], 100, 40, 4089), ([AHEAD, REDUCE], 100, 41, 5120), ([AHEAD, REDUCE], 257, 3001, 2100), ([AHEAD, REDUCE], 257, 3000, 2432),
     ([TILES, REDUCE], 257, 3000, 3200), ([TILES, REDUCE], 300, 3001, 5100),
-    ([LARGE], 2049, 4100, 500), ([LARGE], 4000, 2049, 640), ([LARGE], 5000, 2001, 1000),
+    ([TILES], 128, 50000, 130), ([AHEAD], 64, 20001, 1000), ([LARGE], 2049, 4100, 500), ([LARGE], 4000, 2049, 640), ([LARGE], 5000, 2001, 1000),
 ]
 FEW = [(1, 40, 5000), (16, 48, 4096), (9, 4000, 4500), (5, 10201, 130), (9, 10200, 130), (16, 5101, 200), (20, 10200, 300), (32, 5100, 640), (33, 5100, 129),
        (48, 10201, 200), (64, 10200, 130), (50, 5101, 1000), (70, 900, 1300)]
@@ -46,7 +46,7 @@ def test_products(kernels, n, m, k):
 GATED = [
     (["gated8_tiles128"], 1000, 2001, 100), (["gated8_tiles128"], 640, 3000, 130), (["gated8_tiles128"], 1000, 2000, 384), (["gated8_tiles128"], 999, 2000, 1000),
     (["gated8_tiles256"], 1500, 3001, 128), (["gated8_tiles256"], 1025, 4000, 200), (["gated8_tiles256"], 2000, 2999, 640),
-    ([AHEAD, "gated8_reduce"], 130, 200, 2048), ([AHEAD, "gated8_reduce"], 65, 41, 3100), ([AHEAD, "gated8_reduce"], 257, 4000, 760),
+    ([AHEAD, "gated8_reduce"], 130, 200, 4096), (["gated8_few", "rows8_write"], 130, 200, 2048), ([AHEAD, "gated8_reduce"], 65, 41, 3100), ([AHEAD, "gated8_reduce"], 257, 4000, 760),
     ([TILES, "gated8_reduce"], 513, 2000, 2940), ([TILES, "gated8_reduce"], 257, 4001, 4096),
     *((["gated8_few", "rows8_write"], *s) for s in [(1, 500, 5000), (16, 130, 400), (20, 1000, 300), (40, 8200, 130), (64, 8300, 257), (33, 129, 1000)]),
 ]
