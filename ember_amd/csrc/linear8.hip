@@ -648,8 +648,8 @@ bool launch_few(const Linear8Args &g)
 // What a call costs with each kernel, in us, fitted to measured times of 24 products
 // (65 x 4096 x 4096 to 8192 x 8192 x 8192) and 18 gated layers with every kernel and
 // 1 to 16 splits of k, and of 56 and 66 with 1 to 128 rows and 2730 to 50000 columns:
-// the choice by it is within 9 % of the fastest for all of those, within 5 % for nearly
-// all.  Few rows: a launch, and what a CU's workgroups read (13 bytes a cycle); the
+// the choice by it is within 10 % of the fastest for those, within 5 % for nearly all;
+// over 69 others at random 0.9 % on average, 19 % at most.  Few rows: a launch, and what a CU's workgroups read (13 bytes a cycle); the
 // largest workgroups, of which a CU has one (a gated layer's: two), in whole rounds
 // with their ends.  Tiles: a launch, and for each round over the CUs the ends of a tile
 // and its stages, whose time is one workgroup's latency with the chip nearly empty and
