@@ -62,7 +62,7 @@ template <int NT, int MB, int W, bool GATED>
 __global__ __launch_bounds__(64 * W) void linear8_few(Linear8Args g)
 {
     constexpr int NB = GATED ? 2 : 1, WB = NB * MB;
-    constexpr int S = (WB + NT) * 32 <= 128 ? 4 : 2;  // groups in registers
+    constexpr int S = (WB + NT) * 32 <= 128 ? 4 : 2;  // groups in registers (37 x 4096 x 16384 with four: 20.2 us, with two 18.5)
     __shared__ f32x4 sums[W][WB][NT][64];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -136,6 +136,7 @@ def test_blocks(calls):
             nn.DecoderBlock(64, 2, **more)
     shapes = lambda **kw: [p.shape for p in nn.DecoderBlock(64, 2, **kw).parameters()]  # noqa: E731
     assert shapes() == [(64,), (64,), (64, 192), (192,), (64, 64), (64,), (64,), (64,), (64, 256), (256,), (256, 64), (64,)]
+    assert shapes(hidden=100)[8:] == [(64, 100), (100,), (100, 64), (64,)] and shapes(mlp_ratio=2)[8:] == [(64, 128), (128,), (128, 64), (64,)]
     assert shapes(norm="rms", gated="silu", hidden=100) == [(64,), (64, 192), (192,), (64, 64), (64,), (64,), (64, 200), (200,), (100, 64), (64,)]
     with pytest.raises(ValueError):
         nn.DecoderBlock(64, 2, causal=False).quantize8()

@@ -49,6 +49,28 @@ def test_functions_of_8_bit_matrices():
     np.testing.assert_array_equal(y.to_tensor().to_np(), 2)
 
 
+def test_binding_refuses_other_sizes():
+    t = _core._Tensor
+    a, w = (t(3 * 64), t(3), 3, 200), (t(5 * 64), t(5), 5, 200)  # 256 bytes of codes and 4 of scales a row
+    _core._linear8(a, w, None, None, 0)
+    bad = [
+        lambda: _core._rows8_read((t(3 * 64), t(2), 3, 200)), lambda: _core._rows8_read((t(3 * 50), t(3), 3, 200)),
+        lambda: _core._rows8_read((t(0), t(0), -1, 200)), lambda: _core._rows8_read((t(0), t(0), 0, 0)), lambda: _core._rows8_read((t(0), t(0), 0, 2 ** 24)),
+        lambda: _core._rows8_write(t(15), 4, 4, False), lambda: _core._rows8_write(t(16), 2 ** 27, 4, False),
+        lambda: _core._linear8(a, (t(5 * 32), t(5), 5, 100), None, None, 0), lambda: _core._linear8(a, w, t(3), None, 0),
+        lambda: _core._linear8(a, w, None, t(14), 0), lambda: _core._linear8(a, w, None, None, 2),
+        lambda: _core._gated8(a, w, None, 2), lambda: _core._gated8(a, (t(4 * 64), t(4), 4, 200), t(2), 2), lambda: _core._gated8(a, (t(4 * 64), t(4), 4, 200), None, 0),
+        lambda: _core._rmsnorm_fwd(t(8), t(4), t(4), 2, 4, 0.0), lambda: _core._rmsnorm_fwd(t(8), None, t(3), 2, 4, 0.0), lambda: _core._rmsnorm_fwd(t(8), None, t(4), 2, 4, -1.0),
+        lambda: _core._rmsnorm_fwd(t(6), None, t(3), 2, 3, 0.0), lambda: _core._rmsnorm_fwd8(t(8), t(9), t(4), 2, 4, 0.0), lambda: _core._rmsnorm_fwd8(t(7), None, t(4), 2, 4, 0.0),
+        lambda: _core._rmsnorm_bwd(t(8), t(4), t(1), t(8), None, 2, 4), lambda: _core._rmsnorm_bwd(t(8), t(4), t(2), t(8), t(4), 2, 4),
+        lambda: _core._gated_fwd(t(8), t(23), None, 2, 3, 4, 1, True), lambda: _core._gated_fwd(t(8), t(24), t(3), 2, 3, 4, 1, True), lambda: _core._gated_fwd(t(8), t(24), None, 2, 3, 4, 0, True),
+        lambda: _core._gated_bwd(t(8), t(12), t(6), 2, 3, 4, 1), lambda: _core._gated_bwd(t(8), t(12), t(12), 2, 3, 4, 3),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+
+
 @pytest.mark.parametrize("shape", [(5, 64), (2, 9, 1028)])
 def test_rms_norm_layer(shape):
     rng = np.random.default_rng(2)
