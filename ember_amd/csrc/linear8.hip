@@ -13,6 +13,7 @@
 #include "activation.h"
 #include "lds_dma.h"
 #include "linear8.h"
+#include "linear8_shape.h"
 #include "wave.h"
 
 namespace ember {
@@ -31,12 +32,10 @@ __device__ __forceinline__ void dma16_at(__amdgpu_buffer_rsrc_t rsrc, unsigned o
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lvoid *)to, 16, offset, at, 0, 0);
 }
 
-// An offset past all of a buffer: such a load gives 0 and reads nothing.
-constexpr unsigned kPastAll = 0x80000000u;
-// 2^31 bytes from p on, no fewer than a tile's rows have.
+// The buffer of a tile whose first row is at p (linear8_shape.h).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t bytes_from(const uint8_t *p)
 {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, (int)kPastAll, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, (int)kBufferBytes, 0x00020000);
 }
 
 // 16 (4) bytes from base + offset + at (the same in all lanes).
@@ -101,24 +100,26 @@ __global__ __launch_bounds__(64 * W) void linear8_few(Linear8Args g)
         u32x4 x[S][WB][2], y[S][NT][2];
         unsigned sx[WB], sy[NT], nx[WB], ny[NT];
         // No branches around the loads, so that they stay ahead of their use: past
-        // the run's end their offset is past the buffer's, and nothing is read.
+        // the run's end nothing is read.
         auto load = [&](int k, int i) {
-            const unsigned at = i < end ? i * kGroup8 : kPastAll;
+            const unsigned at = i * kGroup8;
+            const bool there = i < end;
 #pragma unroll
             for (int b = 0; b < WB; ++b)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) x[k][b][h] = load16(wc[b / MB], wo[b % MB], at + 64 * h);
+                for (int h = 0; h < 2; ++h) x[k][b][h] = load16(wc[b / MB], lane_offset(wo[b % MB], there) + 64 * h, at);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) y[k][t][h] = load16(ac, ao[t], at + 64 * h);
+                for (int h = 0; h < 2; ++h) y[k][t][h] = load16(ac, lane_offset(ao[t], there) + 64 * h, at);
         };
         auto load_scales = [&](int i) {
-            const unsigned at = i < end ? i & ~3 : kPastAll;
+            const unsigned at = i & ~3;
+            const bool there = i < end;
 #pragma unroll
-            for (int b = 0; b < WB; ++b) nx[b] = load4(ws[b / MB], wso[b % MB], at);
+            for (int b = 0; b < WB; ++b) nx[b] = load4(ws[b / MB], lane_offset(wso[b % MB], there), at);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) ny[t] = load4(as, aso[t], at);
+            for (int t = 0; t < NT; ++t) ny[t] = load4(as, lane_offset(aso[t], there), at);
         };
         load_scales(begin);
 #pragma unroll
@@ -284,13 +285,14 @@ __global__ __launch_bounds__(64 * WR * WC, TM * TN == 128 * 128 && NBUF == 2 ? 2
     }
     // Copies `from` to `to` (of CA + CW) of stage s.
     auto request = [&](int s, u32x4 *as, u32x4 *bs, int from, int to) {
-        const unsigned at = s < stages ? (unsigned)s * kGroup8 : kPastAll;
+        const unsigned at = (unsigned)s * kGroup8;
+        const bool there = s < stages;
 #pragma unroll
         for (int c = from; c < to; ++c)
             if (c < CA)
-                dma16_at(ra, aoff[c], at, as + (c * NW + w) * 64);
+                dma16_at(ra, lane_offset(aoff[c], there), at, as + (c * NW + w) * 64);
             else
-                dma16_at(c - CA < CW / 2 ? rw : ru, woff[c - CA], at, bs + ((c - CA) * NW + w) * 64);
+                dma16_at(c - CA < CW / 2 ? rw : ru, lane_offset(woff[c - CA], there), at, bs + ((c - CA) * NW + w) * 64);
     };
 
     // This lane's rows of both tiles, 32 apart, and their scales.
