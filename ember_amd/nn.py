@@ -497,7 +497,48 @@ class GatedFeedForward(Layer):
         return input_grad(dpre, self.w_in)
 
 
-class DecoderBlock(Layer):
+class _Decoding:
+    """What decoding takes beside the products, for a block of ``d`` features and ``h``
+    heads whose norms are ``norm``."""
+
+    d: int
+    h: int
+    causal: bool
+    norm: str
+
+    def make_cache(self, sequences: int, tokens: int, page_size: int = 64, pages: int | None = None) -> KVCache:
+        """An empty cache for ``decode``: ``sequences`` of up to ``tokens`` tokens."""
+        return KVCache(sequences, self.h, self.d // self.h, tokens, page_size, pages)
+
+    def _new_tokens(self, x: Tensor, cache: KVCache) -> int:
+        """T of ``decode``'s arguments, which it checks."""
+        if not self.causal:
+            raise ValueError("decode() needs a causal block")
+        rows, d = _rows(x)
+        if (cache.heads, cache.head_dim) != (self.h, self.d // self.h):
+            raise ValueError(f"the cache has {cache.heads} heads of {cache.head_dim}, the block {self.h} of {self.d // self.h}")
+        if d != self.d or rows % cache.sequences:
+            raise ValueError(f"x must be ({cache.sequences} * T, {self.d}), got {x.shape}")
+        return rows // cache.sequences
+
+    def _normed(self, x: Tensor, norm: LayerNorm | RMSNorm) -> Tensor:
+        rows, d = _rows(x)
+        if self.norm == "rms":
+            y = C._rmsnorm_fwd(x._core, None, norm.gamma._core, rows, d, norm.eps)[0]
+        else:
+            y = C._layernorm_fwd(x._core, norm.gamma._core, norm.beta._core, rows, d, norm.eps)[0]
+        return Tensor._from_core(y, x.shape)
+
+    def _attend(self, qkv: Tensor, cache: KVCache, T: int, count: Sequence[int] | None) -> Tensor:
+        """Appends the keys and values of qkv (rows, 3 d) and attends to the cache."""
+        d, D = self.d, cache.head_dim
+        strides = (T * 3 * d, D, 3 * d)
+        cache._append(qkv._core, d, qkv._core, 2 * d, T, strides, count)
+        o, _ = cache._attend(qkv._core, 0, T, self.h, strides, True, float(1.0 / math.sqrt(D)))
+        return Tensor._from_core(o, (qkv.shape[0], d))
+
+
+class DecoderBlock(_Decoding, Layer):
     """One pre-norm transformer decoder block on (B*S, d) token rows:
         h = N1(x);  x2 = x + Attention(h Wqkv + bqkv) Wo + bo
         y = x2 + GELU(N2(x2) W1 + b1) W2 + b2
@@ -599,10 +640,6 @@ class DecoderBlock(Layer):
         self._grads = [*self.ln1.gradients(), g_wqkv, g_bqkv, g_wo, g_bo, *self.ln2.gradients(), g_w1, g_b1, g_w2, g_b2]
         return dx
 
-    def make_cache(self, sequences: int, tokens: int, page_size: int = 64, pages: int | None = None) -> KVCache:
-        """An empty cache for ``decode``: ``sequences`` of up to ``tokens`` tokens."""
-        return KVCache(sequences, self.h, self.d // self.h, tokens, page_size, pages)
-
     def decode(self, x: Tensor, cache: KVCache, count: Sequence[int] | None = None) -> Tensor:
         """The block on rows that follow what ``cache`` holds: x is (sequences *
         T, d), T new tokens of each sequence (``count[b]`` of them where given,
@@ -622,76 +659,59 @@ class DecoderBlock(Layer):
         y, _ = linear(a, self.w_2, self.b_2, residual=x2)
         return y
 
-    def _new_tokens(self, x: Tensor, cache: KVCache) -> int:
-        """T of ``decode``'s arguments, which it checks."""
-        if not self.causal:
-            raise ValueError("decode() needs a causal block")
-        rows, d = _rows(x)
-        if (cache.heads, cache.head_dim) != (self.h, self.d // self.h):
-            raise ValueError(f"the cache has {cache.heads} heads of {cache.head_dim}, the block {self.h} of {self.d // self.h}")
-        if d != self.d or rows % cache.sequences:
-            raise ValueError(f"x must be ({cache.sequences} * T, {self.d}), got {x.shape}")
-        return rows // cache.sequences
-
-    def _normed(self, x: Tensor, norm: LayerNorm | RMSNorm) -> Tensor:
-        rows, d = _rows(x)
-        if self.norm == "rms":
-            y = C._rmsnorm_fwd(x._core, None, norm.gamma._core, rows, d, norm.eps)[0]
-        else:
-            y = C._layernorm_fwd(x._core, norm.gamma._core, norm.beta._core, rows, d, norm.eps)[0]
-        return Tensor._from_core(y, x.shape)
-
-    def _attend(self, qkv: Tensor, cache: KVCache, T: int, count: Sequence[int] | None) -> Tensor:
-        """Appends the keys and values of qkv (rows, 3 d) and attends to the cache."""
-        d, D = self.d, cache.head_dim
-        strides = (T * 3 * d, D, 3 * d)
-        cache._append(qkv._core, d, qkv._core, 2 * d, T, strides, count)
-        o, _ = cache._attend(qkv._core, 0, T, self.h, strides, True, float(1.0 / math.sqrt(D)))
-        return Tensor._from_core(o, (qkv.shape[0], d))
-
     def quantize8(self) -> DecoderBlock8:
         """This causal block for decoding with its four matrices in 8 bits, as they are now."""
         return DecoderBlock8(self)
 
 
-class DecoderBlock8:
-    """A ``DecoderBlock`` for inference whose matrices are held in 8 bits, 33/32 byte
+def _copied(x: Tensor) -> Tensor:
+    """A copy: the sum over its one row."""
+    return Tensor._from_core(C._col_sum(x._core, 1, x.size), x.shape)
+
+
+def _copied_norm(norm: LayerNorm | RMSNorm) -> LayerNorm | RMSNorm:
+    new = type(norm)(norm.features, norm.eps)
+    new.gamma = _copied(norm.gamma)
+    if isinstance(norm, LayerNorm):
+        new.beta = _copied(norm.beta)
+    return new
+
+
+class DecoderBlock8(_Decoding):
+    """A ``DecoderBlock`` for inference whose matrices are held in 8 bits, 129/128 byte
     per element; what enters a product is rounded to 8 bits too, by the norm and the
     gate as they write it.  Norms, biases, attention and all sums stay float32.
-    ``block.quantize8()`` makes one: a copy of the block's weights at that time (its
-    norms' and biases' Tensors are shared)."""
+    ``block.quantize8()`` makes one: a copy of the block's weights at that time, which
+    needs the block no longer."""
 
     def __init__(self, block: DecoderBlock):
         if not block.causal:
             raise ValueError("decode() needs a causal block")
-        self.block = block
+        self.d, self.h, self.causal, self.norm, self.gated = block.d, block.h, block.causal, block.norm, block.gated
+        self.ln1, self.ln2 = _copied_norm(block.ln1), _copied_norm(block.ln2)
         self.w_qkv, self.w_o, self.w_1, self.w_2 = (quantize8(w, trans=True) for w in (block.w_qkv, block.w_o, block.w_1, block.w_2))
+        self.b_qkv, self.b_o, self.b_1, self.b_2 = (_copied(b) for b in (block.b_qkv, block.b_o, block.b_1, block.b_2))
 
     @property
     def nbytes(self) -> int:
         """Device memory of the matrices."""
         return sum(w.nbytes for w in (self.w_qkv, self.w_o, self.w_1, self.w_2))
 
-    def make_cache(self, sequences: int, tokens: int, page_size: int = 64, pages: int | None = None) -> KVCache:
-        """An empty cache for ``decode``: ``sequences`` of up to ``tokens`` tokens."""
-        return self.block.make_cache(sequences, tokens, page_size, pages)
-
-    def _normed(self, x: Tensor, norm: LayerNorm | RMSNorm):
-        if self.block.norm == "rms":
+    def _normed8(self, x: Tensor, norm: LayerNorm | RMSNorm):
+        if self.norm == "rms":
             return rms_norm8(x, norm.gamma, norm.eps)[0]
-        return quantize8(self.block._normed(x, norm))
+        return quantize8(self._normed(x, norm))
 
     def decode(self, x: Tensor, cache: KVCache, count: Sequence[int] | None = None) -> Tensor:
         """``DecoderBlock.decode`` with the matrices in 8 bits."""
-        b = self.block
-        T = b._new_tokens(x, cache)
+        T = self._new_tokens(x, cache)
         if T == 0:
             return _random.zeros(x.shape)
-        qkv = linear8(self._normed(x, b.ln1), self.w_qkv, b.b_qkv)
-        x2 = linear8(quantize8(b._attend(qkv, cache, T, count)), self.w_o, b.b_o, residual=x)
-        h2 = self._normed(x2, b.ln2)
-        if b.gated:
-            a = gated8(h2, self.w_1, b.b_1, b.gated)
+        qkv = linear8(self._normed8(x, self.ln1), self.w_qkv, self.b_qkv)
+        x2 = linear8(quantize8(self._attend(qkv, cache, T, count)), self.w_o, self.b_o, residual=x)
+        h2 = self._normed8(x2, self.ln2)
+        if self.gated:
+            a = gated8(h2, self.w_1, self.b_1, self.gated)
         else:
-            a = quantize8(linear8(h2, self.w_1, b.b_1, gelu=True))
-        return linear8(a, self.w_2, b.b_2, residual=x2)
+            a = quantize8(linear8(h2, self.w_1, self.b_1, gelu=True))
+        return linear8(a, self.w_2, self.b_2, residual=x2)

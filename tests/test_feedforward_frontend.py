@@ -144,6 +144,23 @@ def test_blocks(calls):
     assert (block.w_qkv.shape, block.w_o.shape, block.w_1.shape, block.w_2.shape) == ((192, 64), (64, 64), (512, 64), (64, 256))
 
 
+@pytest.mark.parametrize("kind", [dict(norm="rms", gated="gelu"), {}])
+def test_an_8_bit_block_needs_its_block_no_longer(calls, kind):
+    import gc
+    import weakref
+
+    block = nn.DecoderBlock(64, 2, **kind)
+    shapes = [p.shape for p in block.parameters()]
+    block8 = block.quantize8()
+    assert [p.shape for p in block.parameters()] == shapes
+    held = {id(t) for o in (block8, block8.ln1, block8.ln2) for t in vars(o).values() if isinstance(t, Tensor)}
+    assert held and not held & {id(t) for t in block.parameters()}
+    gone = weakref.ref(block)
+    del block
+    gc.collect()
+    assert gone() is None
+
+
 def test_binding_checks_its_arguments():
     for name, args in (("_rows8_write", (None, 1, 1, False)), ("_rows8_read", (None,)), ("_rows8_read", ((None, None, 1, 1),)),
                        ("_rmsnorm_fwd", (None, None, None, 1, 4, 0.0)), ("_rmsnorm_fwd8", (None, None, None, 1, 4, 0.0)),

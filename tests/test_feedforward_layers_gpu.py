@@ -273,6 +273,27 @@ def test_8_bit_block_keeps_its_weights():
     np.testing.assert_array_equal(block8.decode(x, block8.make_cache(3, 4)).to_np(), y)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_8_bit_block_keeps_all_of_its_weights(kind):
+    """Biases and norms too: trained on in place, set anew and reset, the block changes
+    and its block8 does not."""
+    block, rng = some_block(kind)
+    block8 = block.quantize8()
+    x = em.Tensor(normal(rng, 3, 128))
+    y = block8.decode(x, block8.make_cache(3, 4)).to_np()
+    before = block.decode(x, block.make_cache(3, 4)).to_np()
+    grads = [em.Tensor(np.full(p.shape, 0.5, np.float32)) for p in block.parameters()]
+    optim.SGD(block.parameters(), lr=1.0).apply(grads)
+    assert (block.decode(x, block.make_cache(3, 4)).to_np() != before).any()
+    np.testing.assert_array_equal(block8.decode(x, block8.make_cache(3, 4)).to_np(), y)
+    for p in block.parameters():
+        p._adopt(em.Tensor(np.full(p.shape, 3, np.float32)))
+    np.testing.assert_array_equal(block8.decode(x, block8.make_cache(3, 4)).to_np(), y)
+    block.reset()
+    block.norm, block.gated = "layer", None
+    np.testing.assert_array_equal(block8.decode(x, block8.make_cache(3, 4)).to_np(), y)
+
+
 def test_decode_leaves_training_alone():
     block, rng = some_block(KINDS[0], 64, 2)
     x, g = em.Tensor(normal(rng, 60, 64)), em.Tensor(normal(rng, 60, 64))
