@@ -13,7 +13,7 @@
 // The forward's sum and its products with rstd and gamma are formed in 64 bits
 // and y rounded once (the double rate is far above what the bytes need): the
 // rounding of y to 8 bits must not turn on the order of a sum.  The gradient is
-// formed in 32 bits.
+// formed in 32 bits, and dgamma's sum of many rows in 64.
 #include <math.h>
 
 #include <algorithm>
@@ -98,7 +98,11 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void rms_fwd_kernel(NormArgs 
     }
 }
 
-// dx of a run of rows, and their sum of dy*xhat, which goes to part[blockIdx.x].
+// dx of a run of rows, and their sum of dy*xhat, which goes to part[blockIdx.x].  Runs
+// grow with the rows: the sum is formed over kShort rows at a time in 32 bits, and over
+// those in 64, in LDS (in registers fewer workgroups would share a CU), so that its
+// error does not.
+constexpr int kShort = 32;
 template <int W>
 __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void rms_bwd_kernel(const float *__restrict__ s, const float *__restrict__ gamma,
                                                                        const float *__restrict__ rstd_in, const float *__restrict__ dy,
@@ -108,12 +112,26 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void rms_bwd_kernel(const flo
     constexpr int R = W < 4 ? 4 / W : 1;  // rows at a time
     __shared__ float red[2][W];
     const int t = threadIdx.x % (64 * W), which = threadIdx.x / (64 * W);
+    __shared__ double all[4 * kChunks][64 * W * R];
     f32x4 pg[kChunks];
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) pg[c] = f32x4{0, 0, 0, 0};
+    bool some = false;  // of this lane's sums are in `all`
+    const auto put_by = [&] {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                double &to = all[4 * c + j][threadIdx.x];
+                to = (some ? to : 0.0) + (double)pg[c][j];
+                pg[c][j] = 0;
+            }
+        some = true;
+    };
     const int64_t first = (int64_t)blockIdx.x * rows_per_block, end = min(first + rows_per_block, rows);
-    int turn = 0;
+    int turn = 0, summed = 0;
     for (int64_t row = first + which; row < end; row += R, turn ^= 1) {
+        if (summed++ == kShort) put_by(), summed = 1;
         const float rstd = rstd_in[row];
         f32x4 xh[kChunks], g[kChunks], more[kChunks];
         float m = 0;
@@ -140,6 +158,13 @@ __global__ __launch_bounds__(W < 4 ? 256 : 64 * W) void rms_bwd_kernel(const flo
             const int col = 4 * (64 * W * c + t);
             if (col < d) *(f32x4 *)(dx + row * d + col) = rstd * (g[c] - xh[c] * m) + more[c];
         }
+    }
+    if (some) {
+        put_by();
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pg[c][j] = (float)all[4 * c + j][threadIdx.x];
     }
     if (R > 1) {  // the waves' sums in their order
         __shared__ f32x4 sums[R][64];

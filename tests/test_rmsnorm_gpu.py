@@ -148,3 +148,19 @@ def test_no_rows():
     capi.check(L.rmsnorm_fwd8(p, None, gamma.ptr, None, y.view, 1e-5), "rmsnorm_fwd8")
     capi.check(L.rmsnorm_bwd(p, gamma.ptr, p, p, None, p, dg.ptr, 0, 8), "rmsnorm_bwd")
     assert (dg.numpy() == 0).all()
+
+
+@pytest.mark.parametrize("rows,d,run", [((1 << 22) + 5, 4, 1024), ((1 << 19) + 3, 1028, 512), ((1 << 17) + 1, 4100, 512)])
+def test_gradient_of_gamma_of_many_rows(rows, d, run):
+    """The error of a column's sum does not grow with the rows.  All terms dy * xhat are
+    t = 1 + 0.45 of the last place of a sum of run / 2 to run, which is cut off whenever t
+    is added to one: run terms one by one would be off by run / 5 half steps.  At most 32
+    terms are summed in 32 bits, then rounded, the four waves' sums added, and 8, 15 and
+    7 sums of those: 66 half steps."""
+    t = np.float32(1 + 0.45 * run * 2.0 ** -24)
+    ones, rstd, gamma = arr(np.ones((rows, d), np.float32)), arr(np.full(rows, t, np.float32)), arr(np.ones(d, np.float32))
+    dx, dg = DeviceArray((rows, d)), DeviceArray.from_numpy(np.full(d, G.SENTINEL))
+    G.say(f"rmsnorm_bwd rows={rows} d={d}")
+    capi.check(capi.lib().rmsnorm_bwd(ones.ptr, gamma.ptr, rstd.ptr, ones.ptr, None, dx.ptr, dg.ptr, rows, d), "rmsnorm_bwd")
+    exact = rows * float(t)
+    assert (np.abs(dg.numpy() - exact) <= 66 * U * exact).all()
