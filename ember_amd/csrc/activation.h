@@ -18,11 +18,13 @@ __device__ __forceinline__ float gelu08(float x)
     return (x * 0.5f) * (tanhf(x * 0.8f) + 1.0f);
 }
 
-// 1 / (1 + e^-x), within two units in the last place; expf and a division take
+// 1 / (1 + e^-x), for x from -87 on within three units in the last place (half steps
+// of 2^-24: e^-x 2.7, the sum 1, its reciprocal 2); below, where it is under 2^-125, the
+// reciprocal gives 0 for what would not be a normal number.  expf and a division take
 // four times as many instructions, which a matrix product's epilogue shows (a gated
-// layer of 4096 x 4096 x 8192 in 8 bits: 432 us with them, 419 with this).  e^-x is 2^f * 2^n with n
-// whole and f = -x log2(e) - n, |f| <= 1/2, formed with log2(e) in two floats.  Past
-// +-150 the result is 1 or 0 anyway.
+// layer of 4096 x 4096 x 8192 in 8 bits: 432 us with them, 419 with this).  e^-x is 2^f *
+// 2^n with n whole and f = -x log2(e) - n, |f| <= 1/2, formed with log2(e) in two floats.
+// Past +-150 the result is 1 or 0 anyway.
 __device__ __forceinline__ float sigmoid(float x)
 {
     constexpr float kLog2e = 1.442695041f, kLog2eRest = 1.925963033e-8f;
@@ -33,8 +35,9 @@ __device__ __forceinline__ float sigmoid(float x)
 }
 
 // The activations of gated layers: x * sigmoid(c x), with c = 1 SiLU and with c =
-// 1.6 Ember's GELU, as (1 + tanh z) / 2 = sigmoid(2 z).  An x of -infinity gives NaN
-// and far ones below 0 -0, as the formulas do.
+// 1.6 Ember's GELU, as (1 + tanh z) / 2 = sigmoid(2 z); c x is rounded, which far below
+// 0 is 1.25 |c x| half steps of the result.  An x of -infinity gives NaN, as the formulas
+// do, and one with c x below -87 (a result of less than 2^-118) may give -0.
 constexpr float kSteepGelu = 1.6f, kSteepSilu = 1.0f;
 __device__ __forceinline__ float steepness(int act)
 {

@@ -519,9 +519,10 @@ int linear8_fwd(const ember_rows8 *a, const ember_rows8 *w, const float *bias, c
 
 /* A gated layer, h(n x hidden) = act(x wg + bg) * (x wu + bu): x (n x d), w =
  * [wg | wu] (d x 2 hidden), bias = [bg | bu] or NULL, act 1 = Ember's GELU, 2 =
- * SiLU, g / (1 + exp(-g)).  pre (n x 2 hidden), where not NULL, gets both sums,
- * [x wg + bg | x wu + bu], for the backward.  hidden and d from 1, hidden below
- * 2^29.  h and pre overlap no input.  Uses library scratch. */
+ * SiLU, g / (1 + exp(-g)); where act is under 2^-118 in size it may be 0.  pre
+ * (n x 2 hidden), where not NULL, gets both sums, [x wg + bg | x wu + bu], for the
+ * backward.  hidden and d from 1, hidden below 2^29.  h and pre overlap no input.
+ * Uses library scratch. */
 int gated_fwd(const float *x, const float *w, const float *bias, float *h, float *pre, int n, int hidden, int d,
               int act);
 /* The gradient with respect to pre of what follows a gated layer, y = h w_down:

@@ -184,3 +184,52 @@ def test_no_rows():
     p = DeviceArray((64,)).ptr
     capi.check(capi.lib().gated_fwd(p, p, None, p, None, 0, 4, 4, 1), "gated_fwd")
     capi.check(capi.lib().gated_bwd(p, p, p, p, 0, 4, 4, 1), "gated_bwd")
+
+
+def sweep(act):
+    """Gates of all sizes and signs, and the bounds of activation.h in half steps: of
+    sigmoid(c x) 5.7, and 1.25 |c x| (1 - sigmoid) where c x is rounded."""
+    c = dict(gelu=1.6, silu=1.0)[act]
+    rng = np.random.default_rng(11)
+    gate = np.concatenate((rng.uniform(-86 / c, 30, 30000), rng.uniform(-2, 2, 9000), -np.exp(rng.uniform(-60, 4, 3000)), np.linspace(-86 / c, 30, 5001),
+                           [0.0, 1e30, 3e38])).astype(np.float32)
+    x = gate.astype(np.float64)
+    small = np.exp(-np.abs(c * x))
+    s, rest = np.where(x >= 0, 1, small) / (1 + small), np.where(x >= 0, small, 1) / (1 + small)
+    off = (5.7 + (1.25 * np.abs(c * x) * rest if act == "gelu" else 0)) * U
+    return gate, c, x, s, rest, off
+
+
+@pytest.mark.parametrize("act", list(ACT))
+def test_the_gate_is_near_in_relative_terms(act):
+    """act(gate) * 1 within the sigmoid's bound and one rounding of itself, far below 0 too."""
+    gate, _, x, s, _, off = sweep(act)
+    h, pre = forward(gate[:, None], np.float32([[1, 0]]), np.float32([0, 1]), act)
+    np.testing.assert_array_equal(pre, np.stack((gate, np.ones_like(gate)), 1))
+    assert (np.abs(h[:, 0] - x * s) <= (off + 1.1 * U) * np.abs(x * s) + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("act", list(ACT))
+def test_the_gates_gradient_is_near(act):
+    """Both halves of dpre for dh = up = 1: the value as above; the slope is s + c (v (1 -
+    s)), where v = x s carries s's bound and a rounding, 1 - s what s is off by and a
+    rounding, and two products and c round; the sum once more."""
+    gate, c, x, s, rest, off = sweep(act)
+    one = np.ones((len(gate), 1), np.float32)
+    dpre = backward(one, np.ones((1, 1), np.float32), np.stack((gate, one[:, 0]), 1), act)
+    slope = s + c * x * s * rest
+    tol = off * s + c * np.abs(x) * s * ((off + 4.3 * U) * rest + off * s) + 1.1 * U * np.abs(slope)
+    assert (np.abs(dpre[:, 0] - slope) <= 1.001 * tol + 2.0 ** -148).all()
+    assert (np.abs(dpre[:, 1] - x * s) <= (off + 1.1 * U) * np.abs(x * s) + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("act", list(ACT))
+def test_gates_past_the_sigmoids_range(act):
+    """Between the result and 0 from c gate = -86 on down; -0 or NaN, never anything else."""
+    c = dict(gelu=1.6, silu=1.0)[act]
+    gate = -np.concatenate((np.linspace(86, 110, 4001), [120, 150, 200, 1e4, 1e30, 3e38])).astype(np.float32) / np.float32(c)
+    h, _ = forward(gate[:, None], np.float32([[1, 0]]), np.float32([0, 1]), act)
+    x = gate.astype(np.float64)
+    exact = x * np.exp(c * x)  # within 2^-124 of itself
+    assert (h[:, 0] <= 0).all() and (h[:, 0] >= exact * (1 + 300 * U) - 2.0 ** -148).all()
+    assert (exact[h[:, 0] == 0] > -(2.0 ** -118)).all()
