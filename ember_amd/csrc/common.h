@@ -53,5 +53,11 @@ bool deterministic();
 // Compute units of the current device (cached per device), or 0 if the HIP
 // runtime cannot say; records no error.
 int device_cu_count();
+// The same for choices among kernels alone: an unknown count falls back to MI355X's 256.
+inline int num_cus()
+{
+    const int n = device_cu_count();
+    return n > 0 ? n : 256;
+}
 
 }  // namespace ember

@@ -505,12 +505,5 @@ void launch_tiles(GemmArgs &g, int batch, int ksplit)
     }
 }
 
-// Tile-shape choice only: an unknown CU count falls back to MI355X's 256.
-int num_cus()
-{
-    const int n = device_cu_count();
-    return n > 0 ? n : 256;
-}
-
 }  // namespace
 }  // namespace ember

@@ -587,23 +587,8 @@ bool launch_tiles(const Linear8Args &g, int splits, const char *kernel)
 bool launch_small(const Linear8Args &g, int splits)
 {
     const int64_t tiles = (((int64_t)g.n + 127) / 128) * (((int64_t)g.m + 127) / 128);
-    return tiles * splits <= 256 ? launch_tiles<128, 128, 2, 2, 4, false>(g, splits, "linear8_tiles128_ahead")
+    return tiles * splits <= num_cus() ? launch_tiles<128, 128, 2, 2, 4, false>(g, splits, "linear8_tiles128_ahead")
                                  : launch_tiles<128, 128, 2, 2, 2, false>(g, splits, "linear8_tiles128");
-}
-
-// Rows of a few-rows workgroup, in sixteens.
-int few_rows(int64_t n)
-{
-    return n <= 16 ? 1 : n <= 32 ? 2 : n <= 48 ? 3 : 4;
-}
-// Its columns, in sixteens: each workgroup reads all of a's rows, so many where
-// those are, but not so many that CUs are left without one.  16 x 4096 x 16384: 64
-// columns 15.7 us, 16 19.4; 16 x 4096 x 4096: 14.4 and 7.1; 1 x 4096 x 16384: 14.6
-// and 14.0.  A gated layer's workgroup has twice as many rows of w.
-int few_columns(int64_t n, int64_t m, bool gated)
-{
-    if (gated) return n > 32 && m > 255 * 32 ? 2 : 1;
-    return n <= 8 ? 1 : m > 159 * 64 ? 4 : m > 159 * 32 ? 2 : 1;
 }
 
 template <int NT, int MB, int W, bool GATED>
@@ -616,21 +601,17 @@ void launch_few_as(Linear8Args g)
     hipLaunchKernelGGL((linear8_few<NT, MB, W, GATED>), grid, dim3(64 * W), 0, 0, g);
 }
 
-// Two waves to a workgroup, so that several share a CU and none waits for the last;
-// four where a long k is all that there is to share out (1 x 16384 x 4096: 13.9 us,
-// with two 20.3), and for 64 columns, of which a CU has one workgroup (37 x 4096 x
-// 16384: 18.3 and 19.1, 16 x 8192 x 16384: 27.6 and 35.8).
 template <int NT, bool GATED>
 void launch_few_rows(const Linear8Args &g)
 {
-    const int mb = few_columns(g.n, g.m, GATED);
+    const int cus = num_cus(), mb = few_columns(g.n, g.m, GATED, cus);
     if constexpr (GATED) {
         if (NT > 2 && mb == 2) launch_few_as<NT, (NT > 2 ? 2 : 1), 2, true>(g);
         else launch_few_as<NT, 1, 2, true>(g);
     } else {
         if (mb == 4) launch_few_as<NT, 4, 4, false>(g);
         else if (mb == 2) launch_few_as<NT, 2, 2, false>(g);
-        else if (NT == 1 && g.m <= 4096 && g.w.groups >= 32) launch_few_as<NT, 1, (NT == 1 ? 4 : 2), false>(g);
+        else if (NT == 1 && four_waves(g.m, g.w.groups, cus)) launch_few_as<NT, 1, (NT == 1 ? 4 : 2), false>(g);
         else launch_few_as<NT, 1, 2, false>(g);
     }
 }
@@ -645,59 +626,6 @@ bool launch_few(const Linear8Args &g)
         default: launch_few_rows<4, GATED>(g);
     }
     return launch_ok(GATED ? "gated8_few" : "linear8_few");
-}
-
-// What a call costs with each kernel, in us, fitted to measured times of 24 products
-// (65 x 4096 x 4096 to 8192 x 8192 x 8192) and 18 gated layers with every kernel and
-// 1 to 16 splits of k, and of 56 and 66 with 1 to 128 rows and 2730 to 50000 columns:
-// the choice by it is within 10 % of the fastest for those, within 5 % for nearly all;
-// over 69 others at random 0.9 % on average, 19 % at most.  Few rows: a launch, and what a CU's workgroups read (13 bytes a cycle); the
-// largest workgroups, of which a CU has one (a gated layer's: two), in whole rounds
-// with their ends.  Tiles: a launch, and for each round over the CUs the ends of a tile
-// and its stages, whose time is one workgroup's latency with the chip nearly empty and
-// throughput with it full; the sums' way to memory; and for sums that are added or
-// gated in a launch of their own, that and its bytes.
-enum Kernel { kFew, kSmallTiles, kMidTiles, kLargeTiles };
-struct Choice {
-    Kernel kernel;
-    int splits, chunk;
-};
-constexpr int kMostSplits = 16;
-
-Choice choose(int64_t n, int64_t m, int groups, bool gated)
-{
-    const auto over = [](int64_t a, int64_t b) { return (double)((a + b - 1) / b); };
-    const double moved = 4.0 * (gated ? 2 : 1) * n * m / 5e6;  // us to write the sums once
-    Choice best = {kFew, 1, groups};
-    const int nt = few_rows(n), mb = few_columns(n, m, gated);
-    const double units = over(n, 16 * nt) * over(m, 16 * mb);
-    const int blocks = (gated ? 2 : 1) * mb;  // of 16 rows of w
-    double few_rounds = std::max(1.0, units / 256), few_ends = 0.07 * nt * blocks * blocks;
-    if (blocks == 4) few_rounds = gated ? 2 * over((int64_t)units, 512) : over((int64_t)units, 256);
-    if (blocks == 4 && gated) few_ends = 0.5;
-    double least = 2.2 + few_rounds * (few_ends + groups * 0.0656 * (nt + blocks)) + (gated ? 2.5 + moved : 0);
-    const auto consider = [&](Kernel kernel, int splits, int chunk, double us) {
-        if (us < least) least = us, best = {kernel, splits, chunk};
-    };
-    const auto rounds = [&](double tiles, double ends, double empty, double full) {
-        return 3 + over((int64_t)tiles, 256) * (ends + groups * (empty + (full - empty) * std::min(1.0, tiles / 256)));
-    };
-    if (gated) {
-        consider(kLargeTiles, 1, groups, rounds(over(n, 256) * over(m, 128), 9, 2.25, 3.05));
-        consider(kMidTiles, 1, groups, rounds(over(n, 128) * over(m, 128), 8, 1.35, 1.7));
-    } else {
-        consider(kLargeTiles, 1, groups, rounds(over(n, 256) * over(m, 256), 6, 2.25, 2.95) + 0.5 * moved);
-    }
-    for (int want = 1; want <= kMostSplits; want *= 2) {
-        const int chunk = want == 1 ? groups : ((groups + want - 1) / want + 3) / 4 * 4, splits = (groups + chunk - 1) / chunk;
-        if (splits > 1 && splits * moved > 100) break;
-        const double tiles = over(n, 128) * over((gated ? 2 : 1) * m, 128) * splits;
-        double us = 6 + chunk * (tiles <= 256 ? 0.81 + 0.23 * tiles / 256 : over((int64_t)tiles, 512) * 1.77) + 0.5 * splits * moved;
-        if (splits > 1 || gated) us += 3 + (splits + 1) * moved;
-        consider(kSmallTiles, splits, chunk, us);
-        if (splits < want) break;
-    }
-    return best;
 }
 
 // Whether rows of out and residual can be moved 16 bytes at a time (a split's parts,
@@ -726,7 +654,7 @@ int linear8_launch(const Linear8Args &all)
 {
     for (int64_t row = 0; row < all.n; row += kRowsPerLaunch) {
         Linear8Args g = rows_from(all, row);
-        const Choice c = choose(g.n, g.m, g.w.groups, false);
+        const Choice c = choose(g.n, g.m, g.w.groups, false, num_cus());
         const int64_t total = (int64_t)g.n * g.m;
         g.aligned = aligned_rows(g);
         g.chunk = c.chunk;
@@ -750,7 +678,7 @@ int gated8_launch(const Linear8Args &all)
 {
     for (int64_t row = 0; row < all.n; row += kRowsPerLaunch) {
         Linear8Args g = rows_from(all, row);
-        const Choice c = choose(g.n, g.m, g.w.groups, true);
+        const Choice c = choose(g.n, g.m, g.w.groups, true, num_cus());
         g.chunk = c.chunk;
         if (c.kernel == kLargeTiles || c.kernel == kMidTiles) {
             if (!(c.kernel == kMidTiles ? launch_tiles<128, 256, 2, 4, 2, true>(g, 1, "gated8_tiles128")

@@ -178,3 +178,11 @@ def test_gated_nan_marks_its_groups(n):
     assert (s[2, :3] == 255).all() and (s[:, 1] == 255).all() and (s[:, 3] == 127).all()
     assert (np.delete(s[:, [0, 2]], 2, 0) != 255).all()
     assert (h.bytes()[0][:, 128:256] == 0).all()
+
+
+@pytest.mark.parametrize("n,m", [(1, 33), (16, 20), (7, 4096), (2, 4097)])
+@pytest.mark.parametrize("k", [1024, 1025, 1152, 1300, 2048, 2177, 4224])
+def test_runs_of_k_that_few_waves_share(n, m, k):
+    """8 groups of k and 9, 11, 16, 18 and 33, of which two and four waves have uneven runs, some none."""
+    a, w, _ = operands(n, m, k, 9)
+    check_product(linear8(a, w), *product(a, w), k)
