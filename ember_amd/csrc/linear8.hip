@@ -654,14 +654,14 @@ int linear8_launch(const Linear8Args &all)
 {
     for (int64_t row = 0; row < all.n; row += kRowsPerLaunch) {
         Linear8Args g = rows_from(all, row);
-        const Choice c = choose(g.n, g.m, g.w.groups, false, num_cus());
+        Choice c = choose(g.n, g.m, g.w.groups, false, num_cus());
         const int64_t total = (int64_t)g.n * g.m;
         g.aligned = aligned_rows(g);
-        g.chunk = c.chunk;
         if (c.splits > 1) {
-            g.part = (float *)scratch(kScratchLinear8, (size_t)c.splits * total * sizeof(float));
-            if (!g.part) return EMBER_ERR_OUT_OF_MEMORY;
+            g.part = (float *)scratch(kScratchLinear8, (size_t)c.splits * total * sizeof(float), true);
+            if (!g.part) c = without_scratch(g.w.groups, false);
         }
+        g.chunk = c.chunk;
         if (!(c.kernel == kFew ? launch_few<false>(g)
               : c.kernel == kLargeTiles ? launch_tiles<256, 256, 4, 2, 2, false>(g, 1, "linear8_tiles256")
                                         : launch_small(g, c.splits)))
@@ -678,15 +678,19 @@ int gated8_launch(const Linear8Args &all)
 {
     for (int64_t row = 0; row < all.n; row += kRowsPerLaunch) {
         Linear8Args g = rows_from(all, row);
-        const Choice c = choose(g.n, g.m, g.w.groups, true, num_cus());
+        Choice c = choose(g.n, g.m, g.w.groups, true, num_cus());
+        if (c.kernel == kFew || c.kernel == kSmallTiles) {  // h, or the parts of both sums, in fp32
+            const size_t sums = (size_t)g.n * g.m * (c.kernel == kFew ? 1 : 2 * c.splits);
+            float *const p = (float *)scratch(kScratchLinear8, sums * sizeof(float), true);
+            if (!p) c = without_scratch(g.w.groups, true);
+            (c.kernel == kFew ? g.out : g.part) = p;
+        }
         g.chunk = c.chunk;
         if (c.kernel == kLargeTiles || c.kernel == kMidTiles) {
             if (!(c.kernel == kMidTiles ? launch_tiles<128, 256, 2, 4, 2, true>(g, 1, "gated8_tiles128")
                                         : launch_tiles<256, 256, 4, 2, 2, true>(g, 1, "gated8_tiles256")))
                 return EMBER_ERR_DEVICE;
         } else if (c.kernel == kFew) {
-            g.out = (float *)scratch(kScratchLinear8, (size_t)g.n * g.m * sizeof(float));
-            if (!g.out) return EMBER_ERR_OUT_OF_MEMORY;
             g.aligned = aligned_rows(g);
             if (!launch_few<true>(g)) return EMBER_ERR_DEVICE;
             const int st = rows8_write_launch(g.h, g.out, g.m, 0, "rows8_write");
@@ -695,8 +699,6 @@ int gated8_launch(const Linear8Args &all)
             const int64_t tasks = (int64_t)g.n * g.h.scale_pitch;
             g.m *= 2;
             g.aligned = g.m % 4 == 0;
-            g.part = (float *)scratch(kScratchLinear8, (size_t)c.splits * g.n * g.m * sizeof(float));
-            if (!g.part) return EMBER_ERR_OUT_OF_MEMORY;
             if (!launch_small(g, c.splits)) return EMBER_ERR_DEVICE;
             hipLaunchKernelGGL(gated8_reduce, dim3((unsigned)std::min<int64_t>((tasks + 7) / 8, 1 << 13)), dim3(256), 0, 0, g, c.splits, tasks);
             if (!launch_ok("gated8_reduce")) return EMBER_ERR_DEVICE;

@@ -102,4 +102,11 @@ inline Choice choose(int64_t n, int64_t m, int groups, bool gated, int cus)
     return best;
 }
 
+// The same call where there is no memory for sums on their way: whole sums, which the
+// kernel writes to the output itself.
+inline Choice without_scratch(int groups, bool gated)
+{
+    return {gated ? kMidTiles : kSmallTiles, 1, groups};
+}
+
 }  // namespace ember

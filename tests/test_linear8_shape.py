@@ -20,6 +20,11 @@ extern "C" void choose(int64_t n, int64_t m, int groups, int gated, int cus, int
     const ember::Choice c = ember::choose(n, m, groups, gated != 0, cus);
     out[0] = c.kernel, out[1] = c.splits, out[2] = c.chunk;
 }
+extern "C" void without_scratch(int groups, int gated, int *out)
+{
+    const ember::Choice c = ember::without_scratch(groups, gated != 0);
+    out[0] = c.kernel, out[1] = c.splits, out[2] = c.chunk;
+}
 """
 FEW, SMALL, MID, LARGE = range(4)
 
@@ -34,6 +39,7 @@ def shape(tmp_path_factory):
     L.lane_offset.argtypes = [C.c_uint, C.c_int]
     L.few_columns.argtypes = [C.c_int64, C.c_int64, C.c_int, C.c_int]
     L.four_waves.argtypes = [C.c_int64, C.c_int, C.c_int]
+    L.without_scratch.argtypes = [C.c_int, C.c_int, C.c_void_p]
     L.choose.argtypes = [C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p]
     return L
 
@@ -81,3 +87,12 @@ def test_rules_follow_the_cards_units(shape):
     assert [shape.four_waves(m, 9, 256) for m in (1, 4096, 4097)] == [1, 1, 0] and not shape.four_waves(1, 8, 256)
     assert [shape.few_columns(9, m, 0, 256) for m in (159 * 32, 159 * 32 + 1, 159 * 64, 159 * 64 + 1)] == [1, 2, 2, 4]
     assert [shape.few_columns(33, m, 1, 256) for m in (255 * 32, 255 * 32 + 1)] == [1, 2]
+
+
+@pytest.mark.parametrize("groups", [1, 32, 65536])
+def test_without_memory_for_sums_there_are_none(shape, groups):
+    """Kernels that write to the output: of a product any with one split, of a gated layer the gated tiles."""
+    for gated, kernel in ((0, SMALL), (1, MID)):
+        out = (C.c_int * 3)()
+        shape.without_scratch(groups, gated, out)
+        assert tuple(out) == (kernel, 1, groups)
