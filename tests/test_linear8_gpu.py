@@ -186,3 +186,14 @@ def test_runs_of_k_that_few_waves_share(n, m, k):
     """8 groups of k and 9, 11, 16, 18 and 33, of which two and four waves have uneven runs, some none."""
     a, w, _ = operands(n, m, k, 9)
     check_product(linear8(a, w), *product(a, w), k)
+
+
+@pytest.mark.parametrize("n,m,k", [(40, 5101, 300), (100, 40, 4089), (257, 3001, 2100), (500, 4000, 384), (1500, 4001, 100), (4000, 2049, 640)])
+def test_out_may_be_residual_in_every_kernel(n, m, k):
+    from ember_amd import capi
+    from ember_amd.capi import DeviceArray
+    a, w, rng = operands(n, m, k, 12)
+    bias, r = rng.standard_normal(m).astype(np.float32), rng.standard_normal((n, m)).astype(np.float32)
+    dev, b = DeviceArray.from_numpy(r), DeviceArray.from_numpy(bias)
+    capi.check(capi.lib().linear8_fwd(a.view, w.view, b.ptr, dev.ptr, dev.ptr, 1), "linear8_fwd")
+    np.testing.assert_array_equal(dev.numpy(), linear8(a, w, bias, r, 1))

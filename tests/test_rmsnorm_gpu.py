@@ -164,3 +164,23 @@ def test_gradient_of_gamma_of_many_rows(rows, d, run):
     capi.check(capi.lib().rmsnorm_bwd(ones.ptr, gamma.ptr, rstd.ptr, ones.ptr, None, dx.ptr, dg.ptr, rows, d), "rmsnorm_bwd")
     exact = rows * float(t)
     assert (np.abs(dg.numpy() - exact) <= 66 * U * exact).all()
+
+
+@pytest.mark.parametrize("rows,d", [(5, 60), (70, 1024), (3, 4096), (40, 1540), (3, 16384)])
+def test_calls_that_write_over_an_input(rows, d):
+    """dx over dres; the sum in 8 bits' forward over x, and over the residual."""
+    s, more, gamma = inputs(rows, d, True, seed=13)
+    dy = np.random.default_rng(d).standard_normal(s.shape).astype(np.float32)
+    rstd = ff.rmsnorm_fwd(s, gamma, 1e-5)[1].astype(np.float32)
+    dx, dgamma = backward(s, gamma, rstd, dy, more)
+    dev, over, dg = [arr(a) for a in (s, gamma, rstd, dy)], arr(more), DeviceArray((d,))
+    capi.check(capi.lib().rmsnorm_bwd(*(a.ptr for a in dev), over.ptr, over.ptr, dg.ptr, rows, d), "rmsnorm_bwd")
+    np.testing.assert_array_equal(over.numpy(), dx)
+    np.testing.assert_array_equal(dg.numpy(), dgamma)
+    held, total = norm8(s, more, gamma)
+    for which in (0, 1):
+        pair, g, y = [arr(s), arr(more)], arr(gamma), Rows8(rows, d)
+        capi.check(capi.lib().rmsnorm_fwd8(pair[0].ptr, pair[1].ptr, g.ptr, pair[which].ptr, y.view, 1e-5), "rmsnorm_fwd8")
+        np.testing.assert_array_equal(pair[which].numpy(), total)
+        for got, want in zip(y.bytes(), held.bytes()):
+            np.testing.assert_array_equal(got, want)
