@@ -5,7 +5,10 @@
 // round.  A half wave takes a group, 4 neighbours a lane, so that a wave reads 1
 // KiB in a row; the largest size is found in register moves.  A matrix that is
 // stored transposed (a Linear layer's weight, in x out) is read with the lanes
-// along its rows: a lane holds a whole group and writes its 128 bytes.
+// along its rows: a lane holds a whole group and writes its 128 bytes, 16 at a time at
+// a row's pitch, which holds it back.  21846 x 4096: written in 82 us, 5.4 TB/s (a copy
+// of 4 GiB 4.75), transposed in 127, 3.5, read in 90, 5.0; 8 x 4096, a launch: 3.1, 5.6
+// and 3.0.
 #include <algorithm>
 
 #include "rows8.h"

@@ -3,7 +3,7 @@ reference, whose tensors are all float32).
 
 ``quantize8`` rounds a matrix to a ``Rows8``: 128 neighbours of a row share a
 power of two and each has 4 bits of exponent and 3 of fraction
-(``include/ember_amd.h`` describes the format), 33/32 byte per element.
+(``include/ember_amd.h`` describes the format), 129/128 byte per element.
 ``linear8`` multiplies two of them with the epilogue of ``nn.linear``,
 ``rms_norm8`` and ``gated8`` are layers whose output is one.  What they hold
 enters products exactly, and sums are float32, so rounding to 8 bits is the only
