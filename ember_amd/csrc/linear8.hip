@@ -588,7 +588,7 @@ bool launch_small(const Linear8Args &g, int splits)
 {
     const int64_t tiles = (((int64_t)g.n + 127) / 128) * (((int64_t)g.m + 127) / 128);
     return tiles * splits <= num_cus() ? launch_tiles<128, 128, 2, 2, 4, false>(g, splits, "linear8_tiles128_ahead")
-                                 : launch_tiles<128, 128, 2, 2, 2, false>(g, splits, "linear8_tiles128");
+                                       : launch_tiles<128, 128, 2, 2, 2, false>(g, splits, "linear8_tiles128");
 }
 
 template <int NT, int MB, int W, bool GATED>
